@@ -86,7 +86,7 @@ def draw(rng):
         B, H, W = _log(rng, 1, 256), _log(rng, 1, 96), _log(rng, 1, 96)
         while H * W * (C // G) < 64:  # statistics of a handful of values are of no use to anybody
             H, W = 2 * H, W + 1
-        while B * H * W * C > 40_000_000:
+        while B * H * W * C > 30_000_000:
             B, H = max(1, B // 2), max(1, H - H // 3)
         return _norm(None, rng.random() < 0.75, dtype, B, H, W, C, G, rng.choice(["none", "silu", "sigmoid"]))
     if kind == "drop":
