@@ -17,7 +17,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # DIFFLUT_HIP_LIB points at another build of the same library (kernel experiments)
 LIB_PATH = os.environ.get("DIFFLUT_HIP_LIB") or os.path.join(_HERE, "lib", "libdifflut_hip.so")
 
-_P, _I, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+_P, _I, _F, _Z, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
 
 # name -> (restype, argtypes); mirrors include/difflut_hip.h one to one
 SIGNATURES = {
@@ -106,6 +106,16 @@ SIGNATURES = {
     "dl_adam_step": (_I, [_P, _P, _P, _P, _P, _I, _F, _F, _F, _F, _F, _I, _I, _P]),
     "dl_grad_stabilize_workspace_bytes": (_Z, [ctypes.c_longlong, ctypes.c_longlong, _I]),
     "dl_grad_stabilize": (_I, [_P, _P, ctypes.c_longlong, ctypes.c_longlong, _I, _F, _I, _F, _P, _Z, _P]),
+    "dl_embedding_fwd": (_I, [_P, _I, _P, _L, _P, _I, _L, _L, _I, _F, _P]),
+    "dl_embedding_bwd_workspace_bytes": (_Z, [_L, _L, _I]),
+    "dl_embedding_bwd": (_I, [_P, _I, _P, _P, _I, _L, _L, _I, _F, _L, _P, _Z, _P]),
+    "dl_group_norm_fwd_workspace_bytes": (_Z, [_I, _I, _L, _I, _I]),
+    "dl_group_norm_fwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _L, _I, _I, _F, _I, _P, _Z, _P]),
+    "dl_group_norm_bwd_workspace_bytes": (_Z, [_I, _I, _L, _I, _I]),
+    "dl_group_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _I, _I, _I, _P, _Z, _P]),
+    "dl_dropout": (_I, [_P, _P, _I, _L, ctypes.c_double, _I, ctypes.c_ulonglong, ctypes.c_ulonglong, _P, _P, _P]),
+    "dl_sample_workspace_bytes": (_Z, [_I, _I]),
+    "dl_sample": (_I, [_P, _L, _I, _P, _P, _P, _P, _P, _F, _I, _F, _F, _P, _P, _Z, _I, _I, _P]),
     "dl_profile_enable": (_I, [_I]),
     "dl_profile_read": (_I, [ctypes.c_char_p, _Z, ctypes.POINTER(_F), _I]),
 }

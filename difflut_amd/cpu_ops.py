@@ -9,6 +9,8 @@ argument conventions of `ops.py`, vectorised over batch, nodes and the 2^k table
 reference's interpreter loops.  Like the reference's CPU path the EFD sums are accumulated in float64 and
 rounded once.  Nothing here touches the HIP library, and nothing of the device path comes through here.
 """
+import math
+
 import torch
 
 _NODE_CHUNK = 256  # nodes per pass of the per-node weight tensors [chunk, k, L, L]
@@ -273,3 +275,110 @@ def group_sum(x, groups, tau):
     if pad:
         x = torch.nn.functional.pad(x, (0, pad))
     return x.float().view(B, groups, -1).sum(-1) / tau
+
+
+# ----------------------------------------------------------------------------- around the layers
+def _wide(t):
+    """float32 for the 16-bit types; float32 and float64 stay."""
+    if t.dtype not in (torch.float64, torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"expected a float tensor, got {t.dtype}")
+    return t if t.dtype is torch.float64 else t.float()
+
+
+def embedding(tokens, weight, scale, padding):
+    V = weight.shape[0]
+    known = ((tokens >= 0) & (tokens < V)).unsqueeze(-1)
+    rows = _wide(weight)[tokens.long().clamp(0, V - 1)] * scale
+    rows = torch.where((tokens == padding).unsqueeze(-1), rows.detach(), rows)
+    return torch.where(known, rows, torch.zeros_like(rows)).to(weight.dtype)
+
+
+def group_norm(x, groups, weight, bias, eps, activation):
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
+        raise TypeError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
+    B, C = x.shape[0], x.shape[-1]
+    xg = _wide(x).reshape(B, -1, groups, C // groups)
+    centred = xg - xg.mean((1, 3), keepdim=True)
+    z = (centred / torch.sqrt(centred.square().mean((1, 3), keepdim=True) + eps)).reshape(x.shape)
+    if weight is not None:
+        z = z * _wide(weight)
+    if bias is not None:
+        z = z + _wide(bias)
+    if activation == "sigmoid":
+        z = torch.sigmoid(z)
+    elif activation == "silu":
+        z = z * torch.sigmoid(z)
+    elif activation == "relu":
+        z = torch.relu(z)
+    return z.to(x.dtype).contiguous()  # as on the device
+
+
+def philox_words(seed, offset, numel):
+    """The words of Philox 4x32-10 (Salmon, Moraes, Dror, Shaw 2011) that belong to entries 0 .. numel - 1, as int64 [numel]."""
+    low = 0xFFFFFFFF
+
+    def product(a, m):  # high and low word: int64 holds the partial products of m's halves
+        part = a * (m & 0xFFFF)
+        upper = a * (m >> 16) + (part >> 16)
+        return upper >> 16, ((upper & 0xFFFF) << 16) | (part & 0xFFFF)
+
+    counter = torch.arange(-(-numel // 4), dtype=torch.int64)
+    c = [counter & low, counter >> 32, torch.full_like(counter, offset & low), torch.full_like(counter, (offset >> 32) & low)]
+    k0, k1 = seed & low, (seed >> 32) & low
+    for _ in range(10):
+        (h0, l0), (h1, l1) = product(c[0], 0xD2511F53), product(c[2], 0xCD9E8D57)
+        c = [h1 ^ c[1] ^ k0, l1, h0 ^ c[3] ^ k1, l0]
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    return torch.stack(c, dim=1).reshape(-1)[:numel]
+
+
+def dropout(x, p, state, mode):
+    wide = _wide(x)
+    hit = (philox_words(*state, x.numel()) < math.floor(p * 2.0 ** 32 + 0.5)).view(x.shape)
+    if mode == "flip":
+        flipped = torch.where(hit, 1.0 - wide.detach(), wide.detach()).to(x.dtype)
+        return _PassGradient.apply(x, flipped)
+    factor = 1.0 / (1.0 - p) if p < 1.0 else 0.0
+    return torch.where(hit, torch.zeros_like(wide), wide * factor).to(x.dtype)
+
+
+class _PassGradient(torch.autograd.Function):
+    """The second argument's values, the first one's place in the graph."""
+
+    @staticmethod
+    def forward(ctx, x, values):
+        return values
+
+    @staticmethod
+    def backward(ctx, g):
+        return g, None
+
+
+@torch.no_grad()
+def sample(logits, uniform, temperature, top_k, top_p, min_p):
+    """In float64.  Settings are float32 values, like those that the device kernels read."""
+    B, V = logits.shape
+    x = logits.double()
+    x = torch.where(x.isnan(), -math.inf, x)
+
+    def column(v):
+        return (v if torch.is_tensor(v) else torch.full((B,), float(v))).float().double().view(B, 1)
+
+    T, p, m, u = column(temperature), column(top_p), column(min_p), column(uniform)
+    k = top_k.long().view(B, 1) if torch.is_tensor(top_k) else torch.full((B, 1), int(top_k))
+    k = torch.where((T > 0) & (p > 0) & (m <= 1), k, 1)
+    ordered, order = torch.sort(x, dim=1, descending=True, stable=True)
+    top, rank = ordered[:, :1], torch.arange(V)
+    w = torch.where(ordered == top, 1.0, torch.exp((ordered - top) / torch.where(T > 0, T, 1.0)))
+    w = torch.where(ordered > -math.inf, w, 0.0).nan_to_num(0.0)
+    keep = (ordered > -math.inf) & ((rank < k) | (k <= 0))
+    running = torch.cumsum(w * keep, 1)
+    before = torch.cat([torch.zeros_like(top), running[:, :-1]], 1)
+    keep &= (before < p * running[:, -1:]) | (p >= 1) | (rank == 0)
+    keep &= (w >= m) | (rank == 0)
+    kept = torch.zeros_like(x).scatter_(1, order, w * keep)
+    running = torch.cumsum(kept, 1)
+    u = torch.where(u > 0, u, 0.0)
+    last = torch.where(kept > 0, rank, -1).amax(1)
+    token = torch.minimum((running <= u * running[:, -1:]).sum(1), last)
+    return torch.where(top.view(B) > -math.inf, token, -1)

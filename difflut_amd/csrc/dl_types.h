@@ -1,0 +1,44 @@
+// Element types of the operators that take float32, bfloat16 and float16 tensors: loads widen to float, stores round once
+// (to nearest, ties to even).
+#pragma once
+#include "dl_common.h"
+
+typedef __bf16 dl_bf16;
+typedef _Float16 dl_f16;
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) DlVec {
+    T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ void dl_load(const T *p, float (&f)[N]) {
+    const DlVec<T, N> t = *reinterpret_cast<const DlVec<T, N> *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = (float)t.v[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void dl_store(T *p, const float (&f)[N]) {
+    DlVec<T, N> t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t.v[i] = (T)f[i];
+    *reinterpret_cast<DlVec<T, N> *>(p) = t;
+}
+
+static inline bool dl_type_known(int type) { return type == DL_F32 || type == DL_BF16 || type == DL_F16; }
+static inline int dl_type_bytes(int type) { return type == DL_F32 ? 4 : 2; }
+static inline bool dl_aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// DL_BY_TYPE(type, T, statement): the statement with T as the element type
+#define DL_BY_TYPE(type, T, ...)                    \
+    do {                                            \
+        if ((type) == DL_F32) {                     \
+            typedef float T;                        \
+            __VA_ARGS__;                            \
+        } else if ((type) == DL_BF16) {             \
+            typedef dl_bf16 T;                      \
+            __VA_ARGS__;                            \
+        } else {                                    \
+            typedef dl_f16 T;                       \
+            __VA_ARGS__;                            \
+        }                                           \
+    } while (0)

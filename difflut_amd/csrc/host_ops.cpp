@@ -36,7 +36,10 @@ namespace {
     X(dl_dwn_layer_fwd_planes_groups) X(dl_dwn_layer_eval_planes) X(dl_dwn_layer_eval_planes_groups) X(dl_dwn_layer_rows) X(dl_dwn_rows_pay) \
     X(dl_dwn_layer_bwd_groups) X(dl_dwn_layer_bwd_tiled) X(dl_dwn_chain_fusable) X(dl_dwn_bwd_fused_workspace_bytes)     \
     X(dl_dwn_layer_bwd_chain_fused) X(dl_dwn_chain_first_fusable) X(dl_dwn_bwd_first_workspace_bytes)                    \
-    X(dl_dwn_layer_bwd_chain_first) X(dl_cross_entropy_workspace_bytes) X(dl_cross_entropy) X(dl_adam_step)
+    X(dl_dwn_layer_bwd_chain_first) X(dl_cross_entropy_workspace_bytes) X(dl_cross_entropy) X(dl_adam_step) \
+    X(dl_embedding_fwd) X(dl_embedding_bwd_workspace_bytes) X(dl_embedding_bwd) X(dl_group_norm_fwd_workspace_bytes)     \
+    X(dl_group_norm_fwd) X(dl_group_norm_bwd_workspace_bytes) X(dl_group_norm_bwd) X(dl_dropout)                         \
+    X(dl_sample_workspace_bytes) X(dl_sample)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     DL_FUNCTIONS(X)
@@ -765,6 +768,168 @@ Tensor dwn_stack_eval(const Tensor &x_, const Maybe &thresholds, const std::vect
     return y;
 }
 
+// ------------------------------------------------------------------ around the layers: embedding, group norm, dropout, sampling
+// These take float32, bfloat16 and float16 tensors as they are, and work on the device of their tensors whatever the current one.
+int type_of(const Tensor &t, const char *what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return DL_F32;
+        case at::kBFloat16: return DL_BF16;
+        case at::kHalf: return DL_F16;
+        default: TORCH_CHECK_TYPE(false, what, " must be float32, bfloat16 or float16 on the device, got ", t.scalar_type());
+    }
+}
+void same_device(const Tensor &first, const Tensor &t, const char *what) {
+    require_device(t);
+    TORCH_CHECK(!t.defined() || t.device() == first.device(), what, " is on ", t.device(), ", expected ", first.device());
+}
+void once(const char *what) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (a backward with create_graph=True)");
+}
+const void *raw_in(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+struct Embedding : torch::autograd::Function<Embedding> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &tokens_, const Tensor &weight_, double scale, int64_t padding) {
+        const c10::DeviceGuard guard(weight_.device());
+        const Tensor tokens = tokens_.contiguous();
+        // rows may lie apart, as in a slice of a wider matrix
+        const bool rows = weight_.stride(1) == 1 && weight_.stride(0) >= weight_.size(1);
+        const Tensor weight = rows ? weight_ : weight_.contiguous();
+        const int64_t V = weight.size(0), D = weight.size(1);
+        auto sizes = tokens.sizes().vec();
+        sizes.push_back(D);
+        const Tensor y = at::empty(sizes, weight.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+        check(L.dl_embedding_fwd(raw_in(tokens), tokens.scalar_type() == at::kInt ? 32 : 64, raw_in(weight),
+                                 V > 1 ? weight.stride(0) : std::max(D, weight.stride(0)), raw(y), type_of(weight, "weight"), tokens.numel(), V, D,
+                                 (float)scale, stream()));
+        ctx->save_for_backward({tokens});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding;
+        ctx->saved_data["V"] = V;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        once("embedding");
+        const Tensor tokens = ctx->get_saved_variables()[0], gy = grads[0].contiguous();
+        const c10::DeviceGuard guard(gy.device());
+        const int64_t V = ctx->saved_data["V"].toInt(), D = gy.size(-1), n = tokens.numel();
+        const Tensor gw = at::empty({V, D}, gy.options()), ws = bytes(L.dl_embedding_bwd_workspace_bytes(n, V, D), gy);
+        check(L.dl_embedding_bwd(raw_in(tokens), tokens.scalar_type() == at::kInt ? 32 : 64, raw_in(gy), raw(gw), type_of(gy, "gradient"), n, V, D,
+                                 (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), raw(ws), ws.numel(), stream()));
+        return {Tensor(), gw, Tensor(), Tensor()};
+    }
+};
+Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale, int64_t padding) {
+    require_device(weight);
+    same_device(weight, tokens, "tokens");
+    TORCH_CHECK_TYPE(tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong, "tokens must be int32 or int64, got ", tokens.scalar_type());
+    type_of(weight, "weight");
+    return Embedding::apply(tokens, weight, scale, padding);
+}
+
+// x [B, ..., C], the channels last
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Maybe &weight_, const Maybe &bias_, int64_t groups, double eps, int64_t act) {
+        const c10::DeviceGuard guard(x_.device());
+        const Tensor x = x_.contiguous(), weight = weight_ ? weight_->contiguous() : Tensor(), bias = bias_ ? bias_->contiguous() : Tensor();
+        const int64_t B = x.size(0), C = x.size(-1), P = x.numel() / (B * C);
+        const Tensor y = at::empty_like(x), stats = floats({B, groups, 2}, x);
+        const int type = type_of(x, "x"), ptype = weight.defined() ? type_of(weight, "weight") : bias.defined() ? type_of(bias, "bias") : type;
+        const Tensor ws = bytes(L.dl_group_norm_fwd_workspace_bytes(type, B, P, C, groups), x);
+        check(L.dl_group_norm_fwd(raw_in(x), raw_in(weight), raw_in(bias), raw(y), out(stats), type, ptype, B, P, C, groups, (float)eps, (int)act,
+                                  raw(ws), ws.numel(), stream()));
+        ctx->save_for_backward({x, weight, bias, stats});
+        ctx->saved_data["act"] = act;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        once("group_norm");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+        const c10::DeviceGuard guard(x.device());
+        const Tensor gy = grads[0].contiguous();
+        const int64_t B = x.size(0), C = x.size(-1), P = x.numel() / (B * C), groups = stats.size(1);
+        const int type = type_of(x, "x"), ptype = weight.defined() ? type_of(weight, "weight") : bias.defined() ? type_of(bias, "bias") : type;
+        const Tensor gx = ctx->needs_input_grad(0) ? at::empty_like(x) : Tensor(),
+                     gw = weight.defined() && ctx->needs_input_grad(1) ? at::empty_like(weight) : Tensor(),
+                     // (inputs are counted without those that are missing)
+                     gb = bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1) ? at::empty_like(bias) : Tensor();
+        const Tensor ws = bytes(L.dl_group_norm_bwd_workspace_bytes(type, B, P, C, groups), x);
+        check(L.dl_group_norm_bwd(raw_in(x), raw_in(gy), raw_in(weight), raw_in(bias), in(stats), raw(gx), raw(gw), raw(gb), type, ptype, B, P, C,
+                                  groups, (int)ctx->saved_data["act"].toInt(), raw(ws), ws.numel(), stream()));
+        return {gx, gw, gb, Tensor(), Tensor(), Tensor()};
+    }
+};
+Tensor group_norm(const Tensor &x, int64_t groups, const Maybe &weight_, const Maybe &bias_, double eps, int64_t act) {
+    const Tensor weight = tensor_of(weight_), bias = tensor_of(bias_);
+    require_device(x);
+    same_device(x, weight, "weight");
+    same_device(x, bias, "bias");
+    type_of(x, "x");
+    if (weight.defined()) type_of(weight, "weight");
+    if (bias.defined()) type_of(bias, "bias");
+    TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), "weight and bias must be of one type, got ",
+                     weight.scalar_type(), " and ", bias.scalar_type());
+    return GroupNorm::apply(x, weight_, bias_, groups, eps, act);
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, double p, int64_t mode, int64_t seed, int64_t offset, const Maybe &state_) {
+        const c10::DeviceGuard guard(x_.device());
+        const Tensor x = x_.contiguous(), y = at::empty_like(x), state = tensor_of(state_);
+        // what the state held is kept for the backward: by then the caller may have moved it on
+        const Tensor used = state.defined() ? at::empty_like(state) : Tensor();
+        check(L.dl_dropout(raw_in(x), raw(y), type_of(x, "x"), x.numel(), p, (int)mode, (unsigned long long)seed, (unsigned long long)offset,
+                           state.defined() ? (const long long *)state.const_data_ptr<int64_t>() : nullptr, (long long *)raw(used), stream()));
+        ctx->save_for_backward({used});
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["mode"] = mode;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["offset"] = offset;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const int64_t mode = ctx->saved_data["mode"].toInt();
+        const Tensor used = ctx->get_saved_variables()[0];
+        const Tensor g = mode == DL_DROP_FLIP ? grads[0]
+                                              : apply(grads[0], ctx->saved_data["p"].toDouble(), mode, ctx->saved_data["seed"].toInt(),
+                                                      ctx->saved_data["offset"].toInt(), used.defined() ? Maybe(used) : Maybe());
+        return {g, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+Tensor dropout(const Tensor &x, double p, int64_t mode, int64_t seed, int64_t offset, const Maybe &state_) {
+    const Tensor state = tensor_of(state_);
+    require_device(x);
+    same_device(x, state, "state");
+    type_of(x, "x");
+    return Dropout::apply(x, p, mode, seed, offset, state_);
+}
+
+// Settings are a number, or a tensor [B] with every row's own
+Tensor sample(const Tensor &logits_, const Tensor &uniform_, const Maybe &temperature, const Maybe &top_k, const Maybe &top_p, const Maybe &min_p,
+              double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all) {
+    at::NoGradGuard no_grad;
+    require_device(logits_);
+    const c10::DeviceGuard guard(logits_.device());
+    const int64_t B = logits_.size(0), V = logits_.size(1);
+    const int type = type_of(logits_, "logits");
+    const auto rows = [&](const Maybe &t, at::ScalarType dtype, const char *what) {
+        if (!t) return Tensor();
+        same_device(logits_, *t, what);
+        TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == B, what, " must be [", B, "], got ", t->sizes());
+        return t->to(dtype).contiguous();
+    };
+    const Tensor logits = logits_.stride(1) == 1 && (logits_.stride(0) >= V || B <= 1) ? logits_ : logits_.contiguous();
+    const Tensor uniform = rows(uniform_, at::kFloat, "uniform"), T = rows(temperature, at::kFloat, "temperature"),
+                 k = rows(top_k, at::kInt, "top_k"), p = rows(top_p, at::kFloat, "top_p"), m = rows(min_p, at::kFloat, "min_p");
+    const Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong).requires_grad(false));
+    const size_t need = L.dl_sample_workspace_bytes((int)B, (int)V);
+    const Tensor ws = need ? bytes(need, logits) : Tensor();
+    check(L.dl_sample(raw_in(logits), B > 1 ? logits.stride(0) : V, type, in(uniform), in(T), k.defined() ? ints(k) : nullptr, in(p), in(m),
+                      (float)temperature_all, (int)std::min<int64_t>(top_k_all, INT_MAX), (float)top_p_all, (float)min_p_all,
+                      (long long *)raw(tokens), raw(ws), need, (int)B, (int)V, stream()));
+    return tokens;
+}
+
 // Whether rows 0, n - 1 and `count` rows from `start` on (around the end) of a bank's nodes still hold the views the bank handed out:
 // nodes[keys[row]]._buffers[name] is views[row].  In Python, 18 rows took 3.5 us a bank, two banks a call of a layer.
 bool views_hold(const py::dict &nodes, const py::tuple &keys, const py::str &name, const py::list &views, Py_ssize_t start, Py_ssize_t count) {
@@ -808,5 +973,9 @@ PYBIND11_MODULE(difflut_host, m) {
     m.def("dwn_stack", &dwn_stack, free_gil);
     m.def("dwn_stack_eval", &dwn_stack_eval, free_gil);
     m.def("adam_step", &adam_step);
+    m.def("embedding", &embedding, free_gil);
+    m.def("group_norm", &group_norm, free_gil);
+    m.def("dropout", &dropout, free_gil);
+    m.def("sample", &sample, free_gil);
     m.def("cross_entropy", [](const Tensor &logits, const Tensor &labels) { return CrossEntropy::apply(logits, labels); }, free_gil);
 }

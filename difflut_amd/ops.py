@@ -496,3 +496,110 @@ def cross_entropy(logits, labels):
     if logits.is_cuda:
         return CrossEntropyFunction.apply(logits, labels)
     return torch.nn.functional.cross_entropy(logits.float(), labels.long())
+
+
+# ----------------------------------------------------------------------------- around the layers
+# Tokens in, normalised activations and noise between the layers, tokens out.  Unlike the layers these take float32, bfloat16
+# and float16 tensors as they are (on the CPU float64 as well), and work on their tensors' device whatever the current one is.
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "sigmoid": 3}
+DROP_MODES = {"zero": 0, "flip": 1}
+
+
+def embedding(tokens, weight, scale=1.0, padding_idx=None):
+    """scale * weight[tokens]: rows of weight [V, D] for int32 or int64 tokens of any shape -> [*tokens.shape, D] in weight's type.
+
+    A token outside [0, V) gives a row of zeros and no gradient (as cross_entropy leaves out such labels); `padding_idx` is looked
+    up like any other token but gets no gradient.  The weight's gradient is dense, summed in float32 in the order of the
+    positions: the same bits from run to run.  Rows of `weight` may lie apart (a slice of a wider matrix)."""
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"embedding weight must be a non-empty matrix (tokens, features), got {tuple(weight.shape)}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"tokens must be int32 or int64, got {tokens.dtype}")
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}), got {padding_idx}")
+    padding = -1 if padding_idx is None else int(padding_idx)
+    if weight.is_cuda:
+        return nat.host().embedding(tokens, weight, float(scale), padding)
+    return cpu_ops.embedding(tokens, weight, float(scale), padding)
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
+    """Group norm of x [B, ..., C] (channels last) over the positions and the C / groups channels of each group, then weight [C]
+    and bias [C] (of one type; either may be missing), then `activation`: "none", "relu", "silu" or "sigmoid"."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    if x.dim() < 2 or x.numel() == 0:
+        raise ValueError(f"group_norm expects a non-empty (batch, ..., channels), got shape {tuple(x.shape)}")
+    channels = x.shape[-1]
+    if not isinstance(groups, int) or groups <= 0 or channels % groups != 0:
+        raise ValueError(f"groups must be a positive divisor of the {channels} channels, got {groups}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (channels,):
+            raise ValueError(f"group_norm {name} must be [{channels}], got {tuple(t.shape)}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if x.is_cuda:
+        return nat.host().group_norm(x, groups, weight, bias, float(eps), ACTIVATIONS[activation])
+    return cpu_ops.group_norm(x, groups, weight, bias, float(eps), activation)
+
+
+def dropout(x, p, state, mode="zero"):
+    """Noise from a counter-based generator whose mask is never stored; `state` = (seed, offset) says which one.
+
+    mode "zero": entries become 0 with probability p and the others x / (1 - p); the gradient goes through the same mask.
+    mode "flip": entries become 1 - x with probability p, the bit-flip augmentation of the LUT layers: the gradient passes as if
+    nothing had been flipped.
+    Entry e (in row-major order, whatever the strides) is hit where word e % 4 of Philox 4x32-10 at counter (e // 4, offset) under
+    the key `seed` is below round(p * 2^32), on the device and on the CPU.  `state` is a pair of numbers, or an int64 tensor [2] on
+    x's device that is read when the call runs: a captured call then draws another mask once the tensor has changed."""
+    if mode not in DROP_MODES:
+        raise ValueError(f"mode must be one of {list(DROP_MODES)}, got {mode!r}")
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be in [0, 1], got {p}")
+    if torch.is_tensor(state):
+        if state.dtype is not torch.int64 or tuple(state.shape) != (2,) or not state.is_contiguous():
+            raise TypeError(f"a state tensor is contiguous int64 [2], got {state.dtype} {tuple(state.shape)}")
+        seed, offset, tensor = 0, 0, state
+    else:
+        (seed, offset), tensor = (_signed64(v) for v in state), None
+    if x.is_cuda:
+        return nat.host().dropout(x, float(p), DROP_MODES[mode], seed, offset, tensor)
+    return cpu_ops.dropout(x, float(p), (seed, offset) if tensor is None else tuple(tensor.tolist()), mode)
+
+
+def _signed64(v):
+    """A whole number modulo 2^64, as the int64 of the same bits."""
+    v = int(v) % (1 << 64)
+    return v - (1 << 64) if v >= 1 << 63 else v
+
+
+def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One index per row of logits [B, V], drawn with the given random numbers uniform [B] in [0, 1) -> int64 [B].
+
+    The row's indices are ordered by logit, equal ones by index.  top_k keeps the first k (0: all), top_p of these the shortest
+    prefix whose weights exp((logit - max) / temperature) reach top_p times their sum (1: all), min_p of these the ones whose
+    weight is at least min_p; the first always stays.  The answer is the first kept index whose running sum, in index order, exceeds
+    uniform times the kept sum.  temperature 0 takes the first of the order.  NaN counts as -infinity; a row with nothing above
+    that gives -1.  Weights are summed in 64 bits: the answer does not depend on how the work is split.
+
+    Each setting is a number or a tensor [B] with every row's own (whose values are not looked at on the host: temperature <= 0,
+    top_p <= 0 and min_p > 1 leave the first index alone)."""
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"sample expects logits (batch, classes), got shape {tuple(logits.shape)}")
+    B = logits.shape[0]
+    if tuple(uniform.shape) != (B,) or not uniform.is_floating_point():
+        raise ValueError(f"uniform must be a floating-point tensor [{B}], got {uniform.dtype} {tuple(uniform.shape)}")
+    settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    fine = {"temperature": lambda v: v >= 0, "top_k": lambda v: v >= 0 and int(v) == v, "top_p": lambda v: 0 < v <= 1,
+            "min_p": lambda v: 0 <= v <= 1}
+    for name, v in settings.items():
+        if torch.is_tensor(v):
+            if tuple(v.shape) != (B,):
+                raise ValueError(f"{name} must be a number or a tensor [{B}], got {tuple(v.shape)}")
+        elif not fine[name](v):
+            raise ValueError(f"{name} out of range: {v}")
+    if not logits.is_cuda:
+        return cpu_ops.sample(logits, uniform, **settings)
+    tensors = [v if torch.is_tensor(v) else None for v in settings.values()]
+    numbers = [0 if torch.is_tensor(v) else v for v in settings.values()]
+    return nat.host().sample(logits, uniform, *tensors, float(numbers[0]), int(numbers[1]), float(numbers[2]), float(numbers[3]))

@@ -486,6 +486,61 @@ int dl_unfold_flip(const float *x, const uint8_t *flip, float *patches, void *pl
                    int KH, int KW, int SH, int SW, int PH, int PW, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Around the layers, in models over tokens and deep convolutional stacks.  No counterpart in the reference.
+ * `type` / `ptype`: element type of tensors / of gamma and beta; 16-bit values are widened to float, results rounded once.
+ * ------------------------------------------------------------------------ */
+#define DL_F32 0
+#define DL_BF16 1
+#define DL_F16 2
+
+/* Embedding lookup: y[t] = scale * weight[token_t], tokens int32 or int64 (token_bits) [n], weight [V, D] with ldw elements
+ * between rows, y [n, D].  A token outside [0, V) gives a row of zeros.
+ * Its gradient: gw[v] = scale * sum_{t: token_t = v} gy[t], [V, D], every row written; tokens outside [0, V) and those equal to
+ * `padding` (-1: none) add nothing.  Positions are sorted by token on the device and added in that order, in float: the same bits from run to run. */
+int dl_embedding_fwd(const void *tokens, int token_bits, const void *weight, long long ldw, void *y, int type, long long n,
+                     long long V, int D, float scale, void *stream);
+size_t dl_embedding_bwd_workspace_bytes(long long n, long long V, int D);
+int dl_embedding_bwd(const void *tokens, int token_bits, const void *gy, void *gw, int type, long long n, long long V, int D,
+                     float scale, long long padding, void *ws, size_t ws_bytes, void *stream);
+
+/* Group norm over channels-last activations x [B, P, C] (P positions, G groups of C / G neighbouring channels), with an
+ * activation: y = act((x - mean) * rstd * gamma + beta), rstd = 1 / sqrt(var + eps); gamma / beta [C] may be null (1 / 0).
+ * stats [B, G, 2] receives mean and rstd for the backward, which writes gx, ggamma, gbeta (each may be null). */
+#define DL_ACT_NONE 0
+#define DL_ACT_RELU 1
+#define DL_ACT_SILU 2
+#define DL_ACT_SIGMOID 3
+size_t dl_group_norm_fwd_workspace_bytes(int type, int B, long long P, int C, int G);
+int dl_group_norm_fwd(const void *x, const void *gamma, const void *beta, void *y, float *stats, int type, int ptype, int B,
+                      long long P, int C, int G, float eps, int act, void *ws, size_t ws_bytes, void *stream);
+size_t dl_group_norm_bwd_workspace_bytes(int type, int B, long long P, int C, int G);
+int dl_group_norm_bwd(const void *x, const void *gy, const void *gamma, const void *beta, const float *stats, void *gx,
+                      void *ggamma, void *gbeta, int type, int ptype, int B, long long P, int C, int G, int act, void *ws,
+                      size_t ws_bytes, void *stream);
+
+/* Dropout from a counter-based generator, no mask stored: element e is hit where word e % 4 of Philox 4x32-10 at counter
+ * (e / 4, offset) under the key `seed` is below round(p * 2^32).  DL_DROP_ZERO: y = hit ? 0 : x / (1 - p), and called on gy with
+ * the same seed and offset its own backward; DL_DROP_FLIP: y = hit ? 1 - x : x (the bit-flip augmentation, whose backward is
+ * the identity).  state (nullable): device int64 [2] read instead of seed and offset (then a captured call draws anew when the
+ * values change); used (nullable, with state): receives the pair that was read.  x and y do not overlap. */
+#define DL_DROP_ZERO 0
+#define DL_DROP_FLIP 1
+int dl_dropout(const void *x, void *y, int type, long long numel, double p, int mode, unsigned long long seed,
+               unsigned long long offset, const long long *state, long long *used, void *stream);
+
+/* One index per row of logits [B, V] (ldl elements between rows), from given random numbers uniform [B] in [0, 1).
+ * Order: logit descending, equal ones by index.  top_k keeps the first k (<= 0: all), top_p of these the shortest prefix whose
+ * weights exp((l - max) / T) reach p times their sum (>= 1: all), min_p of these the ones that weigh at least m; the first always
+ * stays.  out[b]: the first kept index, in index order, whose running sum exceeds uniform[b] times the kept sum; T <= 0: the
+ * first of the order; -1 where no logit is above -infinity (NaN counts as that).
+ * Settings: device arrays [B] where given, else the numbers behind them for every row.
+ * Workspace: dl_sample_workspace_bytes(B, V), 0 up to V = 4096. */
+size_t dl_sample_workspace_bytes(int B, int V);
+int dl_sample(const void *logits, long long ldl, int type, const float *uniform, const float *temperature, const int *top_k,
+              const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all, float min_p_all,
+              long long *out, void *ws, size_t ws_bytes, int B, int V, void *stream);
+
+/* ------------------------------------------------------------------------
  * Per-kernel timing.  No counterpart in the reference (it has no tracing at all).
  * After dl_profile_enable(1) every kernel launched by the entry points above is
  * bracketed by HIP events on its stream (at most 64 kernels between two reads).

@@ -1,0 +1,705 @@
+"""Embedding, group norm, dropout and sampling on the CPU (the branch of the same entry points that CPU tensors take) and on the
+device, against the definitions in 64 bits.
+
+Tolerances are sums of roundings.  u = 2^-24 is float32's half step; a value that is rounded to type t at the end is off by
+half a step of it, eps(t) / 2 times its size.  A float32 sum of terms a_i in which no term goes through more than d additions is
+off by d u sum |a_i|; the bounds below are taken element by element from the exact values.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from difflut_amd import ops
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+CPU_AND_GPU = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def close(got, want, bound, dtype):
+    """|got - want| within `bound` (of what was computed) and the rounding to `dtype` (of what came out)."""
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    bound = torch.as_tensor(bound, dtype=torch.float64).cpu() if not torch.is_tensor(bound) else bound.double().cpu()
+    limit = bound * (1 + half(dtype)) + half(dtype) * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    off = (got - want).abs()
+    assert bool((off <= limit).all()), f"off by {float((off - limit).max())} more than {float(limit.max())}"
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ----------------------------------------------------------------------------- embedding
+def embedding_64(tokens, weight, scale, gy, padding=None):
+    V, D = weight.shape
+    flat = tokens.reshape(-1).long()
+    known = (flat >= 0) & (flat < V)
+    y = torch.zeros(flat.numel(), D, dtype=torch.float64)
+    y[known] = weight.double()[flat[known]] * scale
+    gw, size, terms = (torch.zeros(V, n, dtype=torch.float64) for n in (D, D, 1))
+    summed = known if padding is None else known & (flat != padding)
+    g = gy.double().reshape(-1, D)[summed]
+    gw.index_add_(0, flat[summed], g)
+    size.index_add_(0, flat[summed], g.abs())
+    terms.index_add_(0, flat[summed], torch.ones(len(g), 1, dtype=torch.float64))
+    return y.view(*tokens.shape, D), gw * scale, size * abs(scale), terms
+
+
+# a single token; rows shorter than a vector, odd, of a vector, of several teams; pieces that end inside a token's run
+EMBED = [((1,), 1, 1), ((1,), 7, 5), ((3, 5), 9, 8), ((16,), 3, 64), ((17,), 1, 33), ((33, 2), 5, 257), ((300,), 1000, 16), ((0,), 6, 12),
+         ((4, 129), 2, 1030), ((2049,), 700, 4)]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("shape,V,D", EMBED)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding(device, shape, V, D, dtype):
+    g = gen(V + D)
+    tokens = (torch.rand(shape, generator=g) ** 3 * V).long().clamp_(0, V - 1)
+    weight, gy = torch.randn(V, D, generator=g).to(dtype), torch.randn(*shape, D, generator=g).to(dtype)
+    scale = 1.75
+    want, want_g, size, terms = embedding_64(tokens, weight, scale, gy)
+    for ids in (tokens, tokens.int()):
+        w = weight.to(device).requires_grad_()
+        y = ops.embedding(ids.to(device), w, scale)
+        assert y.shape == want.shape and y.dtype is dtype
+        close(y, want, want.abs() * U, dtype)
+        grad, = torch.autograd.grad(y, w, gy.to(device))
+        assert grad.dtype is dtype
+        close(grad, want_g, size * (terms + 1) * U, dtype)  # the terms' additions and the product with scale
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_embedding_of_tokens_outside_and_padding(device):
+    V, D, g = 10, 12, gen(3)
+    weight, gy = torch.randn(V, D, generator=g), torch.randn(9, D, generator=g)
+    tokens = torch.tensor([-1, 3, 10, 3, 0, 9, 2 ** 40, 0, -2 ** 40])
+    want, want_g, size, terms = embedding_64(tokens, weight, 1.0, gy, padding=0)
+    w = weight.to(device).requires_grad_()
+    y = ops.embedding(tokens.to(device), w, padding_idx=0)
+    assert torch.equal(y.cpu().double(), want) and torch.equal(y[4].cpu(), weight[0])  # padding is looked up all the same
+    grad, = torch.autograd.grad(y, w, gy.to(device))
+    close(grad, want_g, size * terms * U, torch.float32)
+    assert not grad[0].any() and not grad[1].any()
+    # nothing but padding, nothing but strangers
+    for ids in (torch.zeros(40, dtype=torch.long), torch.full((40,), -7)):
+        y = ops.embedding(ids.to(device), w, padding_idx=0)
+        grad, = torch.autograd.grad(y, w, torch.ones_like(y))
+        assert not grad.any()
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_embedding_strides(device):
+    """Rows apart, a transposed matrix, tokens and a gradient that are not contiguous, one that is expanded."""
+    g = gen(5)
+    wide, tokens = torch.randn(20, 40, generator=g), torch.randint(0, 20, (6, 8), generator=g)
+    for cut in (lambda t: t[:, 4:20], lambda t: t[:, 3:20], lambda t: t.t()[:16], lambda t: t[::2]):
+        base = wide.clone().to(device).requires_grad_()
+        w = cut(base)
+        ids = tokens.to(device).t() % w.shape[0]
+        y = ops.embedding(ids, w, 2.0)
+        close(y, 2.0 * cut(wide).double()[ids.cpu()], 0.0, torch.float32)
+        gy = torch.randn(1, 1, w.shape[1], generator=g).to(device).expand(*ids.shape, -1)
+        grad, = torch.autograd.grad(y, base, gy)
+        _, want, size, terms = embedding_64(ids.cpu(), cut(wide), 2.0, gy.cpu())
+        close(cut(grad), want, size * (terms + 1) * U, torch.float32)
+
+
+def test_embedding_gradient_against_differences():
+    w = torch.randn(5, 3, dtype=torch.float64, generator=gen(1)).requires_grad_()
+    tokens = torch.tensor([0, 4, 4, 1, -1])
+    assert torch.autograd.gradcheck(lambda t: ops.embedding(tokens, t, 0.7), (w,))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V,D,dtype", [(20011, 3000, 68, torch.float32), (5000, 1, 24, torch.float32), (9000, 70001, 8, torch.bfloat16),
+                                         (40000, 5, 129, torch.float16)])
+def test_embedding_gradient_of_many_tokens(n, V, D, dtype):
+    """Uneven frequencies, all tokens equal, more tokens of the vocabulary than of the text: the formula, and the same bits twice."""
+    g = gen(n)
+    tokens = ((V + 1.0) ** torch.rand(n, generator=g, dtype=torch.float64) - 1).long().clamp_(0, V - 1)
+    gy = torch.randn(n, D, generator=g).to(dtype)
+    w = torch.zeros(V, D, dtype=dtype, device="cuda").requires_grad_()
+    y = ops.embedding(tokens.cuda(), w)
+    grad, = torch.autograd.grad(y, w, gy.cuda(), retain_graph=True)
+    again, = torch.autograd.grad(y, w, gy.cuda())
+    _, want, size, terms = embedding_64(tokens, w.cpu(), 1.0, gy)
+    close(grad, want, size * terms.clamp_max(2 * math.sqrt(n) + 64) * U, dtype)  # pieces first, then the pieces' sums
+    assert torch.equal(grad, again)
+
+
+# ----------------------------------------------------------------------------- group norm
+def sigmoid(z):
+    return 1 / (1 + torch.exp(-z))
+
+
+def norm_64(x, G, weight, bias, eps, act, gy, depth):
+    """The definition, its gradients, and bounds of what float32 makes of them (depth: additions a term of a group's sum goes through)."""
+    B, C = x.shape[0], x.shape[-1]
+    x, gy = x.double().reshape(B, -1, G, C // G), gy.double().reshape(B, -1, G, C // G)
+    ga = torch.ones(G, C // G, dtype=torch.float64) if weight is None else weight.double().view(G, -1)
+    be = torch.zeros(G, C // G, dtype=torch.float64) if bias is None else bias.double().view(G, -1)
+    mean = lambda t: t.mean((1, 3), keepdim=True)  # noqa: E731
+    m = mean(x)
+    rstd = 1 / torch.sqrt(mean((x - m) ** 2) + eps)
+    hat = (x - m) * rstd
+    z = hat * ga + be
+    s = sigmoid(z)
+    y, slope = {"none": (z, torch.ones_like(z)), "relu": (z.clamp_min(0), (z > 0).double()), "silu": (z * s, s * (1 + z * (1 - s))),
+                "sigmoid": (s, s * (1 - s))}[act]
+    d = depth * U
+    off_m = d * mean(x.abs()) + 2 * U * x.abs()              # the mean, the difference with it
+    off_hat = off_m * rstd + hat.abs() * (2 * d + (d * mean(x.abs()) * rstd) ** 2 + 4 * U)  # ... and 1 / sqrt(var + eps)
+    off_z = off_hat * ga.abs() + 3 * U * ((hat * ga).abs() + be.abs())
+    off_y = 1.1 * off_z + 8 * U * (1 + z.abs()) * y.abs()    # |act'| <= 1.1; an exponential of z is off by (1 + |z|) u
+    g = gy * slope
+    off_g = gy.abs() * (0.5 * off_z + 16 * U * (1 + z.abs()) * (s if act != "none" else 0 * s))  # |act''| <= 1/2
+    gb, gw = g.sum((0, 1)), (g * hat).sum((0, 1))
+    many = (depth + 4 * B) * U
+    off_b = off_g.sum((0, 1)) + many * g.abs().sum((0, 1))
+    off_w = (off_g * hat.abs() + g.abs() * off_hat).sum((0, 1)) + many * (g * hat).abs().sum((0, 1))
+    gh, off_h = g * ga, (off_g + 2 * U * g.abs()) * ga.abs()
+    a, q = mean(gh), mean(gh * hat)
+    off_a = mean(off_h) + d * mean(gh.abs())
+    off_q = mean(off_h * hat.abs() + gh.abs() * off_hat) + d * mean((gh * hat).abs())
+    gx = rstd * (gh - a - hat * q)
+    size = gh.abs() + a.abs() + (hat * q).abs()
+    rel = 2 * d + (d * mean(x.abs()) * rstd) ** 2 + 4 * U    # of rstd
+    off_x = rstd * (off_h + off_a + hat.abs() * off_q + q.abs() * off_hat + size * (rel + 6 * U))
+    flat = lambda t: t.reshape(B, -1, C)  # noqa: E731
+    return [(flat(y), flat(off_y)), (flat(gx), flat(off_x)), (gw.reshape(-1), off_w.reshape(-1)), (gb.reshape(-1), off_b.reshape(-1))]
+
+
+# positions x channels: one value, one position, channels fewer than a vector, groups of odd width, groups across vectors, one group
+# wider than a block's tile, as many groups as channels, many positions, positions and channels that end inside a tile
+NORM = [(1, (1,), 1, 1), (3, (), 24, 4), (2, (5,), 3, 3), (2, (7, 9), 20, 4), (1, (64,), 30, 3), (4, (11,), 8, 2), (2, (3, 5), 36, 12),
+        (2, (2,), 2500, 1), (1, (3,), 5001, 3), (3, (13,), 64, 64), (2, (700,), 16, 2), (1, (50, 60), 40, 8), (5, (19,), 320, 32)]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("B,space,C,G", NORM)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_group_norm(device, B, space, C, G, dtype):
+    g = gen(C + G)
+    x, gy = ((torch.randn(B, *space, C, generator=g) * 0.4 + m).to(dtype) for m in (0.5, 0.0))
+    weight, bias = ((torch.randn(C, generator=g) * 0.2 + m).to(dtype) for m in (1.0, 0.0))
+    for act in ("none", "silu", "sigmoid"):
+        want = norm_64(x, G, weight, bias, 1e-2, act, gy, depth=256)
+        leaves = [t.to(device).requires_grad_() for t in (x, weight, bias)]
+        y = ops.group_norm(leaves[0], G, *leaves[1:], eps=1e-2, activation=act)
+        assert y.shape == x.shape and y.dtype is dtype
+        got = [y, *torch.autograd.grad(y, leaves, gy.to(device))]
+        for t, (exact, bound) in zip(got, want):
+            assert t.dtype is dtype
+            close(t.reshape(exact.shape), exact, bound, dtype)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_group_norm_parameters_of_another_type_or_none(device):
+    g = gen(7)
+    x, gy = torch.randn(3, 10, 24, generator=g).bfloat16(), torch.randn(3, 10, 24, generator=g).bfloat16()
+    weight, bias = torch.randn(24, generator=g), torch.randn(24, generator=g)
+    for w, b in ((weight, bias), (weight, None), (None, bias), (None, None)):
+        want = norm_64(x, 3, w, b, 1e-5, "sigmoid", gy, depth=256)
+        leaves = [t.to(device).requires_grad_() for t in (x, w, b) if t is not None]
+        it = iter(leaves[1:])
+        y = ops.group_norm(leaves[0], 3, next(it) if w is not None else None, next(it) if b is not None else None, activation="sigmoid")
+        close(y, *want[0], torch.bfloat16)
+        got = torch.autograd.grad(y, leaves, gy.to(device))
+        close(got[0], *want[1], torch.bfloat16)
+        for t, pair in zip(got[1:], [want[2 + i] for i, p in enumerate((w, b)) if p is not None]):
+            assert t.dtype is torch.float32
+            close(t, *pair, torch.float32)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_group_norm_relu_and_constant_groups(device):
+    """A group of equal values has no variance: xhat is 0 and the output the bias; relu's gradient stops below 0."""
+    x = torch.tensor([[[2.0, 2.0, 1.0, 3.0]], [[-5.0, -5.0, 4.0, 0.0]]])
+    leaf = x.to(device).requires_grad_()
+    bias = torch.tensor([0.5, -0.5, 0.0, 0.0], device=device)
+    y = ops.group_norm(leaf, 2, None, bias, eps=1e-5, activation="relu")
+    want = torch.tensor([[[0.5, 0.0, 0.0, 1.0]], [[0.5, 0.0, 1.0, 0.0]]])
+    close(y, want, 1e-5, torch.float32)  # eps: 1 / sqrt(1 + 1e-5), 1 / sqrt(4 + 1e-5) of a difference of 2
+    gx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    scale = 1 / math.sqrt(1e-5)
+    close(gx[0, 0, :2], torch.tensor([0.5, -0.5]) * scale, scale * 8 * U, torch.float32)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_group_norm_far_from_zero(device):
+    """Values around 1000 with a spread of 1: E[x^2] - mean^2 would have lost the variance."""
+    x = (torch.randn(2, 900, 8, generator=gen(9)) + 1000.0)
+    y = ops.group_norm(x.to(device), 2)
+    wide = x.double().view(2, -1, 2, 4)
+    want = ((wide - wide.mean((1, 3), keepdim=True)) / torch.sqrt(wide.var((1, 3), unbiased=False, keepdim=True) + 1e-5)).view(x.shape)
+    # the mean is a float32 near 1000: off by its own rounding and the sum's, (1 + depth) u 1000
+    close(y, want, 1000 * 64 * U, torch.float32)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_group_norm_leaves_other_samples_alone_when_one_is_not_finite(device):
+    x = torch.randn(3, 6, 8, generator=gen(2))
+    x[1, 2, 3] = float("nan")
+    y = ops.group_norm(x.to(device), 2).cpu()
+    assert y[1, :, :4].isnan().all() and not y[1, :, 4:].isnan().any() and not y[0].isnan().any() and not y[2].isnan().any()
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_group_norm_module_on_images(device):
+    from difflut_amd.utils import GroupNorm
+
+    torch.manual_seed(0)
+    x = torch.randn(2, 12, 5, 7)
+    norm = GroupNorm(3, 12, activation="sigmoid").to(device)
+    with torch.no_grad():
+        norm.weight.normal_(), norm.bias.normal_()
+    want = norm_64(x.movedim(1, -1), 3, norm.weight.cpu(), norm.bias.cpu(), 1e-5, "sigmoid", x.movedim(1, -1), depth=256)[0]
+    for layout in (torch.contiguous_format, torch.channels_last):
+        y = norm(x.to(device).contiguous(memory_format=layout))
+        assert y.shape == x.shape and y.is_contiguous(memory_format=torch.channels_last)
+        close(y.movedim(1, -1).reshape(2, -1, 12), *want, torch.float32)
+    flat = norm(x[:, :, 0, 0].to(device))
+    assert flat.shape == (2, 12)
+    with pytest.raises(ValueError):
+        norm(x[:, :5].to(device))
+
+
+def test_group_norm_gradient_against_differences():
+    g = gen(4)
+    x, w, b = (torch.randn(s, dtype=torch.float64, generator=g).requires_grad_() for s in ((2, 5, 6), (6,), (6,)))
+    for act in ("none", "silu", "sigmoid"):
+        assert torch.autograd.gradcheck(lambda *t: ops.group_norm(t[0], 2, *t[1:], activation=act), (x, w, b))
+
+
+# ----------------------------------------------------------------------------- dropout
+def philox(seed, offset, numel):
+    """By numpy's 64-bit products, from the generator's definition."""
+    counter = np.arange(-(-numel // 4), dtype=np.uint64)
+    low, s32 = np.uint64(0xFFFFFFFF), np.uint64(32)
+    c = [counter & low, counter >> s32, np.full_like(counter, offset & 0xFFFFFFFF), np.full_like(counter, offset >> 32)]
+    key = [seed & 0xFFFFFFFF, seed >> 32]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> s32) ^ c[1] ^ np.uint64(key[0]), b & low, (a >> s32) ^ c[3] ^ np.uint64(key[1]), a & low]
+        key = [(key[0] + 0x9E3779B9) % 2 ** 32, (key[1] + 0xBB67AE85) % 2 ** 32]
+    return np.stack(c, axis=1).reshape(-1)[:numel]
+
+
+def test_philox_known_answers():
+    """The generator's published test vectors (counter and key all zeros; all ones)."""
+    from difflut_amd.cpu_ops import philox_words
+
+    assert [f"{w:08x}" for w in philox(0, 0, 4)] == ["6627e8d5", "e169c58d", "bc57ac4c", "9b00dbd8"]
+    for seed, offset in ((0, 0), (1, 2), (2 ** 64 - 1, 2 ** 64 - 1), (0x0123456789ABCDEF, 0xFEDCBA9876543210)):
+        assert philox_words(ops._signed64(seed), ops._signed64(offset), 1001).tolist() == philox(seed, offset, 1001).tolist()
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("shape", [(1,), (3, 5), (64, 100), (7, 1025), (0, 4)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("p", [0.0, 0.25, 1 / 3, 0.999, 1.0])
+def test_dropout(device, shape, dtype, p):
+    seed, offset = 2 ** 63 + 12345, 2 ** 40 + 7
+    g = gen(11)
+    x, gy = (torch.randn(shape, generator=g).to(dtype) for _ in range(2))
+    hit = torch.from_numpy(philox(seed, offset, x.numel()) < math.floor(p * 2.0 ** 32 + 0.5)).view(shape)
+    if p in (0.0, 1.0):
+        assert hit.all() == (p == 1.0) or not hit.numel()
+    factor = 0.0 if p == 1.0 else 1 / (1 - p)
+    for state in ((seed, offset), torch.tensor([ops._signed64(seed), offset], device=device)):
+        leaf = x.to(device).requires_grad_()
+        y = ops.dropout(leaf, p, state)
+        gx, = torch.autograd.grad(y, leaf, gy.to(device))
+        for got, of in ((y, x), (gx, gy)):
+            assert got.dtype is dtype
+            want = torch.where(hit, 0.0, of.double() * factor)
+            close(got, want, want.abs() * 2 * U, dtype)  # the factor and the product
+            assert not got.detach().cpu()[hit].any()
+        y = ops.dropout(leaf, p, state, mode="flip")
+        gx, = torch.autograd.grad(y, leaf, gy.to(device))
+        assert torch.equal(y.detach().cpu(), torch.where(hit, 1 - x.float(), x.float()).to(dtype)) and torch.equal(gx.cpu(), gy)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_dropout_of_views_and_values_that_are_not_finite(device):
+    """The mask goes by the row-major order whatever the strides and the alignment; what is hit is gone whatever it was."""
+    base = torch.randn(40, 30, generator=gen(3))
+    for view in (lambda t: t.t(), lambda t: t[:, 3:], lambda t: t.reshape(-1)[1:], lambda t: t[::3, ::2]):
+        x = view(base.to(device))
+        hit = torch.from_numpy(philox(5, 6, x.numel()) < 2 ** 31).view(x.shape)
+        assert torch.equal(ops.dropout(x, 0.5, (5, 6)).cpu(), torch.where(hit, 0.0, view(base) * 2))
+    for bad in (math.inf, -math.inf, math.nan):
+        y = ops.dropout(torch.full((64,), bad, device=device), 0.5, (1, 1)).cpu()
+        hit = torch.from_numpy(philox(1, 1, 64) < 2 ** 31)
+        assert not y[hit].any() and not y[~hit].isfinite().any()
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_dropout_module(device):
+    from difflut_amd.utils import Dropout
+
+    x = torch.ones(50, 40, device=device)
+    drop = Dropout(0.25, seed=9).to(device)
+    first, second = drop(x), drop(x)
+    assert not torch.equal(first, second) and drop.state.tolist() == [9, 2]
+    other = Dropout(0.25).to(device)
+    other.load_state_dict({"state": torch.tensor([9, 1])})
+    assert torch.equal(other(x), second)  # a resumed run goes on with the same masks
+    # the backward draws the mask of its forward, also after further calls
+    leaf = x.clone().requires_grad_()
+    y = drop(leaf)
+    drop(x)
+    gx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    assert torch.equal(gx, y.detach())
+    assert drop.eval()(x) is x
+
+
+def test_dropout_gradient_against_differences():
+    x = torch.randn(4, 9, dtype=torch.float64, generator=gen(8)).requires_grad_()
+    assert torch.autograd.gradcheck(lambda t: ops.dropout(t, 0.4, (3, 1)), (x,))
+
+
+# ----------------------------------------------------------------------------- sampling
+def sample_64(logits, uniform, T, k, p, m):
+    """Row by row from the definition, in float64 (settings: float32 values, a list per row)."""
+    out = []
+    for row, u, t, kk, pp, mm in zip(logits.double().numpy(), uniform.double().numpy(), T, k, p, m):
+        row = np.where(np.isnan(row), -np.inf, row)
+        order = [i for i in sorted(range(len(row)), key=lambda i: (-row[i], i)) if row[i] > -np.inf]
+        if not order:
+            out.append(-1)
+            continue
+        top = row[order[0]]
+        if not t > 0:
+            out.append(order[0])
+            continue
+        w = {i: 1.0 if row[i] == top else (0.0 if top == np.inf else math.exp((row[i] - top) / t)) for i in order}
+        if 0 < kk < len(order):
+            order = order[:kk]
+        total, run, kept = math.fsum(w[i] for i in order), 0.0, []
+        for i in order:
+            if kept and pp < 1 and not run < pp * total:
+                break
+            kept.append(i)
+            run += w[i]
+        kept = sorted(i for n, i in enumerate(kept) if n == 0 or w[i] >= mm)
+        total, run, token = math.fsum(w[i] for i in kept), 0.0, kept[-1]
+        for i in kept:
+            run += w[i]
+            if run > u * total:
+                token = i
+                break
+        out.append(token)
+    return torch.tensor(out)
+
+
+def f32(v):
+    return float(np.float32(v))
+
+
+def check_sample(device, logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    B = len(logits)
+    rows = [v.float().tolist() if torch.is_tensor(v) else [f32(v)] * B for v in (temperature, top_k, top_p, min_p)]
+    want = sample_64(logits, uniform, rows[0], [int(v) for v in rows[1]], *rows[2:])
+    args = [v.to(device) if torch.is_tensor(v) else v for v in (temperature, top_k, top_p, min_p)]
+    got = ops.sample(logits.to(device), uniform.to(device), *args)
+    assert got.dtype is torch.int64 and got.cpu().tolist() == want.tolist()
+
+
+# columns: one, a few lanes per row, a sorted row (power of two, odd), split rows with one chunk and several
+COLUMNS = [1, 2, 10, 33, 64, 65, 128, 1000, 1025, 4096, 4097, 9001]
+FILTERS = [dict(), dict(temperature=0.0), dict(top_k=1), dict(top_k=7), dict(top_p=0.5), dict(top_p=0.95, min_p=0.05),
+           dict(temperature=0.7, top_k=50, top_p=0.9), dict(temperature=3.0, top_k=3000, top_p=0.999, min_p=0.001)]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V", COLUMNS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample(device, V, dtype):
+    g = gen(V)
+    B = 5 if V > 2000 else 13
+    logits, uniform = (torch.randn(B, V, generator=g) * 3).to(dtype), torch.rand(B, generator=g)
+    for settings in FILTERS:
+        check_sample(device, logits, uniform, **settings)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V", [12, 700, 6000])
+def test_sample_settings_per_row(device, V):
+    g = gen(V + 1)
+    B = 24
+    r = torch.rand(4, B, generator=g)
+    T, k, p, m = r[0] * 2, (r[1] * 2 * V).int(), 0.3 + r[2], r[3] * 0.2
+    T[3], k[4], p[5], m[6] = 0.0, 1, 1.0, 0.0
+    check_sample(device, torch.randn(B, V, generator=g) * 2, torch.rand(B, generator=g), T, k.long(), p, m)
+    check_sample(device, torch.randn(B, V, generator=g) * 2, torch.rand(B, generator=g), T, 5, p, 0.01)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V", [10, 64, 300, 5000, 20000])
+def test_sample_equal_logits(device, V):
+    """Sums of bits, as GroupSum's are, have many equal values: the cuts fall among those, by index."""
+    g = gen(V + 2)
+    B = 6
+    uniform = torch.rand(B, generator=g)
+    for levels in (1, 2, 7):
+        logits = torch.randint(0, levels, (B, V), generator=g).float()
+        for settings in (dict(), dict(top_k=3), dict(top_k=max(1, V // 3)), dict(top_p=0.3), dict(top_k=max(1, V // 2), top_p=0.7),
+                         dict(top_k=max(1, V - 1), top_p=0.9, temperature=0.25)):
+            check_sample(device, logits, uniform, **settings)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V", [9, 200, 4500])
+def test_sample_masked_rows(device, V):
+    """Masks of -infinity and of the type's lowest value, rows with one or nothing left, NaN and +infinity."""
+    g = gen(V + 3)
+    logits = torch.randn(9, V, generator=g)
+    logits[0] = -math.inf
+    logits[1, 1:] = -math.inf
+    logits[2, :-1] = torch.finfo(torch.float32).min
+    logits[3, ::2] = -math.inf
+    logits[4] = torch.finfo(torch.float32).min
+    logits[5, 3] = math.nan
+    logits[6] = math.nan
+    logits[7, 2] = logits[7, 5] = math.inf
+    logits[8, 0], logits[8, 1] = 0.0, -0.0
+    for u in (0.0, 0.3, 0.999999):
+        for settings in FILTERS:
+            check_sample(device, logits, torch.full((9,), u), **settings)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_sample_strides_and_empty(device):
+    g = gen(6)
+    wide, uniform = torch.randn(8, 6000, generator=g), torch.rand(8, generator=g)
+    for view in (lambda t: t[:, 1:50], lambda t: t[:, 3:], lambda t: t[:, ::2], lambda t: t.t()[:8, :8], lambda t: t[:1].expand(8, -1)):
+        logits = view(wide.to(device))
+        got = ops.sample(logits, uniform.to(device), top_k=20, top_p=0.8)
+        assert got.cpu().tolist() == sample_64(view(wide), uniform, [1.0] * 8, [20] * 8, [f32(0.8)] * 8, [0.0] * 8).tolist()
+    assert ops.sample(wide[:0].to(device), uniform[:0].to(device)).shape == (0,)
+
+
+def test_sample_frequencies():
+    """What is drawn for evenly spaced numbers has the softmax's frequencies to one part in their count."""
+    logits = torch.tensor([0.0, 1.0, 2.0, -1.0])
+    n = 4096
+    tokens = ops.sample(logits.expand(n, -1), torch.arange(n) / n)
+    assert (torch.bincount(tokens, minlength=4) / n - torch.softmax(logits, 0)).abs().max() <= 1 / n
+
+
+# ----------------------------------------------------------------------------- refusals
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_refusals(device):
+    w, t = torch.zeros(4, 3, device=device), torch.zeros(2, dtype=torch.long, device=device)
+    x = torch.zeros(2, 5, 6, device=device)
+    u = torch.zeros(2, device=device)
+    logits = torch.zeros(2, 5, device=device)
+    for error, call in [
+            (ValueError, lambda: ops.embedding(t, w[0])), (ValueError, lambda: ops.embedding(t, w[:0])),
+            (TypeError, lambda: ops.embedding(t.float(), w)), (TypeError, lambda: ops.embedding(t.short(), w)),
+            (ValueError, lambda: ops.embedding(t, w, padding_idx=4)), (ValueError, lambda: ops.embedding(t, w, padding_idx=-1)),
+            (TypeError, lambda: ops.embedding(t, w.int())),
+            (ValueError, lambda: ops.group_norm(x, 4)), (ValueError, lambda: ops.group_norm(x, 0)), (ValueError, lambda: ops.group_norm(x, 2.0)),
+            (ValueError, lambda: ops.group_norm(x[:0], 2)), (ValueError, lambda: ops.group_norm(x[0, 0], 2)),
+            (ValueError, lambda: ops.group_norm(x, 2, activation="tanh")), (ValueError, lambda: ops.group_norm(x, 2, eps=-1.0)),
+            (ValueError, lambda: ops.group_norm(x, 2, w[0])), (ValueError, lambda: ops.group_norm(x, 2, None, w[0])),
+            (TypeError, lambda: ops.group_norm(x.int(), 2)),
+            (TypeError, lambda: ops.group_norm(x, 2, torch.ones(6, device=device), torch.ones(6, device=device).half())),
+            (ValueError, lambda: ops.dropout(x, -0.1, (0, 0))), (ValueError, lambda: ops.dropout(x, 1.1, (0, 0))),
+            (ValueError, lambda: ops.dropout(x, math.nan, (0, 0))), (ValueError, lambda: ops.dropout(x, 0.1, (0, 0), mode="noise")),
+            (TypeError, lambda: ops.dropout(x, 0.1, t.int())), (TypeError, lambda: ops.dropout(x, 0.1, torch.zeros(3, dtype=torch.long, device=device))),
+            (TypeError, lambda: ops.dropout(x.int(), 0.1, (0, 0))),
+            (ValueError, lambda: ops.sample(logits[0], u)), (ValueError, lambda: ops.sample(logits[:, :0], u)),
+            (ValueError, lambda: ops.sample(logits, u[:1])), (ValueError, lambda: ops.sample(logits, t)),
+            (ValueError, lambda: ops.sample(logits, u, temperature=-1.0)), (ValueError, lambda: ops.sample(logits, u, temperature=math.nan)),
+            (ValueError, lambda: ops.sample(logits, u, top_k=-1)), (ValueError, lambda: ops.sample(logits, u, top_k=1.5)),
+            (ValueError, lambda: ops.sample(logits, u, top_p=0.0)), (ValueError, lambda: ops.sample(logits, u, top_p=1.5)),
+            (ValueError, lambda: ops.sample(logits, u, min_p=1.5)), (ValueError, lambda: ops.sample(logits, u, top_p=u[:1]))]:
+        with pytest.raises(error):
+            call()
+
+
+def test_module_refusals():
+    from difflut_amd.utils import Dropout, GroupNorm, TokenEmbedding
+
+    for call in (lambda: TokenEmbedding(0, 4), lambda: TokenEmbedding(4, 0), lambda: TokenEmbedding(4, 4, padding_idx=4),
+                 lambda: GroupNorm(3, 8), lambda: GroupNorm(0, 8), lambda: GroupNorm(2, 8, activation="gelu"),
+                 lambda: Dropout(1.5), lambda: Dropout(0.5, mode="bits")):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.gpu
+def test_refusals_of_mixed_devices_float64_and_second_derivatives():
+    w, t = torch.zeros(4, 3, device="cuda"), torch.zeros(2, dtype=torch.long)
+    x = torch.randn(2, 5, 6, device="cuda")
+    for call in (lambda: ops.embedding(t, w), lambda: ops.group_norm(x, 2, torch.ones(6)), lambda: ops.dropout(x, 0.5, t),
+                 lambda: ops.sample(x[0], torch.zeros(5)), lambda: ops.sample(x[0], x[0, :, 0].abs(), top_p=torch.ones(5))):
+        with pytest.raises(RuntimeError):
+            call()
+    for call in (lambda: ops.embedding(t.cuda(), w.double()), lambda: ops.group_norm(x.double(), 2), lambda: ops.dropout(x.double(), 0.5, (0, 0)),
+                 lambda: ops.sample(x[0].double(), x[0, :, 0].abs())):
+        with pytest.raises(TypeError):
+            call()
+    for call, leaf in ((lambda v: ops.embedding(t.cuda(), v), w), (lambda v: ops.group_norm(v, 2), x)):
+        leaf = leaf.clone().requires_grad_()
+        y = call(leaf)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(y, leaf, torch.ones_like(y), create_graph=True)
+    leaf = x.clone().requires_grad_()  # dropout is linear: its gradient has one of its own
+    gy = torch.ones_like(x).requires_grad_()
+    gx, = torch.autograd.grad(ops.dropout(leaf, 0.5, (1, 2)), leaf, gy, create_graph=True)
+    gg, = torch.autograd.grad(gx, gy, torch.ones_like(gx))
+    assert torch.equal(gg, gx.detach())
+
+
+# ----------------------------------------------------------------------------- streams, graphs, a model
+@pytest.mark.gpu
+def test_on_another_stream():
+    g = gen(12)
+    w, t = torch.randn(50, 20, generator=g), torch.randint(0, 50, (300,), generator=g)
+    x, logits, uniform = torch.randn(4, 200, 16, generator=g), torch.randn(3, 7000, generator=g), torch.rand(3, generator=g)
+
+    def everything():
+        leaf, xl = w.cuda().requires_grad_(), x.cuda().requires_grad_()
+        y = ops.embedding(t.cuda(), leaf, 3.0)
+        z = ops.dropout(ops.group_norm(xl, 4, activation="silu"), 0.2, (1, 2))
+        return [y, *torch.autograd.grad(y, leaf, y.detach()), z, *torch.autograd.grad(z, xl, z.detach()),
+                ops.sample(logits.cuda(), uniform.cuda(), 0.9, 100, 0.9)]
+
+    want = everything()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = everything()
+    stream.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed():
+    """Every operator, forward and backward, in a graph: replays with new inputs against eager calls, eager work between them; the
+    dropout module draws a new mask on every replay."""
+    from difflut_amd.utils import Dropout
+
+    g = gen(13)
+    w, x = torch.randn(900, 64, generator=g).cuda().requires_grad_(), torch.randn(6, 300, 64, generator=g).cuda().requires_grad_()
+    gamma, beta = torch.randn(64, generator=g).cuda().requires_grad_(), torch.randn(64, generator=g).cuda().requires_grad_()
+    tokens, gy = torch.zeros(6, 300, dtype=torch.long, device="cuda"), torch.zeros(6, 300, 64, device="cuda")
+    logits, uniform = torch.zeros(5, 9000, device="cuda"), torch.zeros(5, device="cuda")
+    few = torch.zeros(5, 300, device="cuda")
+    drop = Dropout(0.3, seed=4).cuda()
+
+    def step():
+        y = ops.embedding(tokens, w, 2.0)
+        gw, = torch.autograd.grad(y, w, gy)
+        z = ops.group_norm(x, 8, gamma, beta, activation="sigmoid")
+        grads = torch.autograd.grad(z, [x, gamma, beta], gy)
+        d = drop(x)
+        gd, = torch.autograd.grad(d, x, gy)
+        return [y, gw, z, *grads, d, gd, ops.sample(logits, uniform, 0.8, 300, 0.9, 0.001), ops.sample(few, uniform, 1.0, 0, 0.8)]
+
+    def fill(seed):
+        s = torch.Generator(device="cuda").manual_seed(seed)
+        with torch.no_grad():
+            tokens.copy_((torch.rand(6, 300, generator=s, device="cuda") ** 4 * 900).long())
+            gy.normal_(generator=s), logits.normal_(0, 2, generator=s), uniform.uniform_(generator=s), few.normal_(generator=s)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    masks = set()
+    for replay in range(4):
+        fill(replay)
+        before = drop.state.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        assert drop.state.tolist() == [4, int(before[1]) + 1]
+        drop.state.copy_(before)
+        want = step()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), replay
+        masks.add(int((got[6] == 0).long().mul(torch.arange(got[6].numel(), device="cuda").view(got[6].shape) % 997).sum()))
+    assert len(masks) == 4
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_token_model_trains_and_answers(device):
+    """Tokens -> embedding -> group norm with a sigmoid -> bit flips -> LUT layers -> GroupSum -> cross-entropy, every parameter's
+    gradient; then one token at a time with sampling."""
+    from difflut_amd.layers import RandomLayer
+    from difflut_amd.nodes import NodeConfig, ProbabilisticNode
+    from difflut_amd.nodes.utils import uniform_init
+    from difflut_amd.utils import BankAdam, Dropout, GroupNorm, GroupSum, TokenEmbedding, cross_entropy, sample
+
+    torch.manual_seed(5)
+    V, D, T = 30, 24, 4
+    node = NodeConfig(input_dim=4, output_dim=1, init_fn=uniform_init, init_kwargs={"a": -1.0, "b": 1.0})
+    embed, norm = TokenEmbedding(V, D, scale=math.sqrt(D)).to(device), GroupNorm(4, D, activation="sigmoid").to(device)
+    drop = Dropout(0.1, mode="flip", seed=1).to(device)
+    layer = RandomLayer(T * D, 10 * V, ProbabilisticNode, node, seed=3).to(device)
+    head = GroupSum(V, tau=2.0, use_randperm=False)
+    parts = [embed, norm, drop, layer]
+
+    def logits_of(tokens):
+        h = norm(embed(tokens).movedim(-1, 1)).movedim(1, -1)
+        assert h.shape == (*tokens.shape, D) and bool(((h > 0) & (h < 1)).all())
+        return head(layer(drop(h.flatten(1))))
+
+    tokens, targets = torch.randint(0, V, (16, T), device=device), torch.randint(0, V, (16,), device=device)
+    leaves = [embed.weight, norm.weight, norm.bias, *layer.bank_parameters()]
+    optimizer = BankAdam(leaves, lr=1e-2)
+    for _ in range(2):
+        loss = cross_entropy(logits_of(tokens), targets)
+        optimizer.zero_grad()
+        loss.backward()
+        for p in leaves:
+            assert p.grad is not None and p.grad.isfinite().all() and p.grad.any()
+        optimizer.step()
+    assert drop.state.tolist() == [1, 2]
+    for m in parts:
+        m.eval()
+    g = gen(1)
+    with torch.no_grad():
+        for _ in range(5):
+            nxt = sample(logits_of(tokens[:, -T:]), torch.rand(16, generator=g).to(device), temperature=0.8, top_k=10, top_p=0.9)
+            assert nxt.shape == (16,) and bool(((nxt >= 0) & (nxt < V)).all())
+            tokens = torch.cat([tokens, nxt.unsqueeze(1)], dim=1)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_convolution_with_norm_and_flips(device):
+    """ConvolutionalLayer -> GroupNorm with a sigmoid -> bit flips -> a second layer: the norm takes the layer's memory as it is."""
+    from difflut_amd.layers import ConvolutionalLayer, ConvolutionConfig, RandomLayer
+    from difflut_amd.nodes import DWNNode, NodeConfig
+    from difflut_amd.nodes.utils import uniform_init
+    from difflut_amd.utils import Dropout, GroupNorm
+
+    torch.manual_seed(6)
+    node = NodeConfig(input_dim=3, output_dim=1, init_fn=uniform_init, init_kwargs={"a": -1.0, "b": 1.0})
+    conv = ConvolutionalLayer(ConvolutionConfig(tree_depth=1, in_channels=2, out_channels=8, receptive_field=3, seed=1), DWNNode, node,
+                              RandomLayer, n_inputs_per_node=3).to(device)
+    norm, drop = GroupNorm(2, 8, activation="sigmoid").to(device), Dropout(0.05, mode="flip").to(device)
+    layer = RandomLayer(8 * 16, 20, DWNNode, node, seed=2).to(device)
+    x = torch.rand(4, 2, 6, 6, device=device).requires_grad_()
+    h = conv(x)
+    assert h.movedim(1, -1).is_contiguous()
+    y = layer(drop(norm(h)).flatten(1))
+    y.sum().backward()
+    assert x.grad.isfinite().all() and norm.weight.grad.any() and norm.bias.grad.any()
