@@ -24,6 +24,20 @@ __device__ __forceinline__ void dl_store(T *p, const float (&f)[N]) {
     *reinterpret_cast<DlVec<T, N> *>(p) = t;
 }
 
+// The same past the caches' retention: for results that a launch does not read again and that would push out what it does
+template <typename T, int N>
+__device__ __forceinline__ void dl_store_past(T *p, const float (&f)[N]) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    if constexpr (sizeof(T) * N == 16) {
+        DlVec<T, N> t;
+#pragma unroll
+        for (int i = 0; i < N; ++i) t.v[i] = (T)f[i];
+        __builtin_nontemporal_store(__builtin_bit_cast(words, t), reinterpret_cast<words *>(p));
+    } else {
+        dl_store(p, f);
+    }
+}
+
 static inline bool dl_type_known(int type) { return type == DL_F32 || type == DL_BF16 || type == DL_F16; }
 static inline int dl_type_bytes(int type) { return type == DL_F32 ? 4 : 2; }
 static inline bool dl_aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }

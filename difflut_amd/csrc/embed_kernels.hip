@@ -8,7 +8,7 @@
 //   embed_sort   positions sorted by token, ascending within one.  Block b owns the tokens v with v mod blocks = b and reads
 //                the whole token list (it stays in the L2): how many tokens belong to lower blocks is where its own begin.  Owning
 //                every blocks-th token spreads the frequent ones, which lie together at the low ids of a vocabulary.
-//   embed_sum    teams of threads walk pieces of EMB_PIECE sorted positions - equal work however uneven the frequencies - and write
+//   embed_sum    teams of threads walk pieces of 16 or 32 sorted positions - equal work however uneven the frequencies - and write
 //                a token's sum where all of its positions lie in the piece, else a partial; the rest of the grid writes the rows of
 //                tokens that do not occur.
 //   embed_join   adds the partials of tokens that reach over pieces, in order.
@@ -18,7 +18,11 @@
 #define EMB_SORT_THREADS 1024
 #define EMB_SORT_WAVES (EMB_SORT_THREADS / 64)
 #define EMB_MAX_OWNED 512  // tokens that a block of the sort owns at most (a thread each; 32 KB of counts)
-#define EMB_PIECE 16
+#define EMB_AHEAD 8         // groups of 64 tokens that a wavefront of the sort has in flight
+#define EMB_FOUND 480       // tokens of its own that a wavefront remembers, as 23 bits of position and 9 bits of place (EMB_MAX_OWNED)
+#define EMB_ROWS(E) ((E) == 8 ? 8 : 16)  // rows that a team of the sums has in flight (more registers leave too few wavefronts)
+#define EMB_JOIN_THREADS 512
+#define EMB_JOIN_WAVES (EMB_JOIN_THREADS / 64)
 
 // ---------------------------------------------------------------------------------- lookup
 // A team of `lanes` threads per row (a power of two), R rows of a team in flight at once.
@@ -50,62 +54,65 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_lookup(const TOKEN *__restr
             if (t >= n) continue;
 #pragma unroll
             for (int e = 0; e < E; ++e) f[r][e] *= scale;
-            dl_store(y + t * D + c, f[r]);
+            dl_store_past(y + t * D + c, f[r]);
         }
     }
 }
 
 // ---------------------------------------------------------------------------------- sort
-// The block and the place in it of a token; -1: not summed.
+// A token as 32 bits; ~0: not summed (V < 2^31).
 template <typename TOKEN>
-__device__ __forceinline__ int emb_token(const TOKEN *__restrict__ tokens, int t, int n, long long V, long long padding) {
-    if (t >= n) return -1;
-    const long long v = (long long)tokens[t];
-    return v >= 0 && v < V && v != padding ? (int)v : -1;
+__device__ __forceinline__ unsigned emb_token(TOKEN t, unsigned V, unsigned padding) {
+    const unsigned v = (unsigned)t;
+    const bool known = v < V && v != padding && (sizeof(TOKEN) == 4 || (unsigned)((unsigned long long)t >> 32) == 0u);
+    return known ? v : ~0u;
 }
 
 template <typename TOKEN>
-__global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__restrict__ tokens, int n, long long V, long long padding,
+__global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__restrict__ tokens, int n, unsigned V, unsigned padding,
                                                                 int block_bits, int *__restrict__ order, int *__restrict__ token_of,
-                                                                int *__restrict__ count, int *__restrict__ total) {
+                                                                int *__restrict__ begin_of, int *__restrict__ count, int *__restrict__ total) {
     extern __shared__ int place[];  // [waves][owned]: counts, then where the wave's next position of a token goes
+    __shared__ unsigned found[EMB_SORT_WAVES][EMB_FOUND];  // a wave's own tokens, in order
     __shared__ int below_of[EMB_SORT_WAVES], scan[EMB_SORT_WAVES];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, b = blockIdx.x, mask = (1 << block_bits) - 1;
-    const int owned = (int)((V - b + mask) >> block_bits);  // tokens b, b + blocks, ...
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned b = blockIdx.x, mask = (1u << block_bits) - 1;
+    const int owned = (int)((V - b + mask) >> block_bits);  // tokens b, b + blocks, ...  (b <= mask: no wrap below -mask)
     for (int i = threadIdx.x; i < EMB_SORT_WAVES * owned; i += EMB_SORT_THREADS) place[i] = 0;
     __syncthreads();
-    // a wave takes a run of whole groups of 64 positions
+    // a wave takes a run of whole groups of 64 positions, EMB_AHEAD of them in flight
     const int groups = (n + 63) >> 6, per_wave = (groups + EMB_SORT_WAVES - 1) / EMB_SORT_WAVES;
     const int g0 = min(wave * per_wave, groups), g1 = min(g0 + per_wave, groups);
     int below = 0, mine = 0;
-#pragma unroll 4
-    for (int g = g0; g < g1; ++g) {
-        const int v = emb_token(tokens, g * 64 + lane, n, V, padding);
-        if (v < 0) continue;
-        const int owner = v & mask;
-        below += owner < b;
-        if (owner == b) {
-            atomicAdd(&place[wave * owned + (v >> block_bits)], 1);
-            ++mine;
-        }
-    }
+    for (int g = g0; g < g1; g += EMB_AHEAD) {
+        TOKEN t[EMB_AHEAD];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        below += __shfl_xor(below, o);
-        mine += __shfl_xor(mine, o);
+        for (int u = 0; u < EMB_AHEAD; ++u) t[u] = g + u < g1 && (g + u) * 64 + lane < n ? tokens[(g + u) * 64 + lane] : (TOKEN)-1;
+#pragma unroll
+        for (int u = 0; u < EMB_AHEAD; ++u) {
+            const unsigned v = emb_token(t[u], V, padding), owner = v & mask;
+            const bool known = v != ~0u, here = known && owner == b;
+            below += __popcll(__ballot(known && owner < b));
+            const unsigned long long takes = __ballot(here);
+            if (takes == 0) continue;
+            if (here) {
+                atomicAdd(&place[wave * owned + (v >> block_bits)], 1);
+                const int at = mine + __popcll(takes & ((1ull << lane) - 1));
+                if (at < EMB_FOUND) found[wave][at] = (unsigned)((g + u - g0) * 64 + lane) << 9 | v >> block_bits;
+            }
+            mine += __popcll(takes);
+        }
     }
     if (lane == 0) below_of[wave] = below;
     __syncthreads();
     // per token, where each wave's positions begin (a thread per token: owned <= EMB_MAX_OWNED)
     int tokens_here = 0;
-    if ((int)threadIdx.x < owned) {
+    if ((int)threadIdx.x < owned)
         for (int w = 0; w < EMB_SORT_WAVES; ++w) {
             const int c = place[w * owned + threadIdx.x];
             place[w * owned + threadIdx.x] = tokens_here;
             tokens_here += c;
         }
-        count[b + ((long long)threadIdx.x << block_bits)] = tokens_here;
-    }
     int before = tokens_here;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -121,18 +128,19 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
         all += scan[w];
     }
     before += base - tokens_here;
-    if ((int)threadIdx.x < owned)
+    if ((int)threadIdx.x < owned) {
         for (int w = 0; w < EMB_SORT_WAVES; ++w) place[w * owned + threadIdx.x] += before;
+        const unsigned v = b + (threadIdx.x << block_bits);
+        count[v] = tokens_here;
+        begin_of[v] = before;
+    }
     if (b == mask && threadIdx.x == 0) *total = base + all;
     __syncthreads();
-    if (mine == 0) return;
     // the positions themselves, in order: lanes of one token are ranked among themselves (volatile: a wavefront's lanes see each other's
     // stores, which are in order)
     volatile int *next = place;
-    for (int g = g0; g < g1; ++g) {
-        const int t = g * 64 + lane, v = emb_token(tokens, t, n, V, padding);
-        const bool here = v >= 0 && (v & mask) == b;
-        const int slot = here ? wave * owned + (v >> block_bits) : -1;
+    const auto put = [&](bool here, int t, unsigned v) {
+        const int slot = here ? wave * owned + (int)(v >> block_bits) : -1;
         unsigned long long left = __ballot(here);
         while (left) {
             const int leader = __builtin_ctzll(left), its = __builtin_amdgcn_readlane(slot, leader);
@@ -141,20 +149,37 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
             if (slot == its) {
                 const int at = first + __popcll(same & ((1ull << lane) - 1));
                 order[at] = t;
-                token_of[at] = v;
+                token_of[at] = (int)v;
             }
             if (lane == leader) next[its] = first + __popcll(same);
             left &= ~same;
+        }
+    };
+    if (mine <= EMB_FOUND && per_wave <= 1 << 17) {
+        for (int i = 0; i < mine; i += 64) {
+            const unsigned f = i + lane < mine ? found[wave][i + lane] : 0;
+            put(i + lane < mine, g0 * 64 + (int)(f >> 9), (f & 511) << block_bits | b);
+        }
+    } else {  // a frequent token: the list was too short, the tokens are read again
+        for (int g = g0; g < g1; g += EMB_AHEAD) {
+            TOKEN t[EMB_AHEAD];
+#pragma unroll
+            for (int u = 0; u < EMB_AHEAD; ++u) t[u] = g + u < g1 && (g + u) * 64 + lane < n ? tokens[(g + u) * 64 + lane] : (TOKEN)-1;
+#pragma unroll
+            for (int u = 0; u < EMB_AHEAD; ++u) {
+                const unsigned v = emb_token(t[u], V, padding);
+                put(v != ~0u && (v & mask) == b, (g + u) * 64 + lane, v);
+            }
         }
     }
 }
 
 // ---------------------------------------------------------------------------------- sums
 struct EmbArgs {
-    const int *order, *token_of, *count, *total;
+    const int *order, *token_of, *begin_of, *count, *total;
     float *part;  // [pieces][2][D]: of the token that began in an earlier piece, of the one that goes on into the next
     long long V, ldg;
-    int D, lane_bits, pieces;
+    int D, lane_bits, pieces, piece;  // sorted positions are walked in `pieces` pieces of `piece`
     unsigned sum_blocks;
     float scale;
 };
@@ -167,68 +192,97 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_sum(const T *__restrict__ g
     if (blockIdx.x >= a.sum_blocks) {  // rows of tokens that do not occur
         const float zero[E] = {};
         const long long teams = (long long)(gridDim.x - a.sum_blocks) * teams_here;
-        for (long long v = (long long)(blockIdx.x - a.sum_blocks) * teams_here + team_here; v < a.V; v += teams)
-            if (a.count[v] == 0)
-                for (int c = lane * E; c < a.D; c += E << a.lane_bits) dl_store(gw + v * a.D + c, zero);
+        for (long long v0 = (long long)(blockIdx.x - a.sum_blocks) * teams_here + team_here; v0 < a.V; v0 += 4 * teams) {
+            int n[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) n[u] = v0 + u * teams < a.V ? a.count[v0 + u * teams] : 1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (n[u] == 0)
+                    for (int c = lane * E; c < a.D; c += E << a.lane_bits) dl_store_past(gw + (v0 + u * teams) * a.D + c, zero);
+        }
         return;
     }
+    constexpr int ROWS = EMB_ROWS(E);
     const int total = *a.total, piece = blockIdx.x * teams_here + team_here;
-    const int i0 = piece * EMB_PIECE, i1 = min(i0 + EMB_PIECE, total);
+    const int i0 = piece * a.piece, i1 = min(i0 + a.piece, total);
     if (piece >= a.pieces || i0 >= total) return;
     const int before = i0 > 0 ? a.token_of[i0 - 1] : -1, after = i1 < total ? a.token_of[i1] : -1;
     for (int c = lane * E; c < a.D; c += E << a.lane_bits) {
-        float f[EMB_PIECE][E], acc[E] = {};
-#pragma unroll
-        for (int j = 0; j < EMB_PIECE; ++j)
-            if (i0 + j < i1) dl_load(gy + (long long)a.order[i0 + j] * a.D + c, f[j]);
+        float acc[E] = {};
         bool first = true;  // of the piece's tokens
+        for (int j0 = i0; j0 < i1; j0 += ROWS) {
+            float f[ROWS][E];
 #pragma unroll
-        for (int j = 0; j < EMB_PIECE; ++j) {
-            if (i0 + j >= i1) break;
-            const int v = a.token_of[i0 + j], next = i0 + j + 1 < i1 ? a.token_of[i0 + j + 1] : after;
+            for (int j = 0; j < ROWS; ++j)
+                if (j0 + j < i1) dl_load(gy + (long long)a.order[j0 + j] * a.D + c, f[j]);
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += f[j][e];
-            const bool last = i0 + j + 1 == i1;
-            if (next == v && !last) continue;
-            if (first && before == v) dl_store(a.part + ((long long)piece * 2) * a.D + c, acc);
-            else if (last && next == v) dl_store(a.part + ((long long)piece * 2 + 1) * a.D + c, acc);
-            else {
+            for (int j = 0; j < ROWS; ++j) {
+                if (j0 + j >= i1) break;
+                const bool last = j0 + j + 1 == i1;
+                const int v = a.token_of[j0 + j], next = last ? after : a.token_of[j0 + j + 1];
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] *= a.scale;
-                dl_store(gw + (long long)v * a.D + c, acc);
+                for (int e = 0; e < E; ++e) acc[e] += f[j][e];
+                if (next == v && !last) continue;
+                if (first && before == v) dl_store(a.part + ((long long)piece * 2) * a.D + c, acc);
+                else if (last && next == v) dl_store(a.part + ((long long)piece * 2 + 1) * a.D + c, acc);
+                else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] *= a.scale;
+                    dl_store_past(gw + (long long)v * a.D + c, acc);
+                }
+                first = false;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = 0.0f;
             }
-            first = false;
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = 0.0f;
         }
     }
 }
 
+// Tokens that reach over pieces.  A frequent one has thousands of partials: they are split over the block's wavefronts, whose sums are
+// added in order; with few partials the wavefronts take columns of their own instead.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(EMB_THREADS) void embed_join(T *__restrict__ gw, EmbArgs a) {
-    constexpr int E = VEC ? 16 / sizeof(T) : 1;
-    const int lanes = 1 << a.lane_bits, lane = threadIdx.x & (lanes - 1), teams_here = EMB_THREADS >> a.lane_bits;
-    const int total = *a.total, piece = blockIdx.x * teams_here + (threadIdx.x >> a.lane_bits);
-    const long long i0 = (long long)piece * EMB_PIECE, i1 = i0 + EMB_PIECE;
-    if (i1 >= total) return;  // nothing goes on behind the last piece
-    const int v = a.token_of[i1 - 1];
-    if (a.token_of[i1] != v || (a.token_of[i0] == v && i0 > 0 && a.token_of[i0 - 1] == v)) return;  // ends here, or began earlier
-    // the last piece that holds v
-    int last = piece + 1;
-    while ((long long)(last + 1) * EMB_PIECE < total && a.token_of[(long long)(last + 1) * EMB_PIECE] == v) ++last;
-    for (int c = lane * E; c < a.D; c += E << a.lane_bits) {
-        float acc[E];
-        dl_load(a.part + ((long long)piece * 2 + 1) * a.D + c, acc);
+__global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join(T *__restrict__ gw, EmbArgs a) {
+    constexpr int E = VEC ? 4 : 1;
+    __shared__ DlVec<float, E> sums[EMB_JOIN_WAVES][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, total = *a.total;
+    for (long long piece = blockIdx.x; piece < a.pieces; piece += gridDim.x) {
+        const long long i0 = piece * a.piece, i1 = i0 + a.piece;
+        if (i1 >= total) return;  // nothing goes on behind the last piece
+        const int v = a.token_of[i1 - 1], begin = a.begin_of[v], end = begin + a.count[v];
+        if (end <= i1 || begin < i0) continue;  // ends here, or began earlier
+        const int parts = (end - 1) / a.piece - (int)piece;  // whose sums begin the pieces behind this one
+        const float *own = a.part + ((long long)piece * 2 + 1) * a.D, *rest = a.part + ((long long)piece + 1) * 2 * a.D;
+        const bool split = parts >= EMB_JOIN_WAVES;
+        const int per = split ? (parts + EMB_JOIN_WAVES - 1) / EMB_JOIN_WAVES : parts, p0 = split ? min(wave * per, parts) : 0, p1 = min(p0 + per, parts);
+        for (int c0 = split ? 0 : wave * 64 * E; c0 < a.D; c0 += (split ? 1 : EMB_JOIN_WAVES) * 64 * E) {
+            const int c = c0 + lane * E;
+            float acc[E] = {};
+            if (c < a.D) {
+                if (p0 == 0) dl_load(own + c, acc);
 #pragma unroll 8
-        for (int p = piece + 1; p <= last; ++p) {
-            float f[E];
-            dl_load(a.part + (long long)p * 2 * a.D + c, f);
+                for (int p = p0; p < p1; ++p) {
+                    float f[E];
+                    dl_load(rest + (long long)p * 2 * a.D + c, f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += f[e];
+                    for (int e = 0; e < E; ++e) acc[e] += f[e];
+                }
+            }
+            if (split) {
+                __syncthreads();  // the last columns' sums have been read
+                dl_store(&sums[wave][lane].v[0], acc);
+                __syncthreads();
+                if (wave > 0) continue;
+#pragma unroll
+                for (int w = 1; w < EMB_JOIN_WAVES; ++w)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += sums[w][lane].v[e];
+            }
+            if (c >= a.D) continue;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] *= a.scale;
+            dl_store(gw + (long long)v * a.D + c, acc);
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] *= a.scale;
-        dl_store(gw + (long long)v * a.D + c, acc);
     }
 }
 
@@ -239,9 +293,9 @@ static int emb_lane_bits(int D, int E) {  // a team of up to a block's threads, 
     while (bits < 8 && ((long long)E << bits) < D) ++bits;
     return bits;
 }
-static int emb_block_bits(long long V) {  // blocks of the sort: 512 of them, more where a block would own too many tokens
+static int emb_block_bits(long long V) {  // blocks of the sort: one per CU, more where a block would own too many tokens
     int bits = 0;
-    while (bits < 9 && (1LL << bits) < V) ++bits;
+    while (bits < 8 && (1LL << bits) < V) ++bits;
     while (((V + (1LL << bits) - 1) >> bits) > EMB_MAX_OWNED) ++bits;
     return bits;
 }
@@ -272,12 +326,15 @@ extern "C" int dl_embedding_fwd(const void *tokens, int token_bits, const void *
     return dl_launch_status();
 }
 
-static long long emb_pieces(long long n) { return (n + EMB_PIECE - 1) / EMB_PIECE; }
+// Sorted positions per piece: a piece ends inside a token's run twice, for two partials to write and to read again, so longer ones move
+// less; but there have to be enough teams.  (65521 x 1024 bf16: 32; 12544 x 784 fp32: 16, 17 us for 24.)
+static int emb_piece(long long n, int D) { return n * D >= (1LL << 24) + (1LL << 23) ? 32 : 16; }
+static long long emb_pieces(long long n, int D) { return (n + emb_piece(n, D) - 1) / emb_piece(n, D); }
 
 extern "C" size_t dl_embedding_bwd_workspace_bytes(long long n, long long V, int D) {
     if (!emb_sizes_ok(n, V, D)) return 0;
-    return 256 + 2 * dl_align256((size_t)n * sizeof(int)) + dl_align256((size_t)V * sizeof(int)) +
-           dl_align256((size_t)emb_pieces(n) * 2 * D * sizeof(float));
+    return 256 + 2 * dl_align256((size_t)n * sizeof(int)) + 2 * dl_align256((size_t)V * sizeof(int)) +
+           dl_align256((size_t)emb_pieces(n, D) * 2 * D * sizeof(float));
 }
 
 extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *gy, void *gw, int type, long long n, long long V, int D,
@@ -292,25 +349,30 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
     int *total = (int *)ws, *order = (int *)((char *)ws + 256);
     int *token_of = (int *)((char *)order + dl_align256((size_t)n * sizeof(int)));
     int *count = (int *)((char *)token_of + dl_align256((size_t)n * sizeof(int)));
+    int *begin_of = (int *)((char *)count + dl_align256((size_t)V * sizeof(int)));
     EmbArgs a = {};
-    a.order = order, a.token_of = token_of, a.count = count, a.total = total;
-    a.part = (float *)((char *)count + dl_align256((size_t)V * sizeof(int)));
+    a.order = order, a.token_of = token_of, a.begin_of = begin_of, a.count = count, a.total = total;
+    a.part = (float *)((char *)begin_of + dl_align256((size_t)V * sizeof(int)));
     a.V = V, a.D = D, a.scale = scale;
     a.lane_bits = emb_lane_bits(D, vec ? E : 1);
-    a.pieces = (int)emb_pieces(n);
+    a.piece = emb_piece(n, D), a.pieces = (int)emb_pieces(n, D);
     const int teams = EMB_THREADS >> a.lane_bits;
     a.sum_blocks = (unsigned)((a.pieces + teams - 1) / teams);
     const int bits = emb_block_bits(V);
     const size_t lds = (size_t)EMB_SORT_WAVES * (size_t)((V + (1LL << bits) - 1) >> bits) * sizeof(int);
+    const unsigned skip = padding >= 0 && padding < V ? (unsigned)padding : ~0u;
+#define SORT(TOKEN) \
+    embed_sort<TOKEN><<<1 << bits, EMB_SORT_THREADS, lds, s>>>((const TOKEN *)tokens, (int)n, (unsigned)V, skip, bits, order, token_of, begin_of, count, total)
     dl_prof_begin("embed_sort", s);
-    if (token_bits == 32) embed_sort<int><<<1 << bits, EMB_SORT_THREADS, lds, s>>>((const int *)tokens, (int)n, V, padding, bits, order, token_of, count, total);
-    else embed_sort<long long><<<1 << bits, EMB_SORT_THREADS, lds, s>>>((const long long *)tokens, (int)n, V, padding, bits, order, token_of, count, total);
+    if (token_bits == 32) SORT(int);
+    else SORT(long long);
     dl_prof_end(s);
+#undef SORT
     const long long zero_teams = (V + teams - 1) / teams;
-    const unsigned zero_blocks = (unsigned)(zero_teams < 4096 ? zero_teams : 4096);
+    const unsigned zero_blocks = (unsigned)(zero_teams < 2048 ? zero_teams : 2048);
 #define SUMS(VEC)                                                                                                                    \
     DL_TIMED("embed_sum", s, (embed_sum<T, VEC><<<a.sum_blocks + zero_blocks, EMB_THREADS, 0, s>>>((const T *)gy, (T *)gw, a)));     \
-    if (a.pieces > 1) DL_TIMED("embed_join", s, (embed_join<T, VEC><<<a.sum_blocks, EMB_THREADS, 0, s>>>((T *)gw, a)))
+    if (a.pieces > 1) DL_TIMED("embed_join", s, (embed_join<T, VEC><<<a.pieces < 1024 ? a.pieces : 1024, EMB_JOIN_THREADS, 0, s>>>((T *)gw, a)))
     DL_BY_TYPE(type, T, if (vec) { SUMS(true); } else { SUMS(false); });
 #undef SUMS
     return dl_launch_status();

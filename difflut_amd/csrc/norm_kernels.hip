@@ -11,6 +11,8 @@
 // are joined by the pairwise formula (Chan, Golub, LeVeque 1979), in a fixed order: results are the same bits from run to run.
 #include "dl_types.h"
 
+#define GN_ONE_WIDTH 2048  // channels of a tile of the one-block forms
+
 enum { GN_NONE = DL_ACT_NONE, GN_RELU = DL_ACT_RELU, GN_SILU = DL_ACT_SILU, GN_SIGMOID = DL_ACT_SIGMOID };
 
 struct GnShape {
@@ -24,18 +26,21 @@ struct GnShape {
     int piece_rows;    // positions of a piece
 };
 
-__device__ __forceinline__ float gn_sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
-__device__ __forceinline__ float gn_act(int act, float z) {
-    if (act == GN_RELU) return z > 0.0f || z != z ? z : 0.0f;
-    if (act == GN_SILU) return z * gn_sigmoid(z);
-    if (act == GN_SIGMOID) return gn_sigmoid(z);
+// (exponential and reciprocal as the hardware has them: an ulp each, and |z| u from the product with log2 e)
+__device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+template <int ACT>
+__device__ __forceinline__ float gn_act(float z) {
+    if (ACT == GN_RELU) return z > 0.0f || z != z ? z : 0.0f;
+    if (ACT == GN_SILU) return z * gn_sigmoid(z);
+    if (ACT == GN_SIGMOID) return gn_sigmoid(z);
     return z;
 }
-__device__ __forceinline__ float gn_slope(int act, float z) {
-    if (act == GN_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    if (act == GN_NONE) return 1.0f;
-    const float s = gn_sigmoid(z);
-    return act == GN_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
+template <int ACT>
+__device__ __forceinline__ float gn_slope(float z) {
+    if (ACT == GN_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    if (ACT == GN_NONE) return 1.0f;
+    const float s = gn_sigmoid(z), r = fmaf(-s, s, s);  // s (1 - s)
+    return ACT == GN_SILU ? fmaf(z, r, s) : r;
 }
 // gamma or beta of channel c (stored as `type`); `fallback` where the norm has none
 __device__ __forceinline__ float gn_param(const void *p, int type, int c, float fallback) {
@@ -148,85 +153,173 @@ __device__ void gn_group_sums(const GnShape &s, const GnPlace &w, const float (&
     __syncthreads();
 }
 
-// ---------------------------------------------------------------------------------- forward
-// Statistics of a piece: mean and sum of squares about it per group, [B][G][slices * pieces] (mean, M2).  The piece stays in
-// registers between the two sums.  ONE: the piece is the whole sample, so the block goes on to write y.
-template <typename T, int E, bool VEC, int NV, int THREADS, bool ONE>
-__global__ __launch_bounds__(THREADS) void gn_forward(const T *__restrict__ x, const void *__restrict__ gamma,
-                                                       const void *__restrict__ beta, int ptype, T *__restrict__ y,
-                                                       float2 *__restrict__ stats, float2 *__restrict__ part, GnShape s, float eps, int act) {
-    __shared__ float slots[THREADS * E];
-    __shared__ float sums[THREADS * E], mean[THREADS * E];
-    const int tile = blockIdx.x % s.tiles, piece = blockIdx.x / s.tiles % s.pieces, b = blockIdx.x / s.tiles / s.pieces;
-    const GnPlace w = gn_place<E>(s, tile, piece, THREADS);
-    const int real = w.c_end - w.c;
-    float v[NV][E];
-    float t[E] = {};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const long long p = w.p_begin + w.row0 + (long long)i * w.rows;
-        if (w.active && p < w.p_end) gn_read<T, E, VEC>(x + ((long long)b * s.P + p) * s.C + w.c, real, v[i]);
-        else
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[i][e] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < E; ++e) t[e] += v[i][e];
-    gn_group_sums<E, THREADS>(s, w, t, slots, sums);
-    const int c0 = w.c - w.col * E;
-    const float n = (float)(w.p_end - w.p_begin) * (float)(s.tile_groups ? s.cg : w.c_end - c0);
-    for (int g = threadIdx.x; g < w.groups; g += THREADS) mean[g] = sums[g] / n;
+// Per channel of the tile, the sum over the block's rows of threads: every thread brings E values, totals[c] (LDS, may be slots) gets
+// them.  Two steps: every thread adds a share of one channel's rows, then a thread per channel adds the shares.
+template <int E, int THREADS>
+__device__ void gn_channel_sums(const GnPlace &w, int width, const float (&v)[E], float *slots, float *totals) {
+    const int vectors = (width + E - 1) / E, padded = vectors * E;
     __syncthreads();
-    int group[E];
-    float m[E];
+    if (w.active) dl_store(slots + threadIdx.x * E, v);
+    __syncthreads();
+    const int shares = max(1, THREADS / padded);
+    float t = 0.0f;
+    if (shares > 1 && (int)threadIdx.x < shares * padded) {
+        const int c = threadIdx.x % padded, first = threadIdx.x / padded;
+#pragma unroll 4
+        for (int r = first; r < w.rows; r += shares) t += slots[r * padded + c];
+    }
+    __syncthreads();
+    if (shares > 1) {
+        if ((int)threadIdx.x < shares * padded) slots[threadIdx.x] = t;
+        __syncthreads();
+    }
+    const int parts = shares > 1 ? shares : w.rows;
+    float sum[E] = {};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        group[e] = s.tile_groups && w.active && e < real ? (w.c + e - c0) / s.cg : 0;
-        m[e] = mean[group[e]];
-        t[e] = 0.0f;
+        const int c = threadIdx.x + e * THREADS;  // (padded <= THREADS * E)
+        if (c < padded)
+#pragma unroll 4
+            for (int r = 0; r < parts; ++r) sum[e] += slots[r * padded + c];
     }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if ((int)(threadIdx.x + e * THREADS) < padded) totals[threadIdx.x + e * THREADS] = sum[e];
+    __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------- forward
+// E neighbouring elements as they lie in memory (16 bytes)
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ DlVec<T, E> gn_raw(const T *p, int real) {
+    if constexpr (VEC) return *reinterpret_cast<const DlVec<T, E> *>(p);
+    DlVec<T, E> t;
+#pragma unroll
+    for (int e = 0; e < E; ++e) t.v[e] = e < real ? p[e] : (T)0.0f;
+    return t;
+}
+
+// A sample's tile in one block: the values stay in registers from the one read to y.
+template <typename T, bool VEC, int NV, int THREADS, int ACT>
+__global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ x, const void *__restrict__ gamma,
+                                                           const void *__restrict__ beta, int ptype, T *__restrict__ y,
+                                                           float2 *__restrict__ stats, GnShape s, float eps) {
+    constexpr int E = 16 / sizeof(T);
+    __shared__ float slots[THREADS * E], sums[GN_ONE_WIDTH];
+    const int tile = blockIdx.x % s.tiles, b = blockIdx.x / s.tiles;
+    const GnPlace w = gn_place<E>(s, tile, 0, THREADS);
+    const int real = w.c_end - w.c, c0 = w.c - w.col * E;
+    const long long base = (long long)b * s.P * s.C + w.c;
+    const int P = (int)s.P;
+    DlVec<T, E> v[NV];
+    int group[E];
+    float t[E], m[E], ga[E], be[E];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const long long p = w.p_begin + w.row0 + (long long)i * w.rows;
-        if (!w.active || p >= w.p_end) continue;
+        const int p = w.row0 + i * w.rows;
+        if (w.active && p < P) v[i] = gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[i].v[e] = (T)0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        group[e] = w.active && e < real ? (w.c + e - c0) / s.cg : 0;
+        ga[e] = w.active && e < real ? gn_param(gamma, ptype, w.c + e, 1.0f) : 0.0f;
+        be[e] = w.active && e < real ? gn_param(beta, ptype, w.c + e, 0.0f) : 0.0f;
+        t[e] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) t[e] += (float)v[i].v[e];
+    }
+    gn_group_sums<E, THREADS>(s, w, t, slots, sums);
+    const float per = 1.0f / ((float)P * (float)s.cg);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        m[e] = sums[group[e]] * per;
+        t[e] = 0.0f;
+    }
+    __syncthreads();
+    float mean[E];  // of the groups that this thread reports
+#pragma unroll
+    for (int k = 0; k < E; ++k) mean[k] = (int)(threadIdx.x + k * THREADS) < w.groups ? sums[threadIdx.x + k * THREADS] * per : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (!w.active || w.row0 + i * w.rows >= P) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float d = e < real ? v[i][e] - m[e] : 0.0f;
-            t[e] += d * d;
+            const float d = e < real ? (float)v[i].v[e] - m[e] : 0.0f;
+            t[e] = fmaf(d, d, t[e]);
         }
     }
     gn_group_sums<E, THREADS>(s, w, t, slots, sums);
-    if (!ONE) {
-        const int slice = s.tile_groups ? 0 : tile % s.slices;
-        for (int g = threadIdx.x; g < w.groups; g += THREADS)
-            part[((long long)b * s.G + w.first_group + g) * (s.slices * s.pieces) + (long long)piece * s.slices + slice] = make_float2(mean[g], sums[g]);
-        return;
-    }
-    for (int g = threadIdx.x; g < w.groups; g += THREADS) {
-        const float rstd = 1.0f / sqrtf(sums[g] / n + eps);
-        sums[g] = rstd;
-        if (stats) stats[(long long)b * s.G + w.first_group + g] = make_float2(mean[g], rstd);
-    }
-    __syncthreads();
-    if (!w.active) return;
-    float ga[E], be[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        ga[e] = e < real ? gn_param(gamma, ptype, w.c + e, 1.0f) : 0.0f;
-        be[e] = e < real ? gn_param(beta, ptype, w.c + e, 0.0f) : 0.0f;
-        t[e] = sums[group[e]];
+    for (int k = 0; k < E; ++k) {
+        const int g = threadIdx.x + k * THREADS;
+        if (g < w.groups) stats[(long long)b * s.G + w.first_group + g] = make_float2(mean[k], 1.0f / sqrtf(fmaf(sums[g], per, eps)));
     }
+    if (!w.active) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ga[e] *= 1.0f / sqrtf(fmaf(sums[group[e]], per, eps));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const long long p = w.p_begin + w.row0 + (long long)i * w.rows;
-        if (p >= w.p_end) continue;
+        const int p = w.row0 + i * w.rows;
+        if (p >= P) continue;
         float o[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = gn_act(act, (v[i][e] - m[e]) * t[e] * ga[e] + be[e]);
-        gn_write<T, E, VEC>(y + ((long long)b * s.P + p) * s.C + w.c, real, o);
+        for (int e = 0; e < E; ++e) o[e] = gn_act<ACT>(fmaf((float)v[i].v[e] - m[e], ga[e], be[e]));
+        gn_write<T, E, VEC>(y + base + (long long)p * s.C, real, o);
     }
+}
+
+// Statistics of a piece of a sample: mean and sum of squares about it per group, [B][G][slices * pieces] (mean, M2).  One read:
+// a thread's sums are about its own first value, whose square about the mean is one of the terms that it sums, so that no more than
+// a factor of its number of rows is lost to cancellation, whatever the values.
+template <typename T, bool VEC, int THREADS>
+__global__ __launch_bounds__(THREADS) void gn_stats(const T *__restrict__ x, float2 *__restrict__ part, GnShape s) {
+    constexpr int E = 16 / sizeof(T);
+    __shared__ float slots[THREADS * E], sums[THREADS * E];
+    const int tile = blockIdx.x % s.tiles, piece = blockIdx.x / s.tiles % s.pieces, b = blockIdx.x / s.tiles / s.pieces;
+    const GnPlace w = gn_place<E>(s, tile, piece, THREADS);
+    const int real = w.c_end - w.c, c0 = w.c - w.col * E;
+    const T *from = x + ((long long)b * s.P + w.p_begin) * s.C + w.c;
+    const int rows = (int)(w.p_end - w.p_begin);
+    float first[E], sum[E] = {}, square[E] = {}, t[E];
+    if (w.active && w.row0 < rows) {
+        gn_read<T, E, VEC>(from + (long long)w.row0 * s.C, real, first);
+#pragma unroll 4
+        for (int p = w.row0 + w.rows; p < rows; p += w.rows) {
+            float v[E];
+            gn_read<T, E, VEC>(from + (long long)p * s.C, real, v);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = v[e] - first[e];
+                sum[e] += d;
+                square[e] = fmaf(d, d, square[e]);
+            }
+        }
+    }
+    const float n = w.active && w.row0 < rows ? (float)((rows - 1 - w.row0) / w.rows + 1) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) t[e] = n > 0.0f ? fmaf(n, first[e], sum[e]) : 0.0f;
+    gn_group_sums<E, THREADS>(s, w, t, slots, sums);
+    const float all = (float)rows * (float)(s.tile_groups ? s.cg : w.c_end - c0);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int group = s.tile_groups && w.active && e < real ? (w.c + e - c0) / s.cg : 0;
+        t[e] = 0.0f;
+        if (n > 0.0f && e < real) {
+            const float mine = sum[e] / n, d = first[e] + mine - sums[group] / all;
+            t[e] = fmaxf(square[e] - sum[e] * mine, 0.0f) + n * d * d;
+            if (square[e] != square[e]) t[e] = square[e];  // (fmaxf drops a NaN)
+        }
+    }
+    const int slice = s.tile_groups ? 0 : tile % s.slices;
+    float2 *to = part + ((long long)b * s.G + w.first_group) * (s.slices * s.pieces) + (long long)piece * s.slices + slice;
+    for (int g = threadIdx.x; g < w.groups; g += THREADS) to[(long long)g * (s.slices * s.pieces)].x = sums[g] / all;
+    __syncthreads();
+    gn_group_sums<E, THREADS>(s, w, t, slots, sums);
+    for (int g = threadIdx.x; g < w.groups; g += THREADS) to[(long long)g * (s.slices * s.pieces)].y = sums[g];
 }
 
 // mean and rstd of every (sample, group) from its parts: one wavefront each.
@@ -251,13 +344,15 @@ __global__ __launch_bounds__(256) void gn_join_stats(const float2 *__restrict__ 
 }
 
 // y = act((x - mean) rstd gamma + beta) where the statistics are known
-template <typename T, int E, bool VEC, int THREADS>
+template <typename T, bool VEC, int THREADS, int ACT>
 __global__ __launch_bounds__(THREADS) void gn_apply(const T *__restrict__ x, const void *__restrict__ gamma, const void *__restrict__ beta,
-                                                     int ptype, T *__restrict__ y, const float2 *__restrict__ stats, GnShape s, int act) {
+                                                     int ptype, T *__restrict__ y, const float2 *__restrict__ stats, GnShape s) {
+    constexpr int E = 16 / sizeof(T);
     const int tile = blockIdx.x % s.tiles, piece = blockIdx.x / s.tiles % s.pieces, b = blockIdx.x / s.tiles / s.pieces;
     const GnPlace w = gn_place<E>(s, tile, piece, THREADS);
     if (!w.active) return;
-    const int real = w.c_end - w.c;
+    const int real = w.c_end - w.c, rows = (int)(w.p_end - w.p_begin);
+    const long long base = ((long long)b * s.P + w.p_begin) * s.C + w.c;
     float scale[E], shift[E], mean[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -268,29 +363,21 @@ __global__ __launch_bounds__(THREADS) void gn_apply(const T *__restrict__ x, con
         shift[e] = gn_param(beta, ptype, c, 0.0f);
     }
 #pragma unroll 4
-    for (long long p = w.p_begin + w.row0; p < w.p_end; p += w.rows) {
-        const long long at = ((long long)b * s.P + p) * s.C + w.c;
+    for (int p = w.row0; p < rows; p += w.rows) {
         float v[E];
-        gn_read<T, E, VEC>(x + at, real, v);
+        gn_read<T, E, VEC>(x + base + (long long)p * s.C, real, v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = gn_act(act, (v[e] - mean[e]) * scale[e] + shift[e]);
-        gn_write<T, E, VEC>(y + at, real, v);
+        for (int e = 0; e < E; ++e) v[e] = gn_act<ACT>(fmaf(v[e] - mean[e], scale[e], shift[e]));
+        gn_write<T, E, VEC>(y + base + (long long)p * s.C, real, v);
     }
 }
 
 // ---------------------------------------------------------------------------------- backward
-// Per channel of a piece: sum g and sum g xhat, [B][pieces][2][C].
-template <typename T, int E, bool VEC, int THREADS>
-__global__ __launch_bounds__(THREADS) void gn_backward_sums(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
-                                                             const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
-                                                             float *__restrict__ part, GnShape s, int act) {
-    __shared__ float slots[2][THREADS * E];
-    const int tile = blockIdx.x % s.tiles, piece = blockIdx.x / s.tiles % s.pieces, b = blockIdx.x / s.tiles / s.pieces;
-    const GnPlace w = gn_place<E>(s, tile, piece, THREADS);
-    const int real = w.c_end - w.c;
-    float sg[E] = {}, sx[E] = {};
-    if (w.active) {
-        float mean[E], rstd[E], ga[E], be[E];
+// A thread's channels: what g and xhat are made of
+template <int E>
+struct GnChannels {
+    float mean[E], rstd[E], ga[E], be[E];
+    __device__ __forceinline__ GnChannels(const GnShape &s, const GnPlace &w, int b, const float2 *stats, const void *gamma, const void *beta, int ptype) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int c = min(w.c + e, s.C - 1);
@@ -298,54 +385,155 @@ __global__ __launch_bounds__(THREADS) void gn_backward_sums(const T *__restrict_
             mean[e] = st.x, rstd[e] = st.y;
             ga[e] = gn_param(gamma, ptype, c, 1.0f), be[e] = gn_param(beta, ptype, c, 0.0f);
         }
-#pragma unroll 2
-        for (long long p = w.p_begin + w.row0; p < w.p_end; p += w.rows) {
-            const long long at = ((long long)b * s.P + p) * s.C + w.c;
-            float v[E], g[E];
-            gn_read<T, E, VEC>(x + at, real, v);
-            gn_read<T, E, VEC>(gy + at, real, g);
+    }
+    template <int ACT>
+    __device__ __forceinline__ void at(int e, float x, float gy, float &hat, float &g) const {
+        hat = (x - mean[e]) * rstd[e];
+        g = ACT == GN_NONE ? gy : gy * gn_slope<ACT>(fmaf(hat, ga[e], be[e]));
+    }
+};
+
+// A sample's tile in one block: x and gy stay in registers from the one read to gx; the channels' sums go to [B][2][C].
+template <typename T, bool VEC, int NV, int THREADS, int ACT>
+__global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
+                                                            const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
+                                                            float *__restrict__ channel, T *__restrict__ gx, GnShape s) {
+    constexpr int E = 16 / sizeof(T);
+    __shared__ float slots[THREADS * E], sum_g[GN_ONE_WIDTH + E], sum_x[GN_ONE_WIDTH + E], mean_g[GN_ONE_WIDTH];
+    const int tile = blockIdx.x % s.tiles, b = blockIdx.x / s.tiles;
+    const GnPlace w = gn_place<E>(s, tile, 0, THREADS);
+    const int real = w.c_end - w.c, c0 = w.c - w.col * E, width = w.c_end - c0, P = (int)s.P;
+    const long long base = (long long)b * s.P * s.C + w.c;
+    DlVec<T, E> v[NV], d[NV];
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float hat = (v[e] - mean[e]) * rstd[e], d = g[e] * gn_slope(act, hat * ga[e] + be[e]);
-                sg[e] += d;
-                sx[e] += d * hat;
-            }
+    for (int i = 0; i < NV; ++i) {
+        const int p = w.row0 + i * w.rows;
+        if (w.active && p < P) {
+            v[i] = gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real);
+            d[i] = gn_raw<T, E, VEC>(gy + base + (long long)p * s.C, real);
         }
     }
-    const int vectors = (w.c_end - (w.c - w.col * E) + E - 1) / E;
+    const GnChannels<E> ch(s, w, b, stats, gamma, beta, ptype);
+    float sg[E] = {}, sx[E] = {};
 #pragma unroll
-    for (int e = 0; e < E; ++e) slots[0][threadIdx.x * E + e] = w.active ? sg[e] : 0.0f, slots[1][threadIdx.x * E + e] = w.active ? sx[e] : 0.0f;
+    for (int i = 0; i < NV; ++i) {
+        if (!w.active || w.row0 + i * w.rows >= P) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float hat, g;
+            ch.template at<ACT>(e, (float)v[i].v[e], (float)d[i].v[e], hat, g);
+            sg[e] += g;
+            sx[e] = fmaf(g, hat, sx[e]);
+        }
+    }
+    gn_channel_sums<E, THREADS>(w, width, sg, slots, sum_g);
+    gn_channel_sums<E, THREADS>(w, width, sx, slots, sum_x);
+    for (int c = threadIdx.x; c < width; c += THREADS) {
+        channel[(long long)b * 2 * s.C + c0 + c] = sum_g[c];
+        channel[(long long)b * 2 * s.C + s.C + c0 + c] = sum_x[c];
+    }
+    if (!gx) return;
+    // the groups' means, a wavefront each
+    float *const mean_x = slots;  // (a group has a channel, a channel a slot)
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float per = 1.0f / ((float)P * (float)s.cg);
+    for (int g = wave; g < w.groups; g += THREADS / 64) {
+        float a = 0.0f, q = 0.0f;
+        for (int c = lane; c < s.cg; c += 64) {
+            const float gam = gn_param(gamma, ptype, c0 + g * s.cg + c, 1.0f);
+            a = fmaf(gam, sum_g[g * s.cg + c], a);
+            q = fmaf(gam, sum_x[g * s.cg + c], q);
+        }
+        a = gn_wave_sum(a), q = gn_wave_sum(q);
+        if (lane == 0) mean_g[g] = a * per, mean_x[g] = q * per;
+    }
     __syncthreads();
-    // column sums over the rows of threads, in order
-    const int c0 = w.c - w.col * E, width = w.c_end - c0;
-    float *out = part + ((long long)b * s.pieces + piece) * 2 * s.C + c0;
-    for (int j = threadIdx.x; j < 2 * width; j += THREADS) {
-        const int which = j >= width, c = j - which * width;
-        float t = 0.0f;
-        for (int r = 0; r < w.rows; ++r) t += slots[which][r * vectors * E + c];
-        out[(long long)which * s.C + c] = t;
+    if (!w.active) return;
+    float ma[E], mq[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int g = e < real ? (w.c + e - c0) / s.cg : 0;
+        ma[e] = mean_g[g], mq[e] = mean_x[g];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int p = w.row0 + i * w.rows;
+        if (p >= P) continue;
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float hat, g;
+            ch.template at<ACT>(e, (float)v[i].v[e], (float)d[i].v[e], hat, g);
+            o[e] = ch.rstd[e] * (fmaf(g, ch.ga[e], -ma[e]) - hat * mq[e]);
+        }
+        gn_write<T, E, VEC>(gx + base + (long long)p * s.C, real, o);
     }
 }
 
+// Per channel of a piece: sum g and sum g xhat, [B][pieces][2][C].
+template <typename T, bool VEC, int THREADS, int ACT>
+__global__ __launch_bounds__(THREADS) void gn_backward_sums(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
+                                                             const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
+                                                             float *__restrict__ part, GnShape s) {
+    constexpr int E = 16 / sizeof(T);
+    __shared__ float slots[THREADS * E];
+    const int tile = blockIdx.x % s.tiles, piece = blockIdx.x / s.tiles % s.pieces, b = blockIdx.x / s.tiles / s.pieces;
+    const GnPlace w = gn_place<E>(s, tile, piece, THREADS);
+    const int real = w.c_end - w.c, c0 = w.c - w.col * E, width = w.c_end - c0, rows = (int)(w.p_end - w.p_begin);
+    const long long base = ((long long)b * s.P + w.p_begin) * s.C + w.c;
+    float sg[E] = {}, sx[E] = {};
+    if (w.active) {
+        const GnChannels<E> ch(s, w, b, stats, gamma, beta, ptype);
+#pragma unroll 4
+        for (int p = w.row0; p < rows; p += w.rows) {
+            float v[E], d[E];
+            gn_read<T, E, VEC>(x + base + (long long)p * s.C, real, v);
+            gn_read<T, E, VEC>(gy + base + (long long)p * s.C, real, d);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                float hat, g;
+                ch.template at<ACT>(e, v[e], d[e], hat, g);
+                sg[e] += g;
+                sx[e] = fmaf(g, hat, sx[e]);
+            }
+        }
+    }
+    float *out = part + ((long long)b * s.pieces + piece) * 2 * s.C + c0;
+    gn_channel_sums<E, THREADS>(w, width, sg, slots, slots);
+    for (int c = threadIdx.x; c < width; c += THREADS) out[c] = slots[c];
+    gn_channel_sums<E, THREADS>(w, width, sx, slots, slots);
+    for (int c = threadIdx.x; c < width; c += THREADS) out[s.C + c] = slots[c];
+}
+
 // Per sample: the channels' sums over its pieces ([B][2][C]) and, per group, mean(gamma g) and mean(gamma g xhat).
-// One block per (sample, group).
+// One block per (sample, group): threads are (channel, share of the pieces).
 __global__ __launch_bounds__(256) void gn_backward_join(const float *__restrict__ part, const void *__restrict__ gamma, int ptype,
                                                          float *__restrict__ channel, float2 *__restrict__ group, GnShape s) {
-    __shared__ float red[2][4];
+    __shared__ float share[2][256], red[2][4];
     const int g = blockIdx.x % s.G, b = blockIdx.x / s.G;
+    const int across = min(s.cg, 256), shares = 256 / across, mine = threadIdx.x / across, col = threadIdx.x % across;
     float a = 0.0f, q = 0.0f;
-    for (int c = g * s.cg + threadIdx.x; c < (g + 1) * s.cg; c += 256) {
+    for (int c0 = 0; c0 < s.cg; c0 += across) {
+        const int c = g * s.cg + c0 + col;
         float sg = 0.0f, sx = 0.0f;
-        for (int i = 0; i < s.pieces; ++i) {
-            const float *row = part + ((long long)b * s.pieces + i) * 2 * s.C + c;
-            sg += row[0];
-            sx += row[s.C];
+        if (mine < shares && c0 + col < s.cg)
+#pragma unroll 4
+            for (int i = mine; i < s.pieces; i += shares) {
+                const float *row = part + ((long long)b * s.pieces + i) * 2 * s.C + c;
+                sg += row[0];
+                sx += row[s.C];
+            }
+        __syncthreads();
+        share[0][threadIdx.x] = sg, share[1][threadIdx.x] = sx;
+        __syncthreads();
+        if (mine == 0 && c0 + col < s.cg) {
+            for (int i = 1; i < shares; ++i) sg += share[0][i * across + col], sx += share[1][i * across + col];
+            channel[(long long)b * 2 * s.C + c] = sg;
+            channel[(long long)b * 2 * s.C + s.C + c] = sx;
+            const float ga = gn_param(gamma, ptype, c, 1.0f);
+            a = fmaf(ga, sg, a);
+            q = fmaf(ga, sx, q);
         }
-        channel[(long long)b * 2 * s.C + c] = sg;
-        channel[(long long)b * 2 * s.C + s.C + c] = sx;
-        const float ga = gn_param(gamma, ptype, c, 1.0f);
-        a += ga * sg;
-        q += ga * sx;
     }
     a = gn_wave_sum(a), q = gn_wave_sum(q);
     if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = a, red[1][threadIdx.x >> 6] = q;
@@ -357,34 +545,35 @@ __global__ __launch_bounds__(256) void gn_backward_join(const float *__restrict_
     }
 }
 
-template <typename T, int E, bool VEC, int THREADS>
+template <typename T, bool VEC, int THREADS, int ACT>
 __global__ __launch_bounds__(THREADS) void gn_backward_apply(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
                                                               const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
-                                                              const float2 *__restrict__ group, T *__restrict__ gx, GnShape s, int act) {
+                                                              const float2 *__restrict__ group, T *__restrict__ gx, GnShape s) {
+    constexpr int E = 16 / sizeof(T);
     const int tile = blockIdx.x % s.tiles, piece = blockIdx.x / s.tiles % s.pieces, b = blockIdx.x / s.tiles / s.pieces;
     const GnPlace w = gn_place<E>(s, tile, piece, THREADS);
     if (!w.active) return;
-    const int real = w.c_end - w.c;
-    float mean[E], rstd[E], ga[E], be[E], ma[E], mq[E];
+    const int real = w.c_end - w.c, rows = (int)(w.p_end - w.p_begin);
+    const long long base = ((long long)b * s.P + w.p_begin) * s.C + w.c;
+    const GnChannels<E> ch(s, w, b, stats, gamma, beta, ptype);
+    float ma[E], mq[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int c = min(w.c + e, s.C - 1);
-        const float2 st = stats[(long long)b * s.G + c / s.cg], gr = group[(long long)b * s.G + c / s.cg];
-        mean[e] = st.x, rstd[e] = st.y, ma[e] = gr.x, mq[e] = gr.y;
-        ga[e] = gn_param(gamma, ptype, c, 1.0f), be[e] = gn_param(beta, ptype, c, 0.0f);
+        const float2 gr = group[(long long)b * s.G + min(w.c + e, s.C - 1) / s.cg];
+        ma[e] = gr.x, mq[e] = gr.y;
     }
-#pragma unroll 2
-    for (long long p = w.p_begin + w.row0; p < w.p_end; p += w.rows) {
-        const long long at = ((long long)b * s.P + p) * s.C + w.c;
-        float v[E], g[E];
-        gn_read<T, E, VEC>(x + at, real, v);
-        gn_read<T, E, VEC>(gy + at, real, g);
+#pragma unroll 4
+    for (int p = w.row0; p < rows; p += w.rows) {
+        float v[E], d[E];
+        gn_read<T, E, VEC>(x + base + (long long)p * s.C, real, v);
+        gn_read<T, E, VEC>(gy + base + (long long)p * s.C, real, d);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float hat = (v[e] - mean[e]) * rstd[e], d = g[e] * gn_slope(act, hat * ga[e] + be[e]);
-            v[e] = rstd[e] * (d * ga[e] - ma[e] - hat * mq[e]);
+            float hat, g;
+            ch.template at<ACT>(e, v[e], d[e], hat, g);
+            v[e] = ch.rstd[e] * (fmaf(g, ch.ga[e], -ma[e]) - hat * mq[e]);
         }
-        gn_write<T, E, VEC>(gx + at, real, v);
+        gn_write<T, E, VEC>(gx + base + (long long)p * s.C, real, v);
     }
 }
 
@@ -456,24 +645,61 @@ static int gn_rows_per_step(const GnShape &s, int E, int threads) {
     return threads / vectors > 0 ? threads / vectors : 1;
 }
 #define GN_THREADS 256
-#define GN_NV 8  // positions that a thread of the statistics kernel holds
+#define GN_ONE_THREADS 1024
+// 16-byte units that a thread of the one-block forms holds: 64 values either way, of x or of x and gy (128 spill)
+#define GN_ONE_FORWARD(E) (64 / (E))
+#define GN_ONE_BACKWARD(E) (32 / (E))
 
-static GnShape gn_stats_shape(int B, long long P, int C, int G, int E) {
-    GnShape s = gn_tiles(B, P, C, G, E, GN_THREADS);
-    s.piece_rows = gn_rows_per_step(s, E, GN_THREADS) * GN_NV;
-    s.pieces = (int)((P + s.piece_rows - 1) / s.piece_rows);
-    return s;
-}
-static GnShape gn_sums_shape(int B, long long P, int C, int G, int E) {
+static GnShape gn_pieces_shape(int B, long long P, int C, int G, int E) {
     GnShape s = gn_tiles(B, P, C, G, E, GN_THREADS);
     gn_pieces(s, gn_rows_per_step(s, E, GN_THREADS) * 4, 2048);
     return s;
 }
 static bool gn_grid_ok(const GnShape &s) { return (long long)s.B * s.tiles * s.pieces < (1LL << 31); }
 
+// The one-block form: tiles of whole groups over all of a sample's positions that a block's registers hold; false where there are
+// none, or only tiles of less than 64 bytes per position of a large tensor, whose lines every block would fetch anew.
+static bool gn_one_shape(GnShape &s, int B, long long P, int C, int G, int E, int units, int threads) {
+    const int cg = C / G;
+    const long long vectors = (long long)threads * units / P < threads ? (long long)threads * units / P : threads;
+    long long groups = vectors * E / cg < G ? vectors * E / cg : G;  // as many as could fit; fewer are tried below
+    // enough blocks for the card's 256 CUs, as long as a position's piece is 64 bytes
+    while (groups > 1 && (long long)B * dl_ceil_div(G, groups) < 256 && (groups / 2) * cg >= 4 * E) groups /= 2;
+    for (; groups >= 1; --groups) {
+        if (groups < G && groups > 1 && groups * cg % E) continue;  // tiles that begin at whole vectors
+        s = gn_tiles(B, P, C, G, E, threads);
+        s.tile_groups = (int)groups;
+        s.slices = 1;
+        s.tile_width = (int)groups * cg;
+        s.tiles = dl_ceil_div(G, groups);
+        s.pieces = 1;
+        s.piece_rows = (int)P;
+        if ((s.tile_width + E - 1) / E <= threads && s.tile_width <= GN_ONE_WIDTH && (long long)gn_rows_per_step(s, E, threads) * units >= P)
+            return groups == G || s.tile_width >= 4 * E || (long long)B * P * C <= (1 << 18);
+    }
+    return false;
+}
+
+#define GN_BY_ACT(act, ACT, ...)                   \
+    do {                                           \
+        if ((act) == GN_NONE) {                    \
+            constexpr int ACT = GN_NONE;           \
+            __VA_ARGS__;                           \
+        } else if ((act) == GN_RELU) {             \
+            constexpr int ACT = GN_RELU;           \
+            __VA_ARGS__;                           \
+        } else if ((act) == GN_SILU) {             \
+            constexpr int ACT = GN_SILU;           \
+            __VA_ARGS__;                           \
+        } else {                                   \
+            constexpr int ACT = GN_SIGMOID;        \
+            __VA_ARGS__;                           \
+        }                                          \
+    } while (0)
+
 extern "C" size_t dl_group_norm_fwd_workspace_bytes(int type, int B, long long P, int C, int G) {
     if (!dl_type_known(type) || !gn_shape_ok(B, P, C, G)) return 0;
-    const GnShape s = gn_stats_shape(B, P, C, G, 16 / dl_type_bytes(type));
+    const GnShape s = gn_pieces_shape(B, P, C, G, 16 / dl_type_bytes(type));
     return dl_align256((size_t)B * G * s.slices * s.pieces * sizeof(float2));
 }
 
@@ -485,16 +711,29 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
     if (ws_bytes < dl_group_norm_fwd_workspace_bytes(type, B, P, C, G)) return DL_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     const int E = 16 / dl_type_bytes(type);
-    const GnShape a = gn_stats_shape(B, P, C, G, E), b = gn_sums_shape(B, P, C, G, E);
-    if (!gn_grid_ok(a) || !gn_grid_ok(b)) return DL_ERR_UNSUPPORTED;
-    const bool vec = gn_vectors(a, E, x, y, nullptr);
-    const int blocks_a = B * a.tiles * a.pieces, blocks_b = B * b.tiles * b.pieces;
+    GnShape s;
+    for (const int threads : {GN_THREADS, GN_ONE_THREADS})
+        if (gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_FORWARD(E), threads)) {
+            if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+            const bool vec = gn_vectors(s, E, x, y, nullptr);
+            dl_prof_begin("gn_forward_one", st);
+#define ONE(VEC, NV, THREADS) \
+    gn_forward_one<T, VEC, NV, THREADS, ACT><<<s.B * s.tiles, THREADS, 0, st>>>((const T *)x, gamma, beta, ptype, (T *)y, (float2 *)stats, s, eps)
+            DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
+                                          else { if (vec) ONE(true, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
+#undef ONE
+            dl_prof_end(st);
+            return dl_launch_status();
+        }
+    s = gn_pieces_shape(B, P, C, G, E);
+    if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+    const bool vec = gn_vectors(s, E, x, y, nullptr);
+    const int blocks = B * s.tiles * s.pieces;
 #define FORWARD(VEC)                                                                                                                  \
-    DL_TIMED("gn_forward", st, (gn_forward<T, 16 / sizeof(T), VEC, GN_NV, GN_THREADS, false><<<blocks_a, GN_THREADS, 0, st>>>(        \
-        (const T *)x, gamma, beta, ptype, (T *)y, (float2 *)stats, (float2 *)ws, a, eps, act)));                                      \
-    DL_TIMED("gn_join_stats", st, (gn_join_stats<<<dl_ceil_div((long long)B * G, 4), 256, 0, st>>>((const float2 *)ws, (float2 *)stats, a, eps))); \
-    DL_TIMED("gn_apply", st, (gn_apply<T, 16 / sizeof(T), VEC, GN_THREADS><<<blocks_b, GN_THREADS, 0, st>>>(                          \
-        (const T *)x, gamma, beta, ptype, (T *)y, (const float2 *)stats, b, act)))
+    DL_TIMED("gn_stats", st, (gn_stats<T, VEC, GN_THREADS><<<blocks, GN_THREADS, 0, st>>>((const T *)x, (float2 *)ws, s)));           \
+    DL_TIMED("gn_join_stats", st, (gn_join_stats<<<dl_ceil_div((long long)B * G, 4), 256, 0, st>>>((const float2 *)ws, (float2 *)stats, s, eps))); \
+    GN_BY_ACT(act, ACT, DL_TIMED("gn_apply", st, (gn_apply<T, VEC, GN_THREADS, ACT><<<blocks, GN_THREADS, 0, st>>>(                   \
+        (const T *)x, gamma, beta, ptype, (T *)y, (const float2 *)stats, s))))
     DL_BY_TYPE(type, T, if (vec) { FORWARD(true); } else { FORWARD(false); });
 #undef FORWARD
     return dl_launch_status();
@@ -502,7 +741,7 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
 
 extern "C" size_t dl_group_norm_bwd_workspace_bytes(int type, int B, long long P, int C, int G) {
     if (!dl_type_known(type) || !gn_shape_ok(B, P, C, G)) return 0;
-    const GnShape s = gn_sums_shape(B, P, C, G, 16 / dl_type_bytes(type));
+    const GnShape s = gn_pieces_shape(B, P, C, G, 16 / dl_type_bytes(type));
     return dl_align256((size_t)B * s.pieces * 2 * C * sizeof(float)) + dl_align256((size_t)B * 2 * C * sizeof(float)) +
            dl_align256((size_t)B * G * sizeof(float2));
 }
@@ -516,22 +755,41 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     if (ws_bytes < dl_group_norm_bwd_workspace_bytes(type, B, P, C, G)) return DL_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     const int E = 16 / dl_type_bytes(type);
-    const GnShape s = gn_sums_shape(B, P, C, G, E);
-    if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
-    const bool vec = gn_vectors(s, E, x, gy, gx);
-    float *part = (float *)ws;
-    float *channel = (float *)((char *)part + dl_align256((size_t)B * s.pieces * 2 * C * sizeof(float)));
+    float *channel = (float *)ws;
     float2 *group = (float2 *)((char *)channel + dl_align256((size_t)B * 2 * C * sizeof(float)));
-    const int blocks = B * s.tiles * s.pieces;
+    float *part = (float *)((char *)group + dl_align256((size_t)B * G * sizeof(float2)));
+    GnShape s;
+    bool one = false;
+    for (const int threads : {GN_THREADS, GN_ONE_THREADS}) {
+        one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD(E), threads);
+        if (!one) continue;
+        if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+        const bool vec = gn_vectors(s, E, x, gy, gx);
+        dl_prof_begin("gn_backward_one", st);
+#define ONE(VEC, NV, THREADS) \
+    gn_backward_one<T, VEC, NV, THREADS, ACT><<<s.B * s.tiles, THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
+                                                                                 (const float2 *)stats, channel, (T *)gx, s)
+        DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
+                                      else { if (vec) ONE(true, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
+#undef ONE
+        dl_prof_end(st);
+        break;
+    }
+    if (!one) {
+        s = gn_pieces_shape(B, P, C, G, E);
+        if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+        const bool vec = gn_vectors(s, E, x, gy, gx);
+        const int blocks = B * s.tiles * s.pieces;
 #define BACKWARD(VEC)                                                                                                            \
-    DL_TIMED("gn_backward_sums", st, (gn_backward_sums<T, 16 / sizeof(T), VEC, GN_THREADS><<<blocks, GN_THREADS, 0, st>>>(        \
-        (const T *)x, (const T *)gy, gamma, beta, ptype, (const float2 *)stats, part, s, act)));                                  \
+    GN_BY_ACT(act, ACT, DL_TIMED("gn_backward_sums", st, (gn_backward_sums<T, VEC, GN_THREADS, ACT><<<blocks, GN_THREADS, 0, st>>>( \
+        (const T *)x, (const T *)gy, gamma, beta, ptype, (const float2 *)stats, part, s))));                                      \
     DL_TIMED("gn_backward_join", st, (gn_backward_join<<<B * G, 256, 0, st>>>(part, gamma, ptype, channel, group, s)));           \
     if (gx)                                                                                                                       \
-        DL_TIMED("gn_backward_apply", st, (gn_backward_apply<T, 16 / sizeof(T), VEC, GN_THREADS><<<blocks, GN_THREADS, 0, st>>>(  \
-            (const T *)x, (const T *)gy, gamma, beta, ptype, (const float2 *)stats, group, (T *)gx, s, act)))
-    DL_BY_TYPE(type, T, if (vec) { BACKWARD(true); } else { BACKWARD(false); });
+        GN_BY_ACT(act, ACT, DL_TIMED("gn_backward_apply", st, (gn_backward_apply<T, VEC, GN_THREADS, ACT><<<blocks, GN_THREADS, 0, st>>>( \
+            (const T *)x, (const T *)gy, gamma, beta, ptype, (const float2 *)stats, (const float2 *)group, (T *)gx, s))))
+        DL_BY_TYPE(type, T, if (vec) { BACKWARD(true); } else { BACKWARD(false); });
 #undef BACKWARD
+    }
     if (ggamma || gbeta)
         DL_TIMED("gn_param_grads", st, (gn_param_grads<<<dl_ceil_div(C, 32), 256, 0, st>>>(channel, ggamma, gbeta, ptype, B, C)));
     return dl_launch_status();
