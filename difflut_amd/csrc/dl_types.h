@@ -24,15 +24,36 @@ __device__ __forceinline__ void dl_store(T *p, const float (&f)[N]) {
     *reinterpret_cast<DlVec<T, N> *>(p) = t;
 }
 
-// The same past the caches' retention: for results that a launch does not read again and that would push out what it does
+// 16 bytes as they lie in memory (arrays of 16-bit elements would take a register each), and their values
+typedef uint32_t dl_words __attribute__((ext_vector_type(4)));
+template <typename T, int N>
+__device__ __forceinline__ void dl_unpack(dl_words w, float (&f)[N]) {
+    static_assert(sizeof(T) * N == 16, "16 bytes");
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if constexpr (__is_same(T, dl_bf16)) {
+                f[2 * i] = __uint_as_float(w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            } else {
+                f[2 * i] = (float)__builtin_bit_cast(dl_f16, (uint16_t)w[i]);
+                f[2 * i + 1] = (float)__builtin_bit_cast(dl_f16, (uint16_t)(w[i] >> 16));
+            }
+        }
+    }
+}
+
+// A store past the caches' retention: for results that a launch does not read again and that would push out what it does
 template <typename T, int N>
 __device__ __forceinline__ void dl_store_past(T *p, const float (&f)[N]) {
-    typedef uint32_t words __attribute__((ext_vector_type(4)));
     if constexpr (sizeof(T) * N == 16) {
         DlVec<T, N> t;
 #pragma unroll
         for (int i = 0; i < N; ++i) t.v[i] = (T)f[i];
-        __builtin_nontemporal_store(__builtin_bit_cast(words, t), reinterpret_cast<words *>(p));
+        __builtin_nontemporal_store(__builtin_bit_cast(dl_words, t), reinterpret_cast<dl_words *>(p));
     } else {
         dl_store(p, f);
     }

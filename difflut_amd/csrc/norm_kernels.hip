@@ -190,14 +190,20 @@ __device__ void gn_channel_sums(const GnPlace &w, int width, const float (&v)[E]
 }
 
 // ---------------------------------------------------------------------------------- forward
-// E neighbouring elements as they lie in memory (16 bytes)
+// E neighbouring elements as they lie in memory (16 bytes); those past `real` are 0
 template <typename T, int E, bool VEC>
-__device__ __forceinline__ DlVec<T, E> gn_raw(const T *p, int real) {
-    if constexpr (VEC) return *reinterpret_cast<const DlVec<T, E> *>(p);
+__device__ __forceinline__ dl_words gn_raw(const T *p, int real) {
+    if constexpr (VEC) return *reinterpret_cast<const dl_words *>(p);
     DlVec<T, E> t;
 #pragma unroll
     for (int e = 0; e < E; ++e) t.v[e] = e < real ? p[e] : (T)0.0f;
-    return t;
+    return __builtin_bit_cast(dl_words, t);
+}
+// Their values, unpacked anew at every use: kept as floats, two uses' worth would not fit the registers
+template <typename T, int E>
+__device__ __forceinline__ void gn_values(dl_words &w, float (&f)[E]) {
+    asm volatile("" : "+v"(w));
+    dl_unpack<T>(w, f);
 }
 
 // A sample's tile in one block: the values stay in registers from the one read to y.
@@ -212,16 +218,13 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
     const int real = w.c_end - w.c, c0 = w.c - w.col * E;
     const long long base = (long long)b * s.P * s.C + w.c;
     const int P = (int)s.P;
-    DlVec<T, E> v[NV];
+    dl_words v[NV];
     int group[E];
     float t[E], m[E], ga[E], be[E];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int p = w.row0 + i * w.rows;
-        if (w.active && p < P) v[i] = gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real);
-        else
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[i].v[e] = (T)0.0f;
+        v[i] = w.active && p < P ? gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real) : dl_words{0, 0, 0, 0};
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -229,8 +232,13 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
         ga[e] = w.active && e < real ? gn_param(gamma, ptype, w.c + e, 1.0f) : 0.0f;
         be[e] = w.active && e < real ? gn_param(beta, ptype, w.c + e, 0.0f) : 0.0f;
         t[e] = 0.0f;
+    }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) t[e] += (float)v[i].v[e];
+    for (int i = 0; i < NV; ++i) {
+        float f[E];
+        gn_values<T>(v[i], f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) t[e] += f[e];
     }
     gn_group_sums<E, THREADS>(s, w, t, slots, sums);
     const float per = 1.0f / ((float)P * (float)s.cg);
@@ -245,10 +253,12 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
     for (int k = 0; k < E; ++k) mean[k] = (int)(threadIdx.x + k * THREADS) < w.groups ? sums[threadIdx.x + k * THREADS] * per : 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+        float f[E];
+        gn_values<T>(v[i], f);
         if (!w.active || w.row0 + i * w.rows >= P) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float d = e < real ? (float)v[i].v[e] - m[e] : 0.0f;
+            const float d = e < real ? f[e] - m[e] : 0.0f;
             t[e] = fmaf(d, d, t[e]);
         }
     }
@@ -264,10 +274,11 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int p = w.row0 + i * w.rows;
-        if (p >= P) continue;
         float o[E];
+        gn_values<T>(v[i], o);
+        if (p >= P) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = gn_act<ACT>(fmaf((float)v[i].v[e] - m[e], ga[e], be[e]));
+        for (int e = 0; e < E; ++e) o[e] = gn_act<ACT>(fmaf(o[e] - m[e], ga[e], be[e]));
         gn_write<T, E, VEC>(y + base + (long long)p * s.C, real, o);
     }
 }
@@ -404,7 +415,7 @@ __global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__
     const GnPlace w = gn_place<E>(s, tile, 0, THREADS);
     const int real = w.c_end - w.c, c0 = w.c - w.col * E, width = w.c_end - c0, P = (int)s.P;
     const long long base = (long long)b * s.P * s.C + w.c;
-    DlVec<T, E> v[NV], d[NV];
+    dl_words v[NV] = {}, d[NV] = {};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int p = w.row0 + i * w.rows;
@@ -417,11 +428,13 @@ __global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__
     float sg[E] = {}, sx[E] = {};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+        float x_[E], d_[E];
+        gn_values<T>(v[i], x_), gn_values<T>(d[i], d_);
         if (!w.active || w.row0 + i * w.rows >= P) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             float hat, g;
-            ch.template at<ACT>(e, (float)v[i].v[e], (float)d[i].v[e], hat, g);
+            ch.template at<ACT>(e, x_[e], d_[e], hat, g);
             sg[e] += g;
             sx[e] = fmaf(g, hat, sx[e]);
         }
@@ -458,12 +471,13 @@ __global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int p = w.row0 + i * w.rows;
+        float x_[E], o[E];
+        gn_values<T>(v[i], x_), gn_values<T>(d[i], o);
         if (p >= P) continue;
-        float o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             float hat, g;
-            ch.template at<ACT>(e, (float)v[i].v[e], (float)d[i].v[e], hat, g);
+            ch.template at<ACT>(e, x_[e], o[e], hat, g);
             o[e] = ch.rstd[e] * (fmaf(g, ch.ga[e], -ma[e]) - hat * mq[e]);
         }
         gn_write<T, E, VEC>(gx + base + (long long)p * s.C, real, o);
@@ -646,9 +660,9 @@ static int gn_rows_per_step(const GnShape &s, int E, int threads) {
 }
 #define GN_THREADS 256
 #define GN_ONE_THREADS 1024
-// 16-byte units that a thread of the one-block forms holds: 64 values either way, of x or of x and gy (128 spill)
-#define GN_ONE_FORWARD(E) (64 / (E))
-#define GN_ONE_BACKWARD(E) (32 / (E))
+// 16-byte units that a thread of the one-block forms holds, of x, or of x and of gy: about 48 registers (64 spill)
+#define GN_ONE_FORWARD(E) ((E) == 8 ? 10 : 12)
+#define GN_ONE_BACKWARD 6
 
 static GnShape gn_pieces_shape(int B, long long P, int C, int G, int E) {
     GnShape s = gn_tiles(B, P, C, G, E, GN_THREADS);
@@ -761,7 +775,7 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     GnShape s;
     bool one = false;
     for (const int threads : {GN_THREADS, GN_ONE_THREADS}) {
-        one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD(E), threads);
+        one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD, threads);
         if (!one) continue;
         if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
         const bool vec = gn_vectors(s, E, x, gy, gx);
@@ -770,7 +784,7 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     gn_backward_one<T, VEC, NV, THREADS, ACT><<<s.B * s.tiles, THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
                                                                                  (const float2 *)stats, channel, (T *)gx, s)
         DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
-                                      else { if (vec) ONE(true, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
+                                      else { if (vec) ONE(true, GN_ONE_BACKWARD, GN_ONE_THREADS); else ONE(false, GN_ONE_BACKWARD, GN_ONE_THREADS); }));
 #undef ONE
         dl_prof_end(st);
         break;

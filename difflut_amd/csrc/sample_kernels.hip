@@ -7,27 +7,30 @@
 //   The draw: in index order, the first kept one whose running sum of weights exceeds u times the kept sum.
 // T <= 0, p <= 0, k = 1 and m > 1 leave the first alone.  NaN counts as -infinity; a row without a larger logit gives -1.
 //
-// Neighbouring running sums lie close together, so weights are 64-bit integers, round(2^shift w) with shift = 62 - ceil(log2 V), from
-// exponentials in double: sums fit, are exact in any order - blocks and atomics can split them as they like, every run gives the
+// Neighbouring running sums lie close together, so weights are 64-bit integers, round(2^shift w) with shift = min(51, 62 - ceil(log2 V)),
+// from exponentials in double: sums fit, are exact in any order - blocks and atomics can split them as they like, every run gives the
 // same index - and a weight is off by 2^-(shift + 1), 2^-46 at V = 131072.
 //
-// Up to 64 columns: a few lanes per row compare every pair.  Up to SMP_SORTED: a block sorts the row in LDS.  More: the row is
-// split over blocks, four launches:
-//   sample_max      the chunks' largest logits
-//   sample_hist     number and weight of the logits in SMP_BINS classes of (max - l) / T (a monotone function of l)
-//   sample_collect  the classes that the cuts can fall into are known now: weights of the classes before them, by chunk, and a
-//                   list of the indices in them
-//   sample_draw     sorts the list, finds the cut, then the chunk and in it the index.  A list that is too long (many equal
-//                   logits) is searched over the whole row instead.
+// Up to 64 columns: a few lanes per row compare every pair.  Up to SMP_SORTED: a block sorts the row in LDS.  More: a block per row
+// (sample_row), which reads it once into its registers where it fits; or, for few long rows, four launches over pieces of rows
+// (sample_max, sample_hist, sample_collect, sample_draw).  Both go the same way:
+//   - the largest logit;
+//   - number or weight of the logits in SMP_BINS classes of (max - l) / T, a monotone function of l: they say which classes the cuts
+//     fall into;
+//   - the weights of what lies before those classes, piece by piece of the row, and a list of the indices in them (with a small
+//     enough top-k: a list of all that is kept, and no sums over the row);
+//   - the list, sorted, gives the cut; then the piece that the target falls into, then the index.  A list that is too long
+//     (many equal logits) is searched over the whole row instead.
 #include "dl_types.h"
 
 #define SMP_SORTED 4096
 #define SMP_BINS 2048
-#define SMP_BINS_PER_Z 32.0  // classes per unit of (max - l) / T: the last one holds what weighs less than e^-63.9
+#define SMP_BINS_PER_Z 32.0  // classes per unit of (max - l) / T: the last one holds what weighs less than e^-63.9, so nothing
 #define SMP_LIST 4096
 #define SMP_THREADS 256
 #define SMP_DRAW_THREADS 1024
 #define SMP_MAX_CHUNKS 256
+#define SMP_FEW 768  // top-k up to this goes by the threads' largest logits
 
 typedef unsigned long long u64;
 
@@ -51,7 +54,9 @@ struct SampleArgs {
 
 // A row's settings in the form the kernels use
 struct SampleRow {
-    double rT, p, m, u;
+    double scale, p, u;  // log2(e) / T
+    double classes;      // SMP_BINS_PER_Z / T: classes per logit
+    u64 least;           // min-p's weight
     int k;
     bool first_only, cut_k, cut_p;
 };
@@ -61,8 +66,10 @@ __device__ __forceinline__ SampleRow smp_row(const SampleArgs &a, int b) {
     const int k = a.top_k ? a.top_k[b] : a.k;
     const float u = a.uniform[b];
     r.first_only = !(T > 0.0f) || !(p > 0.0f) || !(m <= 1.0f) || k == 1;
-    r.rT = 1.0 / (double)T;
-    r.p = p, r.m = m;
+    r.scale = 1.44269504088896341 / (double)T;
+    r.classes = SMP_BINS_PER_Z / (double)T;
+    r.p = p;
+    r.least = m > 0.0f && m <= 1.0f ? (u64)ceil(ldexp((double)m, a.shift)) : 0;
     r.u = u > 0.0f ? fmin((double)u, 1.0) : 0.0;
     r.cut_k = k > 0 && k < a.V;
     r.k = r.cut_k ? k : a.V;
@@ -80,17 +87,32 @@ __device__ __forceinline__ float smp_logit(uint32_t key) { return __uint_as_floa
 // (key, index) pairs in the row's order: larger ones first
 __device__ __forceinline__ u64 smp_pair(uint32_t key, uint32_t index) { return (u64)key << 32 | (0xFFFFFFFFu - index); }
 
-__device__ __forceinline__ double smp_exp(uint32_t key, uint32_t top, const SampleRow &r) {
-    if (key == top) return 1.0;
-    const double M = smp_logit(top);
-    if (key <= SMP_DEAD || M > 3.5e38) return 0.0;
-    return exp(((double)smp_logit(key) - M) * r.rT);
+// round(2^shift exp((l - max) / T)).  2^y = 2^n 2^f, |f| <= 1/2: 2^f by its polynomial through the Chebyshev nodes of degree 10 (off by
+// 2^-51.5), both roundings to whole numbers by adding a power of two: double instructions, which run at float's rate here.
+// 2^shift at the maximum itself, 0 at -infinity.
+__device__ __forceinline__ u64 smp_fixed(uint32_t key, uint32_t top, const SampleRow &r, int shift) {
+    const float M = smp_logit(top);
+    if (M > 3.4e38f && __builtin_isinf(M)) return key == top ? 1ull << shift : 0;
+    const double y = fmax(((double)smp_logit(key) - (double)M) * r.scale, -1000.0);  // (0 times -infinity, T infinite: -1000)
+    const double n = y + 6755399441055744.0, f = y - (n - 6755399441055744.0);
+    double e = 7.072585949269223e-09;
+    e = fma(e, f, 1.0208690299958306e-07);
+    e = fma(e, f, 1.321544258792169e-06);
+    e = fma(e, f, 1.5252657260200837e-05);
+    e = fma(e, f, 0.0001540353044173605);
+    e = fma(e, f, 0.0013333558230164974);
+    e = fma(e, f, 0.009618129107606888);
+    e = fma(e, f, 0.05550410866444772);
+    e = fma(e, f, 0.24022650695910097);
+    e = fma(e, f, 0.69314718055995);
+    e = fma(e, f, 1.0);
+    const double x = ldexp(e, (int)(uint32_t)__double_as_longlong(n) + shift) + 4503599627370496.0;
+    return (u64)__double_as_longlong(x) & ((1ull << 52) - 1);
 }
-__device__ __forceinline__ u64 smp_fixed(double e, int shift) { return (u64)(ldexp(e, shift) + 0.5); }
 // weight of an index that no cut but min-p takes away
 __device__ __forceinline__ u64 smp_weight(uint32_t key, uint32_t top, const SampleRow &r, int shift) {
-    const double e = smp_exp(key, top, r);
-    return e >= r.m || key == top ? smp_fixed(e, shift) : 0;
+    const u64 w = smp_fixed(key, top, r, shift);
+    return w >= r.least || key == top ? w : 0;
 }
 __device__ __forceinline__ u64 smp_target(const SampleRow &r, u64 total) {  // the running sum that has to be exceeded
     const u64 t = (u64)(r.u * (double)total);
@@ -141,7 +163,7 @@ __device__ __forceinline__ uint32_t smp_max(uint32_t v, u64 *red) {
 }
 // Descending, n a power of two
 template <int THREADS>
-__device__ void smp_sort(u64 *pairs, int n) {
+__device__ __forceinline__ void smp_sort(u64 *pairs, int n) {
     for (int size = 2; size <= n; size <<= 1)
         for (int step = size >> 1; step > 0; step >>= 1) {
             __syncthreads();
@@ -152,6 +174,29 @@ __device__ void smp_sort(u64 *pairs, int n) {
             }
         }
     __syncthreads();
+}
+
+// The same for n pairs of any number (all different; `size` slots, n <= size): few by counting who is larger, without a barrier per
+// step (64 of them: 1 us for 4).
+template <int THREADS>
+__device__ __forceinline__ void smp_order(u64 *pairs, int n) {
+    if (n <= 256) {
+        const u64 mine = (int)threadIdx.x < n ? pairs[threadIdx.x] : 0;
+        int rank = 0;
+        __syncthreads();
+        if ((int)threadIdx.x < n) {
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) rank += pairs[j] > mine;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < n) pairs[rank] = mine;
+        __syncthreads();
+        return;
+    }
+    int size = 512;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += THREADS) pairs[i] = 0;
+    smp_sort<THREADS>(pairs, size);
 }
 
 // ---------------------------------------------------------------------------------- up to 64 columns
@@ -165,8 +210,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pairs(SampleArgs a) {
     uint32_t top = key;
 #pragma unroll
     for (int o = SEG / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, SEG));
-    const double e = r.first_only ? (key == top ? 1.0 : 0.0) : smp_exp(key, top, r);
-    const u64 w = smp_fixed(e, a.shift);
+    const u64 w = r.first_only ? (key == top ? 1ull << a.shift : 0) : smp_fixed(key, top, r, a.shift);
     int rank = 0;
     u64 before = 0;
 #pragma unroll 8
@@ -180,7 +224,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pairs(SampleArgs a) {
 #pragma unroll
     for (int o = SEG / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, SEG);
     const bool in_p = !r.cut_p || (double)before < r.p * (double)sum;
-    const bool keep = alive && (rank == 0 || (!r.first_only && rank < r.k && in_p && e >= r.m));
+    const bool keep = alive && (rank == 0 || (!r.first_only && rank < r.k && in_p && w >= r.least));
     u64 run = keep ? w : 0;
 #pragma unroll
     for (int o = 1; o < SEG; o <<= 1) {
@@ -196,7 +240,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pairs(SampleArgs a) {
 // ---------------------------------------------------------------------------------- a row in LDS
 // In index order, over [i0, i1): the first index whose running sum of kept weights exceeds `target`; a thread per run of indices.
 template <typename T, int THREADS>
-__device__ void smp_draw(const SampleArgs &a, const SampleRow &r, int b, int i0, int i1, u64 cut, uint32_t top, bool draw_rest, u64 target,
+__device__ __forceinline__ void smp_draw(const SampleArgs &a, const SampleRow &r, int b, int i0, int i1, u64 cut, uint32_t top, bool draw_rest, u64 target,
                          u64 *red) {
     const T *row = (const T *)a.logits + b * a.ldl;
     const int per = (i1 - i0 + THREADS - 1) / THREADS, begin = min(i0 + (int)threadIdx.x * per, i1), end = min(begin + per, i1);
@@ -247,13 +291,13 @@ __global__ __launch_bounds__(THREADS) void sample_sorted(SampleArgs a, int n) {
         const int per = max(1, n / THREADS), begin = min((int)threadIdx.x * per, n), end = min(begin + per, n);
         u64 mine = 0, total, kept = 0;
         for (int j = begin; j < end; ++j)
-            if (j < r.k) mine += smp_fixed(smp_exp((uint32_t)(pairs[j] >> 32), top, r), a.shift);
+            if (j < r.k) mine += smp_fixed((uint32_t)(pairs[j] >> 32), top, r, a.shift);
         u64 before = smp_scan<THREADS>(mine, total, red);
         const double limit = r.p * (double)total;
         for (int j = begin; j < end; ++j) {
             const uint32_t key = (uint32_t)(pairs[j] >> 32);
             if (j >= r.k || key <= SMP_DEAD || (j > 0 && r.cut_p && !((double)before < limit))) break;
-            before += smp_fixed(smp_exp(key, top, r), a.shift);
+            before += smp_fixed(key, top, r, a.shift);
             ++kept;
         }
         smp_scan<THREADS>(kept, total, red);
@@ -263,9 +307,34 @@ __global__ __launch_bounds__(THREADS) void sample_sorted(SampleArgs a, int n) {
 }
 
 // ---------------------------------------------------------------------------------- rows split over blocks
-__device__ __forceinline__ int smp_bin(uint32_t key, double M, const SampleRow &r) {
-    return (int)fmin((M - (double)smp_logit(key)) * r.rT * SMP_BINS_PER_Z, (double)(SMP_BINS - 1));
+// The class of a logit: (max - l) / T in 32nds, to the nearest one, and what is left of it (-1/2 .. 1/2; within the last class: anything)
+__device__ __forceinline__ int smp_bin(uint32_t key, uint32_t top, const SampleRow &r, double &rest) {
+    const double M = smp_logit(top), l = smp_logit(key);
+    double y = fmin((M - l) * r.classes, (double)(SMP_BINS - 1));  // (infinity times 0, T infinite: the last class)
+    if (M > 3.5e38) y = key == top ? 0.0 : (double)(SMP_BINS - 1);
+    const double n = y + 6755399441055744.0;
+    rest = y - (n - 6755399441055744.0);
+    return (int)(uint32_t)__double_as_longlong(n);
 }
+__device__ __forceinline__ int smp_bin(uint32_t key, uint32_t top, const SampleRow &r) {
+    double rest;
+    return smp_bin(key, top, r, rest);
+}
+// A class's weight is e^(-class / 32) times the sum of e^(-rest / 32) over its logits; that sum, whose terms lie within 1.6 % of 1, is kept
+// as 2^(62 - ceil(log2 V)) of it: a polynomial of degree 4 (off by 6 2^-44) and no power of two per logit.
+__device__ __forceinline__ u64 smp_class_term(double rest, double unit) {
+    const double d = rest * (-1.0 / SMP_BINS_PER_Z);
+    double e = fma(d, 1.0 / 24.0, 1.0 / 6.0);
+    e = fma(e, d, 0.5);
+    e = fma(e, d, 1.0);
+    e = fma(e, d, 1.0);
+    return (u64)__double_as_longlong(fma(e, unit, 4503599627370496.0)) & ((1ull << 52) - 1);
+}
+__device__ __forceinline__ u64 smp_class_weight(int bin, u64 sum, int shift, int term_shift) {
+    return sum ? (u64)((double)sum * exp(bin * (-1.0 / SMP_BINS_PER_Z)) * ldexp(1.0, shift - term_shift) + 0.5) : 0;
+}
+// terms of 2^term_shift: under 2^52, and their sum under 2^63
+__device__ __forceinline__ int smp_term_shift(const SampleArgs &a) { return a.shift < 51 ? a.shift : 50; }
 template <int THREADS>
 __device__ __forceinline__ uint32_t smp_top(const SampleArgs &a, int b, u64 *red) {
     uint32_t v = 0;
@@ -304,20 +373,20 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_hist(SampleArgs a) {
     __syncthreads();
     const T *row = (const T *)a.logits + b * a.ldl;
     const int i1 = min((c + 1) * (long long)a.chunk, (long long)a.V);
-    const double M = smp_logit(top);
+    const double unit = ldexp(1.0, smp_term_shift(a));
     for (int i = c * a.chunk + threadIdx.x; i < i1; i += SMP_THREADS) {
         const uint32_t key = smp_key((float)row[i]);
         if (key <= SMP_DEAD) continue;
-        const int bin = key == top ? 0 : smp_bin(key, M, r);
-        atomicAdd(&count[bin], 1u);
-        if (bin < SMP_BINS - 1) atomicAdd(&weight[bin], smp_fixed(smp_exp(key, top, r), a.shift));
+        double rest;
+        const int bin = smp_bin(key, top, r, rest);
+        if (r.cut_k) atomicAdd(&count[bin], 1u);
+        if (r.cut_p) atomicAdd(&weight[bin], smp_class_term(rest, unit));
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < SMP_BINS; i += SMP_THREADS)
-        if (count[i]) {
-            atomicAdd(&a.bin_count[(long long)b * SMP_BINS + i], count[i]);
-            if (weight[i]) atomicAdd(&a.bin_weight[(long long)b * SMP_BINS + i], weight[i]);
-        }
+    for (int i = threadIdx.x; i < SMP_BINS; i += SMP_THREADS) {
+        if (count[i]) atomicAdd(&a.bin_count[(long long)b * SMP_BINS + i], count[i]);
+        if (weight[i]) atomicAdd(&a.bin_weight[(long long)b * SMP_BINS + i], weight[i]);
+    }
 }
 
 // Where the cuts can be: the class of the k-th index, the classes of top-p's last one
@@ -329,15 +398,16 @@ struct SampleCut {
 };
 __device__ __forceinline__ bool smp_open(const SampleCut &c, int bin) { return bin == c.k_bin || (bin >= c.p_first && bin <= c.p_last); }
 
+// (count and sum: the row's classes, in LDS or in memory; those that no cut asks for are zero)
 template <int THREADS>
-__device__ SampleCut smp_resolve(const SampleArgs &a, const SampleRow &r, int b, u64 *red, SampleCut *shared) {
+__device__ __forceinline__ SampleCut smp_resolve(const SampleArgs &a, const uint32_t *count, const u64 *sum, const SampleRow &r, u64 *red, SampleCut *shared) {
     constexpr int PER = SMP_BINS / THREADS;
     uint32_t n[PER];
     u64 w[PER], mine_n = 0, mine_w = 0, all_n, all_w;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        n[j] = a.bin_count[(long long)b * SMP_BINS + threadIdx.x * PER + j];
-        w[j] = a.bin_weight[(long long)b * SMP_BINS + threadIdx.x * PER + j];
+        n[j] = count[threadIdx.x * PER + j];
+        w[j] = smp_class_weight(threadIdx.x * PER + j, sum[threadIdx.x * PER + j], a.shift, smp_term_shift(a));
         mine_n += n[j], mine_w += w[j];
     }
     const u64 n0 = smp_scan<THREADS>(mine_n, all_n, red), w0 = smp_scan<THREADS>(mine_w, all_w, red);
@@ -356,7 +426,7 @@ __device__ SampleCut smp_resolve(const SampleArgs &a, const SampleRow &r, int b,
     const int k_bin = shared->k_bin;
     const u64 low = shared->k_weight;
     u64 high = low;
-    if (k_bin < SMP_BINS) high += a.bin_weight[(long long)b * SMP_BINS + k_bin];
+    if (k_bin < SMP_BINS) high += smp_class_weight(k_bin, sum[k_bin], a.shift, smp_term_shift(a));
     if (r.cut_p) {
         cw = w0;
 #pragma unroll
@@ -385,16 +455,15 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_collect(SampleArgs a) {
     if (top <= SMP_DEAD) return;
     const bool cuts = r.cut_k || r.cut_p;
     SampleCut cut = {SMP_BINS, SMP_BINS, SMP_BINS, SMP_BINS, 0, 0, 0};
-    if (cuts) cut = smp_resolve<SMP_THREADS>(a, r, b, red, &shared);
+    if (cuts) cut = smp_resolve<SMP_THREADS>(a, a.bin_count + (long long)b * SMP_BINS, a.bin_weight + (long long)b * SMP_BINS, r, red, &shared);
     const T *row = (const T *)a.logits + b * a.ldl;
     const int i1 = min((c + 1) * (long long)a.chunk, (long long)a.V);
-    const double M = smp_logit(top);
     const int lane = threadIdx.x & 63;
     u64 sum = 0;
     for (int i0 = c * a.chunk; i0 < i1; i0 += SMP_THREADS) {
         const int i = i0 + threadIdx.x;
         const uint32_t key = i < i1 ? smp_key((float)row[i]) : 0;
-        const int bin = key <= SMP_DEAD ? SMP_BINS : key == top ? 0 : smp_bin(key, M, r);
+        const int bin = key <= SMP_DEAD ? SMP_BINS : smp_bin(key, top, r);
         if (bin < cut.sure) sum += smp_weight(key, top, r, a.shift);
         const bool open = bin < SMP_BINS && smp_open(cut, bin);
         const u64 takes = __ballot(open);
@@ -412,28 +481,27 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_collect(SampleArgs a) {
 
 // Sums over the whole row by one block: number and weight of the keys >= `least` (of those in open classes: their extremes)
 template <typename T, int THREADS>
-__device__ void smp_row_sums(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, uint32_t least, u64 &count, u64 &weight, u64 *red) {
+__device__ __forceinline__ void smp_row_sums(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, uint32_t least, u64 &count, u64 &weight, u64 *red) {
     const T *row = (const T *)a.logits + b * a.ldl;
     u64 n = 0, w = 0;
     for (int i = threadIdx.x; i < a.V; i += THREADS) {
         const uint32_t key = smp_key((float)row[i]);
         if (key < least || key <= SMP_DEAD) continue;
         ++n;
-        w += smp_fixed(smp_exp(key, top, r), a.shift);
+        w += smp_fixed(key, top, r, a.shift);
     }
     smp_scan<THREADS>(n, count, red);
     smp_scan<THREADS>(w, weight, red);
 }
 // The least and the largest key in classes [first, last]
 template <typename T, int THREADS>
-__device__ void smp_key_range(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, int first, int last, uint32_t &low, uint32_t &high, u64 *red) {
+__device__ __forceinline__ void smp_key_range(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, int first, int last, uint32_t &low, uint32_t &high, u64 *red) {
     const T *row = (const T *)a.logits + b * a.ldl;
-    const double M = smp_logit(top);
     uint32_t lo = 0, hi = 0;  // (lo: of the complements)
     for (int i = threadIdx.x; i < a.V; i += THREADS) {
         const uint32_t key = smp_key((float)row[i]);
         if (key <= SMP_DEAD) continue;
-        const int bin = key == top ? 0 : smp_bin(key, M, r);
+        const int bin = smp_bin(key, top, r);
         if (bin < first || bin > last) continue;
         hi = max(hi, key), lo = max(lo, ~key);
     }
@@ -443,7 +511,7 @@ __device__ void smp_key_range(const SampleArgs &a, const SampleRow &r, int b, ui
 
 // The cut of a row whose open classes hold more than the list: by bisection over the keys, then over equal ones by index.
 template <typename T, int THREADS>
-__device__ u64 smp_search(const SampleArgs &a, const SampleRow &r, const SampleCut &c, int b, uint32_t top, u64 *red) {
+__device__ __forceinline__ u64 smp_search(const SampleArgs &a, const SampleRow &r, const SampleCut &c, int b, uint32_t top, u64 *red) {
     uint32_t lo, hi, cut_key = SMP_DEAD + 1;
     u64 n, w, ties = ~0ull, sum = c.k_weight;  // the indices kept among those with cut_key; the weight under top-k
     if (c.k_bin < SMP_BINS) {
@@ -457,7 +525,7 @@ __device__ u64 smp_search(const SampleArgs &a, const SampleRow &r, const SampleC
         cut_key = lo;
         smp_row_sums<T, THREADS>(a, r, b, top, lo + 1, n, w, red);
         ties = (u64)r.k - n;
-        sum = w + ties * smp_fixed(smp_exp(lo, top, r), a.shift);
+        sum = w + ties * smp_fixed(lo, top, r, a.shift);
     }
     if (r.cut_p && c.p_first < SMP_BINS) {
         const double limit = r.p * (double)sum;
@@ -470,7 +538,7 @@ __device__ u64 smp_search(const SampleArgs &a, const SampleRow &r, const SampleC
             else hi = mid - 1;
         }
         smp_row_sums<T, THREADS>(a, r, b, top, lo + 1, n, w, red);
-        const u64 each = smp_fixed(smp_exp(lo, top, r), a.shift);
+        const u64 each = smp_fixed(lo, top, r, a.shift);
         u64 take = each ? (u64)fmax((limit - (double)w) / (double)each, 0.0) : 0;
         while (each && (double)(w + take * each) < limit) ++take;
         while (take > 1 && !((double)(w + (take - 1) * each) < limit)) --take;
@@ -495,6 +563,42 @@ __device__ u64 smp_search(const SampleArgs &a, const SampleRow &r, const SampleC
     const u64 cut = red[0];
     __syncthreads();
     return cut;
+}
+
+// The cut from the list of the n indices in open classes (from `list`, or in pairs already where that is null): sorted into pairs, the
+// first `kept` of them stay.
+template <int THREADS>
+__device__ __forceinline__ u64 smp_list_cut(const SampleArgs &a, const SampleRow &r, const SampleCut &c, uint32_t top, u64 *pairs, int n, const u64 *list,
+                            u64 *red, u64 &cut) {
+    if (list)
+        for (int i = threadIdx.x; i < n; i += THREADS) pairs[i] = list[i];
+    __syncthreads();
+    smp_order<THREADS>(pairs, n);
+    // in order: classes [p_first, p_last], then k_bin where that is another one
+    const int per = (n + THREADS - 1) / THREADS, begin = min((int)threadIdx.x * per, n), end = min(begin + per, n);
+    u64 in_k = 0, k_from = 0, kept = 0, mine = 0, total;
+    for (int j = begin; j < end; ++j) k_from += smp_bin((uint32_t)(pairs[j] >> 32), top, r) != c.k_bin;  // entries before the k-th's class
+    smp_scan<THREADS>(k_from, total, red);
+    k_from = total;
+    const u64 k_end = c.k_bin < SMP_BINS ? k_from + ((u64)r.k - c.k_before) : (u64)n;  // list entries that top-k keeps
+    for (int j = begin; j < end; ++j) {
+        const u64 w = smp_fixed((uint32_t)(pairs[j] >> 32), top, r, a.shift);
+        if ((u64)j >= k_from && (u64)j < k_end) in_k += w;
+        mine += w;
+    }
+    smp_scan<THREADS>(in_k, total, red);
+    const double limit = r.p * (double)(c.k_weight + total);
+    u64 before = smp_scan<THREADS>(mine, total, red) + c.p_weight;
+    for (int j = begin; j < end; ++j) {
+        const uint32_t key = (uint32_t)(pairs[j] >> 32);
+        const bool in_p = !r.cut_p || (smp_bin(key, top, r) <= c.p_last && ((double)before < limit || (j == 0 && c.p_weight == 0)));
+        if ((u64)j >= k_end || !in_p) break;
+        before += smp_fixed(key, top, r, a.shift);
+        ++kept;
+    }
+    smp_scan<THREADS>(kept, total, red);
+    cut = total ? pairs[total - 1] : pairs[0] + 1;
+    return total;
 }
 
 template <typename T>
@@ -527,7 +631,7 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_draw(SampleArgs a) {
     for (int c = threadIdx.x; c < a.chunks; c += THREADS) chunk_sum[c] = a.chunk_sum[(long long)b * a.chunks + c];
     u64 cut = (u64)(SMP_DEAD + 1) << 32, total;
     if (r.cut_k || r.cut_p) {
-        const SampleCut c = smp_resolve<THREADS>(a, r, b, red, &shared);
+        const SampleCut c = smp_resolve<THREADS>(a, a.bin_count + (long long)b * SMP_BINS, a.bin_weight + (long long)b * SMP_BINS, r, red, &shared);
         const uint32_t n = a.listed[b];
         if (n > SMP_LIST) {
             cut = smp_search<T, THREADS>(a, r, c, b, top, red);
@@ -543,39 +647,8 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_draw(SampleArgs a) {
                 if ((threadIdx.x & 63) == 0) chunk_sum[q] = sum;
             }
         } else if (n > 0) {
-            int size = 1;
-            while (size < (int)n) size <<= 1;
-            for (int i = threadIdx.x; i < size; i += THREADS) pairs[i] = i < (int)n ? a.list[(long long)b * SMP_LIST + i] : 0;
-            smp_sort<THREADS>(pairs, size);
-            const double M = smp_logit(top);
-            // the list in order: classes [p_first, p_last], then k_bin where that is another one
-            const int per = max(1, size / THREADS), begin = min((int)threadIdx.x * per, (int)n), end = min(begin + per, (int)n);
-            u64 in_k = 0, k_from = 0, kept = 0, mine = 0;
-            for (int j = begin; j < end; ++j) {  // entries before the k-th's class
-                const uint32_t key = (uint32_t)(pairs[j] >> 32);
-                k_from += (key == top ? 0 : smp_bin(key, M, r)) != c.k_bin;
-            }
-            smp_scan<THREADS>(k_from, k_from, red);
-            const u64 k_end = c.k_bin < SMP_BINS ? k_from + ((u64)r.k - c.k_before) : n;  // list entries that top-k keeps
-            for (int j = begin; j < end; ++j) {
-                const u64 w = smp_fixed(smp_exp((uint32_t)(pairs[j] >> 32), top, r), a.shift);
-                if ((u64)j >= k_from && (u64)j < k_end) in_k += w;
-                mine += w;
-            }
-            smp_scan<THREADS>(in_k, total, red);
-            const double limit = r.p * (double)(c.k_weight + total);
-            u64 before = smp_scan<THREADS>(mine, total, red) + c.p_weight;
-            for (int j = begin; j < end; ++j) {
-                const uint32_t key = (uint32_t)(pairs[j] >> 32);
-                const int bin = key == top ? 0 : smp_bin(key, M, r);
-                const bool in_p = !r.cut_p || (bin <= c.p_last && ((double)before < limit || (j == 0 && c.p_weight == 0)));
-                if ((u64)j >= k_end || !in_p) break;
-                before += smp_fixed(smp_exp(key, top, r), a.shift);
-                ++kept;
-            }
-            smp_scan<THREADS>(kept, total, red);
-            cut = total ? pairs[total - 1] : pairs[0] + 1;
-            for (int j = threadIdx.x; j < (int)total; j += THREADS) {
+            const u64 kept = smp_list_cut<THREADS>(a, r, c, top, pairs, (int)n, a.list + (long long)b * SMP_LIST, red, cut);
+            for (int j = threadIdx.x; j < (int)kept; j += THREADS) {
                 const u64 w = smp_weight((uint32_t)(pairs[j] >> 32), top, r, a.shift);
                 if (w) atomicAdd(&chunk_sum[(0xFFFFFFFFu - (uint32_t)pairs[j]) / a.chunk], w);
             }
@@ -589,6 +662,331 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_draw(SampleArgs a) {
     __syncthreads();
     const int c = chosen;
     smp_draw<T, THREADS>(a, r, b, c * a.chunk, (int)min((c + 1) * (long long)a.chunk, (long long)a.V), cut, top, true, shared.k_weight, red);
+}
+
+// ---------------------------------------------------------------------------------- a block per row
+// A list in LDS that wavefronts append to; `size` counts what did not fit as well
+__device__ __forceinline__ void smp_append(u64 *list, uint32_t *size, bool take, u64 pair) {
+    const u64 takes = __ballot(take);
+    if (!take) return;
+    const int lane = threadIdx.x & 63, leader = __builtin_ctzll(takes);
+    uint32_t at = 0;
+    if (lane == leader) at = atomicAdd(size, (uint32_t)__popcll(takes));
+    at = (uint32_t)__builtin_amdgcn_readlane((int)at, leader) + __popcll(takes & ((1ull << lane) - 1));
+    if (at < SMP_LIST) list[at] = pair;
+}
+
+// A row's elements, 16 bytes at a time: a wavefront takes a run of units, NR per thread in registers, or (NR = 0) read again for every
+// pass.  The up to E - 1 elements before the first whole unit and behind the last one are single ones.
+template <typename T, int NR>
+struct SampleReader {
+    static constexpr int E = 16 / sizeof(T), THREADS = SMP_DRAW_THREADS;
+    const T *row;
+    int V, head, units, run;  // units of a wavefront (whole groups of 64)
+    dl_words raw[NR > 0 ? NR : 1];
+
+    __device__ __forceinline__ SampleReader(const T *row, int V) : row(row), V(V) {
+        head = min((int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T), V);
+        units = (V - head) / E;
+        run = (units + THREADS - 1) / THREADS * 64;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (i * 64 < run && first() + i * 64 < units) raw[i] = unit(first() + i * 64);
+    }
+    __device__ __forceinline__ dl_words unit(int j) const { return *reinterpret_cast<const dl_words *>(row + head + j * E); }
+    __device__ __forceinline__ int first() const { return (threadIdx.x >> 6) * run + (threadIdx.x & 63); }
+    // f(unit number, values, whether the thread has one), by all threads of a wavefront.  The units go through the loop by turns of
+    // the registers: one copy of f's code, whose exponentials would fill the registers in unrolled ones.
+    template <int N, typename F>
+    __device__ __forceinline__ void by_turns(dl_words (&v)[N], int i0, F f) const {
+#pragma unroll 1
+        for (int u = 0; u < N; ++u) {
+            const dl_words now = v[0];
+#pragma unroll
+            for (int k = 0; k + 1 < N; ++k) v[k] = v[k + 1];
+            v[N - 1] = now;
+            const int i = i0 + u * 64, j = first() + i;
+            if (i < run) {
+                float values[E];
+                dl_unpack<T>(now, values);
+                f(j, values, j < units);
+            }
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void units_of(F f) {
+        if constexpr (NR > 0) {
+            by_turns(raw, 0, f);
+        } else {
+            constexpr int AHEAD = 4;  // units in flight while as many are worked on
+            dl_words v[AHEAD], next[AHEAD];
+            const auto fetch = [&](dl_words (&to)[AHEAD], int i0) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int i = i0 + u * 64;
+                    if (i < run && first() + i < units) to[u] = unit(first() + i);
+                }
+            };
+            fetch(v, 0);
+#pragma unroll 1
+            for (int i0 = 0; i0 < run; i0 += AHEAD * 64) {
+                fetch(next, i0 + AHEAD * 64);
+                by_turns(v, i0, f);
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) v[u] = next[u];
+            }
+        }
+    }
+    // the single element of a thread: its index, or -1
+    __device__ __forceinline__ int single() const {
+        const int t = threadIdx.x, tail = head + units * E;
+        return t < head ? t : tail + (t - head) < V ? tail + (t - head) : -1;
+    }
+    // the thread's largest element, as a key
+    __device__ __forceinline__ uint32_t largest() {
+        const int i = single();
+        float m = i >= 0 ? fmaxf((float)row[i], -INFINITY) : -INFINITY;  // (the larger of a NaN and a number is the number)
+        units_of([&](int, const float (&v)[E], bool has) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) m = has ? fmaxf(m, v[e]) : m;
+        });
+        return smp_key(m);
+    }
+    // f(key, index) for every element
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
+        const int i = single();
+        if (i >= 0) f(smp_key((float)row[i]), i);
+        units_of([&](int j, const float (&v)[E], bool has) {
+            if (!has) return;
+#pragma unroll
+            for (int e = 0; e < E; ++e) f(smp_key(v[e]), head + j * E + e);
+        });
+    }
+    // Appends the elements that take(value) says (not a NaN) to a list in LDS; `size` counts what does not fit as well
+    template <typename F>
+    __device__ __forceinline__ void list(u64 *pairs, uint32_t *size, F take) {
+        const int i = single();
+        const float l = i >= 0 ? (float)row[i] : 0.0f;
+        smp_append(pairs, size, i >= 0 && take(l), smp_pair(smp_key(l), i));
+        units_of([&](int j, const float (&v)[E], bool has) {
+            uint32_t mask = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) mask |= (uint32_t)(has && take(v[e])) << e;
+            if (__ballot(mask != 0) == 0) return;
+#pragma unroll
+            for (int e = 0; e < E; ++e) smp_append(pairs, size, mask >> e & 1, smp_pair(smp_key(v[e]), head + j * E + e));
+        });
+    }
+};
+
+// The least key (above -infinity) of a class or a lower one: classes go down as keys go up.  32 steps, by every thread alike.
+__device__ __forceinline__ uint32_t smp_first_key(int bin, uint32_t top, const SampleRow &r) {
+    uint32_t lo = SMP_DEAD + 1, hi = top;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (smp_bin(mid, top, r) <= bin) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// All that top-k keeps is in the list of n: the cuts, and the draw.
+template <int THREADS>
+__device__ __forceinline__ void smp_list_draw(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, u64 *pairs, int n, u64 *red) {
+    smp_order<THREADS>(pairs, n);
+    n = min(n, r.k);
+    const int per = (n + THREADS - 1) / THREADS, begin = min((int)threadIdx.x * per, n), end = min(begin + per, n);
+    u64 mine = 0, total, kept = 0;
+    for (int j = begin; j < end; ++j) mine += smp_fixed((uint32_t)(pairs[j] >> 32), top, r, a.shift);
+    u64 before = smp_scan<THREADS>(mine, total, red);
+    const double limit = r.p * (double)total;
+    for (int j = begin; j < end; ++j) {
+        const u64 w = smp_fixed((uint32_t)(pairs[j] >> 32), top, r, a.shift);
+        if (j > 0 && ((r.cut_p && !((double)before < limit)) || (w < r.least && (uint32_t)(pairs[j] >> 32) != top))) break;
+        before += w;
+        ++kept;
+    }
+    smp_scan<THREADS>(kept, total, red);
+    n = (int)total;
+    // what is left in index order: the halves of the pairs change places
+    for (int j = threadIdx.x; j < n; j += THREADS) pairs[j] = pairs[j] << 32 | pairs[j] >> 32;
+    __syncthreads();
+    smp_order<THREADS>(pairs, n);
+    const int per_n = (n + THREADS - 1) / THREADS, first = min((int)threadIdx.x * per_n, n), last = min(first + per_n, n);
+    mine = 0;
+    for (int j = first; j < last; ++j) mine += smp_fixed((uint32_t)pairs[j], top, r, a.shift);
+    u64 run = smp_scan<THREADS>(mine, total, red);
+    const u64 target = smp_target(r, total);
+    if (run <= target && target < run + mine)
+        for (int j = first; j < last; ++j) {
+            run += smp_fixed((uint32_t)pairs[j], top, r, a.shift);
+            if (run > target) {
+                a.out[b] = (long long)(0xFFFFFFFFu - (uint32_t)(pairs[j] >> 32));
+                break;
+            }
+        }
+}
+
+template <typename T, int NR>
+__global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
+    constexpr int THREADS = SMP_DRAW_THREADS, E = 16 / sizeof(T), WAVES = THREADS / 64;
+    __shared__ u64 weight[SMP_BINS], pairs[SMP_LIST], red[WAVES], slot[WAVES + 2], left;
+    __shared__ uint32_t count[SMP_BINS], limit[4], listed, least;
+    __shared__ SampleCut shared;
+    __shared__ int chosen;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    SampleReader<T, NR> row((const T *)a.logits + b * a.ldl, a.V);
+    const SampleRow r = smp_row(a, b);
+    if (threadIdx.x == 0) listed = 0;
+    const uint32_t own = row.largest();
+    const uint32_t top = smp_max<THREADS>(own, red);
+    if (top <= SMP_DEAD) {
+        if (threadIdx.x == 0) a.out[b] = -1;
+        return;
+    }
+    if (r.first_only) {
+        uint32_t low = 0;
+        row.each([&](uint32_t key, int i) { low = key == top ? max(low, ~(uint32_t)i) : low; });
+        low = smp_max<THREADS>(low, red);
+        if (threadIdx.x == 0) a.out[b] = (long long)(uint32_t)~low;
+        return;
+    }
+    if (r.cut_k && r.k <= SMP_FEW) {
+        // k of the threads' largest logits reach some number, so at least k logits do, and hardly more: every thread has the largest of
+        // its own.  A wavefront looks for that number, by bisection.
+        count[threadIdx.x] = own;
+        __syncthreads();
+        if (wave == 0) {
+            uint32_t v[WAVES], most = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) v[w] = count[w * 64 + lane], most = max(most, v[w]);
+            uint32_t lo = r.k <= 64 ? ~smp_wave_max(~most) : 0, hi = top;  // 64 reach the least of the lanes' largest
+            while (lo < hi) {
+                const uint32_t mid = lo + (hi - lo) / 2 + 1;
+                int n = 0;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) n += __popcll(__ballot(v[w] >= mid));
+                if (n >= r.k) lo = mid;
+                else hi = mid - 1;
+                if (n >= r.k && n <= r.k + r.k / 8) break;
+            }
+            if (lane == 0) least = max(lo, SMP_DEAD + 1);
+        }
+        __syncthreads();
+        const float from = smp_logit(least);
+        row.list(pairs, &listed, [&](float l) { return l >= from; });
+        __syncthreads();
+        const uint32_t n = listed;
+        if (n <= SMP_LIST) {
+            smp_list_draw<THREADS>(a, r, b, top, pairs, (int)n, red);
+            return;
+        }
+        __syncthreads();  // (many equal ones)
+        if (threadIdx.x == 0) listed = 0;
+    }
+    for (int i = threadIdx.x; i < SMP_BINS; i += THREADS) weight[i] = 0, count[i] = 0;
+    __syncthreads();
+    SampleCut c = {SMP_BINS, SMP_BINS, SMP_BINS, SMP_BINS, 0, 0, 0};
+    if (r.cut_k) {
+        row.each([&](uint32_t key, int) {
+            if (key > SMP_DEAD) atomicAdd(&count[smp_bin(key, top, r)], 1u);
+        });
+        __syncthreads();
+        SampleRow only_k = r;
+        only_k.cut_p = false;
+        c = smp_resolve<THREADS>(a, count, weight, only_k, red, &shared);
+        if (c.k_bin < SMP_BINS && c.k_before + count[c.k_bin] <= SMP_LIST) {  // all that top-k keeps fits the list
+            const float from = smp_logit(smp_first_key(c.k_bin, top, r));
+            row.list(pairs, &listed, [&](float l) { return l >= from; });
+            __syncthreads();
+            smp_list_draw<THREADS>(a, r, b, top, pairs, (int)listed, red);
+            return;
+        }
+    }
+    if (r.cut_p) {
+        const double unit = ldexp(1.0, smp_term_shift(a));
+        row.each([&](uint32_t key, int) {
+            double rest;
+            const int bin = smp_bin(key, top, r, rest);
+            if (key > SMP_DEAD) atomicAdd(&weight[bin], smp_class_term(rest, unit));
+        });
+        __syncthreads();
+        c = smp_resolve<THREADS>(a, count, weight, r, red, &shared);
+    }
+    // Pieces of the row in index order: the elements before the first unit, the wavefronts' runs of units, those behind.
+    const auto slot_of = [&](int i) { return i < row.head ? 0 : i >= row.head + row.units * E ? WAVES + 1 : (i - row.head) / (row.run * E) + 1; };
+    if (threadIdx.x < WAVES + 2) slot[threadIdx.x] = 0;
+    // the classes' limits as logits: kept for certain from `sure` on, open are those of [p_from, sure) down to top-p's last class and [k_from, k_to)
+    if (wave < 4) {
+        const int bin = wave == 0 ? c.sure - 1 : wave == 1 ? c.p_last : wave == 2 ? c.k_bin - 1 : c.k_bin;
+        const uint32_t key = bin < 0 ? top + 1 : bin >= SMP_BINS - 1 ? SMP_DEAD + 1 : smp_first_key(bin, top, r);
+        if (lane == 0) limit[wave] = key;
+    }
+    __syncthreads();
+    // (top + 1 of an infinite maximum is a NaN, which nothing reaches)
+    const float sure = smp_logit(limit[0]), p_from = c.p_first < SMP_BINS ? smp_logit(limit[1]) : INFINITY,
+                k_to = smp_logit(limit[2]), k_from = c.k_bin < SMP_BINS ? smp_logit(limit[3]) : INFINITY;
+    const auto is_sure = [&](float l) { return l >= sure; };
+    const auto is_open = [&](float l) { return !(l >= sure) && ((c.p_first < SMP_BINS && l >= p_from) || (c.k_bin < SMP_BINS && l >= k_from && !(l >= k_to))); };
+    {
+        const int i = row.single();
+        const float l = i >= 0 ? (float)row.row[i] : -INFINITY;
+        if (is_sure(l)) atomicAdd(&slot[slot_of(i)], smp_weight(smp_key(l), top, r, a.shift));
+        smp_append(pairs, &listed, is_open(l), smp_pair(smp_key(l), i));
+    }
+    u64 sum = 0;
+    row.units_of([&](int j, const float (&v)[E], bool has) {
+        uint32_t kept = 0, open = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) kept |= (uint32_t)(has && is_sure(v[e])) << e, open |= (uint32_t)(has && is_open(v[e])) << e;
+        // (few of a nucleus' lanes have more than one: a turn for the lanes' first ones, then for the second ones)
+        while (__ballot(kept != 0)) {
+            float l = v[0];
+            const int at = __builtin_ctz(kept | 1u << E);
+#pragma unroll
+            for (int e = 1; e < E; ++e) l = at == e ? v[e] : l;
+            if (kept) sum += smp_weight(smp_key(l), top, r, a.shift);
+            kept &= kept - 1;
+        }
+        if (__ballot(open != 0))
+#pragma unroll
+            for (int e = 0; e < E; ++e) smp_append(pairs, &listed, open >> e & 1, smp_pair(smp_key(v[e]), row.head + j * E + e));
+    });
+    sum = smp_wave_sum(sum);
+    if (lane == 0) slot[wave + 1] = sum;
+    __syncthreads();
+    u64 cut = (u64)(SMP_DEAD + 1) << 32, total;
+    const uint32_t n = listed;
+    if (n > SMP_LIST) {
+        cut = smp_search<T, THREADS>(a, r, c, b, top, red);
+        if (threadIdx.x < WAVES + 2) slot[threadIdx.x] = 0;
+        __syncthreads();
+        sum = 0;
+        row.units_of([&](int j, const float (&v)[E], bool has) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (has && smp_pair(smp_key(v[e]), row.head + j * E + e) >= cut) sum += smp_weight(smp_key(v[e]), top, r, a.shift);
+        });
+        sum = smp_wave_sum(sum);
+        if (lane == 0) slot[wave + 1] = sum;
+        const int i = row.single();
+        if (i >= 0 && smp_pair(smp_key((float)row.row[i]), i) >= cut) atomicAdd(&slot[slot_of(i)], smp_weight(smp_key((float)row.row[i]), top, r, a.shift));
+    } else if (n > 0) {
+        const u64 kept = smp_list_cut<THREADS>(a, r, c, top, pairs, (int)n, nullptr, red, cut);
+        for (int j = threadIdx.x; j < (int)kept; j += THREADS) {
+            const u64 w = smp_weight((uint32_t)(pairs[j] >> 32), top, r, a.shift);
+            if (w) atomicAdd(&slot[slot_of((int)(0xFFFFFFFFu - (uint32_t)pairs[j]))], w);
+        }
+    }
+    __syncthreads();
+    const u64 mine = threadIdx.x < WAVES + 2 ? slot[threadIdx.x] : 0, before = smp_scan<THREADS>(mine, total, red);
+    const u64 target = smp_target(r, total);
+    if (before <= target && target < before + mine) chosen = threadIdx.x, left = target - before;
+    __syncthreads();
+    const int piece = chosen, last = row.head + row.units * E;
+    const int i0 = piece == 0 ? 0 : piece == WAVES + 1 ? last : row.head + (piece - 1) * row.run * E;
+    smp_draw<T, THREADS>(a, r, b, i0, piece == 0 ? row.head : piece == WAVES + 1 ? a.V : min(i0 + row.run * E, last), cut, top, true, left, red);
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -618,8 +1016,11 @@ static size_t smp_layout(SampleArgs &a, char *ws) {
     return at;
 }
 
+// A block per row: its time is that of V / 1024 logits per thread, whatever the number of rows up to the card's 256 CUs.
+static bool smp_by_row(int B, int V) { return V <= 65536 || B >= 32; }
+
 extern "C" size_t dl_sample_workspace_bytes(int B, int V) {
-    if (B <= 0 || V <= SMP_SORTED) return 0;
+    if (B <= 0 || V <= SMP_SORTED || smp_by_row(B, V)) return 0;
     SampleArgs a = {};
     a.B = B, a.V = V;
     return smp_layout(a, nullptr);
@@ -642,7 +1043,7 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
     a.T = temperature_all, a.k = top_k_all, a.p = top_p_all, a.m = min_p_all, a.out = out, a.B = B, a.V = V;
     int bits = 0;
     while ((1LL << bits) < V) ++bits;
-    a.shift = 62 - bits;
+    a.shift = 62 - bits < 51 ? 62 - bits : 51;
     if (V <= 64) {
         const int seg = V <= 8 ? 8 : V <= 16 ? 16 : V <= 32 ? 32 : 64;
         const long long blocks = ((long long)B * seg + SMP_THREADS - 1) / SMP_THREADS;
@@ -660,6 +1061,15 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
         dl_prof_begin("sample_sorted", s);
         DL_BY_TYPE(type, T, if (n <= 1024) sample_sorted<T, 256><<<B, 256, n * sizeof(u64), s>>>(a, n);
                    else sample_sorted<T, 1024><<<B, 1024, n * sizeof(u64), s>>>(a, n));
+        dl_prof_end(s);
+        return dl_launch_status();
+    }
+    if (smp_by_row(B, V)) {
+        const int units = dl_ceil_div(V / (16 / dl_type_bytes(type)), SMP_DRAW_THREADS);  // of a thread
+        dl_prof_begin("sample_row", s);
+#define ROW(NR) sample_row<T, NR><<<B, SMP_DRAW_THREADS, 0, s>>>(a)
+        DL_BY_TYPE(type, T, if (units <= 2) ROW(2); else ROW(0));
+#undef ROW
         dl_prof_end(s);
         return dl_launch_status();
     }
