@@ -30,6 +30,8 @@
 #define SMP_THREADS 256
 #define SMP_DRAW_THREADS 1024
 #define SMP_MAX_CHUNKS 256
+#define SMP_GATHER 320  // logits that a wavefront gathers: fewer than 64 left and 4 of every lane
+#define SMP_FEW_LISTED 128
 #define SMP_FEW 768  // top-k up to this goes by the threads' largest logits
 
 typedef unsigned long long u64;
@@ -245,9 +247,12 @@ __device__ __forceinline__ void smp_draw(const SampleArgs &a, const SampleRow &r
     const T *row = (const T *)a.logits + b * a.ldl;
     const int per = (i1 - i0 + THREADS - 1) / THREADS, begin = min(i0 + (int)threadIdx.x * per, i1), end = min(begin + per, i1);
     u64 mine = 0, total;
-    for (int i = begin; i < end; ++i) {
-        const uint32_t key = smp_key((float)row[i]);
-        if (smp_pair(key, i) >= cut) mine += smp_weight(key, top, r, a.shift);
+    // 16 at a time: which of them are kept, then their weights, the lanes' first ones together
+    for (int i0 = begin; i0 < end; i0 += 16) {
+        uint32_t kept = 0;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) kept |= (uint32_t)(i0 + u < end && smp_pair(smp_key((float)row[i0 + u < end ? i0 + u : begin]), i0 + u) >= cut) << u;
+        for (; kept; kept &= kept - 1) mine += smp_weight(smp_key((float)row[i0 + __builtin_ctz(kept)]), top, r, a.shift);
     }
     u64 run = smp_scan<THREADS>(mine, total, red);
     if (!draw_rest) target = total ? smp_target(r, total) : 0;
@@ -255,15 +260,29 @@ __device__ __forceinline__ void smp_draw(const SampleArgs &a, const SampleRow &r
         if (threadIdx.x == 0) a.out[b] = -1;
         return;
     }
-    if (run <= target && target < run + mine)
-        for (int i = begin; i < end; ++i) {
-            const uint32_t key = smp_key((float)row[i]);
-            if (smp_pair(key, i) >= cut) run += smp_weight(key, top, r, a.shift);
-            if (run > target) {
-                a.out[b] = i;
-                break;
-            }
+    // in the run of the thread that it falls into: a wavefront, an index a lane
+    __shared__ int chosen;
+    __shared__ u64 chosen_run;
+    if (run <= target && target < run + mine) chosen = begin, chosen_run = run;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    run = chosen_run;
+    for (int i = chosen + (int)threadIdx.x;; i += 64) {
+        const uint32_t key = i < i1 ? smp_key((float)row[i]) : 0;
+        u64 up, sum = i < i1 && smp_pair(key, i) >= cut ? smp_weight(key, top, r, a.shift) : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            up = __shfl_up(sum, o);
+            if ((int)threadIdx.x >= o) sum += up;
         }
+        const u64 past = __ballot(run + sum > target);
+        if (past) {
+            if ((int)threadIdx.x == __builtin_ctzll(past)) a.out[b] = i;
+            return;
+        }
+        run += __shfl(sum, 63);
+        if (i - (int)threadIdx.x + 64 >= i1) return;
+    }
 }
 
 template <typename T, int THREADS>
@@ -308,13 +327,20 @@ __global__ __launch_bounds__(THREADS) void sample_sorted(SampleArgs a, int n) {
 
 // ---------------------------------------------------------------------------------- rows split over blocks
 // The class of a logit: (max - l) / T in 32nds, to the nearest one, and what is left of it (-1/2 .. 1/2; within the last class: anything)
-__device__ __forceinline__ int smp_bin(uint32_t key, uint32_t top, const SampleRow &r, double &rest) {
-    const double M = smp_logit(top), l = smp_logit(key);
-    double y = fmin((M - l) * r.classes, (double)(SMP_BINS - 1));  // (infinity times 0, T infinite: the last class)
-    if (M > 3.5e38) y = key == top ? 0.0 : (double)(SMP_BINS - 1);
+// (of a finite maximum; -infinity and NaN are of the last class)
+__device__ __forceinline__ int smp_class(float l, double M, const SampleRow &r, double &rest) {
+    const double y = fmin((M - (double)l) * r.classes, (double)(SMP_BINS - 1));  // (infinity times 0, T infinite: the last class)
     const double n = y + 6755399441055744.0;
     rest = y - (n - 6755399441055744.0);
     return (int)(uint32_t)__double_as_longlong(n);
+}
+__device__ __forceinline__ int smp_bin(uint32_t key, uint32_t top, const SampleRow &r, double &rest) {
+    const float M = smp_logit(top);
+    if (__builtin_isinf(M)) {  // only its equals weigh anything
+        rest = 0.0;
+        return key == top ? 0 : SMP_BINS - 1;
+    }
+    return smp_class(smp_logit(key), (double)M, r, rest);
 }
 __device__ __forceinline__ int smp_bin(uint32_t key, uint32_t top, const SampleRow &r) {
     double rest;
@@ -676,65 +702,48 @@ __device__ __forceinline__ void smp_append(u64 *list, uint32_t *size, bool take,
     if (at < SMP_LIST) list[at] = pair;
 }
 
-// A row's elements, 16 bytes at a time: a wavefront takes a run of units, NR per thread in registers, or (NR = 0) read again for every
-// pass.  The up to E - 1 elements before the first whole unit and behind the last one are single ones.
-template <typename T, int NR>
+// A row's elements, 16 bytes at a time: a wavefront takes a run of units.  The up to E - 1 elements before the first whole unit and behind
+// the last one are single ones.  (Rows are read again for every pass, mostly from the L2: held in registers they left too few of those.)
+template <typename T>
 struct SampleReader {
     static constexpr int E = 16 / sizeof(T), THREADS = SMP_DRAW_THREADS;
     const T *row;
     int V, head, units, run;  // units of a wavefront (whole groups of 64)
-    dl_words raw[NR > 0 ? NR : 1];
 
     __device__ __forceinline__ SampleReader(const T *row, int V) : row(row), V(V) {
         head = min((int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T), V);
         units = (V - head) / E;
         run = (units + THREADS - 1) / THREADS * 64;
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-            if (i * 64 < run && first() + i * 64 < units) raw[i] = unit(first() + i * 64);
     }
     __device__ __forceinline__ dl_words unit(int j) const { return *reinterpret_cast<const dl_words *>(row + head + j * E); }
     __device__ __forceinline__ int first() const { return (threadIdx.x >> 6) * run + (threadIdx.x & 63); }
-    // f(unit number, values, whether the thread has one), by all threads of a wavefront.  The units go through the loop by turns of
-    // the registers: one copy of f's code, whose exponentials would fill the registers in unrolled ones.
-    template <int N, typename F>
-    __device__ __forceinline__ void by_turns(dl_words (&v)[N], int i0, F f) const {
-#pragma unroll 1
-        for (int u = 0; u < N; ++u) {
-            const dl_words now = v[0];
-#pragma unroll
-            for (int k = 0; k + 1 < N; ++k) v[k] = v[k + 1];
-            v[N - 1] = now;
-            const int i = i0 + u * 64, j = first() + i;
-            if (i < run) {
-                float values[E];
-                dl_unpack<T>(now, values);
-                f(j, values, j < units);
-            }
-        }
-    }
+    // f(unit number, values, whether the thread has one), by all threads of a wavefront
     template <typename F>
-    __device__ __forceinline__ void units_of(F f) {
-        if constexpr (NR > 0) {
-            by_turns(raw, 0, f);
-        } else {
-            constexpr int AHEAD = 4;  // units in flight while as many are worked on
-            dl_words v[AHEAD], next[AHEAD];
-            const auto fetch = [&](dl_words (&to)[AHEAD], int i0) {
+    __device__ __forceinline__ void units_of(F f) const {
+        constexpr int AHEAD = E == 4 ? 4 : 2;  // units in flight while as many are worked on
+        dl_words v[AHEAD], next[AHEAD];
+        const auto fetch = [&](dl_words (&to)[AHEAD], int i0) {
 #pragma unroll
-                for (int u = 0; u < AHEAD; ++u) {
-                    const int i = i0 + u * 64;
-                    if (i < run && first() + i < units) to[u] = unit(first() + i);
-                }
-            };
-            fetch(v, 0);
-#pragma unroll 1
-            for (int i0 = 0; i0 < run; i0 += AHEAD * 64) {
-                fetch(next, i0 + AHEAD * 64);
-                by_turns(v, i0, f);
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u) v[u] = next[u];
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = i0 + u * 64;
+                if (i < run && first() + i < units) to[u] = unit(first() + i);
             }
+        };
+        fetch(v, 0);
+#pragma unroll 1
+        for (int i0 = 0; i0 < run; i0 += AHEAD * 64) {
+            fetch(next, i0 + AHEAD * 64);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = i0 + u * 64, j = first() + i;
+                if (i < run) {
+                    float values[E];
+                    dl_unpack<T>(v[u], values);
+                    f(j, values, j < units);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) v[u] = next[u];
         }
     }
     // the single element of a thread: its index, or -1
@@ -743,7 +752,7 @@ struct SampleReader {
         return t < head ? t : tail + (t - head) < V ? tail + (t - head) : -1;
     }
     // the thread's largest element, as a key
-    __device__ __forceinline__ uint32_t largest() {
+    __device__ __forceinline__ uint32_t largest() const {
         const int i = single();
         float m = i >= 0 ? fmaxf((float)row[i], -INFINITY) : -INFINITY;  // (the larger of a NaN and a number is the number)
         units_of([&](int, const float (&v)[E], bool has) {
@@ -754,7 +763,7 @@ struct SampleReader {
     }
     // f(key, index) for every element
     template <typename F>
-    __device__ __forceinline__ void each(F f) {
+    __device__ __forceinline__ void each(F f) const {
         const int i = single();
         if (i >= 0) f(smp_key((float)row[i]), i);
         units_of([&](int j, const float (&v)[E], bool has) {
@@ -765,7 +774,7 @@ struct SampleReader {
     }
     // Appends the elements that take(value) says (not a NaN) to a list in LDS; `size` counts what does not fit as well
     template <typename F>
-    __device__ __forceinline__ void list(u64 *pairs, uint32_t *size, F take) {
+    __device__ __forceinline__ void list(u64 *pairs, uint32_t *size, F take) const {
         const int i = single();
         const float l = i >= 0 ? (float)row[i] : 0.0f;
         smp_append(pairs, size, i >= 0 && take(l), smp_pair(smp_key(l), i));
@@ -791,7 +800,57 @@ __device__ __forceinline__ uint32_t smp_first_key(int bin, uint32_t top, const S
     return lo;
 }
 
-// All that top-k keeps is in the list of n: the cuts, and the draw.
+// All that top-k keeps is in a list of n <= SMP_FEW_LISTED: the cuts and the draw by one wavefront, two pairs a lane, every pair against
+// every other one (no barrier and no sorting).  The list's room behind the pairs takes their weights.
+__device__ __forceinline__ void smp_few_draw(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, u64 *pairs, int n) {
+    const int lane = threadIdx.x & 63;
+    u64 *const weights = pairs + SMP_FEW_LISTED;
+    u64 p[2], w[2], before[2] = {}, run[2] = {}, in_k = 0, all = 0;
+    int rank[2] = {};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const int i = m * 64 + lane;
+        p[m] = i < n ? pairs[i] : 0;
+        w[m] = i < n ? smp_fixed((uint32_t)(p[m] >> 32), top, r, a.shift) : 0;
+        weights[i] = w[m];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+        const u64 pj = pairs[j], wj = weights[j];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const bool ahead = pj > p[m];
+            rank[m] += ahead;
+            before[m] += ahead ? wj : 0;
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) in_k += rank[m] < r.k ? w[m] : 0;
+    const double limit = r.p * (double)smp_wave_sum(in_k);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const bool stays = (!r.cut_p || (double)before[m] < limit) && (w[m] >= r.least || (uint32_t)(p[m] >> 32) == top);
+        if (!(p[m] != 0 && rank[m] < r.k && (rank[m] == 0 || stays))) w[m] = 0;  // (of weight 0: never drawn)
+        weights[m * 64 + lane] = w[m];
+        all += w[m];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+        const u64 wj = weights[j];
+        const uint32_t at = (uint32_t)pairs[j];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) run[m] += at >= (uint32_t)p[m] ? wj : 0;  // (indices are complements: those up to its own)
+    }
+    const u64 target = smp_target(r, smp_wave_sum(all));
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+        if (w[m] > 0 && run[m] > target && run[m] - w[m] <= target) a.out[b] = (long long)(0xFFFFFFFFu - (uint32_t)p[m]);
+}
+
+// The same for a longer list.
 template <int THREADS>
 __device__ __forceinline__ void smp_list_draw(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, u64 *pairs, int n, u64 *red) {
     smp_order<THREADS>(pairs, n);
@@ -828,15 +887,25 @@ __device__ __forceinline__ void smp_list_draw(const SampleArgs &a, const SampleR
         }
 }
 
-template <typename T, int NR>
+template <typename T>
 __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
     constexpr int THREADS = SMP_DRAW_THREADS, E = 16 / sizeof(T), WAVES = THREADS / 64;
-    __shared__ u64 weight[SMP_BINS], pairs[SMP_LIST], red[WAVES], slot[WAVES + 2], left;
-    __shared__ uint32_t count[SMP_BINS], limit[4], listed, least;
+    __shared__ union {
+        struct {
+            u64 weight[SMP_BINS];
+            uint32_t count[SMP_BINS];
+        } bins;
+        float space[WAVES * SMP_GATHER];
+    } of;
+    static_assert(sizeof(of.space) <= sizeof(of.bins), "the logits that are gathered take the classes' place");
+    __shared__ u64 pairs[SMP_LIST], red[WAVES], slot[WAVES + 2], left;
+    __shared__ uint32_t limit[4], listed, least;
+    u64 *const weight = of.bins.weight;
+    uint32_t *const count = of.bins.count;
     __shared__ SampleCut shared;
     __shared__ int chosen;
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    SampleReader<T, NR> row((const T *)a.logits + b * a.ldl, a.V);
+    const SampleReader<T> row((const T *)a.logits + b * a.ldl, a.V);
     const SampleRow r = smp_row(a, b);
     if (threadIdx.x == 0) listed = 0;
     const uint32_t own = row.largest();
@@ -878,6 +947,10 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
         row.list(pairs, &listed, [&](float l) { return l >= from; });
         __syncthreads();
         const uint32_t n = listed;
+        if (n <= SMP_FEW_LISTED) {
+            if (wave == 0) smp_few_draw(a, r, b, top, pairs, (int)n);
+            return;
+        }
         if (n <= SMP_LIST) {
             smp_list_draw<THREADS>(a, r, b, top, pairs, (int)n, red);
             return;
@@ -905,12 +978,25 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
         }
     }
     if (r.cut_p) {
-        const double unit = ldexp(1.0, smp_term_shift(a));
-        row.each([&](uint32_t key, int) {
-            double rest;
-            const int bin = smp_bin(key, top, r, rest);
-            if (key > SMP_DEAD) atomicAdd(&weight[bin], smp_class_term(rest, unit));
-        });
+        const double unit = ldexp(1.0, smp_term_shift(a)), M = smp_logit(top);
+        if (M <= 3.4028234663852886e38) {
+            const auto add = [&](float l) {
+                double rest;
+                const int bin = smp_class(l, M, r, rest);
+                atomicAdd(&weight[bin], smp_class_term(rest, unit));  // (what is dead as well: the last class weighs nothing)
+            };
+            const int i = row.single();
+            if (i >= 0) add((float)row.row[i]);
+            row.units_of([&](int, const float (&v)[E], bool has) {
+                if (!has) return;
+#pragma unroll
+                for (int e = 0; e < E; ++e) add(v[e]);
+            });
+        } else {
+            row.each([&](uint32_t key, int) {
+                if (key == top) atomicAdd(&weight[0], smp_class_term(0.0, unit));
+            });
+        }
         __syncthreads();
         c = smp_resolve<THREADS>(a, count, weight, r, red, &shared);
     }
@@ -935,24 +1021,34 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
         if (is_sure(l)) atomicAdd(&slot[slot_of(i)], smp_weight(smp_key(l), top, r, a.shift));
         smp_append(pairs, &listed, is_open(l), smp_pair(smp_key(l), i));
     }
+    // Few of a nucleus' logits are kept, most wavefronts have some: they are gathered (where the classes' sums and counts were), so that
+    // all lanes work on every exponential
+    float *const gathered = reinterpret_cast<float *>(of.space) + wave * SMP_GATHER;
+    int waiting = 0;
     u64 sum = 0;
     row.units_of([&](int j, const float (&v)[E], bool has) {
-        uint32_t kept = 0, open = 0;
+        u64 some = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) kept |= (uint32_t)(has && is_sure(v[e])) << e, open |= (uint32_t)(has && is_open(v[e])) << e;
-        // (few of a nucleus' lanes have more than one: a turn for the lanes' first ones, then for the second ones)
-        while (__ballot(kept != 0)) {
-            float l = v[0];
-            const int at = __builtin_ctz(kept | 1u << E);
-#pragma unroll
-            for (int e = 1; e < E; ++e) l = at == e ? v[e] : l;
-            if (kept) sum += smp_weight(smp_key(l), top, r, a.shift);
-            kept &= kept - 1;
+        for (int e = 0; e < E; ++e) {
+            const bool keep = has && is_sure(v[e]);
+            const u64 keeps = __ballot(keep);
+            if (keep) gathered[waiting + __popcll(keeps & ((1ull << lane) - 1))] = v[e];
+            waiting += __popcll(keeps);
+            some |= __ballot(has && is_open(v[e]));
+            if (e % 4 == 3)
+                while (waiting >= 64) {
+                    waiting -= 64;
+                    __builtin_amdgcn_wave_barrier();
+                    sum += smp_weight(smp_key(gathered[waiting + lane]), top, r, a.shift);
+                    __builtin_amdgcn_wave_barrier();
+                }
         }
-        if (__ballot(open != 0))
+        if (some)
 #pragma unroll
-            for (int e = 0; e < E; ++e) smp_append(pairs, &listed, open >> e & 1, smp_pair(smp_key(v[e]), row.head + j * E + e));
+            for (int e = 0; e < E; ++e) smp_append(pairs, &listed, has && is_open(v[e]), smp_pair(smp_key(v[e]), row.head + j * E + e));
     });
+    __builtin_amdgcn_wave_barrier();
+    if (lane < waiting) sum += smp_weight(smp_key(gathered[lane]), top, r, a.shift);
     sum = smp_wave_sum(sum);
     if (lane == 0) slot[wave + 1] = sum;
     __syncthreads();
@@ -1065,11 +1161,8 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
         return dl_launch_status();
     }
     if (smp_by_row(B, V)) {
-        const int units = dl_ceil_div(V / (16 / dl_type_bytes(type)), SMP_DRAW_THREADS);  // of a thread
         dl_prof_begin("sample_row", s);
-#define ROW(NR) sample_row<T, NR><<<B, SMP_DRAW_THREADS, 0, s>>>(a)
-        DL_BY_TYPE(type, T, if (units <= 2) ROW(2); else ROW(0));
-#undef ROW
+        DL_BY_TYPE(type, T, sample_row<T><<<B, SMP_DRAW_THREADS, 0, s>>>(a));
         dl_prof_end(s);
         return dl_launch_status();
     }
