@@ -64,7 +64,7 @@ __global__ __launch_bounds__(DROP_THREADS) void dropout_kernel(const T *__restri
             dl_load(x + e, f);
 #pragma unroll
             for (int j = 0; j < E; ++j) f[j] = drop_one<FLIP>(f[j], w[j], below, scale);
-            dl_store(y + e, f);
+            dl_store_past(y + e, f);
         } else {
 #pragma unroll
             for (int j = 0; j < E; ++j)

@@ -785,6 +785,10 @@ void same_device(const Tensor &first, const Tensor &t, const char *what) {
 void once(const char *what) {
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (a backward with create_graph=True)");
 }
+int size_int(int64_t v, const char *what) {
+    TORCH_CHECK(v <= INT_MAX, what, " of ", v, " is more than the kernels take");
+    return (int)v;
+}
 const void *raw_in(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
 struct Embedding : torch::autograd::Function<Embedding> {
@@ -794,7 +798,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
         // rows may lie apart, as in a slice of a wider matrix
         const bool rows = weight_.stride(1) == 1 && weight_.stride(0) >= weight_.size(1);
         const Tensor weight = rows ? weight_ : weight_.contiguous();
-        const int64_t V = weight.size(0), D = weight.size(1);
+        const int64_t V = weight.size(0), D = size_int(weight.size(1), "a row");
         auto sizes = tokens.sizes().vec();
         sizes.push_back(D);
         const Tensor y = at::empty(sizes, weight.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
@@ -831,7 +835,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Maybe &weight_, const Maybe &bias_, int64_t groups, double eps, int64_t act) {
         const c10::DeviceGuard guard(x_.device());
         const Tensor x = x_.contiguous(), weight = weight_ ? weight_->contiguous() : Tensor(), bias = bias_ ? bias_->contiguous() : Tensor();
-        const int64_t B = x.size(0), C = x.size(-1), P = x.numel() / (B * C);
+        const int64_t B = size_int(x.size(0), "a batch"), C = size_int(x.size(-1), "a number of channels"), P = x.numel() / (B * C);
         const Tensor y = at::empty_like(x), stats = floats({B, groups, 2}, x);
         const int type = type_of(x, "x"), ptype = weight.defined() ? type_of(weight, "weight") : bias.defined() ? type_of(bias, "bias") : type;
         const Tensor ws = bytes(L.dl_group_norm_fwd_workspace_bytes(type, B, P, C, groups), x);
@@ -910,7 +914,7 @@ Tensor sample(const Tensor &logits_, const Tensor &uniform_, const Maybe &temper
     at::NoGradGuard no_grad;
     require_device(logits_);
     const c10::DeviceGuard guard(logits_.device());
-    const int64_t B = logits_.size(0), V = logits_.size(1);
+    const int64_t B = size_int(logits_.size(0), "a batch"), V = size_int(logits_.size(1), "a row");
     const int type = type_of(logits_, "logits");
     const auto rows = [&](const Maybe &t, at::ScalarType dtype, const char *what) {
         if (!t) return Tensor();
@@ -920,7 +924,7 @@ Tensor sample(const Tensor &logits_, const Tensor &uniform_, const Maybe &temper
     };
     const Tensor logits = logits_.stride(1) == 1 && (logits_.stride(0) >= V || B <= 1) ? logits_ : logits_.contiguous();
     const Tensor uniform = rows(uniform_, at::kFloat, "uniform"), T = rows(temperature, at::kFloat, "temperature"),
-                 k = rows(top_k, at::kInt, "top_k"), p = rows(top_p, at::kFloat, "top_p"), m = rows(min_p, at::kFloat, "min_p");
+                 k = rows(top_k && top_k->scalar_type() == at::kLong ? top_k->clamp(0, INT_MAX) : top_k, at::kInt, "top_k"), p = rows(top_p, at::kFloat, "top_p"), m = rows(min_p, at::kFloat, "min_p");
     const Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong).requires_grad(false));
     const size_t need = L.dl_sample_workspace_bytes((int)B, (int)V);
     const Tensor ws = need ? bytes(need, logits) : Tensor();

@@ -108,16 +108,18 @@ __device__ __forceinline__ GnPlace gn_place(const GnShape &s, int tile, int piec
 template <typename T, int E, bool VEC>
 __device__ __forceinline__ void gn_read(const T *p, int real, float (&f)[E]) {
     if constexpr (VEC) {
-        dl_load(p, f);
+        dl_unpack<T>(*reinterpret_cast<const dl_words *>(p), f);
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) f[e] = e < real ? (float)p[e] : 0.0f;
     }
 }
-template <typename T, int E, bool VEC>
+// PAST: of a tensor that no launch of the call reads again, next to ones that the next launch does
+template <typename T, int E, bool VEC, bool PAST>
 __device__ __forceinline__ void gn_write(T *p, int real, const float (&f)[E]) {
     if constexpr (VEC) {
-        dl_store(p, f);
+        if constexpr (PAST) dl_store_past(p, f);
+        else dl_store(p, f);
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -279,7 +281,7 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
         if (p >= P) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = gn_act<ACT>(fmaf(o[e] - m[e], ga[e], be[e]));
-        gn_write<T, E, VEC>(y + base + (long long)p * s.C, real, o);
+        gn_write<T, E, VEC, false>(y + base + (long long)p * s.C, real, o);
     }
 }
 
@@ -379,7 +381,7 @@ __global__ __launch_bounds__(THREADS) void gn_apply(const T *__restrict__ x, con
         gn_read<T, E, VEC>(x + base + (long long)p * s.C, real, v);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = gn_act<ACT>(fmaf(v[e] - mean[e], scale[e], shift[e]));
-        gn_write<T, E, VEC>(y + base + (long long)p * s.C, real, v);
+        gn_write<T, E, VEC, true>(y + base + (long long)p * s.C, real, v);
     }
 }
 
@@ -480,7 +482,7 @@ __global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__
             ch.template at<ACT>(e, x_[e], o[e], hat, g);
             o[e] = ch.rstd[e] * (fmaf(g, ch.ga[e], -ma[e]) - hat * mq[e]);
         }
-        gn_write<T, E, VEC>(gx + base + (long long)p * s.C, real, o);
+        gn_write<T, E, VEC, false>(gx + base + (long long)p * s.C, real, o);
     }
 }
 
@@ -587,7 +589,7 @@ __global__ __launch_bounds__(THREADS) void gn_backward_apply(const T *__restrict
             ch.template at<ACT>(e, v[e], d[e], hat, g);
             v[e] = ch.rstd[e] * (fmaf(g, ch.ga[e], -ma[e]) - hat * mq[e]);
         }
-        gn_write<T, E, VEC>(gx + base + (long long)p * s.C, real, v);
+        gn_write<T, E, VEC, true>(gx + base + (long long)p * s.C, real, v);
     }
 }
 
@@ -666,7 +668,7 @@ static int gn_rows_per_step(const GnShape &s, int E, int threads) {
 
 static GnShape gn_pieces_shape(int B, long long P, int C, int G, int E) {
     GnShape s = gn_tiles(B, P, C, G, E, GN_THREADS);
-    gn_pieces(s, gn_rows_per_step(s, E, GN_THREADS) * 4, 2048);
+    gn_pieces(s, gn_rows_per_step(s, E, GN_THREADS) * 4, 1024);
     return s;
 }
 static bool gn_grid_ok(const GnShape &s) { return (long long)s.B * s.tiles * s.pieces < (1LL << 31); }

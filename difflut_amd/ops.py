@@ -596,6 +596,8 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         if torch.is_tensor(v):
             if tuple(v.shape) != (B,):
                 raise ValueError(f"{name} must be a number or a tensor [{B}], got {tuple(v.shape)}")
+            if name == "top_k" and (v.is_floating_point() or v.dtype is torch.bool):
+                raise TypeError(f"top_k must be whole numbers, got {v.dtype}")
         elif not fine[name](v):
             raise ValueError(f"{name} out of range: {v}")
     if not logits.is_cuda:
