@@ -23,6 +23,7 @@
 #define EMB_ROWS(E) ((E) == 8 ? 8 : 16)  // rows that a team of the sums has in flight (more registers leave too few wavefronts)
 #define EMB_JOIN_THREADS 512
 #define EMB_JOIN_WAVES (EMB_JOIN_THREADS / 64)
+#define EMB_JOIN_SPLIT 16  // partials from which on the block's wavefronts share them
 
 // ---------------------------------------------------------------------------------- lookup
 // A team of `lanes` threads per row (a power of two), R rows of a team in flight at once.
@@ -239,50 +240,72 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_sum(const T *__restrict__ g
     }
 }
 
-// Tokens that reach over pieces.  A frequent one has thousands of partials: they are split over the block's wavefronts, whose sums are
-// added in order; with few partials the wavefronts take columns of their own instead.
+// Tokens that reach over pieces.  A wavefront takes a piece, whose last token may go on, and 64 vectors of columns; the partials of a frequent
+// token (thousands) are split over the block's wavefronts, whose sums are added in order.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join(T *__restrict__ gw, EmbArgs a) {
+__global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join(T *__restrict__ gw, EmbArgs a, int columns) {
     constexpr int E = VEC ? 4 : 1;
     __shared__ DlVec<float, E> sums[EMB_JOIN_WAVES][64];
+    __shared__ int parts_of[EMB_JOIN_WAVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, total = *a.total;
-    for (long long piece = blockIdx.x; piece < a.pieces; piece += gridDim.x) {
+    const int c = (blockIdx.x % columns * 64 + lane) * E;
+    const long long piece0 = (long long)(blockIdx.x / columns) * EMB_JOIN_WAVES;
+    // the pieces behind `piece` that begin with sums of its last token (0: it ends here, began earlier, or there is none)
+    const auto joins = [&](long long piece, int &v) {
         const long long i0 = piece * a.piece, i1 = i0 + a.piece;
-        if (i1 >= total) return;  // nothing goes on behind the last piece
-        const int v = a.token_of[i1 - 1], begin = a.begin_of[v], end = begin + a.count[v];
-        if (end <= i1 || begin < i0) continue;  // ends here, or began earlier
-        const int parts = (end - 1) / a.piece - (int)piece;  // whose sums begin the pieces behind this one
-        const float *own = a.part + ((long long)piece * 2 + 1) * a.D, *rest = a.part + ((long long)piece + 1) * 2 * a.D;
-        const bool split = parts >= EMB_JOIN_WAVES;
-        const int per = split ? (parts + EMB_JOIN_WAVES - 1) / EMB_JOIN_WAVES : parts, p0 = split ? min(wave * per, parts) : 0, p1 = min(p0 + per, parts);
-        for (int c0 = split ? 0 : wave * 64 * E; c0 < a.D; c0 += (split ? 1 : EMB_JOIN_WAVES) * 64 * E) {
-            const int c = c0 + lane * E;
-            float acc[E] = {};
-            if (c < a.D) {
-                if (p0 == 0) dl_load(own + c, acc);
+        if (i1 >= total) return 0;
+        v = a.token_of[i1 - 1];
+        const int begin = a.begin_of[v], end = begin + a.count[v];
+        return end <= i1 || begin < i0 ? 0 : (end - 1) / a.piece - (int)piece;
+    };
+    // sum of partials [p0, p1) behind `piece`, on top of acc
+    const auto add = [&](long long piece, int p0, int p1, float (&acc)[E]) {
+        const float *rest = a.part + (piece + 1) * 2 * a.D + c;
 #pragma unroll 8
-                for (int p = p0; p < p1; ++p) {
-                    float f[E];
-                    dl_load(rest + (long long)p * 2 * a.D + c, f);
+        for (int p = p0; p < p1; ++p) {
+            float f[E];
+            dl_load(rest + (long long)p * 2 * a.D, f);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += f[e];
-                }
-            }
-            if (split) {
-                __syncthreads();  // the last columns' sums have been read
-                dl_store(&sums[wave][lane].v[0], acc);
-                __syncthreads();
-                if (wave > 0) continue;
-#pragma unroll
-                for (int w = 1; w < EMB_JOIN_WAVES; ++w)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += sums[w][lane].v[e];
-            }
-            if (c >= a.D) continue;
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] *= a.scale;
-            dl_store(gw + (long long)v * a.D + c, acc);
+            for (int e = 0; e < E; ++e) acc[e] += f[e];
         }
+    };
+    const auto write = [&](int v, float (&acc)[E]) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= a.scale;
+        dl_store(gw + (long long)v * a.D + c, acc);
+    };
+    int v = 0;
+    const long long own = piece0 + wave;
+    const int parts = own < a.pieces ? joins(own, v) : 0;
+    if (lane == 0) parts_of[wave] = parts;
+    if (parts > 0 && parts < EMB_JOIN_SPLIT && c < a.D) {
+        float acc[E];
+        dl_load(a.part + (own * 2 + 1) * a.D + c, acc);
+        add(own, 0, parts, acc);
+        write(v, acc);
+    }
+    __syncthreads();
+    for (int w = 0; w < EMB_JOIN_WAVES; ++w) {
+        const int n = parts_of[w];
+        if (n < EMB_JOIN_SPLIT) continue;
+        const int per = (n + EMB_JOIN_WAVES - 1) / EMB_JOIN_WAVES, p0 = min(wave * per, n);
+        float acc[E] = {};
+        if (c < a.D) {
+            if (wave == 0) dl_load(a.part + ((piece0 + w) * 2 + 1) * a.D + c, acc);
+            add(piece0 + w, p0, min(p0 + per, n), acc);
+        }
+        dl_store(&sums[wave][lane].v[0], acc);
+        __syncthreads();
+        if (wave == w && c < a.D) {  // (v is this wavefront's)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = sums[0][lane].v[e];
+#pragma unroll
+            for (int k = 1; k < EMB_JOIN_WAVES; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += sums[k][lane].v[e];
+            write(v, acc);
+        }
+        __syncthreads();
     }
 }
 
@@ -360,6 +383,7 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
     a.sum_blocks = (unsigned)((a.pieces + teams - 1) / teams);
     const int bits = emb_block_bits(V);
     const size_t lds = (size_t)EMB_SORT_WAVES * (size_t)((V + (1LL << bits) - 1) >> bits) * sizeof(int);
+    if ((long long)dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * dl_ceil_div(D, vec ? 256 : 64) > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
     const unsigned skip = padding >= 0 && padding < V ? (unsigned)padding : ~0u;
 #define SORT(TOKEN) \
     embed_sort<TOKEN><<<1 << bits, EMB_SORT_THREADS, lds, s>>>((const TOKEN *)tokens, (int)n, (unsigned)V, skip, bits, order, token_of, begin_of, count, total)
@@ -372,7 +396,11 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
     const unsigned zero_blocks = (unsigned)(zero_teams < 2048 ? zero_teams : 2048);
 #define SUMS(VEC)                                                                                                                    \
     DL_TIMED("embed_sum", s, (embed_sum<T, VEC><<<a.sum_blocks + zero_blocks, EMB_THREADS, 0, s>>>((const T *)gy, (T *)gw, a)));     \
-    if (a.pieces > 1) DL_TIMED("embed_join", s, (embed_join<T, VEC><<<a.pieces < 1024 ? a.pieces : 1024, EMB_JOIN_THREADS, 0, s>>>((T *)gw, a)))
+    if (a.pieces > 1) {                                                                                                              \
+        const int columns = dl_ceil_div(D, VEC ? 256 : 64);                                                                          \
+        const int joins = dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * columns;                                                           \
+        DL_TIMED("embed_join", s, (embed_join<T, VEC><<<joins, EMB_JOIN_THREADS, 0, s>>>((T *)gw, a, columns)));                \
+    }
     DL_BY_TYPE(type, T, if (vec) { SUMS(true); } else { SUMS(false); });
 #undef SUMS
     return dl_launch_status();
