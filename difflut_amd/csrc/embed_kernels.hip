@@ -64,9 +64,20 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_lookup(const TOKEN *__restr
 // A token as 32 bits; ~0: not summed (V < 2^31).
 template <typename TOKEN>
 __device__ __forceinline__ unsigned emb_token(TOKEN t, unsigned V, unsigned padding) {
-    const unsigned v = (unsigned)t;
-    const bool known = v < V && v != padding && (sizeof(TOKEN) == 4 || (unsigned)((unsigned long long)t >> 32) == 0u);
-    return known ? v : ~0u;
+    const bool known = sizeof(TOKEN) == 4 ? (unsigned)t < V : (unsigned long long)t < (unsigned long long)V;
+    return known && (unsigned)t != padding ? (unsigned)t : ~0u;
+}
+// EMB_AHEAD groups of 64 tokens from group g on, those before g1 and n; -1 past them
+template <typename TOKEN>
+__device__ __forceinline__ void emb_fetch(const TOKEN *__restrict__ tokens, int g, int g1, int n, TOKEN (&t)[EMB_AHEAD]) {
+    const TOKEN *from = tokens + (long long)g * 64 + (threadIdx.x & 63);
+    if (g + EMB_AHEAD <= g1 && (long long)(g + EMB_AHEAD) * 64 <= n) {
+#pragma unroll
+        for (int u = 0; u < EMB_AHEAD; ++u) t[u] = from[u * 64];
+    } else {
+#pragma unroll
+        for (int u = 0; u < EMB_AHEAD; ++u) t[u] = g + u < g1 && (g + u) * 64 + (int)(threadIdx.x & 63) < n ? from[u * 64] : (TOKEN)-1;
+    }
 }
 
 template <typename TOKEN>
@@ -85,15 +96,15 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
     const int groups = (n + 63) >> 6, per_wave = (groups + EMB_SORT_WAVES - 1) / EMB_SORT_WAVES;
     const int g0 = min(wave * per_wave, groups), g1 = min(g0 + per_wave, groups);
     int below = 0, mine = 0;
+    TOKEN t[EMB_AHEAD], ahead[EMB_AHEAD];
+    emb_fetch(tokens, g0, g1, n, t);
     for (int g = g0; g < g1; g += EMB_AHEAD) {
-        TOKEN t[EMB_AHEAD];
-#pragma unroll
-        for (int u = 0; u < EMB_AHEAD; ++u) t[u] = g + u < g1 && (g + u) * 64 + lane < n ? tokens[(g + u) * 64 + lane] : (TOKEN)-1;
+        emb_fetch(tokens, g + EMB_AHEAD, g1, n, ahead);
 #pragma unroll
         for (int u = 0; u < EMB_AHEAD; ++u) {
-            const unsigned v = emb_token(t[u], V, padding), owner = v & mask;
-            const bool known = v != ~0u, here = known && owner == b;
-            below += __popcll(__ballot(known && owner < b));
+            const unsigned v = emb_token(t[u], V, padding), owner = v == ~0u ? v : v & mask;
+            const bool here = owner == b;
+            below += __popcll(__ballot(owner < b));
             const unsigned long long takes = __ballot(here);
             if (takes == 0) continue;
             if (here) {
@@ -103,6 +114,8 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
             }
             mine += __popcll(takes);
         }
+#pragma unroll
+        for (int u = 0; u < EMB_AHEAD; ++u) t[u] = ahead[u];
     }
     if (lane == 0) below_of[wave] = below;
     __syncthreads();
@@ -163,9 +176,7 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
         }
     } else {  // a frequent token: the list was too short, the tokens are read again
         for (int g = g0; g < g1; g += EMB_AHEAD) {
-            TOKEN t[EMB_AHEAD];
-#pragma unroll
-            for (int u = 0; u < EMB_AHEAD; ++u) t[u] = g + u < g1 && (g + u) * 64 + lane < n ? tokens[(g + u) * 64 + lane] : (TOKEN)-1;
+            emb_fetch(tokens, g, g1, n, t);
 #pragma unroll
             for (int u = 0; u < EMB_AHEAD; ++u) {
                 const unsigned v = emb_token(t[u], V, padding);

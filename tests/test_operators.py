@@ -278,10 +278,54 @@ def test_group_norm_gradient_against_differences():
         assert torch.autograd.gradcheck(lambda *t: ops.group_norm(t[0], 2, *t[1:], activation=act), (x, w, b))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,space,C,G", [(2, (130, 130), 40, 8), (1, (40000,), 6, 3), (3, (900,), 1100, 1), (1, (6001,), 2500, 1), (1, (70, 300), 64, 64),
+                                         (300, (64,), 96, 4), (9, (130,), 250, 5)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_group_norm_of_larger_tensors(B, space, C, G, dtype):
+    """Samples split over blocks, wide groups in slices, and what still fits one block; twice the same bits."""
+    g = gen(C + G)
+    x, gy = ((torch.randn(B, *space, C, generator=g) * 0.4 + m).to(dtype) for m in (0.5, 0.0))
+    weight, bias = ((torch.randn(C, generator=g) * 0.2 + m).to(dtype) for m in (1.0, 0.0))
+    want = norm_64(x, G, weight, bias, 1e-2, "silu", gy, depth=256)
+    leaves = [t.cuda().requires_grad_() for t in (x, weight, bias)]
+    runs = []
+    for _ in range(2):
+        y = ops.group_norm(leaves[0], G, *leaves[1:], eps=1e-2, activation="silu")
+        runs.append([y, *torch.autograd.grad(y, leaves, gy.cuda())])
+    for t, again, (exact, bound) in zip(*runs, want):
+        close(t.reshape(exact.shape), exact, bound, dtype)
+        assert torch.equal(t, again)
+
+
+@pytest.mark.gpu
+def test_group_norm_far_from_zero_in_pieces():
+    """The variance of a sample that is split over blocks, around 1000, and with an outlier where the sums begin."""
+    x = torch.randn(1, 60000, 8, generator=gen(9)) + 1000.0
+    x[0, 0] = -5000.0
+    y = ops.group_norm(x.cuda(), 2)
+    wide = x.double().view(1, -1, 2, 4)
+    want = ((wide - wide.mean((1, 3), keepdim=True)) / torch.sqrt(wide.var((1, 3), unbiased=False, keepdim=True) + 1e-5)).view(x.shape)
+    rstd = 1 / math.sqrt(float(wide.var((1, 3), unbiased=False).min()))
+    close(y, want, 1000 * rstd * 64 * U + want.abs() * 512 * U, torch.float32)  # the mean's rounding; a thread's rows in the variance
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_group_norm_gradients_of_some_inputs(device):
+    g = gen(14)
+    x, gy, weight, bias = (torch.randn(s, generator=g).to(device) for s in ((3, 40, 12), (3, 40, 12), (12,), (12,)))
+    leaves = [t.clone().requires_grad_() for t in (x, weight, bias)]
+    full = torch.autograd.grad(ops.group_norm(leaves[0], 3, *leaves[1:], activation="silu"), leaves, gy)
+    for i in range(3):
+        some = [t.clone().requires_grad_(n == i) for n, t in enumerate((x, weight, bias))]
+        got, = torch.autograd.grad(ops.group_norm(some[0], 3, *some[1:], activation="silu"), some[i], gy)
+        assert torch.equal(got, full[i])
+
+
 # ----------------------------------------------------------------------------- dropout
-def philox(seed, offset, numel):
-    """By numpy's 64-bit products, from the generator's definition."""
-    counter = np.arange(-(-numel // 4), dtype=np.uint64)
+def philox(seed, offset, numel, start=0):
+    """By numpy's 64-bit products, from the generator's definition; words start .. (a multiple of 4)."""
+    counter = np.arange(start // 4, start // 4 - (-numel // 4), dtype=np.uint64)
     low, s32 = np.uint64(0xFFFFFFFF), np.uint64(32)
     c = [counter & low, counter >> s32, np.full_like(counter, offset & 0xFFFFFFFF), np.full_like(counter, offset >> 32)]
     key = [seed & 0xFFFFFFFF, seed >> 32]
@@ -359,6 +403,27 @@ def test_dropout_module(device):
     gx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
     assert torch.equal(gx, y.detach())
     assert drop.eval()(x) is x
+
+
+@pytest.mark.gpu
+def test_more_than_two_to_the_31_elements():
+    """Offsets past 32 bits: the last entries of a dropout, a lookup and a gradient."""
+    n = 2 ** 31 + 40
+    y = ops.dropout(torch.ones(n, dtype=torch.float16, device="cuda"), 0.5, (3, 4))
+    for start in (0, 2 ** 31 - 64, 2 ** 31):
+        hit = torch.from_numpy(philox(3, 4, min(128, n - start), start) < 2 ** 31)
+        assert torch.equal(y[start:start + len(hit)].cpu() == 0, hit)
+    del y
+    V, D = 2 ** 21 + 3, 1032
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    w[-1], w[-2] = 1.0, 2.0
+    tokens = torch.tensor([V - 1, V - 2, 0, V - 1], device="cuda")
+    w.requires_grad_()
+    y = ops.embedding(tokens, w)
+    assert y[:, 0].tolist() == [1.0, 2.0, 0.0, 1.0] and y[:, -1].tolist() == [1.0, 2.0, 0.0, 1.0]
+    grad, = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert grad[[0, 1, V // 2, V - 3, V - 2, V - 1]].float().mean(1).tolist() == [1.0, 0.0, 0.0, 0.0, 1.0, 2.0]
+    assert float(grad.sum(dtype=torch.float32)) == 4.0 * D
 
 
 def test_dropout_gradient_against_differences():
@@ -476,6 +541,45 @@ def test_sample_masked_rows(device, V):
             check_sample(device, logits, torch.full((9,), u), **settings)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,V", [(1, 65537), (3, 131071), (33, 70001)])
+def test_sample_long_rows(B, V):
+    """Rows split over blocks, and more rows than are split: every kind of cut, equal logits, masks."""
+    g = gen(V)
+    normal, equal = torch.randn(3, V, generator=g) * 3, torch.randint(0, 9, (3, V), generator=g).float()
+    masked = torch.where(torch.rand(3, V, generator=g) < 0.999, torch.full((3, V), -math.inf), normal)
+    masked[0] = -math.inf
+    masked[1, 5] = math.nan
+    for logits in (normal, normal.bfloat16(), equal, masked):
+        rows = torch.arange(B) % 3  # (the oracle's time goes by the row)
+        uniform = torch.rand(3, generator=g)
+        for T, k, p, m in ((1.0, 0, 1.0, 0.0), (0.0, 0, 1.0, 0.0), (0.7, 40, 0.9, 0.01), (1.0, 0, 0.8, 0.0), (1.5, 3000, 0.99, 0.0), (1.0, 60000, 0.7, 1e-3)):
+            want = sample_64(logits, uniform, [f32(T)] * 3, [k] * 3, [f32(p)] * 3, [f32(m)] * 3)[rows]
+            got = ops.sample(logits.cuda()[rows.cuda()], uniform.cuda()[rows.cuda()], T, k, p, m)
+            assert got.cpu().tolist() == want.tolist(), (T, k, p, m)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V", [20, 500, 5000])
+def test_sample_extreme_settings(device, V):
+    """Temperatures near nothing and without end, settings that leave the first index, a top-k past any row."""
+    g = gen(V + 4)
+    logits = torch.randn(6, V, generator=g) * 4
+    logits[1, 3] = math.inf
+    logits[2, ::2] = logits[2].max()
+    uniform = torch.tensor([0.0, 0.2, 0.5, 0.9, 1.0 - 2.0 ** -24, 0.7])
+    for T in (1e-30, 1e-3, 1e30, 3e38):
+        for k, p in ((0, 1.0), (5, 1.0), (0, 0.4), (V, 0.9)):
+            check_sample(device, logits, uniform, T, k, p)
+    first = logits.argmax(1).tolist()
+    for name, v in (("temperature", -1.0), ("temperature", math.nan), ("top_p", 0.0), ("top_p", -3.0), ("top_p", math.nan), ("min_p", 1.5),
+                    ("min_p", math.nan)):
+        assert ops.sample(logits.to(device), uniform.to(device), **{name: torch.full((6,), v, device=device)}).tolist() == first
+    for k in (2 ** 31 - 1, 2 ** 40, -5):
+        top_k = torch.full((6,), k, dtype=torch.int64, device=device)
+        assert ops.sample(logits.to(device), uniform.to(device), top_k=top_k).tolist() == ops.sample(logits.to(device), uniform.to(device)).tolist()
+
+
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 def test_sample_strides_and_empty(device):
     g = gen(6)
@@ -522,7 +626,7 @@ def test_refusals(device):
             (ValueError, lambda: ops.sample(logits, u, temperature=-1.0)), (ValueError, lambda: ops.sample(logits, u, temperature=math.nan)),
             (ValueError, lambda: ops.sample(logits, u, top_k=-1)), (ValueError, lambda: ops.sample(logits, u, top_k=1.5)),
             (ValueError, lambda: ops.sample(logits, u, top_p=0.0)), (ValueError, lambda: ops.sample(logits, u, top_p=1.5)),
-            (ValueError, lambda: ops.sample(logits, u, min_p=1.5)), (ValueError, lambda: ops.sample(logits, u, top_p=u[:1]))]:
+            (ValueError, lambda: ops.sample(logits, u, min_p=1.5)), (TypeError, lambda: ops.sample(logits, u, top_k=u)), (ValueError, lambda: ops.sample(logits, u, top_p=u[:1]))]:
         with pytest.raises(error):
             call()
 
