@@ -114,7 +114,7 @@ SIGNATURES = {
     "dl_group_norm_bwd_workspace_bytes": (_Z, [_I, _I, _L, _I, _I]),
     "dl_group_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _I, _I, _I, _P, _Z, _P]),
     "dl_dropout": (_I, [_P, _P, _I, _L, ctypes.c_double, _I, ctypes.c_ulonglong, ctypes.c_ulonglong, _P, _P, _P]),
-    "dl_sample_workspace_bytes": (_Z, [_I, _I]),
+    "dl_sample_workspace_bytes": (_Z, [_I, _I, _I, _F]),
     "dl_sample": (_I, [_P, _L, _I, _P, _P, _P, _P, _P, _F, _I, _F, _F, _P, _P, _Z, _I, _I, _P]),
     "dl_profile_enable": (_I, [_I]),
     "dl_profile_read": (_I, [ctypes.c_char_p, _Z, ctypes.POINTER(_F), _I]),

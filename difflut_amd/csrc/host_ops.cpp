@@ -926,10 +926,11 @@ Tensor sample(const Tensor &logits_, const Tensor &uniform_, const Maybe &temper
     const Tensor uniform = rows(uniform_, at::kFloat, "uniform"), T = rows(temperature, at::kFloat, "temperature"),
                  k = rows(top_k && top_k->scalar_type() == at::kLong ? top_k->clamp(0, INT_MAX) : top_k, at::kInt, "top_k"), p = rows(top_p, at::kFloat, "top_p"), m = rows(min_p, at::kFloat, "min_p");
     const Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong).requires_grad(false));
-    const size_t need = L.dl_sample_workspace_bytes((int)B, (int)V);
+    const int k_all = (int)std::min<int64_t>(top_k_all, INT_MAX);
+    const size_t need = L.dl_sample_workspace_bytes((int)B, (int)V, k.defined() ? -1 : k_all, p.defined() ? -1.0f : (float)top_p_all);
     const Tensor ws = need ? bytes(need, logits) : Tensor();
     check(L.dl_sample(raw_in(logits), B > 1 ? logits.stride(0) : V, type, in(uniform), in(T), k.defined() ? ints(k) : nullptr, in(p), in(m),
-                      (float)temperature_all, (int)std::min<int64_t>(top_k_all, INT_MAX), (float)top_p_all, (float)min_p_all,
+                      (float)temperature_all, k_all, (float)top_p_all, (float)min_p_all,
                       (long long *)raw(tokens), raw(ws), need, (int)B, (int)V, stream()));
     return tokens;
 }

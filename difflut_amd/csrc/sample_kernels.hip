@@ -30,7 +30,7 @@
 #define SMP_THREADS 256
 #define SMP_DRAW_THREADS 1024
 #define SMP_MAX_CHUNKS 256
-#define SMP_GATHER 320  // logits that a wavefront gathers: fewer than 64 left and 4 of every lane
+#define SMP_GATHER 128  // logits that a wavefront gathers: fewer than 64 left and one of every lane
 #define SMP_FEW_LISTED 128
 #define SMP_FEW 768  // top-k up to this goes by the threads' largest logits
 
@@ -182,7 +182,7 @@ __device__ __forceinline__ void smp_sort(u64 *pairs, int n) {
 // step (64 of them: 1 us for 4).
 template <int THREADS>
 __device__ __forceinline__ void smp_order(u64 *pairs, int n) {
-    if (n <= 256) {
+    if (n <= 512) {
         const u64 mine = (int)threadIdx.x < n ? pairs[threadIdx.x] : 0;
         int rank = 0;
         __syncthreads();
@@ -195,7 +195,7 @@ __device__ __forceinline__ void smp_order(u64 *pairs, int n) {
         __syncthreads();
         return;
     }
-    int size = 512;
+    int size = 1024;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += THREADS) pairs[i] = 0;
     smp_sort<THREADS>(pairs, size);
@@ -895,9 +895,11 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
             u64 weight[SMP_BINS];
             uint32_t count[SMP_BINS];
         } bins;
-        float space[WAVES * SMP_GATHER];
+        struct {
+            float value[WAVES * SMP_GATHER];
+            uint32_t index[WAVES * SMP_GATHER];
+        } gathered;
     } of;
-    static_assert(sizeof(of.space) <= sizeof(of.bins), "the logits that are gathered take the classes' place");
     __shared__ u64 pairs[SMP_LIST], red[WAVES], slot[WAVES + 2], left;
     __shared__ uint32_t limit[4], listed, least;
     u64 *const weight = of.bins.weight;
@@ -1021,34 +1023,46 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
         if (is_sure(l)) atomicAdd(&slot[slot_of(i)], smp_weight(smp_key(l), top, r, a.shift));
         smp_append(pairs, &listed, is_open(l), smp_pair(smp_key(l), i));
     }
-    // Few of a nucleus' logits are kept, most wavefronts have some: they are gathered (where the classes' sums and counts were), so that
-    // all lanes work on every exponential
-    float *const gathered = reinterpret_cast<float *>(of.space) + wave * SMP_GATHER;
+    // Few of a nucleus' logits are kept, most wavefronts have some: they are gathered with their indices (where the classes' sums and counts
+    // were), so that all lanes work on every exponential, and what is open is looked for among them only.
+    const float from = c.k_bin < SMP_BINS ? k_from : c.p_first < SMP_BINS ? p_from : sure;
+    float *const values = of.gathered.value + wave * SMP_GATHER;
+    uint32_t *const indices = of.gathered.index + wave * SMP_GATHER;
     int waiting = 0;
     u64 sum = 0;
-    row.units_of([&](int j, const float (&v)[E], bool has) {
-        u64 some = 0;
+    const auto work_on = [&](int at, bool has) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const float l = has ? values[at] : -INFINITY;
+        const uint32_t index = has ? indices[at] : 0;
+        if (is_sure(l)) sum += smp_weight(smp_key(l), top, r, a.shift);
+        smp_append(pairs, &listed, is_open(l), smp_pair(smp_key(l), index));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    if (!r.cut_k && !r.cut_p) {  // all of them
+        row.units_of([&](int, const float (&v)[E], bool has) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const bool keep = has && is_sure(v[e]);
-            const u64 keeps = __ballot(keep);
-            if (keep) gathered[waiting + __popcll(keeps & ((1ull << lane) - 1))] = v[e];
-            waiting += __popcll(keeps);
-            some |= __ballot(has && is_open(v[e]));
-            if (e % 4 == 3)
-                while (waiting >= 64) {
-                    waiting -= 64;
-                    __builtin_amdgcn_wave_barrier();
-                    sum += smp_weight(smp_key(gathered[waiting + lane]), top, r, a.shift);
-                    __builtin_amdgcn_wave_barrier();
+            for (int e = 0; e < E; ++e) {
+                const u64 w = smp_weight(smp_key(v[e]), top, r, a.shift);
+                sum += has ? w : 0;
+            }
+        });
+    } else {
+        row.units_of([&](int j, const float (&v)[E], bool has) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const bool take = has && v[e] >= from;
+                const u64 takes = __ballot(take);
+                if (take) {
+                    const int at = waiting + __popcll(takes & ((1ull << lane) - 1));
+                    values[at] = v[e];
+                    indices[at] = (uint32_t)(row.head + j * E + e);
                 }
-        }
-        if (some)
-#pragma unroll
-            for (int e = 0; e < E; ++e) smp_append(pairs, &listed, has && is_open(v[e]), smp_pair(smp_key(v[e]), row.head + j * E + e));
-    });
-    __builtin_amdgcn_wave_barrier();
-    if (lane < waiting) sum += smp_weight(smp_key(gathered[lane]), top, r, a.shift);
+                waiting += __popcll(takes);
+                if (waiting >= 64) waiting -= 64, work_on(waiting + lane, true);
+            }
+        });
+        work_on(lane, lane < waiting);
+    }
     sum = smp_wave_sum(sum);
     if (lane == 0) slot[wave + 1] = sum;
     __syncthreads();
@@ -1112,11 +1126,21 @@ static size_t smp_layout(SampleArgs &a, char *ws) {
     return at;
 }
 
-// A block per row: its time is that of V / 1024 logits per thread, whatever the number of rows up to the card's 256 CUs.
-static bool smp_by_row(int B, int V) { return V <= 65536 || B >= 32; }
+// Whether a block takes a row of its own (its time goes by the row's length, whatever the number of rows up to the card's 256 CUs) or
+// rows are split over blocks.  us for fp32 rows, block per row / split:
+//   a small top-k (top_k_all in 1 .. SMP_FEW): 131072 columns, 1 row 25 / 40, 16 rows 25 / 51; 262144, 1 row 39 / 41, 16 rows 39 / 64
+//   no cut at all: 32768, 1 row 23 / 22; 131072, 16 rows 70 / 24, 64 rows 70 / 41
+//   else (top-p of 0.9): 65536, 1 row 43 / 42; 131072, 1 row 70 / 44, 16 rows 71 / 67, 64 rows 72 / 129
+static bool smp_by_row(int B, int V, int top_k_all, bool may_cut) {
+    if (top_k_all > 0 && top_k_all <= SMP_FEW) return V <= 262144 || B >= 16;
+    if (!may_cut) return V <= 32768 || B >= 128;
+    return V <= 65536 || B >= 16;
+}
+// (negative numbers stand for settings on the device: the kernels look for themselves whether a row has cuts)
+static bool smp_may_cut(int V, int top_k_all, float top_p_all) { return top_k_all < 0 || (top_k_all > 0 && top_k_all < V) || !(top_p_all >= 1.0f); }
 
-extern "C" size_t dl_sample_workspace_bytes(int B, int V) {
-    if (B <= 0 || V <= SMP_SORTED || smp_by_row(B, V)) return 0;
+extern "C" size_t dl_sample_workspace_bytes(int B, int V, int top_k_all, float top_p_all) {
+    if (B <= 0 || V <= SMP_SORTED || smp_by_row(B, V, top_k_all, smp_may_cut(V, top_k_all, top_p_all))) return 0;
     SampleArgs a = {};
     a.B = B, a.V = V;
     return smp_layout(a, nullptr);
@@ -1130,7 +1154,10 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
     if (B == 0) return DL_OK;
     if (!logits || !uniform || !out) return DL_ERR_NULL;
     if (V > (1 << 30)) return DL_ERR_UNSUPPORTED;
-    const size_t need = dl_sample_workspace_bytes(B, V);
+    if (!top_k && top_k_all < 0) top_k_all = 0;
+    const int k_rule = top_k ? -1 : top_k_all;
+    const float p_rule = top_p ? -1.0f : top_p_all;
+    const size_t need = dl_sample_workspace_bytes(B, V, k_rule, p_rule);
     if (need && !ws) return DL_ERR_NULL;
     if (ws_bytes < need) return DL_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
@@ -1160,7 +1187,7 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
         dl_prof_end(s);
         return dl_launch_status();
     }
-    if (smp_by_row(B, V)) {
+    if (!need) {
         dl_prof_begin("sample_row", s);
         DL_BY_TYPE(type, T, sample_row<T><<<B, SMP_DRAW_THREADS, 0, s>>>(a));
         dl_prof_end(s);
@@ -1169,10 +1196,8 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
     smp_layout(a, (char *)ws);
     if ((long long)B * a.chunks > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
     const int blocks = B * a.chunks;
-    // (settings on the device: the kernels look for themselves whether a row has cuts)
-    const bool may_cut = top_k || top_p || (top_k_all > 0 && top_k_all < V) || !(top_p_all >= 1.0f);
     DL_BY_TYPE(type, T, DL_TIMED("sample_max", s, (sample_max<T><<<blocks, SMP_THREADS, 0, s>>>(a)));
-               if (may_cut) DL_TIMED("sample_hist", s, (sample_hist<T><<<blocks, SMP_THREADS, 0, s>>>(a)));
+               if (smp_may_cut(V, k_rule, p_rule)) DL_TIMED("sample_hist", s, (sample_hist<T><<<blocks, SMP_THREADS, 0, s>>>(a)));
                DL_TIMED("sample_collect", s, (sample_collect<T><<<blocks, SMP_THREADS, 0, s>>>(a)));
                DL_TIMED("sample_draw", s, (sample_draw<T><<<B, SMP_DRAW_THREADS, 0, s>>>(a))));
     return dl_launch_status();

@@ -534,8 +534,9 @@ int dl_dropout(const void *x, void *y, int type, long long numel, double p, int 
  * stays.  out[b]: the first kept index, in index order, whose running sum exceeds uniform[b] times the kept sum; T <= 0: the
  * first of the order; -1 where no logit is above -infinity (NaN counts as that).
  * Settings: device arrays [B] where given, else the numbers behind them for every row.
- * Workspace: dl_sample_workspace_bytes(B, V), 0 for all but few long rows. */
-size_t dl_sample_workspace_bytes(int B, int V);
+ * Workspace: dl_sample_workspace_bytes(B, V, top_k_all or -1 with an array, top_p_all or -1 with an array), 0 for all but few
+ * long rows. */
+size_t dl_sample_workspace_bytes(int B, int V, int top_k_all, float top_p_all);
 int dl_sample(const void *logits, long long ldl, int type, const float *uniform, const float *temperature, const int *top_k,
               const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all, float min_p_all,
               long long *out, void *ws, size_t ws_bytes, int B, int V, void *stream);

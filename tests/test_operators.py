@@ -437,31 +437,27 @@ def sample_64(logits, uniform, T, k, p, m):
     out = []
     for row, u, t, kk, pp, mm in zip(logits.double().numpy(), uniform.double().numpy(), T, k, p, m):
         row = np.where(np.isnan(row), -np.inf, row)
-        order = [i for i in sorted(range(len(row)), key=lambda i: (-row[i], i)) if row[i] > -np.inf]
-        if not order:
+        order = np.argsort(-row, kind="stable")
+        order = order[row[order] > -np.inf]
+        if not len(order):
             out.append(-1)
             continue
         top = row[order[0]]
         if not t > 0:
-            out.append(order[0])
+            out.append(int(order[0]))
             continue
-        w = {i: 1.0 if row[i] == top else (0.0 if top == np.inf else math.exp((row[i] - top) / t)) for i in order}
         if 0 < kk < len(order):
             order = order[:kk]
-        total, run, kept = math.fsum(w[i] for i in order), 0.0, []
-        for i in order:
-            if kept and pp < 1 and not run < pp * total:
-                break
-            kept.append(i)
-            run += w[i]
-        kept = sorted(i for n, i in enumerate(kept) if n == 0 or w[i] >= mm)
-        total, run, token = math.fsum(w[i] for i in kept), 0.0, kept[-1]
-        for i in kept:
-            run += w[i]
-            if run > u * total:
-                token = i
-                break
-        out.append(token)
+        with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+            w = np.where(row[order] == top, 1.0, np.exp((row[order] - top) / t) if top < np.inf else 0.0)
+        before = np.concatenate([[0.0], np.cumsum(w)])  # one after the other
+        keep = np.ones(len(order), bool) if pp >= 1 else before[:-1] < pp * before[-1]
+        keep &= w >= mm
+        keep[0] = True
+        by_index = np.argsort(order[keep])
+        kept, running = order[keep][by_index], np.cumsum(w[keep][by_index])
+        past = np.nonzero(running > u * running[-1])[0]
+        out.append(int(kept[past[0]] if len(past) else kept[-1]))
     return torch.tensor(out)
 
 
@@ -542,7 +538,7 @@ def test_sample_masked_rows(device, V):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,V", [(1, 65537), (3, 131071), (33, 70001)])
+@pytest.mark.parametrize("B,V", [(1, 65537), (3, 131071), (33, 70001), (1, 300001)])
 def test_sample_long_rows(B, V):
     """Rows split over blocks, and more rows than are split: every kind of cut, equal logits, masks."""
     g = gen(V)
