@@ -24,6 +24,7 @@ struct GnShape {
     int tiles;         // tiles of channels per sample
     int pieces;        // pieces of a sample's positions
     int piece_rows;    // positions of a piece
+    int samples;       // samples of a block (one-block forms; 1 otherwise)
 };
 
 // (exponential and reciprocal as the hardware has them: an ulp each, and |z| u from the product with log2 e)
@@ -76,7 +77,8 @@ __device__ __forceinline__ GnMoments gn_join(GnMoments a, GnMoments b) {
 // What a thread works on: E channels from `c` on (those below c_end are real), positions row0, row0 + rows, ... of the piece
 struct GnPlace {
     int c, c_end, first_group, groups;  // the tile's groups
-    int col, row0, rows;                // column of vectors, first position, positions per step
+    int col, row0, rows;                // column of vectors, row of threads, rows of threads
+    int sample, first, step;            // one-block forms: the thread's sample in the block, its first position, and how far the next one is
     bool active;
     long long p_begin, p_end;
 };
@@ -100,6 +102,12 @@ __device__ __forceinline__ GnPlace gn_place(const GnShape &s, int tile, int piec
     w.col = threadIdx.x % vectors;
     w.row0 = threadIdx.x / vectors;
     w.active = w.row0 < w.rows;
+    w.sample = 0, w.first = w.row0, w.step = w.rows;
+    if (s.samples > 1) {
+        w.step = (int)s.P;
+        w.sample = w.row0 / w.step, w.first = w.row0 % w.step;
+        w.active = w.active && w.sample < s.samples;
+    }
     w.c = c0 + w.col * E;
     w.p_begin = (long long)piece * s.piece_rows;
     w.p_end = min(w.p_begin + s.piece_rows, s.P);
@@ -127,8 +135,8 @@ __device__ __forceinline__ void gn_write(T *p, int real, const float (&f)[E]) {
     }
 }
 
-// Sums of the tile's groups: every thread brings one value per channel, sums[g] (in LDS) are the groups' totals.  slots: LDS of
-// threads * E floats.
+// Sums of the tile's groups: every thread brings one value per channel, sums[sample * groups + g] (in LDS) are the groups' totals.
+// slots: LDS of threads * E floats.
 template <int E, int THREADS>
 __device__ void gn_group_sums(const GnShape &s, const GnPlace &w, const float (&v)[E], float *slots, float *sums) {
     const int width = w.c_end - (w.c - w.col * E);  // channels of the tile
@@ -145,12 +153,18 @@ __device__ void gn_group_sums(const GnShape &s, const GnPlace &w, const float (&
     }
     __syncthreads();
     const int per_row = by_vector ? vectors : vectors * E, per_group = s.tile_groups == 0 ? per_row : (by_vector ? s.cg / E : s.cg);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int g = wave; g < w.groups; g += THREADS / 64) {
+    // as many lanes as a group has values
+    const int rows = s.samples > 1 ? (int)s.P : w.rows, n = rows * per_group, all = s.samples * w.groups;
+    int lanes = 64;
+    while (lanes > 1 && n <= lanes / 2) lanes >>= 1;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, at_once = 64 / lanes;
+    for (int k0 = wave * at_once; k0 < all; k0 += THREADS / 64 * at_once) {
+        const int k = k0 + lane / lanes, g = k % w.groups, row0 = k / w.groups * rows;
         float t = 0.0f;
-        for (int j = lane; j < w.rows * per_group; j += 64) t += slots[(j / per_group) * per_row + g * per_group + j % per_group];
-        t = gn_wave_sum(t);
-        if (lane == 0) sums[g] = t;
+        if (k < all)
+            for (int j = lane % lanes; j < n; j += lanes) t += slots[(row0 + j / per_group) * per_row + g * per_group + j % per_group];
+        for (int o = lanes >> 1; o > 0; o >>= 1) t += __shfl_xor(t, o);
+        if (k < all && lane % lanes == 0) sums[k] = t;
     }
     __syncthreads();
 }
@@ -161,7 +175,11 @@ template <int E, int THREADS>
 __device__ void gn_channel_sums(const GnPlace &w, int width, const float (&v)[E], float *slots, float *totals) {
     const int vectors = (width + E - 1) / E, padded = vectors * E;
     __syncthreads();
-    if (w.active) dl_store(slots + threadIdx.x * E, v);
+    if ((int)threadIdx.x < w.rows * vectors) {
+        const float zero[E] = {};
+        if (w.active) dl_store(slots + threadIdx.x * E, v);
+        else dl_store(slots + threadIdx.x * E, zero);
+    }
     __syncthreads();
     const int shares = max(1, THREADS / padded);
     float t = 0.0f;
@@ -208,16 +226,17 @@ __device__ __forceinline__ void gn_values(dl_words &w, float (&f)[E]) {
     dl_unpack<T>(w, f);
 }
 
-// A sample's tile in one block: the values stay in registers from the one read to y.
+// A sample's tile - or several small samples - in one block: the values stay in registers from the one read to y.
 template <typename T, bool VEC, int NV, int THREADS, int ACT>
 __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ x, const void *__restrict__ gamma,
                                                            const void *__restrict__ beta, int ptype, T *__restrict__ y,
                                                            float2 *__restrict__ stats, GnShape s, float eps) {
     constexpr int E = 16 / sizeof(T);
     __shared__ float slots[THREADS * E], sums[GN_ONE_WIDTH];
-    const int tile = blockIdx.x % s.tiles, b = blockIdx.x / s.tiles;
-    const GnPlace w = gn_place<E>(s, tile, 0, THREADS);
-    const int real = w.c_end - w.c, c0 = w.c - w.col * E;
+    const int tile = blockIdx.x % s.tiles, b0 = blockIdx.x / s.tiles * s.samples;
+    GnPlace w = gn_place<E>(s, tile, 0, THREADS);
+    const int real = w.c_end - w.c, c0 = w.c - w.col * E, b = b0 + w.sample;
+    w.active = w.active && b < s.B;
     const long long base = (long long)b * s.P * s.C + w.c;
     const int P = (int)s.P;
     dl_words v[NV];
@@ -225,12 +244,12 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
     float t[E], m[E], ga[E], be[E];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int p = w.row0 + i * w.rows;
+        const int p = w.first + i * w.step;
         v[i] = w.active && p < P ? gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real) : dl_words{0, 0, 0, 0};
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        group[e] = w.active && e < real ? (w.c + e - c0) / s.cg : 0;
+        group[e] = w.active && e < real ? w.sample * w.groups + (w.c + e - c0) / s.cg : 0;
         ga[e] = w.active && e < real ? gn_param(gamma, ptype, w.c + e, 1.0f) : 0.0f;
         be[e] = w.active && e < real ? gn_param(beta, ptype, w.c + e, 0.0f) : 0.0f;
         t[e] = 0.0f;
@@ -252,12 +271,12 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
     __syncthreads();
     float mean[E];  // of the groups that this thread reports
 #pragma unroll
-    for (int k = 0; k < E; ++k) mean[k] = (int)(threadIdx.x + k * THREADS) < w.groups ? sums[threadIdx.x + k * THREADS] * per : 0.0f;
+    for (int k = 0; k < E; ++k) mean[k] = (int)(threadIdx.x + k * THREADS) < s.samples * w.groups ? sums[threadIdx.x + k * THREADS] * per : 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float f[E];
         gn_values<T>(v[i], f);
-        if (!w.active || w.row0 + i * w.rows >= P) continue;
+        if (!w.active || w.first + i * w.step >= P) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float d = e < real ? f[e] - m[e] : 0.0f;
@@ -267,15 +286,15 @@ __global__ __launch_bounds__(THREADS) void gn_forward_one(const T *__restrict__ 
     gn_group_sums<E, THREADS>(s, w, t, slots, sums);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-        const int g = threadIdx.x + k * THREADS;
-        if (g < w.groups) stats[(long long)b * s.G + w.first_group + g] = make_float2(mean[k], 1.0f / sqrtf(fmaf(sums[g], per, eps)));
+        const int g = threadIdx.x + k * THREADS, of = b0 + g / w.groups;
+        if (g < s.samples * w.groups && of < s.B) stats[(long long)of * s.G + w.first_group + g % w.groups] = make_float2(mean[k], 1.0f / sqrtf(fmaf(sums[g], per, eps)));
     }
     if (!w.active) return;
 #pragma unroll
     for (int e = 0; e < E; ++e) ga[e] *= 1.0f / sqrtf(fmaf(sums[group[e]], per, eps));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int p = w.row0 + i * w.rows;
+        const int p = w.first + i * w.step;
         float o[E];
         gn_values<T>(v[i], o);
         if (p >= P) continue;
@@ -406,21 +425,22 @@ struct GnChannels {
     }
 };
 
-// A sample's tile in one block: x and gy stay in registers from the one read to gx; the channels' sums go to [B][2][C].
+// A sample's tile in one block: x and gy stay in registers from the one read to gx; the channels' sums over the block's samples go to [blocks][2][C].
 template <typename T, bool VEC, int NV, int THREADS, int ACT>
 __global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
                                                             const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
                                                             float *__restrict__ channel, T *__restrict__ gx, GnShape s) {
     constexpr int E = 16 / sizeof(T);
     __shared__ float slots[THREADS * E], sum_g[GN_ONE_WIDTH + E], sum_x[GN_ONE_WIDTH + E], mean_g[GN_ONE_WIDTH];
-    const int tile = blockIdx.x % s.tiles, b = blockIdx.x / s.tiles;
-    const GnPlace w = gn_place<E>(s, tile, 0, THREADS);
-    const int real = w.c_end - w.c, c0 = w.c - w.col * E, width = w.c_end - c0, P = (int)s.P;
+    const int tile = blockIdx.x % s.tiles, block = blockIdx.x / s.tiles;
+    GnPlace w = gn_place<E>(s, tile, 0, THREADS);
+    const int real = w.c_end - w.c, c0 = w.c - w.col * E, width = w.c_end - c0, P = (int)s.P, b = min(block * s.samples + w.sample, s.B - 1);
+    w.active = w.active && block * s.samples + w.sample < s.B;
     const long long base = (long long)b * s.P * s.C + w.c;
     dl_words v[NV] = {}, d[NV] = {};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int p = w.row0 + i * w.rows;
+        const int p = w.first + i * w.step;
         if (w.active && p < P) {
             v[i] = gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real);
             d[i] = gn_raw<T, E, VEC>(gy + base + (long long)p * s.C, real);
@@ -432,7 +452,7 @@ __global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__
     for (int i = 0; i < NV; ++i) {
         float x_[E], d_[E];
         gn_values<T>(v[i], x_), gn_values<T>(d[i], d_);
-        if (!w.active || w.row0 + i * w.rows >= P) continue;
+        if (!w.active || w.first + i * w.step >= P) continue;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             float hat, g;
@@ -444,35 +464,44 @@ __global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__
     gn_channel_sums<E, THREADS>(w, width, sg, slots, sum_g);
     gn_channel_sums<E, THREADS>(w, width, sx, slots, sum_x);
     for (int c = threadIdx.x; c < width; c += THREADS) {
-        channel[(long long)b * 2 * s.C + c0 + c] = sum_g[c];
-        channel[(long long)b * 2 * s.C + s.C + c0 + c] = sum_x[c];
+        channel[(long long)block * 2 * s.C + c0 + c] = sum_g[c];
+        channel[(long long)block * 2 * s.C + s.C + c0 + c] = sum_x[c];
     }
     if (!gx) return;
-    // the groups' means, a wavefront each
-    float *const mean_x = slots;  // (a group has a channel, a channel a slot)
+    // the groups' means: of one sample from its channels' sums, a wavefront each
+    float *mean_x = slots;  // (a group has a channel, a channel a slot)
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const float per = 1.0f / ((float)P * (float)s.cg);
-    for (int g = wave; g < w.groups; g += THREADS / 64) {
-        float a = 0.0f, q = 0.0f;
-        for (int c = lane; c < s.cg; c += 64) {
-            const float gam = gn_param(gamma, ptype, c0 + g * s.cg + c, 1.0f);
-            a = fmaf(gam, sum_g[g * s.cg + c], a);
-            q = fmaf(gam, sum_x[g * s.cg + c], q);
+    if (s.samples > 1) {
+        mean_x = sum_x;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sg[e] *= ch.ga[e] * per, sx[e] *= ch.ga[e] * per;
+        __syncthreads();  // the channels' sums have been read
+        gn_group_sums<E, THREADS>(s, w, sg, slots, mean_g);
+        gn_group_sums<E, THREADS>(s, w, sx, slots, mean_x);
+    } else {
+        for (int g = wave; g < w.groups; g += THREADS / 64) {
+            float a = 0.0f, q = 0.0f;
+            for (int c = lane; c < s.cg; c += 64) {
+                const float gam = gn_param(gamma, ptype, c0 + g * s.cg + c, 1.0f);
+                a = fmaf(gam, sum_g[g * s.cg + c], a);
+                q = fmaf(gam, sum_x[g * s.cg + c], q);
+            }
+            a = gn_wave_sum(a), q = gn_wave_sum(q);
+            if (lane == 0) mean_g[g] = a * per, mean_x[g] = q * per;
         }
-        a = gn_wave_sum(a), q = gn_wave_sum(q);
-        if (lane == 0) mean_g[g] = a * per, mean_x[g] = q * per;
     }
     __syncthreads();
     if (!w.active) return;
     float ma[E], mq[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int g = e < real ? (w.c + e - c0) / s.cg : 0;
+        const int g = w.sample * w.groups + (e < real ? (w.c + e - c0) / s.cg : 0);
         ma[e] = mean_g[g], mq[e] = mean_x[g];
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int p = w.row0 + i * w.rows;
+        const int p = w.first + i * w.step;
         float x_[E], o[E];
         gn_values<T>(v[i], x_), gn_values<T>(d[i], o);
         if (p >= P) continue;
@@ -593,26 +622,28 @@ __global__ __launch_bounds__(THREADS) void gn_backward_apply(const T *__restrict
     }
 }
 
-// ggamma_c = sum_b sum g xhat, gbeta_c = sum_b sum g: 32 channels x 8 samples a step per block, added in a fixed order.
-__global__ __launch_bounds__(256) void gn_param_grads(const float *__restrict__ channel, void *__restrict__ ggamma, void *__restrict__ gbeta,
-                                                       int ptype, int B, int C) {
+// ggamma_c = sum g xhat, gbeta_c = sum g over n rows of [2][C]: a block takes 32 channels of a share of the rows, 8 at a step, added in a
+// fixed order.  With `part` the shares' sums go there, as rows of the same kind.
+__global__ __launch_bounds__(256) void gn_param_grads(const float *__restrict__ channel, float *__restrict__ part, void *__restrict__ ggamma,
+                                                       void *__restrict__ gbeta, int ptype, int n, int C, int share) {
     __shared__ float red[2][8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+    const int columns = (C + 31) / 32, c = blockIdx.x % columns * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5, mine = blockIdx.x / columns;
     float sg = 0.0f, sx = 0.0f;
+    const int end = min((mine + 1) * (long long)share, (long long)n);
     if (c < C)
 #pragma unroll 8
-        for (int b = r; b < B; b += 8) {
-            sg += channel[(long long)b * 2 * C + c];
-            sx += channel[(long long)b * 2 * C + C + c];
+        for (int i = mine * share + r; i < end; i += 8) {
+            sg += channel[(long long)i * 2 * C + c];
+            sx += channel[(long long)i * 2 * C + C + c];
         }
     red[0][r][threadIdx.x & 31] = sg, red[1][r][threadIdx.x & 31] = sx;
     __syncthreads();
-    if (threadIdx.x >= 64) return;
-    const int which = threadIdx.x >> 5, cc = blockIdx.x * 32 + (threadIdx.x & 31);
-    if (cc >= C) return;
+    if (threadIdx.x >= 64 || c >= C) return;
+    const int which = threadIdx.x >> 5;
     float t = 0.0f;
     for (int i = 0; i < 8; ++i) t += red[which][i][threadIdx.x & 31];
-    gn_param_store(which ? ggamma : gbeta, ptype, cc, t);
+    if (part) part[((long long)mine * 2 + which) * C + c] = t;
+    else gn_param_store(which ? ggamma : gbeta, ptype, c, t);
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -638,7 +669,7 @@ static GnShape gn_tiles(int B, long long P, int C, int G, int E, int threads) {
         s.tile_width = s.tile_groups * s.cg;
         s.tiles = dl_ceil_div(G, s.tile_groups);
     }
-    s.pieces = 1;
+    s.pieces = s.samples = 1;
     s.piece_rows = (int)(P < (1 << 30) ? P : (1 << 30));
     return s;
 }
@@ -664,13 +695,15 @@ static int gn_rows_per_step(const GnShape &s, int E, int threads) {
 #define GN_ONE_THREADS 1024
 // 16-byte units that a thread of the one-block forms holds, of x, or of x and of gy: about 48 registers (64 spill)
 #define GN_ONE_FORWARD(E) ((E) == 8 ? 10 : 12)
-#define GN_ONE_BACKWARD 6
+#define GN_ONE_BACKWARD(E) ((E) == 8 ? 5 : 6)
+#define GN_SHARES 64  // of many samples, in the sums of the parameters' gradients
 
 static GnShape gn_pieces_shape(int B, long long P, int C, int G, int E) {
     GnShape s = gn_tiles(B, P, C, G, E, GN_THREADS);
     gn_pieces(s, gn_rows_per_step(s, E, GN_THREADS) * 4, 1024);
     return s;
 }
+static int gn_blocks(const GnShape &s) { return dl_ceil_div(s.B, s.samples) * s.tiles; }  // of the one-block forms
 static bool gn_grid_ok(const GnShape &s) { return (long long)s.B * s.tiles * s.pieces < (1LL << 31); }
 
 // The one-block form: tiles of whole groups over all of a sample's positions that a block's registers hold; false where there are
@@ -690,8 +723,13 @@ static bool gn_one_shape(GnShape &s, int B, long long P, int C, int G, int E, in
         s.tiles = dl_ceil_div(G, groups);
         s.pieces = 1;
         s.piece_rows = (int)P;
-        if ((s.tile_width + E - 1) / E <= threads && s.tile_width <= GN_ONE_WIDTH && (long long)gn_rows_per_step(s, E, threads) * units >= P)
+        const int rows = gn_rows_per_step(s, E, threads);
+        if ((s.tile_width + E - 1) / E <= threads && s.tile_width <= GN_ONE_WIDTH && (long long)rows * units >= P) {
+            // small samples share a block, as long as there are 512 of those (65536 rows of 64 channels: 16 a block)
+            if (groups == G && threads == GN_THREADS)
+                for (s.samples = P <= rows ? (int)(rows / P) : 1; s.samples > 1 && dl_ceil_div(B, s.samples) < 512;) s.samples /= 2;
             return groups == G || s.tile_width >= 4 * E || (long long)B * P * C <= (1 << 18);
+        }
     }
     return false;
 }
@@ -734,7 +772,7 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
             const bool vec = gn_vectors(s, E, x, y, nullptr);
             dl_prof_begin("gn_forward_one", st);
 #define ONE(VEC, NV, THREADS) \
-    gn_forward_one<T, VEC, NV, THREADS, ACT><<<s.B * s.tiles, THREADS, 0, st>>>((const T *)x, gamma, beta, ptype, (T *)y, (float2 *)stats, s, eps)
+    gn_forward_one<T, VEC, NV, THREADS, ACT><<<gn_blocks(s), THREADS, 0, st>>>((const T *)x, gamma, beta, ptype, (T *)y, (float2 *)stats, s, eps)
             DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
                                           else { if (vec) ONE(true, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
 #undef ONE
@@ -759,7 +797,7 @@ extern "C" size_t dl_group_norm_bwd_workspace_bytes(int type, int B, long long P
     if (!dl_type_known(type) || !gn_shape_ok(B, P, C, G)) return 0;
     const GnShape s = gn_pieces_shape(B, P, C, G, 16 / dl_type_bytes(type));
     return dl_align256((size_t)B * s.pieces * 2 * C * sizeof(float)) + dl_align256((size_t)B * 2 * C * sizeof(float)) +
-           dl_align256((size_t)B * G * sizeof(float2));
+           dl_align256((size_t)B * G * sizeof(float2)) + dl_align256((size_t)GN_SHARES * 2 * C * sizeof(float));
 }
 
 extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamma, const void *beta, const float *stats, void *gx,
@@ -773,20 +811,21 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     const int E = 16 / dl_type_bytes(type);
     float *channel = (float *)ws;
     float2 *group = (float2 *)((char *)channel + dl_align256((size_t)B * 2 * C * sizeof(float)));
-    float *part = (float *)((char *)group + dl_align256((size_t)B * G * sizeof(float2)));
+    float *shares = (float *)((char *)group + dl_align256((size_t)B * G * sizeof(float2)));
+    float *part = (float *)((char *)shares + dl_align256((size_t)GN_SHARES * 2 * C * sizeof(float)));
     GnShape s;
     bool one = false;
     for (const int threads : {GN_THREADS, GN_ONE_THREADS}) {
-        one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD, threads);
+        one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD(E), threads);
         if (!one) continue;
         if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
         const bool vec = gn_vectors(s, E, x, gy, gx);
         dl_prof_begin("gn_backward_one", st);
 #define ONE(VEC, NV, THREADS) \
-    gn_backward_one<T, VEC, NV, THREADS, ACT><<<s.B * s.tiles, THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
+    gn_backward_one<T, VEC, NV, THREADS, ACT><<<gn_blocks(s), THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
                                                                                  (const float2 *)stats, channel, (T *)gx, s)
         DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
-                                      else { if (vec) ONE(true, GN_ONE_BACKWARD, GN_ONE_THREADS); else ONE(false, GN_ONE_BACKWARD, GN_ONE_THREADS); }));
+                                      else { if (vec) ONE(true, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
 #undef ONE
         dl_prof_end(st);
         break;
@@ -806,7 +845,16 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
         DL_BY_TYPE(type, T, if (vec) { BACKWARD(true); } else { BACKWARD(false); });
 #undef BACKWARD
     }
-    if (ggamma || gbeta)
-        DL_TIMED("gn_param_grads", st, (gn_param_grads<<<dl_ceil_div(C, 32), 256, 0, st>>>(channel, ggamma, gbeta, ptype, B, C)));
+    if (ggamma || gbeta) {
+        int n = one ? dl_ceil_div(B, s.samples) : B;
+        const float *rows = channel;
+        const int columns = dl_ceil_div(C, 32);
+        if (n > 512) {  // first in shares
+            const int share = dl_ceil_div(n, GN_SHARES), count = dl_ceil_div(n, share);
+            DL_TIMED("gn_param_grads", st, (gn_param_grads<<<columns * count, 256, 0, st>>>(rows, shares, nullptr, nullptr, ptype, n, C, share)));
+            n = count, rows = shares;
+        }
+        DL_TIMED("gn_param_grads", st, (gn_param_grads<<<columns, 256, 0, st>>>(rows, nullptr, ggamma, gbeta, ptype, n, C, n)));
+    }
     return dl_launch_status();
 }

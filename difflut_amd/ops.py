@@ -517,6 +517,8 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
         raise TypeError(f"tokens must be int32 or int64, got {tokens.dtype}")
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}), got {padding_idx}")
+    if isinstance(scale, bool) or not isinstance(scale, (int, float)):
+        raise TypeError(f"scale must be a number, got {type(scale).__name__}")
     padding = -1 if padding_idx is None else int(padding_idx)
     if weight.is_cuda:
         return nat.host().embedding(tokens, weight, float(scale), padding)

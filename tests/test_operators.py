@@ -280,10 +280,10 @@ def test_group_norm_gradient_against_differences():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,space,C,G", [(2, (130, 130), 40, 8), (1, (40000,), 6, 3), (3, (900,), 1100, 1), (1, (6001,), 2500, 1), (1, (70, 300), 64, 64),
-                                         (300, (64,), 96, 4), (9, (130,), 250, 5)])
+                                         (300, (64,), 96, 4), (9, (130,), 250, 5), (5000, (), 64, 8), (3001, (3,), 24, 6), (2049, (), 7, 7), (1100, (2,), 36, 4)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_group_norm_of_larger_tensors(B, space, C, G, dtype):
-    """Samples split over blocks, wide groups in slices, and what still fits one block; twice the same bits."""
+    """Samples split over blocks, wide groups in slices, what still fits one block, small samples that share one; twice the same bits."""
     g = gen(C + G)
     x, gy = ((torch.randn(B, *space, C, generator=g) * 0.4 + m).to(dtype) for m in (0.5, 0.0))
     weight, bias = ((torch.randn(C, generator=g) * 0.2 + m).to(dtype) for m in (1.0, 0.0))
@@ -606,7 +606,7 @@ def test_refusals(device):
             (ValueError, lambda: ops.embedding(t, w[0])), (ValueError, lambda: ops.embedding(t, w[:0])),
             (TypeError, lambda: ops.embedding(t.float(), w)), (TypeError, lambda: ops.embedding(t.short(), w)),
             (ValueError, lambda: ops.embedding(t, w, padding_idx=4)), (ValueError, lambda: ops.embedding(t, w, padding_idx=-1)),
-            (TypeError, lambda: ops.embedding(t, w.int())),
+            (TypeError, lambda: ops.embedding(t, w.int())), (TypeError, lambda: ops.embedding(t, w, scale=torch.ones(1, requires_grad=True))),
             (ValueError, lambda: ops.group_norm(x, 4)), (ValueError, lambda: ops.group_norm(x, 0)), (ValueError, lambda: ops.group_norm(x, 2.0)),
             (ValueError, lambda: ops.group_norm(x[:0], 2)), (ValueError, lambda: ops.group_norm(x[0, 0], 2)),
             (ValueError, lambda: ops.group_norm(x, 2, activation="tanh")), (ValueError, lambda: ops.group_norm(x, 2, eps=-1.0)),
@@ -625,6 +625,52 @@ def test_refusals(device):
             (ValueError, lambda: ops.sample(logits, u, min_p=1.5)), (TypeError, lambda: ops.sample(logits, u, top_k=u)), (ValueError, lambda: ops.sample(logits, u, top_p=u[:1]))]:
         with pytest.raises(error):
             call()
+
+
+def test_c_entry_points_refuse():
+    """Null pointers, unknown types and options, sizes that do not fit, short workspaces: an error before anything is launched."""
+    from difflut_amd import _native as nat
+
+    if not nat.is_built():
+        pytest.skip("not built")
+    lib = nat.lib()
+    at, null, shape, unsupported, short = 4096, -1, -2, -3, -4  # (an address that is never followed)
+    big = 1 << 40
+    for want, call in [
+            (unsupported, lambda: lib.dl_dropout(at, at, 7, 10, 0.5, 0, 0, 0, None, None, None)),
+            (unsupported, lambda: lib.dl_dropout(at, at, 0, 10, 0.5, 2, 0, 0, None, None, None)),
+            (shape, lambda: lib.dl_dropout(at, at, 0, -1, 0.5, 0, 0, 0, None, None, None)),
+            (shape, lambda: lib.dl_dropout(at, at, 0, 10, 1.5, 0, 0, 0, None, None, None)),
+            (shape, lambda: lib.dl_dropout(at, at, 0, 10, math.nan, 0, 0, 0, None, None, None)),
+            (null, lambda: lib.dl_dropout(None, at, 0, 10, 0.5, 0, 0, 0, None, None, None)),
+            (0, lambda: lib.dl_dropout(None, None, 0, 0, 0.5, 0, 0, 0, None, None, None)),
+            (unsupported, lambda: lib.dl_embedding_fwd(at, 16, at, 8, at, 0, 4, 5, 8, 1.0, None)),
+            (unsupported, lambda: lib.dl_embedding_fwd(at, 64, at, 8, at, 3, 4, 5, 8, 1.0, None)),
+            (shape, lambda: lib.dl_embedding_fwd(at, 64, at, 7, at, 0, 4, 5, 8, 1.0, None)),
+            (shape, lambda: lib.dl_embedding_fwd(at, 64, at, 8, at, 0, big, 5, 8, 1.0, None)),
+            (shape, lambda: lib.dl_embedding_fwd(at, 64, at, 8, at, 0, 4, big, 8, 1.0, None)),
+            (null, lambda: lib.dl_embedding_fwd(at, 64, None, 8, at, 0, 4, 5, 8, 1.0, None)),
+            (null, lambda: lib.dl_embedding_bwd(at, 64, at, None, 0, 4, 5, 8, 1.0, -1, at, big, None)),
+            (null, lambda: lib.dl_embedding_bwd(at, 64, None, at, 0, 4, 5, 8, 1.0, -1, at, big, None)),
+            (short, lambda: lib.dl_embedding_bwd(at, 64, at, at, 0, 4, 5, 8, 1.0, -1, at, lib.dl_embedding_bwd_workspace_bytes(4, 5, 8) - 1, None)),
+            (null, lambda: lib.dl_group_norm_fwd(at, at, at, at, None, 0, 0, 2, 3, 8, 2, 1e-5, 0, at, big, None)),
+            (unsupported, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 9, 2, 3, 8, 2, 1e-5, 0, at, big, None)),
+            (unsupported, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 0, 2, 3, 8, 2, 1e-5, 4, at, big, None)),
+            (shape, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 0, 2, 3, 8, 3, 1e-5, 0, at, big, None)),
+            (shape, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 0, 2, 3, 8, 2, -1.0, 0, at, big, None)),
+            (shape, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 0, 2, big, 8, 2, 1e-5, 0, at, big, None)),
+            (short, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 0, 2, 3, 8, 2, 1e-5, 0, at, 8, None)),
+            (null, lambda: lib.dl_group_norm_bwd(at, at, at, at, at, None, None, None, 0, 0, 2, 3, 8, 2, 0, at, big, None)),
+            (short, lambda: lib.dl_group_norm_bwd(at, at, at, at, at, at, None, None, 0, 0, 2, 3, 8, 2, 0, at, 8, None)),
+            (unsupported, lambda: lib.dl_sample(at, 8, 5, at, None, None, None, None, 1.0, 0, 1.0, 0.0, at, None, 0, 2, 8, None)),
+            (shape, lambda: lib.dl_sample(at, 7, 0, at, None, None, None, None, 1.0, 0, 1.0, 0.0, at, None, 0, 2, 8, None)),
+            (shape, lambda: lib.dl_sample(at, 8, 0, at, None, None, None, None, 1.0, 0, 1.0, 0.0, at, None, 0, 2, 0, None)),
+            (null, lambda: lib.dl_sample(at, 8, 0, None, None, None, None, None, 1.0, 0, 1.0, 0.0, at, None, 0, 2, 8, None)),
+            (null, lambda: lib.dl_sample(at, 1 << 20, 0, at, None, None, None, None, 1.0, 0, 0.5, 0.0, at, None, 0, 1, 1 << 20, None)),
+            (short, lambda: lib.dl_sample(at, 1 << 20, 0, at, None, None, None, None, 1.0, 0, 0.5, 0.0, at, at, 8, 1, 1 << 20, None)),
+            (0, lambda: lib.dl_sample(None, 8, 0, None, None, None, None, None, 1.0, 0, 1.0, 0.0, None, None, 0, 0, 8, None))]:
+        assert call() == want
+    assert lib.dl_group_norm_fwd_workspace_bytes(0, 2, 3, 8, 3) == 0 and lib.dl_embedding_bwd_workspace_bytes(-1, 5, 8) == 0
 
 
 def test_module_refusals():
