@@ -11,6 +11,8 @@
 // are joined by the pairwise formula (Chan, Golub, LeVeque 1979), in a fixed order: results are the same bits from run to run.
 #include "dl_types.h"
 
+#define GN_THREADS 256
+#define GN_ONE_THREADS 1024
 #define GN_ONE_WIDTH 2048  // channels of a tile of the one-block forms
 
 enum { GN_NONE = DL_ACT_NONE, GN_RELU = DL_ACT_RELU, GN_SILU = DL_ACT_SILU, GN_SIGMOID = DL_ACT_SIGMOID };
@@ -162,6 +164,7 @@ __device__ void gn_group_sums(const GnShape &s, const GnPlace &w, const float (&
         const int k = k0 + lane / lanes, g = k % w.groups, row0 = k / w.groups * rows;
         float t = 0.0f;
         if (k < all)
+#pragma unroll 2
             for (int j = lane % lanes; j < n; j += lanes) t += slots[(row0 + j / per_group) * per_row + g * per_group + j % per_group];
         for (int o = lanes >> 1; o > 0; o >>= 1) t += __shfl_xor(t, o);
         if (k < all && lane % lanes == 0) sums[k] = t;
@@ -425,94 +428,91 @@ struct GnChannels {
     }
 };
 
-// A sample's tile in one block: x and gy stay in registers from the one read to gx; the channels' sums over the block's samples go to [blocks][2][C].
+// A sample's tile - or several small samples - in one block: x and gy stay in registers from the one read to gx.  A block takes every
+// gridDim.x / tiles-th one: its channels are the same ones, whose sums stay in registers until the last; they go to
+// [gridDim.x / tiles][2][C].
 template <typename T, bool VEC, int NV, int THREADS, int ACT>
-__global__ __launch_bounds__(THREADS) void gn_backward_one(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
+__global__ __launch_bounds__(THREADS, NV == 1 ? 4 : 1) void gn_backward_one(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
                                                             const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
                                                             float *__restrict__ channel, T *__restrict__ gx, GnShape s) {
     constexpr int E = 16 / sizeof(T);
-    __shared__ float slots[THREADS * E], sum_g[GN_ONE_WIDTH + E], sum_x[GN_ONE_WIDTH + E], mean_g[GN_ONE_WIDTH];
-    const int tile = blockIdx.x % s.tiles, block = blockIdx.x / s.tiles;
-    GnPlace w = gn_place<E>(s, tile, 0, THREADS);
-    const int real = w.c_end - w.c, c0 = w.c - w.col * E, width = w.c_end - c0, P = (int)s.P, b = min(block * s.samples + w.sample, s.B - 1);
-    w.active = w.active && block * s.samples + w.sample < s.B;
-    const long long base = (long long)b * s.P * s.C + w.c;
-    dl_words v[NV] = {}, d[NV] = {};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int p = w.first + i * w.step;
-        if (w.active && p < P) {
-            v[i] = gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real);
-            d[i] = gn_raw<T, E, VEC>(gy + base + (long long)p * s.C, real);
-        }
-    }
-    const GnChannels<E> ch(s, w, b, stats, gamma, beta, ptype);
-    float sg[E] = {}, sx[E] = {};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float x_[E], d_[E];
-        gn_values<T>(v[i], x_), gn_values<T>(d[i], d_);
-        if (!w.active || w.first + i * w.step >= P) continue;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            float hat, g;
-            ch.template at<ACT>(e, x_[e], d_[e], hat, g);
-            sg[e] += g;
-            sx[e] = fmaf(g, hat, sx[e]);
-        }
-    }
-    gn_channel_sums<E, THREADS>(w, width, sg, slots, sum_g);
-    gn_channel_sums<E, THREADS>(w, width, sx, slots, sum_x);
-    for (int c = threadIdx.x; c < width; c += THREADS) {
-        channel[(long long)block * 2 * s.C + c0 + c] = sum_g[c];
-        channel[(long long)block * 2 * s.C + s.C + c0 + c] = sum_x[c];
-    }
-    if (!gx) return;
-    // the groups' means: of one sample from its channels' sums, a wavefront each
-    float *mean_x = slots;  // (a group has a channel, a channel a slot)
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    __shared__ float slots[THREADS * E], mean_g[GN_ONE_WIDTH + E], mean_x[GN_ONE_WIDTH + E];
+    const int tile = blockIdx.x % s.tiles, block0 = blockIdx.x / s.tiles, blocks = gridDim.x / s.tiles;
+    const GnPlace w = gn_place<E>(s, tile, 0, THREADS);
+    const int real = w.c_end - w.c, c0 = w.c - w.col * E, width = w.c_end - c0, P = (int)s.P;
     const float per = 1.0f / ((float)P * (float)s.cg);
-    if (s.samples > 1) {
-        mean_x = sum_x;
+    float all_g[E] = {}, all_x[E] = {};
+    for (int block = block0; (long long)block * s.samples < s.B; block += blocks) {
+        const int b = min(block * s.samples + w.sample, s.B - 1);
+        GnPlace here = w;
+        here.active = w.active && block * s.samples + w.sample < s.B;
+        const long long base = (long long)b * s.P * s.C + w.c;
+        dl_words v[NV] = {}, d[NV] = {};
 #pragma unroll
-        for (int e = 0; e < E; ++e) sg[e] *= ch.ga[e] * per, sx[e] *= ch.ga[e] * per;
-        __syncthreads();  // the channels' sums have been read
-        gn_group_sums<E, THREADS>(s, w, sg, slots, mean_g);
-        gn_group_sums<E, THREADS>(s, w, sx, slots, mean_x);
-    } else {
-        for (int g = wave; g < w.groups; g += THREADS / 64) {
-            float a = 0.0f, q = 0.0f;
-            for (int c = lane; c < s.cg; c += 64) {
-                const float gam = gn_param(gamma, ptype, c0 + g * s.cg + c, 1.0f);
-                a = fmaf(gam, sum_g[g * s.cg + c], a);
-                q = fmaf(gam, sum_x[g * s.cg + c], q);
+        for (int i = 0; i < NV; ++i) {
+            const int p = w.first + i * w.step;
+            if (here.active && p < P) {
+                v[i] = gn_raw<T, E, VEC>(x + base + (long long)p * s.C, real);
+                d[i] = gn_raw<T, E, VEC>(gy + base + (long long)p * s.C, real);
             }
-            a = gn_wave_sum(a), q = gn_wave_sum(q);
-            if (lane == 0) mean_g[g] = a * per, mean_x[g] = q * per;
         }
-    }
-    __syncthreads();
-    if (!w.active) return;
-    float ma[E], mq[E];
+        const GnChannels<E> ch(s, w, b, stats, gamma, beta, ptype);
+        float sg[E] = {}, sx[E] = {};
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int g = w.sample * w.groups + (e < real ? (w.c + e - c0) / s.cg : 0);
-        ma[e] = mean_g[g], mq[e] = mean_x[g];
-    }
+        for (int i = 0; i < NV; ++i) {
+            float x_[E], d_[E];
+            gn_values<T>(v[i], x_), gn_values<T>(d[i], d_);
+            if (!here.active || w.first + i * w.step >= P) continue;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int p = w.first + i * w.step;
-        float x_[E], o[E];
-        gn_values<T>(v[i], x_), gn_values<T>(d[i], o);
-        if (p >= P) continue;
+            for (int e = 0; e < E; ++e) {
+                float hat, g;
+                ch.template at<ACT>(e, x_[e], d_[e], hat, g);
+                sg[e] += g;
+                sx[e] = fmaf(g, hat, sx[e]);
+            }
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            float hat, g;
-            ch.template at<ACT>(e, x_[e], o[e], hat, g);
-            o[e] = ch.rstd[e] * (fmaf(g, ch.ga[e], -ma[e]) - hat * mq[e]);
+            all_g[e] += sg[e], all_x[e] += sx[e];
+            sg[e] *= ch.ga[e] * per, sx[e] *= ch.ga[e] * per;
         }
-        gn_write<T, E, VEC, false>(gx + base + (long long)p * s.C, real, o);
+        if (!gx) {
+            if constexpr (THREADS != GN_THREADS) break;
+            continue;
+        }
+        // the groups' means of gamma g and of gamma g xhat
+        gn_group_sums<E, THREADS>(s, here, sg, slots, mean_g);
+        gn_group_sums<E, THREADS>(s, here, sx, slots, mean_x);
+        if (here.active) {
+            float ma[E], mq[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int g = w.sample * w.groups + (e < real ? (w.c + e - c0) / s.cg : 0);
+                ma[e] = mean_g[g], mq[e] = mean_x[g];
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int p = w.first + i * w.step;
+                float x_[E], o[E];
+                gn_values<T>(v[i], x_), gn_values<T>(d[i], o);
+                if (p >= P) continue;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    float hat, g;
+                    ch.template at<ACT>(e, x_[e], o[e], hat, g);
+                    o[e] = ch.rstd[e] * (fmaf(g, ch.ga[e], -ma[e]) - hat * mq[e]);
+                }
+                gn_write<T, E, VEC, false>(gx + base + (long long)p * s.C, real, o);
+            }
+        }
+        if constexpr (THREADS != GN_THREADS) break;  // (one round: with a second one's values next to these the registers spill)
+        __syncthreads();  // the means have been read
     }
+    float *out = channel + (long long)block0 * 2 * s.C + c0;
+    gn_channel_sums<E, THREADS>(w, width, all_g, slots, slots);
+    for (int c = threadIdx.x; c < width; c += THREADS) out[c] = slots[c];
+    gn_channel_sums<E, THREADS>(w, width, all_x, slots, slots);
+    for (int c = threadIdx.x; c < width; c += THREADS) out[s.C + c] = slots[c];
 }
 
 // Per channel of a piece: sum g and sum g xhat, [B][pieces][2][C].
@@ -691,11 +691,9 @@ static int gn_rows_per_step(const GnShape &s, int E, int threads) {
     const int vectors = (s.tile_width + E - 1) / E;
     return threads / vectors > 0 ? threads / vectors : 1;
 }
-#define GN_THREADS 256
-#define GN_ONE_THREADS 1024
 // 16-byte units that a thread of the one-block forms holds, of x, or of x and of gy: about 48 registers (64 spill)
 #define GN_ONE_FORWARD(E) ((E) == 8 ? 10 : 12)
-#define GN_ONE_BACKWARD(E) ((E) == 8 ? 5 : 6)
+#define GN_ONE_BACKWARD(E) ((E) == 8 ? 4 : 6)
 #define GN_SHARES 64  // of many samples, in the sums of the parameters' gradients
 
 static GnShape gn_pieces_shape(int B, long long P, int C, int G, int E) {
@@ -770,10 +768,14 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
         if (gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_FORWARD(E), threads)) {
             if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
             const bool vec = gn_vectors(s, E, x, y, nullptr);
+            const bool few = s.samples > 1 || P <= gn_rows_per_step(s, E, threads);  // a position per thread
             dl_prof_begin("gn_forward_one", st);
 #define ONE(VEC, NV, THREADS) \
     gn_forward_one<T, VEC, NV, THREADS, ACT><<<gn_blocks(s), THREADS, 0, st>>>((const T *)x, gamma, beta, ptype, (T *)y, (float2 *)stats, s, eps)
-            DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
+            DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) {
+                if (few) { if (vec) ONE(true, 1, GN_THREADS); else ONE(false, 1, GN_THREADS); }
+                else { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
+            }
                                           else { if (vec) ONE(true, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
 #undef ONE
             dl_prof_end(st);
@@ -815,16 +817,24 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     float *part = (float *)((char *)shares + dl_align256((size_t)GN_SHARES * 2 * C * sizeof(float)));
     GnShape s;
     bool one = false;
+    int rows_out = B;  // of sums over samples
     for (const int threads : {GN_THREADS, GN_ONE_THREADS}) {
         one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD(E), threads);
         if (!one) continue;
         if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+        // of 256 threads as many blocks as the card holds at a time, rounds of them after that
+        const int most = 2048 / s.tiles, want = dl_ceil_div(B, s.samples);
+        rows_out = threads != GN_THREADS || want < most ? want : most > 0 ? most : 1;
         const bool vec = gn_vectors(s, E, x, gy, gx);
+        const bool few = s.samples > 1 || P <= gn_rows_per_step(s, E, threads);
         dl_prof_begin("gn_backward_one", st);
 #define ONE(VEC, NV, THREADS) \
-    gn_backward_one<T, VEC, NV, THREADS, ACT><<<gn_blocks(s), THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
+    gn_backward_one<T, VEC, NV, THREADS, ACT><<<rows_out * s.tiles, THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
                                                                                  (const float2 *)stats, channel, (T *)gx, s)
-        DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
+        DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) {
+                if (few) { if (vec) ONE(true, 1, GN_THREADS); else ONE(false, 1, GN_THREADS); }
+                else { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
+            }
                                       else { if (vec) ONE(true, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
 #undef ONE
         dl_prof_end(st);
@@ -846,7 +856,7 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
 #undef BACKWARD
     }
     if (ggamma || gbeta) {
-        int n = one ? dl_ceil_div(B, s.samples) : B;
+        int n = rows_out;
         const float *rows = channel;
         const int columns = dl_ceil_div(C, 32);
         if (n > 512) {  // first in shares

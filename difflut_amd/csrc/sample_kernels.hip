@@ -11,7 +11,7 @@
 // from exponentials in double: sums fit, are exact in any order - blocks and atomics can split them as they like, every run gives the
 // same index - and a weight is off by 2^-(shift + 1), 2^-46 at V = 131072.
 //
-// Up to 64 columns: a few lanes per row compare every pair.  Up to SMP_SORTED: a block sorts the row in LDS.  More: a block per row
+// Up to 64 columns: a few lanes per row compare every pair.  Up to SMP_WAVE: a wavefront per row, in its registers.  More: a block per row
 // (sample_row), which reads it once into its registers where it fits; or, for few long rows, four launches over pieces of rows
 // (sample_max, sample_hist, sample_collect, sample_draw).  Both go the same way:
 //   - the largest logit;
@@ -23,7 +23,7 @@
 //     (many equal logits) is searched over the whole row instead.
 #include "dl_types.h"
 
-#define SMP_SORTED 4096
+#define SMP_WAVE 1024
 #define SMP_BINS 2048
 #define SMP_BINS_PER_Z 32.0  // classes per unit of (max - l) / T: the last one holds what weighs less than e^-63.9, so nothing
 #define SMP_LIST 4096
@@ -239,11 +239,9 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_pairs(SampleArgs a) {
     if (i == 0 && b0 < a.B) a.out[b] = mine ? __builtin_ctzll(mine) : -1;
 }
 
-// ---------------------------------------------------------------------------------- a row in LDS
 // In index order, over [i0, i1): the first index whose running sum of kept weights exceeds `target`; a thread per run of indices.
 template <typename T, int THREADS>
-__device__ __forceinline__ void smp_draw(const SampleArgs &a, const SampleRow &r, int b, int i0, int i1, u64 cut, uint32_t top, bool draw_rest, u64 target,
-                         u64 *red) {
+__device__ __forceinline__ void smp_draw(const SampleArgs &a, const SampleRow &r, int b, int i0, int i1, u64 cut, uint32_t top, u64 target, u64 *red) {
     const T *row = (const T *)a.logits + b * a.ldl;
     const int per = (i1 - i0 + THREADS - 1) / THREADS, begin = min(i0 + (int)threadIdx.x * per, i1), end = min(begin + per, i1);
     u64 mine = 0, total;
@@ -255,11 +253,6 @@ __device__ __forceinline__ void smp_draw(const SampleArgs &a, const SampleRow &r
         for (; kept; kept &= kept - 1) mine += smp_weight(smp_key((float)row[i0 + __builtin_ctz(kept)]), top, r, a.shift);
     }
     u64 run = smp_scan<THREADS>(mine, total, red);
-    if (!draw_rest) target = total ? smp_target(r, total) : 0;
-    if (total == 0) {
-        if (threadIdx.x == 0) a.out[b] = -1;
-        return;
-    }
     // in the run of the thread that it falls into: a wavefront, an index a lane
     __shared__ int chosen;
     __shared__ u64 chosen_run;
@@ -285,44 +278,196 @@ __device__ __forceinline__ void smp_draw(const SampleArgs &a, const SampleRow &r
     }
 }
 
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_sorted(SampleArgs a, int n) {
-    extern __shared__ u64 pairs[];  // [n], n a power of two >= V
-    __shared__ u64 red[THREADS / 64];
-    const int b = blockIdx.x;
+// All that top-k keeps is in a list of n <= SMP_FEW_LISTED: the cuts and the draw by one wavefront, two pairs a lane, every pair against
+// every other one (no barrier and no sorting).  The list's room behind the pairs takes their weights.
+__device__ __forceinline__ void smp_few_draw(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, u64 *pairs, int n) {
+    const int lane = threadIdx.x & 63;
+    u64 *const weights = pairs + SMP_FEW_LISTED;
+    u64 p[2], w[2], before[2] = {}, run[2] = {}, in_k = 0, all = 0;
+    int rank[2] = {};
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const int i = m * 64 + lane;
+        p[m] = i < n ? pairs[i] : 0;
+        w[m] = i < n ? smp_fixed((uint32_t)(p[m] >> 32), top, r, a.shift) : 0;
+        weights[i] = w[m];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+        const u64 pj = pairs[j], wj = weights[j];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const bool ahead = pj > p[m];
+            rank[m] += ahead;
+            before[m] += ahead ? wj : 0;
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) in_k += rank[m] < r.k ? w[m] : 0;
+    const double limit = r.p * (double)smp_wave_sum(in_k);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const bool stays = (!r.cut_p || (double)before[m] < limit) && (w[m] >= r.least || (uint32_t)(p[m] >> 32) == top);
+        if (!(p[m] != 0 && rank[m] < r.k && (rank[m] == 0 || stays))) w[m] = 0;  // (of weight 0: never drawn)
+        weights[m * 64 + lane] = w[m];
+        all += w[m];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+        const u64 wj = weights[j];
+        const uint32_t at = (uint32_t)pairs[j];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) run[m] += at >= (uint32_t)p[m] ? wj : 0;  // (indices are complements: those up to its own)
+    }
+    const u64 target = smp_target(r, smp_wave_sum(all));
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+        if (w[m] > 0 && run[m] > target && run[m] - w[m] <= target) a.out[b] = (long long)(0xFFFFFFFFu - (uint32_t)p[m]);
+}
+
+// ---------------------------------------------------------------------------------- a wavefront per row
+// Up to SMP_WAVE columns, N a lane: index e * 64 + lane.  Cuts by bisection over the keys - the largest one that k logits, or that
+// p of the weight, reach - and equal keys at the cut by index; a small top-k leaves a list for smp_few_draw.
+template <typename T, int N>
+__global__ __launch_bounds__(SMP_THREADS) void sample_wave(SampleArgs a) {
+    __shared__ u64 lists[SMP_THREADS / 64][2 * SMP_FEW_LISTED];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long b0 = (long long)blockIdx.x * (SMP_THREADS / 64) + wave;
+    if (b0 >= a.B) return;  // (no barrier below)
+    const int b = (int)b0;
     const T *row = (const T *)a.logits + b * a.ldl;
     const SampleRow r = smp_row(a, b);
-    u64 best = 0;
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-        const u64 pair = i < a.V ? smp_pair(smp_key((float)row[i]), i) : 0;
-        pairs[i] = pair;
-        best = max(best, pair);
+    uint32_t key[N], top = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        key[e] = e * 64 + lane < a.V ? smp_key((float)row[e * 64 + lane]) : 0;
+        top = max(top, key[e]);
     }
-    const uint32_t top = smp_max<THREADS>((uint32_t)(best >> 32), red);
+    top = smp_wave_max(top);
     if (top <= SMP_DEAD || r.first_only) {
-        const uint32_t low = smp_max<THREADS>((uint32_t)(best >> 32) == top ? (uint32_t)best : 0, red);
-        if (threadIdx.x == 0) a.out[b] = top <= SMP_DEAD ? -1 : (long long)(0xFFFFFFFFu - low);
+        int first = -1;
+#pragma unroll
+        for (int e = N - 1; e >= 0; --e) {
+            const u64 equal = __ballot(key[e] == top);
+            if (equal) first = e * 64 + __builtin_ctzll(equal);
+        }
+        if (lane == 0) a.out[b] = top <= SMP_DEAD ? -1 : first;
         return;
     }
-    u64 cut = (u64)(SMP_DEAD + 1) << 32;  // everything that is not dead
-    if (r.cut_k || r.cut_p) {
-        smp_sort<THREADS>(pairs, n);
-        const int per = max(1, n / THREADS), begin = min((int)threadIdx.x * per, n), end = min(begin + per, n);
-        u64 mine = 0, total, kept = 0;
-        for (int j = begin; j < end; ++j)
-            if (j < r.k) mine += smp_fixed((uint32_t)(pairs[j] >> 32), top, r, a.shift);
-        u64 before = smp_scan<THREADS>(mine, total, red);
-        const double limit = r.p * (double)total;
-        for (int j = begin; j < end; ++j) {
-            const uint32_t key = (uint32_t)(pairs[j] >> 32);
-            if (j >= r.k || key <= SMP_DEAD || (j > 0 && r.cut_p && !((double)before < limit))) break;
-            before += smp_fixed(key, top, r, a.shift);
-            ++kept;
+    const auto reach = [&](uint32_t least) {  // logits of this key or a larger one
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) n += __popcll(__ballot(key[e] >= least));
+        return n;
+    };
+    // keeps the first `most` of the logits with key `least`, and all larger ones
+    uint32_t kept = 0;
+    const auto keep = [&](uint32_t least, int most) {
+        int before = 0;
+        uint32_t now = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const u64 equal = __ballot(key[e] == least);
+            const bool stays = key[e] > least || (key[e] == least && before + __popcll(equal & ((1ull << lane) - 1)) < most);
+            now |= (uint32_t)stays << e;
+            before += __popcll(equal);
         }
-        smp_scan<THREADS>(kept, total, red);
-        cut = pairs[total - 1];
+        kept = now;
+    };
+    uint32_t lo = SMP_DEAD + 1;
+    int most = a.V;
+    if (r.cut_k && reach(lo) > r.k) {
+        uint32_t hi = top;
+        int n = 0;
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2 + 1;
+            n = reach(mid);
+            if (n >= r.k) lo = mid;
+            else hi = mid - 1;
+            if (n == r.k) break;
+        }
+        n = reach(lo);
+        if (n <= SMP_FEW_LISTED) {
+            int at = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const u64 takes = __ballot(key[e] >= lo);
+                if (key[e] >= lo) lists[wave][at + __popcll(takes & ((1ull << lane) - 1))] = smp_pair(key[e], e * 64 + lane);
+                at += __popcll(takes);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            smp_few_draw(a, r, b, top, lists[wave], n);
+            return;
+        }
+        most = r.k - reach(lo + 1);
     }
-    smp_draw<T, THREADS>(a, r, b, 0, a.V, cut, top, false, 0, red);
+    keep(lo, most);
+    u64 w[N], sum = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        w[e] = kept >> e & 1 ? smp_fixed(key[e], top, r, a.shift) : 0;
+        sum += w[e];
+    }
+    if (r.cut_p) {
+        const double limit = r.p * (double)smp_wave_sum(sum);
+        const auto weigh = [&](uint32_t least) {
+            u64 t = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) t += key[e] >= least ? w[e] : 0;
+            return smp_wave_sum(t);
+        };
+        uint32_t hi = top;
+        int from_lo = reach(lo), past_hi = 0;
+        while (lo < hi && from_lo - past_hi > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2 + 1;
+            const int n = reach(mid);
+            if ((double)weigh(mid) >= limit) lo = mid, from_lo = n;
+            else hi = mid - 1, past_hi = n;
+        }
+        if (lo < hi) {  // one logit is left between them
+            lo = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) lo = key[e] <= hi ? max(lo, key[e]) : lo;
+            lo = smp_wave_max(lo);
+        }
+        // of the equal ones those that what lies before them does not reach the limit (the first of the row always)
+        const u64 larger = weigh(lo + 1), each = smp_fixed(lo, top, r, a.shift);
+        int before = 0;
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const u64 equal = __ballot(key[e] == lo);
+            const int mine = before + __popcll(equal & ((1ull << lane) - 1));
+            if (key[e] < lo || (key[e] == lo && !((double)(larger + mine * each) < limit) && !(lo == top && mine == 0))) w[e] = 0;
+            before += __popcll(equal);
+        }
+    }
+    sum = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if (w[e] < r.least && key[e] != top) w[e] = 0;
+        sum += w[e];
+    }
+    const u64 target = smp_target(r, smp_wave_sum(sum));
+    u64 run = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        u64 upto = w[e];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const u64 up = __shfl_up(upto, o);
+            if (lane >= o) upto += up;
+        }
+        const u64 past = __ballot(run + upto > target);
+        if (past) {
+            if (lane == 0) a.out[b] = e * 64 + __builtin_ctzll(past);
+            return;
+        }
+        run += __shfl(upto, 63);
+    }
 }
 
 // ---------------------------------------------------------------------------------- rows split over blocks
@@ -687,7 +832,7 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_draw(SampleArgs a) {
     if (before <= target && target < before + mine) chosen = threadIdx.x, shared.k_weight = target - before;
     __syncthreads();
     const int c = chosen;
-    smp_draw<T, THREADS>(a, r, b, c * a.chunk, (int)min((c + 1) * (long long)a.chunk, (long long)a.V), cut, top, true, shared.k_weight, red);
+    smp_draw<T, THREADS>(a, r, b, c * a.chunk, (int)min((c + 1) * (long long)a.chunk, (long long)a.V), cut, top, shared.k_weight, red);
 }
 
 // ---------------------------------------------------------------------------------- a block per row
@@ -798,56 +943,6 @@ __device__ __forceinline__ uint32_t smp_first_key(int bin, uint32_t top, const S
         else lo = mid + 1;
     }
     return lo;
-}
-
-// All that top-k keeps is in a list of n <= SMP_FEW_LISTED: the cuts and the draw by one wavefront, two pairs a lane, every pair against
-// every other one (no barrier and no sorting).  The list's room behind the pairs takes their weights.
-__device__ __forceinline__ void smp_few_draw(const SampleArgs &a, const SampleRow &r, int b, uint32_t top, u64 *pairs, int n) {
-    const int lane = threadIdx.x & 63;
-    u64 *const weights = pairs + SMP_FEW_LISTED;
-    u64 p[2], w[2], before[2] = {}, run[2] = {}, in_k = 0, all = 0;
-    int rank[2] = {};
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const int i = m * 64 + lane;
-        p[m] = i < n ? pairs[i] : 0;
-        w[m] = i < n ? smp_fixed((uint32_t)(p[m] >> 32), top, r, a.shift) : 0;
-        weights[i] = w[m];
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-        const u64 pj = pairs[j], wj = weights[j];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const bool ahead = pj > p[m];
-            rank[m] += ahead;
-            before[m] += ahead ? wj : 0;
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < 2; ++m) in_k += rank[m] < r.k ? w[m] : 0;
-    const double limit = r.p * (double)smp_wave_sum(in_k);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const bool stays = (!r.cut_p || (double)before[m] < limit) && (w[m] >= r.least || (uint32_t)(p[m] >> 32) == top);
-        if (!(p[m] != 0 && rank[m] < r.k && (rank[m] == 0 || stays))) w[m] = 0;  // (of weight 0: never drawn)
-        weights[m * 64 + lane] = w[m];
-        all += w[m];
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-        const u64 wj = weights[j];
-        const uint32_t at = (uint32_t)pairs[j];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) run[m] += at >= (uint32_t)p[m] ? wj : 0;  // (indices are complements: those up to its own)
-    }
-    const u64 target = smp_target(r, smp_wave_sum(all));
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-        if (w[m] > 0 && run[m] > target && run[m] - w[m] <= target) a.out[b] = (long long)(0xFFFFFFFFu - (uint32_t)p[m]);
 }
 
 // The same for a longer list.
@@ -1096,7 +1191,7 @@ __global__ __launch_bounds__(SMP_DRAW_THREADS) void sample_row(SampleArgs a) {
     __syncthreads();
     const int piece = chosen, last = row.head + row.units * E;
     const int i0 = piece == 0 ? 0 : piece == WAVES + 1 ? last : row.head + (piece - 1) * row.run * E;
-    smp_draw<T, THREADS>(a, r, b, i0, piece == 0 ? row.head : piece == WAVES + 1 ? a.V : min(i0 + row.run * E, last), cut, top, true, left, red);
+    smp_draw<T, THREADS>(a, r, b, i0, piece == 0 ? row.head : piece == WAVES + 1 ? a.V : min(i0 + row.run * E, last), cut, top, left, red);
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -1140,7 +1235,7 @@ static bool smp_by_row(int B, int V, int top_k_all, bool may_cut) {
 static bool smp_may_cut(int V, int top_k_all, float top_p_all) { return top_k_all < 0 || (top_k_all > 0 && top_k_all < V) || !(top_p_all >= 1.0f); }
 
 extern "C" size_t dl_sample_workspace_bytes(int B, int V, int top_k_all, float top_p_all) {
-    if (B <= 0 || V <= SMP_SORTED || smp_by_row(B, V, top_k_all, smp_may_cut(V, top_k_all, top_p_all))) return 0;
+    if (B <= 0 || V <= SMP_WAVE || smp_by_row(B, V, top_k_all, smp_may_cut(V, top_k_all, top_p_all))) return 0;
     SampleArgs a = {};
     a.B = B, a.V = V;
     return smp_layout(a, nullptr);
@@ -1179,11 +1274,13 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
         dl_prof_end(s);
         return dl_launch_status();
     }
-    if (V <= SMP_SORTED) {
-        const int n = 1 << bits;
-        dl_prof_begin("sample_sorted", s);
-        DL_BY_TYPE(type, T, if (n <= 1024) sample_sorted<T, 256><<<B, 256, n * sizeof(u64), s>>>(a, n);
-                   else sample_sorted<T, 1024><<<B, 1024, n * sizeof(u64), s>>>(a, n));
+    if (V <= SMP_WAVE) {
+        const int blocks = dl_ceil_div(B, SMP_THREADS / 64);
+        dl_prof_begin("sample_wave", s);
+        DL_BY_TYPE(type, T, if (V <= 128) sample_wave<T, 2><<<blocks, SMP_THREADS, 0, s>>>(a);
+                   else if (V <= 256) sample_wave<T, 4><<<blocks, SMP_THREADS, 0, s>>>(a);
+                   else if (V <= 512) sample_wave<T, 8><<<blocks, SMP_THREADS, 0, s>>>(a);
+                   else sample_wave<T, 16><<<blocks, SMP_THREADS, 0, s>>>(a));
         dl_prof_end(s);
         return dl_launch_status();
     }

@@ -474,8 +474,8 @@ def check_sample(device, logits, uniform, temperature=1.0, top_k=0, top_p=1.0, m
     assert got.dtype is torch.int64 and got.cpu().tolist() == want.tolist()
 
 
-# columns: one, a few lanes per row, a sorted row (power of two, odd), split rows with one chunk and several
-COLUMNS = [1, 2, 10, 33, 64, 65, 128, 1000, 1025, 4096, 4097, 9001]
+# columns: one, a few lanes per row, a wavefront per row (powers of two, odd), a block per row
+COLUMNS = [1, 2, 10, 33, 64, 65, 128, 129, 300, 1000, 1024, 1025, 4096, 4097, 9001]
 FILTERS = [dict(), dict(temperature=0.0), dict(top_k=1), dict(top_k=7), dict(top_p=0.5), dict(top_p=0.95, min_p=0.05),
            dict(temperature=0.7, top_k=50, top_p=0.9), dict(temperature=3.0, top_k=3000, top_p=0.999, min_p=0.001)]
 
