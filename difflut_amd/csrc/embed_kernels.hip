@@ -4,7 +4,7 @@
 //
 // A token outside [0, V) gives a row of zeros and adds nothing to the gradient; one that equals `padding` adds nothing either.
 //
-// The gradient takes three launches and no atomics on floats, so its bits do not depend on the schedule:
+// The gradient of many tokens takes three launches and no atomics on floats, so its bits do not depend on the schedule:
 //   embed_sort   positions sorted by token, ascending within one.  Block b owns the tokens v with v mod blocks = b and reads
 //                the whole token list (it stays in the L2): how many tokens belong to lower blocks is where its own begin.  Owning
 //                every blocks-th token spreads the frequent ones, which lie together at the low ids of a vocabulary.
@@ -21,6 +21,7 @@
 #define EMB_AHEAD 8         // groups of 64 tokens that a wavefront of the sort has in flight
 #define EMB_FOUND 480       // tokens of its own that a wavefront remembers, as 23 bits of position and 9 bits of place (EMB_MAX_OWNED)
 #define EMB_ROWS(E) ((E) == 8 ? 8 : 16)  // rows that a team of the sums has in flight (more registers leave too few wavefronts)
+#define EMB_FEW 512         // tokens up to which the gradient takes one launch
 #define EMB_JOIN_THREADS 512
 #define EMB_JOIN_WAVES (EMB_JOIN_THREADS / 64)
 #define EMB_JOIN_SPLIT 16  // partials from which on the block's wavefronts share them
@@ -320,6 +321,55 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join(T *__restrict__ g
     }
 }
 
+// ---------------------------------------------------------------------------------- few tokens
+// Up to EMB_FEW tokens the whole gradient takes one launch: a block owns every gridDim.x-th token of the vocabulary, picks their
+// positions out of the list - in order, a wavefront's turn after the other - and writes their rows, most of them zeros.
+template <typename T, typename TOKEN, bool VEC>
+__global__ __launch_bounds__(EMB_THREADS) void embed_few(const TOKEN *__restrict__ tokens, const T *__restrict__ gy, T *__restrict__ gw, int n,
+                                                          unsigned V, unsigned padding, int D, int lane_bits, float scale) {
+    constexpr int E = VEC ? 16 / sizeof(T) : 1, WAVES = EMB_THREADS / 64, TURNS = EMB_FEW / EMB_THREADS;
+    __shared__ unsigned token_of[EMB_FEW];
+    __shared__ int position[EMB_FEW], found_in[TURNS][WAVES];
+    const int wave = threadIdx.x >> 6, lane64 = threadIdx.x & 63;
+    unsigned mine[TURNS];
+    unsigned long long takes[TURNS];
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+        const int t = u * EMB_THREADS + threadIdx.x;
+        mine[u] = t < n ? emb_token(tokens[t], V, padding) : ~0u;
+        takes[u] = __ballot(mine[u] != ~0u && mine[u] % gridDim.x == blockIdx.x);
+        if (lane64 == 0) found_in[u][wave] = __popcll(takes[u]);
+    }
+    __syncthreads();
+    int m = 0;
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u)
+        for (int w = 0; w < WAVES; ++w) {
+            if (w == wave && (takes[u] >> lane64 & 1)) {
+                const int at = m + __popcll(takes[u] & ((1ull << lane64) - 1));
+                token_of[at] = mine[u], position[at] = u * EMB_THREADS + threadIdx.x;
+            }
+            m += found_in[u][w];
+        }
+    __syncthreads();
+    const int lane = threadIdx.x & ((1 << lane_bits) - 1), teams = EMB_THREADS >> lane_bits;
+    for (unsigned long long v = blockIdx.x + (unsigned long long)(threadIdx.x >> lane_bits) * gridDim.x; v < V; v += (unsigned long long)teams * gridDim.x)
+        for (int c = lane * E; c < D; c += E << lane_bits) {
+            float acc[E] = {};
+#pragma unroll 4
+            for (int j = 0; j < m; ++j)
+                if (token_of[j] == (unsigned)v) {
+                    float f[E];
+                    dl_load(gy + (long long)position[j] * D + c, f);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += f[e];
+                }
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] *= scale;
+            dl_store_past(gw + (long long)v * D + c, acc);
+        }
+}
+
 // ---------------------------------------------------------------------------------- host
 static bool emb_sizes_ok(long long n, long long V, int D) { return n >= 0 && n < (1LL << 31) - 64 && V > 0 && V < (1LL << 31) && D > 0; }
 static int emb_lane_bits(int D, int E) {  // a team of up to a block's threads, as many as a row has vectors
@@ -366,7 +416,7 @@ static int emb_piece(long long n, int D) { return n * D >= (1LL << 24) + (1LL <<
 static long long emb_pieces(long long n, int D) { return (n + emb_piece(n, D) - 1) / emb_piece(n, D); }
 
 extern "C" size_t dl_embedding_bwd_workspace_bytes(long long n, long long V, int D) {
-    if (!emb_sizes_ok(n, V, D)) return 0;
+    if (!emb_sizes_ok(n, V, D) || n <= EMB_FEW) return 0;
     return 256 + 2 * dl_align256((size_t)n * sizeof(int)) + 2 * dl_align256((size_t)V * sizeof(int)) +
            dl_align256((size_t)emb_pieces(n, D) * 2 * D * sizeof(float));
 }
@@ -375,11 +425,25 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
                                 float scale, long long padding, void *ws, size_t ws_bytes, void *stream) {
     if (!dl_type_known(type) || (token_bits != 32 && token_bits != 64)) return DL_ERR_UNSUPPORTED;
     if (!emb_sizes_ok(n, V, D)) return DL_ERR_SHAPE;
-    if (!gw || !ws || (n > 0 && (!tokens || !gy))) return DL_ERR_NULL;
-    if (ws_bytes < dl_embedding_bwd_workspace_bytes(n, V, D)) return DL_ERR_WORKSPACE;
+    const size_t need = dl_embedding_bwd_workspace_bytes(n, V, D);
+    if (!gw || (need && !ws) || (n > 0 && (!tokens || !gy))) return DL_ERR_NULL;
+    if (ws_bytes < need) return DL_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     const int E = 16 / dl_type_bytes(type);
     const bool vec = dl_aligned16(gy) && dl_aligned16(gw) && D % E == 0;
+    const unsigned skip = padding >= 0 && padding < V ? (unsigned)padding : ~0u;
+    if (!need) {
+        const int bits = emb_lane_bits(D, vec ? E : 1);
+        const long long rows = (V + (EMB_THREADS >> bits) - 1) / (EMB_THREADS >> bits);
+        const int blocks = (int)(rows < 2048 ? rows : 2048);
+#define FEW(TOKEN, VEC) embed_few<T, TOKEN, VEC><<<blocks, EMB_THREADS, 0, s>>>((const TOKEN *)tokens, (const T *)gy, (T *)gw, (int)n, (unsigned)V, skip, D, bits, scale)
+        dl_prof_begin("embed_few", s);
+        DL_BY_TYPE(type, T, if (token_bits == 32) { if (vec) FEW(int, true); else FEW(int, false); }
+                   else { if (vec) FEW(long long, true); else FEW(long long, false); });
+        dl_prof_end(s);
+#undef FEW
+        return dl_launch_status();
+    }
     int *total = (int *)ws, *order = (int *)((char *)ws + 256);
     int *token_of = (int *)((char *)order + dl_align256((size_t)n * sizeof(int)));
     int *count = (int *)((char *)token_of + dl_align256((size_t)n * sizeof(int)));
@@ -395,7 +459,6 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
     const int bits = emb_block_bits(V);
     const size_t lds = (size_t)EMB_SORT_WAVES * (size_t)((V + (1LL << bits) - 1) >> bits) * sizeof(int);
     if ((long long)dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * dl_ceil_div(D, vec ? 256 : 64) > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
-    const unsigned skip = padding >= 0 && padding < V ? (unsigned)padding : ~0u;
 #define SORT(TOKEN) \
     embed_sort<TOKEN><<<1 << bits, EMB_SORT_THREADS, lds, s>>>((const TOKEN *)tokens, (int)n, (unsigned)V, skip, bits, order, token_of, begin_of, count, total)
     dl_prof_begin("embed_sort", s);

@@ -816,9 +816,10 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const Tensor tokens = ctx->get_saved_variables()[0], gy = grads[0].contiguous();
         const c10::DeviceGuard guard(gy.device());
         const int64_t V = ctx->saved_data["V"].toInt(), D = gy.size(-1), n = tokens.numel();
-        const Tensor gw = at::empty({V, D}, gy.options()), ws = bytes(L.dl_embedding_bwd_workspace_bytes(n, V, D), gy);
+        const size_t need = L.dl_embedding_bwd_workspace_bytes(n, V, D);
+        const Tensor gw = at::empty({V, D}, gy.options()), ws = need ? bytes(need, gy) : Tensor();
         check(L.dl_embedding_bwd(raw_in(tokens), tokens.scalar_type() == at::kInt ? 32 : 64, raw_in(gy), raw(gw), type_of(gy, "gradient"), n, V, D,
-                                 (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), raw(ws), ws.numel(), stream()));
+                                 (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), raw(ws), need, stream()));
         return {Tensor(), gw, Tensor(), Tensor()};
     }
 };

@@ -434,7 +434,8 @@ struct GnChannels {
 template <typename T, bool VEC, int NV, int THREADS, int ACT>
 __global__ __launch_bounds__(THREADS, NV == 1 ? 4 : 1) void gn_backward_one(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
                                                             const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
-                                                            float *__restrict__ channel, T *__restrict__ gx, GnShape s) {
+                                                            float *__restrict__ channel, T *__restrict__ gx, void *__restrict__ ggamma,
+                                                            void *__restrict__ gbeta, GnShape s) {
     constexpr int E = 16 / sizeof(T);
     __shared__ float slots[THREADS * E], mean_g[GN_ONE_WIDTH + E], mean_x[GN_ONE_WIDTH + E];
     const int tile = blockIdx.x % s.tiles, block0 = blockIdx.x / s.tiles, blocks = gridDim.x / s.tiles;
@@ -508,11 +509,17 @@ __global__ __launch_bounds__(THREADS, NV == 1 ? 4 : 1) void gn_backward_one(cons
         if constexpr (THREADS != GN_THREADS) break;  // (one round: with a second one's values next to these the registers spill)
         __syncthreads();  // the means have been read
     }
-    float *out = channel + (long long)block0 * 2 * s.C + c0;
+    // (from a single block of the tile they are the parameters' gradients already)
+    const auto put = [&](int which, void *gradient) {
+        for (int c = threadIdx.x; c < width; c += THREADS) {
+            if (blocks == 1) gn_param_store(gradient, ptype, c0 + c, slots[c]);
+            else channel[((long long)block0 * 2 + which) * s.C + c0 + c] = slots[c];
+        }
+    };
     gn_channel_sums<E, THREADS>(w, width, all_g, slots, slots);
-    for (int c = threadIdx.x; c < width; c += THREADS) out[c] = slots[c];
+    put(0, gbeta);
     gn_channel_sums<E, THREADS>(w, width, all_x, slots, slots);
-    for (int c = threadIdx.x; c < width; c += THREADS) out[s.C + c] = slots[c];
+    put(1, ggamma);
 }
 
 // Per channel of a piece: sum g and sum g xhat, [B][pieces][2][C].
@@ -723,9 +730,13 @@ static bool gn_one_shape(GnShape &s, int B, long long P, int C, int G, int E, in
         s.piece_rows = (int)P;
         const int rows = gn_rows_per_step(s, E, threads);
         if ((s.tile_width + E - 1) / E <= threads && s.tile_width <= GN_ONE_WIDTH && (long long)rows * units >= P) {
-            // small samples share a block, as long as there are 512 of those (65536 rows of 64 channels: 16 a block)
-            if (groups == G && threads == GN_THREADS)
-                for (s.samples = P <= rows ? (int)(rows / P) : 1; s.samples > 1 && dl_ceil_div(B, s.samples) < 512;) s.samples /= 2;
+            // small samples share a block: all of them where that takes a few (the backward then needs no sums over blocks), else as long as
+            // there are 512 blocks (65536 rows of 64 channels: 16 a block)
+            if (groups == G && threads == GN_THREADS) {
+                s.samples = P <= rows ? (int)(rows / P) : 1;
+                if (dl_ceil_div(B, s.samples) > 4)
+                    while (s.samples > 1 && dl_ceil_div(B, s.samples) < 512) s.samples /= 2;
+            }
             return groups == G || s.tile_width >= 4 * E || (long long)B * P * C <= (1 << 18);
         }
     }
@@ -825,12 +836,13 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
         // of 256 threads as many blocks as the card holds at a time, rounds of them after that
         const int most = 2048 / s.tiles, want = dl_ceil_div(B, s.samples);
         rows_out = threads != GN_THREADS || want < most ? want : most > 0 ? most : 1;
+        if (threads == GN_THREADS && want <= 4) rows_out = 1;  // a few rounds instead of a launch for the sums over samples
         const bool vec = gn_vectors(s, E, x, gy, gx);
         const bool few = s.samples > 1 || P <= gn_rows_per_step(s, E, threads);
         dl_prof_begin("gn_backward_one", st);
 #define ONE(VEC, NV, THREADS) \
     gn_backward_one<T, VEC, NV, THREADS, ACT><<<rows_out * s.tiles, THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
-                                                                                 (const float2 *)stats, channel, (T *)gx, s)
+                                                                                 (const float2 *)stats, channel, (T *)gx, ggamma, gbeta, s)
         DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) {
                 if (few) { if (vec) ONE(true, 1, GN_THREADS); else ONE(false, 1, GN_THREADS); }
                 else { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
@@ -855,7 +867,7 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
         DL_BY_TYPE(type, T, if (vec) { BACKWARD(true); } else { BACKWARD(false); });
 #undef BACKWARD
     }
-    if (ggamma || gbeta) {
+    if ((ggamma || gbeta) && !(one && rows_out == 1)) {
         int n = rows_out;
         const float *rows = channel;
         const int columns = dl_ceil_div(C, 32);

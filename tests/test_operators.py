@@ -52,7 +52,7 @@ def embedding_64(tokens, weight, scale, gy, padding=None):
 
 
 # a single token; rows shorter than a vector, odd, of a vector, of several teams; pieces that end inside a token's run
-EMBED = [((1,), 1, 1), ((1,), 7, 5), ((3, 5), 9, 8), ((16,), 3, 64), ((17,), 1, 33), ((33, 2), 5, 257), ((300,), 1000, 16), ((0,), 6, 12),
+EMBED = [((512,), 3, 20), ((513,), 3, 20), ((510,), 9000, 8), ((1,), 1, 1), ((1,), 7, 5), ((3, 5), 9, 8), ((16,), 3, 64), ((17,), 1, 33), ((33, 2), 5, 257), ((300,), 1000, 16), ((0,), 6, 12),
          ((4, 129), 2, 1030), ((2049,), 700, 4)]
 
 
@@ -652,7 +652,8 @@ def test_c_entry_points_refuse():
             (null, lambda: lib.dl_embedding_fwd(at, 64, None, 8, at, 0, 4, 5, 8, 1.0, None)),
             (null, lambda: lib.dl_embedding_bwd(at, 64, at, None, 0, 4, 5, 8, 1.0, -1, at, big, None)),
             (null, lambda: lib.dl_embedding_bwd(at, 64, None, at, 0, 4, 5, 8, 1.0, -1, at, big, None)),
-            (short, lambda: lib.dl_embedding_bwd(at, 64, at, at, 0, 4, 5, 8, 1.0, -1, at, lib.dl_embedding_bwd_workspace_bytes(4, 5, 8) - 1, None)),
+            (null, lambda: lib.dl_embedding_bwd(at, 64, at, at, 0, 4000, 5, 8, 1.0, -1, None, big, None)),
+            (short, lambda: lib.dl_embedding_bwd(at, 64, at, at, 0, 4000, 5, 8, 1.0, -1, at, lib.dl_embedding_bwd_workspace_bytes(4000, 5, 8) - 1, None)),
             (null, lambda: lib.dl_group_norm_fwd(at, at, at, at, None, 0, 0, 2, 3, 8, 2, 1e-5, 0, at, big, None)),
             (unsupported, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 9, 2, 3, 8, 2, 1e-5, 0, at, big, None)),
             (unsupported, lambda: lib.dl_group_norm_fwd(at, at, at, at, at, 0, 0, 2, 3, 8, 2, 1e-5, 4, at, big, None)),
