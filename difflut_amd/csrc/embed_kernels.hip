@@ -12,6 +12,12 @@
 //                a token's sum where all of its positions lie in the piece, else a partial; the rest of the grid writes the rows of
 //                tokens that do not occur.
 //   embed_join   adds the partials of tokens that reach over pieces, in order.
+// Up to EMB_FEW tokens take one launch (embed_few).
+//
+// Bound by memory but for the sort.  us at 65521 tokens, 131072 x 1024 bf16: lookup 32 (results stored past the caches; 52 before), sums and
+// empty rows 78 (435 MB, 5.6 TB/s; 120 with 16 rows of 8 values in flight, which left two wavefronts a SIMD), sort 24 (every block
+// reads 64 tokens per wavefront and step, 16 instructions each; 60 with a second read of the list), join 6 (84 by one team per
+// token).  At 12544 tokens, 16384 x 784 fp32: 12, 17, 11, 5.
 #include "dl_types.h"
 
 #define EMB_THREADS 256
@@ -22,6 +28,8 @@
 #define EMB_FOUND 480       // tokens of its own that a wavefront remembers, as 23 bits of position and 9 bits of place (EMB_MAX_OWNED)
 #define EMB_ROWS(E) ((E) == 8 ? 8 : 16)  // rows that a team of the sums has in flight (more registers leave too few wavefronts)
 #define EMB_FEW 512         // tokens up to which the gradient takes one launch
+#define EMB_LONG 131072     // tokens from which on they are parted by owner before they are sorted
+#define EMB_CHUNKS 1024     // pieces of the list there, at most
 #define EMB_JOIN_THREADS 512
 #define EMB_JOIN_WAVES (EMB_JOIN_THREADS / 64)
 #define EMB_JOIN_SPLIT 16  // partials from which on the block's wavefronts share them
@@ -79,6 +87,24 @@ __device__ __forceinline__ void emb_fetch(const TOKEN *__restrict__ tokens, int 
 #pragma unroll
         for (int u = 0; u < EMB_AHEAD; ++u) t[u] = g + u < g1 && (g + u) * 64 + (int)(threadIdx.x & 63) < n ? from[u * 64] : (TOKEN)-1;
     }
+}
+
+// Lanes of one slot (of `bits` bits) are ranked among themselves and go to next[slot] on; `next`, a wavefront's own in LDS, moves on.  Which
+// lanes share a slot comes from a ballot per bit, so the cost does not go by the number of different slots.  (volatile: a
+// wavefront's lanes see each other's stores, which are in order)
+template <typename F>
+__device__ __forceinline__ void emb_put(bool here, unsigned slot, int bits, volatile int *next, F store) {
+    unsigned long long same = __ballot(here);
+    if (same == 0) return;
+    for (int k = 0; k < bits; ++k) {
+        const bool bit = slot >> k & 1;
+        const unsigned long long set = __ballot(bit);
+        same &= bit ? set : ~set;
+    }
+    if (!here) return;
+    const int lane = threadIdx.x & 63, first = next[slot];
+    store(first + __popcll(same & ((1ull << lane) - 1)));
+    if (lane == __builtin_ctzll(same)) next[slot] = first + __popcll(same);
 }
 
 template <typename TOKEN>
@@ -151,24 +177,10 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
     }
     if (b == mask && threadIdx.x == 0) *total = base + all;
     __syncthreads();
-    // the positions themselves, in order: lanes of one token are ranked among themselves (volatile: a wavefront's lanes see each other's
-    // stores, which are in order)
-    volatile int *next = place;
+    // the positions themselves, in order
+    const int bits = 32 - __clz(max(owned - 1, 0));
     const auto put = [&](bool here, int t, unsigned v) {
-        const int slot = here ? wave * owned + (int)(v >> block_bits) : -1;
-        unsigned long long left = __ballot(here);
-        while (left) {
-            const int leader = __builtin_ctzll(left), its = __builtin_amdgcn_readlane(slot, leader);
-            const unsigned long long same = __ballot(slot == its);
-            const int first = next[its];
-            if (slot == its) {
-                const int at = first + __popcll(same & ((1ull << lane) - 1));
-                order[at] = t;
-                token_of[at] = (int)v;
-            }
-            if (lane == leader) next[its] = first + __popcll(same);
-            left &= ~same;
-        }
+        emb_put(here, v >> block_bits, bits, place + wave * owned, [&](int at) { order[at] = t, token_of[at] = (int)v; });
     };
     if (mine <= EMB_FOUND && per_wave <= 1 << 17) {
         for (int i = 0; i < mine; i += 64) {
@@ -184,6 +196,145 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
                 put(v != ~0u && (v & mask) == b, (g + u) * 64 + lane, v);
             }
         }
+    }
+}
+
+// ---------------------------------------------------------------------------------- long lists
+// From EMB_LONG tokens on every block reading all of them is what the time goes into; they are parted by owner first, in order:
+//   embed_part_count   how many tokens of a chunk belong to each owner, [owner][chunk]
+//   embed_part_scan    where each of those begins
+//   embed_part         positions and tokens, an owner's together
+//   embed_sort_part    an owner's, by token
+// (1 048 576 tokens of 50000, rows of 256 floats: the gradient 1.07 -> 0.51 ms, 0.31 of it the sums; the block of the most frequent token, 6 % of
+// the list, is what embed_sort_part's 0.11 wait for.)
+
+template <typename TOKEN>
+__global__ __launch_bounds__(EMB_SORT_THREADS) void embed_part_count(const TOKEN *__restrict__ tokens, int n, unsigned V, unsigned padding,
+                                                                      int block_bits, int chunk, int chunks, int *__restrict__ counts) {
+    extern __shared__ int place[];  // [owners]
+    const int owners = 1 << block_bits;
+    for (int i = threadIdx.x; i < owners; i += EMB_SORT_THREADS) place[i] = 0;
+    __syncthreads();
+    const int begin = blockIdx.x * chunk, end = (int)min((long long)begin + chunk, (long long)n);
+    for (int t = begin + threadIdx.x; t < end; t += EMB_SORT_THREADS) {
+        const unsigned v = emb_token(tokens[t], V, padding);
+        if (v != ~0u) atomicAdd(&place[v & (owners - 1)], 1);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < owners; i += EMB_SORT_THREADS) counts[(long long)i * chunks + blockIdx.x] = place[i];
+}
+
+// begins[owner][chunk]: where its tokens go, of all in that order; the total stands behind them.  A block per owner (chunks <= its threads)
+// adds up the lower owners' counts for itself.
+__global__ __launch_bounds__(EMB_SORT_THREADS) void embed_part_scan(const int *__restrict__ counts, int chunks, int *__restrict__ begins,
+                                                                     int *__restrict__ total) {
+    __shared__ int scan[EMB_SORT_WAVES], lower[EMB_SORT_WAVES];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, own = blockIdx.x * chunks;
+    int below = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < own; i += EMB_SORT_THREADS) below += counts[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o);
+    const int mine = (int)threadIdx.x < chunks ? counts[own + threadIdx.x] : 0;
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(before, o);
+        if (lane >= o) before += up;
+    }
+    if (lane == 63) scan[wave] = before, lower[wave] = below;
+    __syncthreads();
+    for (int w = 0; w < EMB_SORT_WAVES; ++w) {
+        before += lower[w];
+        if (w < wave) before += scan[w];
+    }
+    if ((int)threadIdx.x < chunks) begins[own + threadIdx.x] = before - mine;
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == EMB_SORT_THREADS - 1) begins[own + chunks] = *total = before;
+}
+
+template <typename TOKEN>
+__global__ __launch_bounds__(EMB_SORT_THREADS) void embed_part(const TOKEN *__restrict__ tokens, int n, unsigned V, unsigned padding,
+                                                                int block_bits, int chunk, int chunks, const int *__restrict__ begins,
+                                                                int *__restrict__ positions, unsigned *__restrict__ parted) {
+    extern __shared__ int place[];  // [waves][owners]
+    const int owners = 1 << block_bits, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int i = threadIdx.x; i < EMB_SORT_WAVES * owners; i += EMB_SORT_THREADS) place[i] = 0;
+    __syncthreads();
+    const int begin = blockIdx.x * chunk, end = (int)min((long long)begin + chunk, (long long)n);
+    const int per_wave = (chunk / 64 + EMB_SORT_WAVES - 1) / EMB_SORT_WAVES * 64;  // (chunk: whole groups of 64)
+    const int t0 = min(begin + wave * per_wave, end), t1 = min(t0 + per_wave, end);
+    for (int t = t0 + lane; t < t1; t += 64) {
+        const unsigned v = emb_token(tokens[t], V, padding);
+        if (v != ~0u) atomicAdd(&place[wave * owners + (v & (owners - 1))], 1);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < owners; i += EMB_SORT_THREADS) {
+        int at = begins[(long long)i * chunks + blockIdx.x];
+        for (int w = 0; w < EMB_SORT_WAVES; ++w) {
+            const int c = place[w * owners + i];
+            place[w * owners + i] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; t += 64) {
+        const unsigned v = t + lane < t1 ? emb_token(tokens[t + lane], V, padding) : ~0u;
+        emb_put(v != ~0u, v & (owners - 1), block_bits, place + wave * owners, [&](int at) { positions[at] = t + lane, parted[at] = v; });
+    }
+}
+
+__global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort_part(const int *__restrict__ positions, const unsigned *__restrict__ parted, unsigned V,
+                                                                     int block_bits, int chunks, const int *__restrict__ begins,
+                                                                     int *__restrict__ order, int *__restrict__ token_of,
+                                                                     int *__restrict__ begin_of, int *__restrict__ count) {
+    extern __shared__ int place[];  // [waves][owned]
+    __shared__ int scan[EMB_SORT_WAVES];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned b = blockIdx.x, mask = (1u << block_bits) - 1;
+    const int owned = (int)((V - b + mask) >> block_bits);
+    for (int i = threadIdx.x; i < EMB_SORT_WAVES * owned; i += EMB_SORT_THREADS) place[i] = 0;
+    __syncthreads();
+    const int begin = begins[(long long)b * chunks], end = begins[(long long)(b + 1) * chunks];  // (the total stands behind the last)
+    const int per_wave = ((end - begin + 63) / 64 + EMB_SORT_WAVES - 1) / EMB_SORT_WAVES * 64;
+    const int i0 = min(begin + wave * per_wave, end), i1 = min(i0 + per_wave, end);
+#pragma unroll 4
+    for (int i = i0 + lane; i < i1; i += 64) atomicAdd(&place[wave * owned + (int)(parted[i] >> block_bits)], 1);
+    __syncthreads();
+    int here = 0;
+    if ((int)threadIdx.x < owned)
+        for (int w = 0; w < EMB_SORT_WAVES; ++w) here += place[w * owned + threadIdx.x];
+    int before = here;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(before, o);
+        if (lane >= o) before += up;
+    }
+    if (lane == 63) scan[wave] = before;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) before += scan[w];
+    before += begin - here;
+    if ((int)threadIdx.x < owned) {
+        const unsigned v = b + (threadIdx.x << block_bits);
+        count[v] = here, begin_of[v] = before;
+        for (int w = 0; w < EMB_SORT_WAVES; ++w) {
+            const int c = place[w * owned + threadIdx.x];
+            place[w * owned + threadIdx.x] = before;
+            before += c;
+        }
+    }
+    __syncthreads();
+    const int bits = 32 - __clz(max(owned - 1, 0));
+    for (int i = i0; i < i1; i += 4 * 64) {
+        unsigned v[4];
+        int t[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int at = i + u * 64 + lane;
+            v[u] = at < i1 ? parted[at] : 0, t[u] = at < i1 ? positions[at] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            emb_put(i + u * 64 + lane < i1, v[u] >> block_bits, bits, place + wave * owned, [&](int at) { order[at] = t[u], token_of[at] = (int)v[u]; });
     }
 }
 
@@ -371,7 +522,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_few(const TOKEN *__restrict
 }
 
 // ---------------------------------------------------------------------------------- host
-static bool emb_sizes_ok(long long n, long long V, int D) { return n >= 0 && n < (1LL << 31) - 64 && V > 0 && V < (1LL << 31) && D > 0; }
+static bool emb_sizes_ok(long long n, long long V, int D) { return n >= 0 && n < (1LL << 31) - 65536 && V > 0 && V < (1LL << 31) && D > 0; }
 static int emb_lane_bits(int D, int E) {  // a team of up to a block's threads, as many as a row has vectors
     int bits = 0;
     while (bits < 8 && ((long long)E << bits) < D) ++bits;
@@ -415,10 +566,19 @@ extern "C" int dl_embedding_fwd(const void *tokens, int token_bits, const void *
 static int emb_piece(long long n, int D) { return n * D >= (1LL << 24) + (1LL << 23) ? 32 : 16; }
 static long long emb_pieces(long long n, int D) { return (n + emb_piece(n, D) - 1) / emb_piece(n, D); }
 
+// Parting a long list: chunks of whole groups of 64 tokens, and the owners that their counts' LDS has room for
+static int emb_chunk(long long n) {
+    const long long chunk = (n + EMB_CHUNKS - 1) / EMB_CHUNKS;
+    return (int)((chunk > 4096 ? chunk + 63 : 4096) / 64 * 64);
+}
+static bool emb_long(long long n, long long V) { return n >= EMB_LONG && emb_block_bits(V) <= 9; }
+
 extern "C" size_t dl_embedding_bwd_workspace_bytes(long long n, long long V, int D) {
     if (!emb_sizes_ok(n, V, D) || n <= EMB_FEW) return 0;
     return 256 + 2 * dl_align256((size_t)n * sizeof(int)) + 2 * dl_align256((size_t)V * sizeof(int)) +
-           dl_align256((size_t)emb_pieces(n, D) * 2 * D * sizeof(float));
+           dl_align256((size_t)emb_pieces(n, D) * 2 * D * sizeof(float)) +
+           (emb_long(n, V) ? 2 * dl_align256((size_t)n * sizeof(int)) +
+                                 2 * dl_align256((((size_t)dl_ceil_div(n, emb_chunk(n)) << emb_block_bits(V)) + 1) * sizeof(int)) : 0);
 }
 
 extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *gy, void *gw, int type, long long n, long long V, int D,
@@ -461,10 +621,29 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
     if ((long long)dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * dl_ceil_div(D, vec ? 256 : 64) > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
 #define SORT(TOKEN) \
     embed_sort<TOKEN><<<1 << bits, EMB_SORT_THREADS, lds, s>>>((const TOKEN *)tokens, (int)n, (unsigned)V, skip, bits, order, token_of, begin_of, count, total)
-    dl_prof_begin("embed_sort", s);
-    if (token_bits == 32) SORT(int);
-    else SORT(long long);
-    dl_prof_end(s);
+    if (emb_long(n, V)) {
+        const int chunk = emb_chunk(n), chunks = dl_ceil_div(n, chunk), owners = 1 << bits;
+        int *positions = (int *)((char *)a.part + dl_align256((size_t)a.pieces * 2 * D * sizeof(float)));
+        unsigned *parted = (unsigned *)((char *)positions + dl_align256((size_t)n * sizeof(int)));
+        int *begins = (int *)((char *)parted + dl_align256((size_t)n * sizeof(int)));
+        int *counts = (int *)((char *)begins + dl_align256(((size_t)owners * chunks + 1) * sizeof(int)));
+#define PART(TOKEN)                                                                                                                    \
+    DL_TIMED("embed_part_count", s, (embed_part_count<TOKEN><<<chunks, EMB_SORT_THREADS, owners * sizeof(int), s>>>(                   \
+        (const TOKEN *)tokens, (int)n, (unsigned)V, skip, bits, chunk, chunks, counts)));                                              \
+    DL_TIMED("embed_part_scan", s, (embed_part_scan<<<owners, EMB_SORT_THREADS, 0, s>>>(counts, chunks, begins, total)));              \
+    DL_TIMED("embed_part", s, (embed_part<TOKEN><<<chunks, EMB_SORT_THREADS, EMB_SORT_WAVES * owners * sizeof(int), s>>>(              \
+        (const TOKEN *)tokens, (int)n, (unsigned)V, skip, bits, chunk, chunks, begins, positions, parted)))
+        if (token_bits == 32) { PART(int); }
+        else { PART(long long); }
+#undef PART
+        DL_TIMED("embed_sort_part", s, (embed_sort_part<<<owners, EMB_SORT_THREADS, lds, s>>>(positions, parted, (unsigned)V, bits, chunks, begins,
+                                                                                             order, token_of, begin_of, count)));
+    } else {
+        dl_prof_begin("embed_sort", s);
+        if (token_bits == 32) SORT(int);
+        else SORT(long long);
+        dl_prof_end(s);
+    }
 #undef SORT
     const long long zero_teams = (V + teams - 1) / teams;
     const unsigned zero_blocks = (unsigned)(zero_teams < 2048 ? zero_teams : 2048);

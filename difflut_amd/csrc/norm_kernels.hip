@@ -9,6 +9,13 @@
 // E neighbouring channels - 16 bytes - of some positions, so that a wavefront's loads are consecutive bytes of channels-last rows.
 // Everything is held in float; variances are sums of squares about a mean that is known (never E[x^2] - mean^2), and pieces
 // are joined by the pairwise formula (Chan, Golub, LeVeque 1979), in a fixed order: results are the same bits from run to run.
+//
+// Where a sample's tile fits the registers of a block (gn_one_shape), one launch reads it once, and small samples share a block; the
+// backward needs one more launch for sums over samples.  Else a direction takes three launches (statistics or sums, a join, the result)
+// and reads its inputs twice; results go past the caches, so that the second read finds its lines there.
+// Bound by memory, or by a block's chain of sums and barriers where samples are small.  us: 256 x 24 x 24 x 32 fp32, 8 groups, forward 13
+// (three launches: 24), backward 18 + 4 (32); 16 x 95 x 97 x 320 bf16, 32 groups, statistics 29, result 34, backward's sums 40 and result
+// 49 (5.8 TB/s), 14 in three small launches; 8192 x 16000 fp32 in 16 groups forward 490, backward 650 (2.1 and 2.4 TB/s: the chain).
 #include "dl_types.h"
 
 #define GN_THREADS 256
@@ -157,17 +164,21 @@ __device__ void gn_group_sums(const GnShape &s, const GnPlace &w, const float (&
     const int per_row = by_vector ? vectors : vectors * E, per_group = s.tile_groups == 0 ? per_row : (by_vector ? s.cg / E : s.cg);
     // as many lanes as a group has values
     const int rows = s.samples > 1 ? (int)s.P : w.rows, n = rows * per_group, all = s.samples * w.groups;
-    int lanes = 64;
-    while (lanes > 1 && n <= lanes / 2) lanes >>= 1;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, at_once = 64 / lanes;
+    int bits = 6;
+    while (bits > 0 && n <= 1 << (bits - 1)) --bits;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = lane & ((1 << bits) - 1), at_once = 64 >> bits;
     for (int k0 = wave * at_once; k0 < all; k0 += THREADS / 64 * at_once) {
-        const int k = k0 + lane / lanes, g = k % w.groups, row0 = k / w.groups * rows;
+        const int k = k0 + (lane >> bits), sample = s.samples > 1 ? k / w.groups : 0, g = k - sample * w.groups;
+        const float *from = slots + sample * rows * per_row + g * per_group;
         float t = 0.0f;
         if (k < all)
 #pragma unroll 2
-            for (int j = lane % lanes; j < n; j += lanes) t += slots[(row0 + j / per_group) * per_row + g * per_group + j % per_group];
-        for (int o = lanes >> 1; o > 0; o >>= 1) t += __shfl_xor(t, o);
-        if (k < all && lane % lanes == 0) sums[k] = t;
+            for (int j = first; j < n; j += 1 << bits) {
+                const int row = j / per_group;
+                t += from[row * (per_row - per_group) + j];
+            }
+        for (int o = 1 << bits >> 1; o > 0; o >>= 1) t += __shfl_xor(t, o);
+        if (k < all && first == 0) sums[k] = t;
     }
     __syncthreads();
 }
@@ -432,7 +443,7 @@ struct GnChannels {
 // gridDim.x / tiles-th one: its channels are the same ones, whose sums stay in registers until the last; they go to
 // [gridDim.x / tiles][2][C].
 template <typename T, bool VEC, int NV, int THREADS, int ACT>
-__global__ __launch_bounds__(THREADS, NV == 1 ? 4 : 1) void gn_backward_one(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
+__global__ __launch_bounds__(THREADS, NV == 1 && sizeof(T) == 4 ? 4 : 1) void gn_backward_one(const T *__restrict__ x, const T *__restrict__ gy, const void *__restrict__ gamma,
                                                             const void *__restrict__ beta, int ptype, const float2 *__restrict__ stats,
                                                             float *__restrict__ channel, T *__restrict__ gx, void *__restrict__ ggamma,
                                                             void *__restrict__ gbeta, GnShape s) {

@@ -119,11 +119,13 @@ def test_embedding_gradient_against_differences():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,V,D,dtype", [(20011, 3000, 68, torch.float32), (5000, 1, 24, torch.float32), (9000, 70001, 8, torch.bfloat16),
-                                         (40000, 5, 129, torch.float16)])
+                                         (40000, 5, 129, torch.float16), (131072, 9000, 4, torch.float32), (300001, 100, 8, torch.float32),
+                                         (200003, 300001, 8, torch.bfloat16), (150000, 1, 4, torch.float32), (140000, 140001, 12, torch.float32)])
 def test_embedding_gradient_of_many_tokens(n, V, D, dtype):
     """Uneven frequencies, all tokens equal, more tokens of the vocabulary than of the text: the formula, and the same bits twice."""
     g = gen(n)
     tokens = ((V + 1.0) ** torch.rand(n, generator=g, dtype=torch.float64) - 1).long().clamp_(0, V - 1)
+    tokens[::17] = -1  # (some of no token)
     gy = torch.randn(n, D, generator=g).to(dtype)
     w = torch.zeros(V, D, dtype=dtype, device="cuda").requires_grad_()
     y = ops.embedding(tokens.cuda(), w)
