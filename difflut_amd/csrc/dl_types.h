@@ -61,6 +61,7 @@ __device__ __forceinline__ void dl_store_past(T *p, const float (&f)[N]) {
 
 static inline bool dl_type_known(int type) { return type == DL_F32 || type == DL_BF16 || type == DL_F16; }
 static inline int dl_type_bytes(int type) { return type == DL_F32 ? 4 : 2; }
+static inline bool dl_grid_ok(long long blocks, int threads) { return blocks * threads < (1LL << 32); }  // work items of a launch
 static inline bool dl_aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // DL_BY_TYPE(type, T, statement): the statement with T as the element type

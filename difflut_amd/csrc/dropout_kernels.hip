@@ -88,7 +88,7 @@ extern "C" int dl_dropout(const void *x, void *y, int type, long long numel, dou
     const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
     const long long per_block = (long long)DROP_THREADS * DROP_UNITS * (16 / dl_type_bytes(type));
     const long long blocks = numel > 0 ? (numel + per_block - 1) / per_block : 1;
-    if (blocks > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
+    if (!dl_grid_ok(blocks, DROP_THREADS)) return DL_ERR_UNSUPPORTED;
     const DropKey key = {seed, offset};
     const bool vec = dl_aligned16(x) && dl_aligned16(y);
     dl_prof_begin("dropout", s);

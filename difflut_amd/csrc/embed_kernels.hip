@@ -548,6 +548,12 @@ extern "C" int dl_embedding_fwd(const void *tokens, int token_bits, const void *
     const long long per_block = EMB_THREADS >> bits;
     const bool many = n >= 4 * 2048 * per_block;  // enough rows for every team to take four
     const long long blocks = (n + per_block * (many ? 4 : 1) - 1) / (per_block * (many ? 4 : 1));
+    if (!dl_grid_ok(blocks, EMB_THREADS)) {  // (tens of millions of odd rows)
+        const long long half = n / 2;
+        const int rc = dl_embedding_fwd(tokens, token_bits, weight, ldw, y, type, half, V, D, scale, stream);
+        return rc != DL_OK ? rc : dl_embedding_fwd((const char *)tokens + half * (token_bits / 8), token_bits, weight, ldw,
+                                                   (char *)y + half * D * dl_type_bytes(type), type, n - half, V, D, scale, stream);
+    }
 #define LOOKUP(TOKEN, VEC, R) \
     embed_lookup<T, TOKEN, VEC, R><<<(int)blocks, EMB_THREADS, 0, s>>>((const TOKEN *)tokens, (const T *)weight, ldw, (T *)y, n, V, D, scale, bits)
 #define LOOKUP_R(TOKEN, VEC) if (many) LOOKUP(TOKEN, VEC, 4); else LOOKUP(TOKEN, VEC, 1)
@@ -571,7 +577,7 @@ static int emb_chunk(long long n) {
     const long long chunk = (n + EMB_CHUNKS - 1) / EMB_CHUNKS;
     return (int)((chunk > 4096 ? chunk + 63 : 4096) / 64 * 64);
 }
-static bool emb_long(long long n, long long V) { return n >= EMB_LONG && emb_block_bits(V) <= 9; }
+static bool emb_long(long long n, long long V) { return n >= EMB_LONG && emb_block_bits(V) <= 10; }  // (64 KB of LDS)
 
 extern "C" size_t dl_embedding_bwd_workspace_bytes(long long n, long long V, int D) {
     if (!emb_sizes_ok(n, V, D) || n <= EMB_FEW) return 0;
@@ -618,7 +624,9 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
     a.sum_blocks = (unsigned)((a.pieces + teams - 1) / teams);
     const int bits = emb_block_bits(V);
     const size_t lds = (size_t)EMB_SORT_WAVES * (size_t)((V + (1LL << bits) - 1) >> bits) * sizeof(int);
-    if ((long long)dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * dl_ceil_div(D, vec ? 256 : 64) > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
+    if (!dl_grid_ok((long long)dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * dl_ceil_div(D, vec ? 256 : 64), EMB_JOIN_THREADS) ||
+        !dl_grid_ok((long long)a.sum_blocks + 2048, EMB_THREADS))
+        return DL_ERR_UNSUPPORTED;
 #define SORT(TOKEN) \
     embed_sort<TOKEN><<<1 << bits, EMB_SORT_THREADS, lds, s>>>((const TOKEN *)tokens, (int)n, (unsigned)V, skip, bits, order, token_of, begin_of, count, total)
     if (emb_long(n, V)) {

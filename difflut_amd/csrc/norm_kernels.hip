@@ -720,7 +720,10 @@ static GnShape gn_pieces_shape(int B, long long P, int C, int G, int E) {
     return s;
 }
 static int gn_blocks(const GnShape &s) { return dl_ceil_div(s.B, s.samples) * s.tiles; }  // of the one-block forms
-static bool gn_grid_ok(const GnShape &s) { return (long long)s.B * s.tiles * s.pieces < (1LL << 31); }
+static bool gn_grid_ok(const GnShape &s, int threads) {
+    return dl_grid_ok(((long long)s.B + s.samples - 1) / s.samples * s.tiles * s.pieces, threads);
+}
+static bool gn_pieces_grid_ok(const GnShape &s) { return gn_grid_ok(s, GN_THREADS) && dl_grid_ok((long long)s.B * s.G, 256); }
 
 // The one-block form: tiles of whole groups over all of a sample's positions that a block's registers hold; false where there are
 // none, or only tiles of less than 64 bytes per position of a large tensor, whose lines every block would fetch anew.
@@ -788,7 +791,7 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
     GnShape s;
     for (const int threads : {GN_THREADS, GN_ONE_THREADS})
         if (gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_FORWARD(E), threads)) {
-            if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+            if (!gn_grid_ok(s, threads)) return DL_ERR_UNSUPPORTED;
             const bool vec = gn_vectors(s, E, x, y, nullptr);
             const bool few = s.samples > 1 || P <= gn_rows_per_step(s, E, threads);  // a position per thread
             dl_prof_begin("gn_forward_one", st);
@@ -804,7 +807,7 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
             return dl_launch_status();
         }
     s = gn_pieces_shape(B, P, C, G, E);
-    if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+    if (!gn_pieces_grid_ok(s)) return DL_ERR_UNSUPPORTED;
     const bool vec = gn_vectors(s, E, x, y, nullptr);
     const int blocks = B * s.tiles * s.pieces;
 #define FORWARD(VEC)                                                                                                                  \
@@ -843,7 +846,7 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     for (const int threads : {GN_THREADS, GN_ONE_THREADS}) {
         one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD(E), threads);
         if (!one) continue;
-        if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+        if (!gn_grid_ok(s, threads)) return DL_ERR_UNSUPPORTED;
         // of 256 threads as many blocks as the card holds at a time, rounds of them after that
         const int most = 2048 / s.tiles, want = dl_ceil_div(B, s.samples);
         rows_out = threads != GN_THREADS || want < most ? want : most > 0 ? most : 1;
@@ -865,7 +868,7 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     }
     if (!one) {
         s = gn_pieces_shape(B, P, C, G, E);
-        if (!gn_grid_ok(s)) return DL_ERR_UNSUPPORTED;
+        if (!gn_pieces_grid_ok(s)) return DL_ERR_UNSUPPORTED;
         const bool vec = gn_vectors(s, E, x, gy, gx);
         const int blocks = B * s.tiles * s.pieces;
 #define BACKWARD(VEC)                                                                                                            \

@@ -33,6 +33,7 @@
 #define SMP_BINS_PER_Z 32.0  // classes per unit of (max - l) / T: the last one holds what weighs less than e^-63.9, so nothing
 #define SMP_LIST 4096
 #define SMP_THREADS 256
+#define SMP_MOST_ROWS (1 << 21)  // of a launch (2^32 work items)
 #define SMP_DRAW_THREADS 1024
 #define SMP_MAX_CHUNKS 256
 #define SMP_GATHER 128  // logits that a wavefront gathers: fewer than 64 left and one of every lane
@@ -1255,6 +1256,15 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
     if (!logits || !uniform || !out) return DL_ERR_NULL;
     if (V > (1 << 30)) return DL_ERR_UNSUPPORTED;
     if (!top_k && top_k_all < 0) top_k_all = 0;
+    if (B > SMP_MOST_ROWS) {  // halves: each still has a block or a wavefront per row, and no workspace
+        const int m = B / 2;
+        const int rc = dl_sample(logits, ldl, type, uniform, temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all, out,
+                                 ws, ws_bytes, m, V, stream);
+        return rc != DL_OK ? rc : dl_sample((const char *)logits + m * ldl * dl_type_bytes(type), ldl, type, uniform + m,
+                                            temperature ? temperature + m : nullptr, top_k ? top_k + m : nullptr, top_p ? top_p + m : nullptr,
+                                            min_p ? min_p + m : nullptr, temperature_all, top_k_all, top_p_all, min_p_all, out + m, ws, ws_bytes,
+                                            B - m, V, stream);
+    }
     const int k_rule = top_k ? -1 : top_k_all;
     const float p_rule = top_p ? -1.0f : top_p_all;
     const size_t need = dl_sample_workspace_bytes(B, V, k_rule, p_rule);
@@ -1270,7 +1280,6 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
     if (V <= 64) {
         const int seg = V <= 8 ? 8 : V <= 16 ? 16 : V <= 32 ? 32 : 64;
         const long long blocks = ((long long)B * seg + SMP_THREADS - 1) / SMP_THREADS;
-        if (blocks > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
         dl_prof_begin("sample_pairs", s);
         DL_BY_TYPE(type, T, if (seg == 8) sample_pairs<T, 8><<<(int)blocks, SMP_THREADS, 0, s>>>(a);
                    else if (seg == 16) sample_pairs<T, 16><<<(int)blocks, SMP_THREADS, 0, s>>>(a);
@@ -1296,8 +1305,7 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
         return dl_launch_status();
     }
     smp_layout(a, (char *)ws);
-    if ((long long)B * a.chunks > 0x7fffffffLL) return DL_ERR_UNSUPPORTED;
-    const int blocks = B * a.chunks;
+    const int blocks = B * a.chunks;  // (about 2048)
     DL_BY_TYPE(type, T, DL_TIMED("sample_max", s, (sample_max<T><<<blocks, SMP_THREADS, 0, s>>>(a)));
                if (smp_may_cut(V, k_rule, p_rule)) DL_TIMED("sample_hist", s, (sample_hist<T><<<blocks, SMP_THREADS, 0, s>>>(a)));
                DL_TIMED("sample_collect", s, (sample_collect<T><<<blocks, SMP_THREADS, 0, s>>>(a)));

@@ -111,7 +111,9 @@ class Dropout(nn.Module):
     """Dropout, or (mode "flip") bit flips in front of a layer, whose mask is drawn from (seed, number of the call) and never
     stored.  The pair is the int64 buffer `state`: it travels with the state dict, so a resumed run goes on with the same masks, and
     it is read and moved on by the device, so that every replay of a captured step draws a new mask.  In evaluation the
-    input is returned as it is.  Modules with the same seed draw the same masks; a module is used on one stream at a time."""
+    input is returned as it is.  Modules with the same seed draw the same masks; a module is used on one stream at a time.
+    Each forward moves the state on, also one that activation checkpointing runs again: `ops.dropout` with a pair of one's own
+    is the call for that."""
 
     def __init__(self, p=0.5, mode="zero", seed=0):
         super().__init__()

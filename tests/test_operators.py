@@ -120,7 +120,7 @@ def test_embedding_gradient_against_differences():
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,V,D,dtype", [(20011, 3000, 68, torch.float32), (5000, 1, 24, torch.float32), (9000, 70001, 8, torch.bfloat16),
                                          (40000, 5, 129, torch.float16), (131072, 9000, 4, torch.float32), (300001, 100, 8, torch.float32),
-                                         (200003, 300001, 8, torch.bfloat16), (150000, 1, 4, torch.float32), (140000, 140001, 12, torch.float32)])
+                                         (200003, 300001, 8, torch.bfloat16), (170003, 600001, 4, torch.float32), (150000, 1, 4, torch.float32), (140000, 140001, 12, torch.float32)])
 def test_embedding_gradient_of_many_tokens(n, V, D, dtype):
     """Uneven frequencies, all tokens equal, more tokens of the vocabulary than of the text: the formula, and the same bits twice."""
     g = gen(n)
@@ -426,6 +426,24 @@ def test_more_than_two_to_the_31_elements():
     grad, = torch.autograd.grad(y, w, torch.ones_like(y))
     assert grad[[0, 1, V // 2, V - 3, V - 2, V - 1]].float().mean(1).tolist() == [1.0, 0.0, 0.0, 0.0, 1.0, 2.0]
     assert float(grad.sum(dtype=torch.float32)) == 4.0 * D
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes():
+    """A launch takes less than 2^32 work items: lookups and samples of more rows are as right at the end as at the beginning."""
+    n, D = 2 ** 26 + 1001, 129
+    w = torch.arange(5 * D, device="cuda").view(5, D).remainder(251).to(torch.bfloat16)  # (whole numbers that bf16 holds)
+    tokens = torch.arange(n, dtype=torch.int32, device="cuda") * 7 % 5
+    y = ops.embedding(tokens, w)
+    for start in range(0, n, 2 ** 22):
+        assert torch.equal(y[start:start + 2 ** 22], w[tokens[start:start + 2 ** 22].long()]), start
+    del y, tokens
+    B, V = 2 ** 22 + 9, 1030
+    best = torch.arange(B, device="cuda") * 13 % V
+    logits = torch.zeros(B, V, dtype=torch.float16, device="cuda").scatter_(1, best[:, None], 1.0)
+    temperature = torch.full((B,), 1e-3, device="cuda")  # (the others weigh exp(-1000))
+    temperature[1::2] = 0.0
+    assert torch.equal(ops.sample(logits, torch.full((B,), 0.5, device="cuda"), temperature=temperature), best)
 
 
 def test_dropout_gradient_against_differences():
