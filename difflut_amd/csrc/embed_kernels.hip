@@ -28,7 +28,7 @@
 #define EMB_FOUND 480       // tokens of its own that a wavefront remembers, as 23 bits of position and 9 bits of place (EMB_MAX_OWNED)
 #define EMB_ROWS(E) ((E) == 8 ? 8 : 16)  // rows that a team of the sums has in flight (more registers leave too few wavefronts)
 #define EMB_FEW 512         // tokens up to which the gradient takes one launch
-#define EMB_LONG 131072     // tokens from which on they are parted by owner before they are sorted
+#define EMB_LONG 81920      // tokens from which on they are parted by owner before they are sorted
 #define EMB_CHUNKS 1024     // pieces of the list there, at most
 #define EMB_JOIN_THREADS 512
 #define EMB_JOIN_WAVES (EMB_JOIN_THREADS / 64)
@@ -205,6 +205,8 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort(const TOKEN *__re
 //   embed_part_scan    where each of those begins
 //   embed_part         positions and tokens, an owner's together
 //   embed_sort_part    an owner's, by token
+// The gradient in us, every block reading all / parted, rows of 64 floats: 65536 tokens of 50000 41 / 48, 131072 146 / 56 (blocks of frequent
+// tokens read the list twice), 262144 271 / 80; of 500000 80 / 70, 112 / 81, 304 / 109.
 // (1 048 576 tokens of 50000, rows of 256 floats: the gradient 1.07 -> 0.51 ms, 0.31 of it the sums; the block of the most frequent token, 6 % of
 // the list, is what embed_sort_part's 0.11 wait for.)
 
