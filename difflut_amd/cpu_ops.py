@@ -356,7 +356,7 @@ class _PassGradient(torch.autograd.Function):
 
 @torch.no_grad()
 def sample(logits, uniform, temperature, top_k, top_p, min_p):
-    """In float64.  Settings are float32 values, like those that the device kernels read."""
+    """In float64, without the weights that round to nothing in the device's 64-bit sums.  Settings are float32 values, like those that the device kernels read."""
     B, V = logits.shape
     x = logits.double()
     x = torch.where(x.isnan(), -math.inf, x)
@@ -371,6 +371,7 @@ def sample(logits, uniform, temperature, top_k, top_p, min_p):
     top, rank = ordered[:, :1], torch.arange(V)
     w = torch.where(ordered == top, 1.0, torch.exp((ordered - top) / torch.where(T > 0, T, 1.0)))
     w = torch.where(ordered > -math.inf, w, 0.0).nan_to_num(0.0)
+    w = torch.where(w < 0.5 * 2.0 ** -min(51, 62 - (V - 1).bit_length()), 0.0, w)
     keep = (ordered > -math.inf) & ((rank < k) | (k <= 0))
     running = torch.cumsum(w * keep, 1)
     before = torch.cat([torch.zeros_like(top), running[:, :-1]], 1)

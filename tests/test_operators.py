@@ -597,6 +597,17 @@ def test_sample_extreme_settings(device, V):
 
 
 @pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V", [5, 64, 65, 1000, 3000, 70001])
+def test_sample_weights_of_nothing(device, V):
+    """A number of 0 takes the first index that weighs anything: exp(-60) < 2^-86 does not, exp(-25) > 2^-37 does."""
+    logits = torch.zeros(2, V)
+    logits[:, V - 1] = 60.0
+    logits[1, 1] = 35.0
+    for settings in (dict(), dict(top_p=1 - 2.0 ** -24), dict(top_k=V)):
+        assert ops.sample(logits.to(device), torch.zeros(2, device=device), **settings).tolist() == [V - 1, 1 if settings.get("top_p", 1) == 1 else V - 1]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
 def test_sample_strides_and_empty(device):
     g = gen(6)
     wide, uniform = torch.randn(8, 6000, generator=g), torch.rand(8, generator=g)
