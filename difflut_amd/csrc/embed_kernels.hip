@@ -626,7 +626,9 @@ extern "C" int dl_embedding_bwd(const void *tokens, int token_bits, const void *
     a.sum_blocks = (unsigned)((a.pieces + teams - 1) / teams);
     const int bits = emb_block_bits(V);
     const size_t lds = (size_t)EMB_SORT_WAVES * (size_t)((V + (1LL << bits) - 1) >> bits) * sizeof(int);
-    if (!dl_grid_ok((long long)dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * dl_ceil_div(D, vec ? 256 : 64), EMB_JOIN_THREADS) ||
+    // every launch of the call, before the first one: those behind a launch that fails would take what it left unwritten for indices
+    if (!dl_grid_ok(1LL << bits, EMB_SORT_THREADS) ||
+        !dl_grid_ok((long long)dl_ceil_div(a.pieces, EMB_JOIN_WAVES) * dl_ceil_div(D, vec ? 256 : 64), EMB_JOIN_THREADS) ||
         !dl_grid_ok((long long)a.sum_blocks + 2048, EMB_THREADS))
         return DL_ERR_UNSUPPORTED;
 #define SORT(TOKEN) \

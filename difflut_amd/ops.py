@@ -510,7 +510,8 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
 
     A token outside [0, V) gives a row of zeros and no gradient (as cross_entropy leaves out such labels); `padding_idx` is looked
     up like any other token but gets no gradient.  The weight's gradient is dense, summed in float32 in the order of the
-    positions: the same bits from run to run.  Rows of `weight` may lie apart (a slice of a wider matrix)."""
+    positions: the same bits from run to run.  Rows of `weight` may lie apart (a slice of a wider matrix).  On the device the gradient
+    of more than 512 tokens takes up to 2^30 rows of `weight` and raises beyond."""
     if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError(f"embedding weight must be a non-empty matrix (tokens, features), got {tuple(weight.shape)}")
     if tokens.dtype not in (torch.int32, torch.int64):

@@ -497,7 +497,7 @@ int dl_unfold_flip(const float *x, const uint8_t *flip, float *patches, void *pl
  * between rows, y [n, D].  A token outside [0, V) gives a row of zeros.
  * Its gradient: gw[v] = scale * sum_{t: token_t = v} gy[t], [V, D], every row written; tokens outside [0, V) and those equal to
  * `padding` (-1: none) add nothing.  Positions are sorted by token on the device and added in that order, in float: the same bits from
- * run to run.  Few tokens (up to 512) need no workspace. */
+ * run to run.  Few tokens (up to 512) need no workspace; more of them are sorted for V <= 2^30 (DL_ERR_UNSUPPORTED beyond). */
 int dl_embedding_fwd(const void *tokens, int token_bits, const void *weight, long long ldw, void *y, int type, long long n,
                      long long V, int D, float scale, void *stream);
 size_t dl_embedding_bwd_workspace_bytes(long long n, long long V, int D);

@@ -705,6 +705,19 @@ def test_c_entry_points_refuse():
     assert lib.dl_group_norm_fwd_workspace_bytes(0, 2, 3, 8, 3) == 0 and lib.dl_embedding_bwd_workspace_bytes(-1, 5, 8) == 0
 
 
+def test_embedding_gradient_refuses_vocabularies_that_the_sort_cannot_launch():
+    """More than 2^30 rows would take 2^32 work items to sort for: refused before the first launch."""
+    from difflut_amd import _native as nat
+
+    if not nat.is_built():
+        pytest.skip("not built")
+    at, unsupported = 4096, -3  # (an address that is never followed)
+    for V in (2 ** 30 + 1, 2 ** 31 - 1):
+        for n in (513, 100000):
+            for bits in (32, 64):
+                assert nat.lib().dl_embedding_bwd(at, bits, at, at, 1, n, V, 16, 1.0, -1, at, 1 << 40, None) == unsupported
+
+
 def test_module_refusals():
     from difflut_amd.utils import Dropout, GroupNorm, TokenEmbedding
 
