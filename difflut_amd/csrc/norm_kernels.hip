@@ -568,7 +568,8 @@ __global__ __launch_bounds__(THREADS) void gn_backward_sums(const T *__restrict_
     for (int c = threadIdx.x; c < width; c += THREADS) out[s.C + c] = slots[c];
 }
 
-// Per sample: the channels' sums over its pieces ([B][2][C]) and, per group, mean(gamma g) and mean(gamma g xhat).
+// Per sample: the channels' sums over its pieces ([B][2][C], or null: of a single piece they are there already) and, per group,
+// mean(gamma g) and mean(gamma g xhat).
 // One block per (sample, group): threads are (channel, share of the pieces).
 __global__ __launch_bounds__(256) void gn_backward_join(const float *__restrict__ part, const void *__restrict__ gamma, int ptype,
                                                          float *__restrict__ channel, float2 *__restrict__ group, GnShape s) {
@@ -591,8 +592,10 @@ __global__ __launch_bounds__(256) void gn_backward_join(const float *__restrict_
         __syncthreads();
         if (mine == 0 && c0 + col < s.cg) {
             for (int i = 1; i < shares; ++i) sg += share[0][i * across + col], sx += share[1][i * across + col];
-            channel[(long long)b * 2 * s.C + c] = sg;
-            channel[(long long)b * 2 * s.C + s.C + c] = sx;
+            if (channel) {
+                channel[(long long)b * 2 * s.C + c] = sg;
+                channel[(long long)b * 2 * s.C + s.C + c] = sx;
+            }
             const float ga = gn_param(gamma, ptype, c, 1.0f);
             a = fmaf(ga, sg, a);
             q = fmaf(ga, sx, q);
@@ -757,6 +760,50 @@ static bool gn_one_shape(GnShape &s, int B, long long P, int C, int G, int E, in
     return false;
 }
 
+// Which form a direction takes: the threads of a block of the one-block form, 0 for pieces.  `units`: of the larger one-block form.
+// (the workspace sizes and the calls both go by this)
+static int gn_form(GnShape &s, int B, long long P, int C, int G, int E, int units) {
+    for (const int threads : {GN_THREADS, GN_ONE_THREADS})
+        if (gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : units, threads)) return threads;
+    s = gn_pieces_shape(B, P, C, G, E);
+    return 0;
+}
+
+// What the backward keeps between its launches, as offsets into the workspace
+struct GnBackwardPlan {
+    GnShape s;
+    int threads;        // gn_form
+    int rows;           // of channels' sums, from which the parameters' gradients come; one of the one-block form: they are written at once
+    int share, shares;  // rows of a share, and how many shares many rows are added in first (0: all in one launch)
+    size_t channel, group, part, share_sums, bytes;
+};
+static GnBackwardPlan gn_backward_plan(int B, long long P, int C, int G, int E) {
+    GnBackwardPlan q = {};
+    q.threads = gn_form(q.s, B, P, C, G, E, GN_ONE_BACKWARD(E));
+    q.rows = B;
+    if (q.threads) {
+        q.rows = dl_ceil_div(B, q.s.samples);
+        if (q.threads == GN_THREADS) {
+            // as many blocks as the card holds at a time, rounds of them after that; a few rounds instead of a launch for the sums over samples
+            const int most = 2048 / q.s.tiles > 0 ? 2048 / q.s.tiles : 1;
+            q.rows = q.rows <= 4 ? 1 : q.rows < most ? q.rows : most;
+        }
+    }
+    if (q.rows > 512) q.share = dl_ceil_div(q.rows, GN_SHARES), q.shares = dl_ceil_div(q.rows, q.share);
+    const auto take = [&](size_t floats) {
+        const size_t at = q.bytes;
+        q.bytes += dl_align256(floats * sizeof(float));
+        return at;
+    };
+    const bool pieces = !q.threads;
+    q.channel = take(pieces ? (q.s.pieces > 1 ? (size_t)B * 2 * C : 0) : q.rows > 1 ? (size_t)q.rows * 2 * C : 0);
+    q.group = take(pieces ? (size_t)B * G * 2 : 0);
+    q.part = take(pieces ? (size_t)B * q.s.pieces * 2 * C : 0);
+    q.share_sums = take((size_t)q.shares * 2 * C);
+    if (!q.bytes) q.bytes = 256;  // (a call always has one)
+    return q;
+}
+
 #define GN_BY_ACT(act, ACT, ...)                   \
     do {                                           \
         if ((act) == GN_NONE) {                    \
@@ -776,7 +823,9 @@ static bool gn_one_shape(GnShape &s, int B, long long P, int C, int G, int E, in
 
 extern "C" size_t dl_group_norm_fwd_workspace_bytes(int type, int B, long long P, int C, int G) {
     if (!dl_type_known(type) || !gn_shape_ok(B, P, C, G)) return 0;
-    const GnShape s = gn_pieces_shape(B, P, C, G, 16 / dl_type_bytes(type));
+    const int E = 16 / dl_type_bytes(type);
+    GnShape s;
+    if (gn_form(s, B, P, C, G, E, GN_ONE_FORWARD(E))) return 256;  // (nothing is kept, but a call always has one)
     return dl_align256((size_t)B * G * s.slices * s.pieces * sizeof(float2));
 }
 
@@ -789,24 +838,23 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
     hipStream_t st = (hipStream_t)stream;
     const int E = 16 / dl_type_bytes(type);
     GnShape s;
-    for (const int threads : {GN_THREADS, GN_ONE_THREADS})
-        if (gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_FORWARD(E), threads)) {
-            if (!gn_grid_ok(s, threads)) return DL_ERR_UNSUPPORTED;
-            const bool vec = gn_vectors(s, E, x, y, nullptr);
-            const bool few = s.samples > 1 || P <= gn_rows_per_step(s, E, threads);  // a position per thread
-            dl_prof_begin("gn_forward_one", st);
+    const int threads = gn_form(s, B, P, C, G, E, GN_ONE_FORWARD(E));
+    if (threads) {
+        if (!gn_grid_ok(s, threads)) return DL_ERR_UNSUPPORTED;
+        const bool vec = gn_vectors(s, E, x, y, nullptr);
+        const bool few = s.samples > 1 || P <= gn_rows_per_step(s, E, threads);  // a position per thread
+        dl_prof_begin("gn_forward_one", st);
 #define ONE(VEC, NV, THREADS) \
     gn_forward_one<T, VEC, NV, THREADS, ACT><<<gn_blocks(s), THREADS, 0, st>>>((const T *)x, gamma, beta, ptype, (T *)y, (float2 *)stats, s, eps)
-            DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) {
+        DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) {
                 if (few) { if (vec) ONE(true, 1, GN_THREADS); else ONE(false, 1, GN_THREADS); }
                 else { if (vec) ONE(true, 4, GN_THREADS); else ONE(false, 4, GN_THREADS); }
             }
-                                          else { if (vec) ONE(true, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
+                                      else { if (vec) ONE(true, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_FORWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
 #undef ONE
-            dl_prof_end(st);
-            return dl_launch_status();
-        }
-    s = gn_pieces_shape(B, P, C, G, E);
+        dl_prof_end(st);
+        return dl_launch_status();
+    }
     if (!gn_pieces_grid_ok(s)) return DL_ERR_UNSUPPORTED;
     const bool vec = gn_vectors(s, E, x, y, nullptr);
     const int blocks = B * s.tiles * s.pieces;
@@ -822,9 +870,7 @@ extern "C" int dl_group_norm_fwd(const void *x, const void *gamma, const void *b
 
 extern "C" size_t dl_group_norm_bwd_workspace_bytes(int type, int B, long long P, int C, int G) {
     if (!dl_type_known(type) || !gn_shape_ok(B, P, C, G)) return 0;
-    const GnShape s = gn_pieces_shape(B, P, C, G, 16 / dl_type_bytes(type));
-    return dl_align256((size_t)B * s.pieces * 2 * C * sizeof(float)) + dl_align256((size_t)B * 2 * C * sizeof(float)) +
-           dl_align256((size_t)B * G * sizeof(float2)) + dl_align256((size_t)GN_SHARES * 2 * C * sizeof(float));
+    return gn_backward_plan(B, P, C, G, 16 / dl_type_bytes(type)).bytes;
 }
 
 extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamma, const void *beta, const float *stats, void *gx,
@@ -833,29 +879,21 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     if (!x || !gy || !stats || !ws || !(gx || ggamma || gbeta)) return DL_ERR_NULL;
     if (!dl_type_known(type) || !dl_type_known(ptype) || act < DL_ACT_NONE || act > DL_ACT_SIGMOID) return DL_ERR_UNSUPPORTED;
     if (!gn_shape_ok(B, P, C, G)) return DL_ERR_SHAPE;
-    if (ws_bytes < dl_group_norm_bwd_workspace_bytes(type, B, P, C, G)) return DL_ERR_WORKSPACE;
-    hipStream_t st = (hipStream_t)stream;
     const int E = 16 / dl_type_bytes(type);
-    float *channel = (float *)ws;
-    float2 *group = (float2 *)((char *)channel + dl_align256((size_t)B * 2 * C * sizeof(float)));
-    float *shares = (float *)((char *)group + dl_align256((size_t)B * G * sizeof(float2)));
-    float *part = (float *)((char *)shares + dl_align256((size_t)GN_SHARES * 2 * C * sizeof(float)));
-    GnShape s;
-    bool one = false;
-    int rows_out = B;  // of sums over samples
-    for (const int threads : {GN_THREADS, GN_ONE_THREADS}) {
-        one = gn_one_shape(s, B, P, C, G, E, threads == GN_THREADS ? 4 : GN_ONE_BACKWARD(E), threads);
-        if (!one) continue;
+    const GnBackwardPlan plan = gn_backward_plan(B, P, C, G, E);
+    if (ws_bytes < plan.bytes) return DL_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    const GnShape &s = plan.s;
+    const int threads = plan.threads;
+    float *channel = (float *)((char *)ws + plan.channel), *part = (float *)((char *)ws + plan.part);
+    float2 *group = (float2 *)((char *)ws + plan.group);
+    if (threads) {
         if (!gn_grid_ok(s, threads)) return DL_ERR_UNSUPPORTED;
-        // of 256 threads as many blocks as the card holds at a time, rounds of them after that
-        const int most = 2048 / s.tiles, want = dl_ceil_div(B, s.samples);
-        rows_out = threads != GN_THREADS || want < most ? want : most > 0 ? most : 1;
-        if (threads == GN_THREADS && want <= 4) rows_out = 1;  // a few rounds instead of a launch for the sums over samples
         const bool vec = gn_vectors(s, E, x, gy, gx);
         const bool few = s.samples > 1 || P <= gn_rows_per_step(s, E, threads);
         dl_prof_begin("gn_backward_one", st);
 #define ONE(VEC, NV, THREADS) \
-    gn_backward_one<T, VEC, NV, THREADS, ACT><<<rows_out * s.tiles, THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
+    gn_backward_one<T, VEC, NV, THREADS, ACT><<<plan.rows * s.tiles, THREADS, 0, st>>>((const T *)x, (const T *)gy, gamma, beta, ptype, \
                                                                                  (const float2 *)stats, channel, (T *)gx, ggamma, gbeta, s)
         DL_BY_TYPE(type, T, GN_BY_ACT(act, ACT, if (threads == GN_THREADS) {
                 if (few) { if (vec) ONE(true, 1, GN_THREADS); else ONE(false, 1, GN_THREADS); }
@@ -864,31 +902,28 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
                                       else { if (vec) ONE(true, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); else ONE(false, GN_ONE_BACKWARD(16 / sizeof(T)), GN_ONE_THREADS); }));
 #undef ONE
         dl_prof_end(st);
-        break;
-    }
-    if (!one) {
-        s = gn_pieces_shape(B, P, C, G, E);
+    } else {
         if (!gn_pieces_grid_ok(s)) return DL_ERR_UNSUPPORTED;
         const bool vec = gn_vectors(s, E, x, gy, gx);
         const int blocks = B * s.tiles * s.pieces;
 #define BACKWARD(VEC)                                                                                                            \
     GN_BY_ACT(act, ACT, DL_TIMED("gn_backward_sums", st, (gn_backward_sums<T, VEC, GN_THREADS, ACT><<<blocks, GN_THREADS, 0, st>>>( \
         (const T *)x, (const T *)gy, gamma, beta, ptype, (const float2 *)stats, part, s))));                                      \
-    DL_TIMED("gn_backward_join", st, (gn_backward_join<<<B * G, 256, 0, st>>>(part, gamma, ptype, channel, group, s)));           \
+    DL_TIMED("gn_backward_join", st, (gn_backward_join<<<B * G, 256, 0, st>>>(part, gamma, ptype, s.pieces > 1 ? channel : nullptr, group, s))); \
     if (gx)                                                                                                                       \
         GN_BY_ACT(act, ACT, DL_TIMED("gn_backward_apply", st, (gn_backward_apply<T, VEC, GN_THREADS, ACT><<<blocks, GN_THREADS, 0, st>>>( \
             (const T *)x, (const T *)gy, gamma, beta, ptype, (const float2 *)stats, (const float2 *)group, (T *)gx, s))))
         DL_BY_TYPE(type, T, if (vec) { BACKWARD(true); } else { BACKWARD(false); });
 #undef BACKWARD
     }
-    if ((ggamma || gbeta) && !(one && rows_out == 1)) {
-        int n = rows_out;
-        const float *rows = channel;
+    if ((ggamma || gbeta) && !(threads && plan.rows == 1)) {
+        int n = plan.rows;
+        const float *rows = threads || s.pieces > 1 ? channel : part;
         const int columns = dl_ceil_div(C, 32);
-        if (n > 512) {  // first in shares
-            const int share = dl_ceil_div(n, GN_SHARES), count = dl_ceil_div(n, share);
-            DL_TIMED("gn_param_grads", st, (gn_param_grads<<<columns * count, 256, 0, st>>>(rows, shares, nullptr, nullptr, ptype, n, C, share)));
-            n = count, rows = shares;
+        if (plan.shares) {
+            float *sums = (float *)((char *)ws + plan.share_sums);
+            DL_TIMED("gn_param_grads", st, (gn_param_grads<<<columns * plan.shares, 256, 0, st>>>(rows, sums, nullptr, nullptr, ptype, n, C, plan.share)));
+            n = plan.shares, rows = sums;
         }
         DL_TIMED("gn_param_grads", st, (gn_param_grads<<<columns, 256, 0, st>>>(rows, nullptr, ggamma, gbeta, ptype, n, C, n)));
     }

@@ -324,6 +324,54 @@ def test_group_norm_gradients_of_some_inputs(device):
         assert torch.equal(got, full[i])
 
 
+# [B, P, C] in G groups and the type's number, by form: rounds of blocks over many samples, small samples that share blocks, one launch for few;
+# a tile per block of 1024 threads; groups wider than a tile, of one position and of many
+NORM_FORMS = [(1, 65536, 1, 2048, 8), (1, 8192, 1, 16000, 16), (0, 8192, 1, 16000, 16), (0, 65536, 1, 64, 8), (0, 4, 1, 64, 8), (0, 256, 576, 32, 8),
+              (2, 600, 3, 1800, 1), (0, 1024, 1, 1500, 1), (1, 8192, 1, 16000, 1), (0, 700, 1, 4104, 2), (1, 16, 9215, 320, 32), (0, 2, 40000, 5000, 1)]
+
+
+@pytest.mark.parametrize("type,B,P,C,G", NORM_FORMS)
+def test_group_norm_workspaces_hold_what_is_kept(type, B, P, C, G):
+    """What a direction keeps between its launches, and no more: a mean and a sum of squares per group of a piece; two
+    sums per channel, of a sample or of a piece, their means per group, and up to 64 shares of many samples' sums."""
+    from difflut_amd import _native as nat
+
+    if not nat.is_built():
+        pytest.skip("not built")
+    x = B * P * C * (4 if type == 0 else 2)
+    forward, backward = nat.lib().dl_group_norm_fwd_workspace_bytes(type, B, P, C, G), nat.lib().dl_group_norm_bwd_workspace_bytes(type, B, P, C, G)
+    assert 0 < forward <= max(x // 16, 4096)
+    assert 0 < backward <= 8 * B * C * (1 if P == 1 else 1 + P / 4) + 8 * B * G + 512 * C + 1024
+    if C // G <= 1024 and P == 1:  # a tile in one block of 256 threads: 2048 blocks' sums at most, of 2048 channels
+        assert forward <= 256 and backward <= 2 ** 25 + 512 * C + 1024
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type,B,P,C,G", [(1, 6000, 1, 2048, 8), (0, 5000, 1, 64, 8), (0, 4, 1, 64, 8), (0, 256, 60, 32, 8), (2, 600, 3, 1800, 1), (0, 1024, 1, 1500, 1),
+                                          (0, 700, 1, 4104, 2), (1, 3, 1, 5001, 3), (1, 3, 3001, 320, 32), (0, 2, 700, 5000, 1), (2, 5, 3, 2, 1)])
+def test_group_norm_stays_within_its_workspaces(type, B, P, C, G):
+    """Workspaces of exactly the size asked for: right results, and nothing written behind them."""
+    from difflut_amd import _native as nat
+
+    lib, dtype, g = nat.lib(), TYPES[type], gen(B + C)
+    x, gy = ((torch.randn(B, P, C, generator=g) * 0.4 + m).to(dtype) for m in (0.5, 0.0))
+    weight, bias = ((torch.randn(C, generator=g) * 0.2 + m).to(dtype) for m in (1.0, 0.0))
+    want = norm_64(x, G, weight, bias, 1e-2, "silu", gy, depth=256)
+    x, gy, weight, bias = (t.cuda() for t in (x, gy, weight, bias))
+    y, gx, gw, gb, stats = torch.empty_like(x), torch.empty_like(x), torch.empty_like(weight), torch.empty_like(bias), torch.empty(B, G, 2, device="cuda")
+    sizes = [lib.dl_group_norm_fwd_workspace_bytes(type, B, P, C, G), lib.dl_group_norm_bwd_workspace_bytes(type, B, P, C, G)]
+    spaces = [torch.full((n + 8192,), 90, dtype=torch.uint8, device="cuda") for n in sizes]
+    at = lambda t: t.data_ptr()  # noqa: E731
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.dl_group_norm_fwd(at(x), at(weight), at(bias), at(y), at(stats), type, type, B, P, C, G, 1e-2, 2, at(spaces[0]), sizes[0], stream) == 0
+    assert lib.dl_group_norm_bwd(at(x), at(gy), at(weight), at(bias), at(stats), at(gx), at(gw), at(gb), type, type, B, P, C, G, 2, at(spaces[1]), sizes[1],
+                                 stream) == 0
+    for t, (exact, bound) in zip((y, gx, gw, gb), want):
+        close(t.reshape(exact.shape), exact, bound, dtype)
+    for n, space in zip(sizes, spaces):
+        assert bool((space[n:] == 90).all())
+
+
 # ----------------------------------------------------------------------------- dropout
 def philox(seed, offset, numel, start=0):
     """By numpy's 64-bit products, from the generator's definition; words start .. (a multiple of 4)."""
