@@ -524,7 +524,10 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_few(const TOKEN *__restrict
 }
 
 // ---------------------------------------------------------------------------------- host
-static bool emb_sizes_ok(long long n, long long V, int D) { return n >= 0 && n < (1LL << 31) - 65536 && V > 0 && V < (1LL << 31) && D > 0; }
+// (positions and columns are counted in 32 bits, some of them by a block's step past the last)
+static bool emb_sizes_ok(long long n, long long V, int D) {
+    return n >= 0 && n < (1LL << 31) - 65536 && V > 0 && V < (1LL << 31) && D > 0 && D < (1LL << 31) - 65536;
+}
 static int emb_lane_bits(int D, int E) {  // a team of up to a block's threads, as many as a row has vectors
     int bits = 0;
     while (bits < 8 && ((long long)E << bits) < D) ++bits;

@@ -668,8 +668,9 @@ __global__ __launch_bounds__(256) void gn_param_grads(const float *__restrict__ 
 }
 
 // ---------------------------------------------------------------------------------- host
+// (channels are counted in 32 bits, some of them by a tile past the last)
 static bool gn_shape_ok(int B, long long P, int C, int G) {
-    return B > 0 && P > 0 && C > 0 && G > 0 && C % G == 0 && P < (1LL << 31) && (long long)B * G < (1LL << 31);
+    return B > 0 && P > 0 && C > 0 && C < (1LL << 31) - 65536 && G > 0 && C % G == 0 && P < (1LL << 31) && (long long)B * G < (1LL << 31);
 }
 // The tiles of channels for blocks of `threads` threads that hold E channels each.
 static GnShape gn_tiles(int B, long long P, int C, int G, int E, int threads) {

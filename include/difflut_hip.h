@@ -488,6 +488,7 @@ int dl_unfold_flip(const float *x, const uint8_t *flip, float *patches, void *pl
 /* ------------------------------------------------------------------------
  * Around the layers, in models over tokens and deep convolutional stacks.  No counterpart in the reference.
  * `type` / `ptype`: element type of tensors / of gamma and beta; 16-bit values are widened to float, results rounded once.
+ * Tokens n, features D and channels C are below 2^31 - 65536 (DL_ERR_SHAPE).
  * ------------------------------------------------------------------------ */
 #define DL_F32 0
 #define DL_BF16 1

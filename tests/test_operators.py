@@ -766,6 +766,21 @@ def test_embedding_gradient_refuses_vocabularies_that_the_sort_cannot_launch():
                 assert nat.lib().dl_embedding_bwd(at, bits, at, at, 1, n, V, 16, 1.0, -1, at, 1 << 40, None) == unsupported
 
 
+def test_rows_whose_last_columns_do_not_fit_32_bits_are_refused():
+    """Features and channels near 2^31: a step past the last column would be a negative number."""
+    from difflut_amd import _native as nat
+
+    if not nat.is_built():
+        pytest.skip("not built")
+    lib, at, shape, big = nat.lib(), 4096, -2, 1 << 40  # (an address that is never followed)
+    for D in (2 ** 31 - 1, 2 ** 31 - 1024, 2 ** 31 - 65536):
+        assert lib.dl_embedding_fwd(at, 64, at, D, at, 1, 3, 1, D, 1.0, None) == shape
+        for n in (3, 600):
+            assert lib.dl_embedding_bwd(at, 64, at, at, 1, n, 1, D, 1.0, -1, at, big, None) == shape
+        assert lib.dl_group_norm_fwd(at, at, at, at, at, 1, 1, 1, 1, D, 1, 1e-5, 0, at, big, None) == shape
+        assert lib.dl_group_norm_bwd(at, at, at, at, at, at, None, None, 1, 1, 1, 1, D, 1, 0, at, big, None) == shape
+
+
 def test_module_refusals():
     from difflut_amd.utils import Dropout, GroupNorm, TokenEmbedding
 
