@@ -646,25 +646,32 @@ __global__ __launch_bounds__(THREADS) void gn_backward_apply(const T *__restrict
 // ggamma_c = sum g xhat, gbeta_c = sum g over n rows of [2][C]: a block takes 32 channels of a share of the rows, 8 at a step, added in a
 // fixed order.  With `part` the shares' sums go there, as rows of the same kind.
 __global__ __launch_bounds__(256) void gn_param_grads(const float *__restrict__ channel, float *__restrict__ part, void *__restrict__ ggamma,
-                                                       void *__restrict__ gbeta, int ptype, int n, int C, int share) {
+                                                       void *__restrict__ gbeta, int ptype, int n, int C, int share, int shares) {
     __shared__ float red[2][8][32];
-    const int columns = (C + 31) / 32, c = blockIdx.x % columns * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5, mine = blockIdx.x / columns;
-    float sg = 0.0f, sx = 0.0f;
-    const int end = min((mine + 1) * (long long)share, (long long)n);
-    if (c < C)
+    const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, columns = (C + 31) / 32;
+    const unsigned items = (unsigned)columns * shares;  // (below 2^26 times GN_SHARES)
+    for (unsigned item = blockIdx.x;; item += gridDim.x) {
+        const int c = (int)(item % columns) * 32 + lane, mine = item / columns;
+        float sg = 0.0f, sx = 0.0f;
+        const int end = min((mine + 1) * (long long)share, (long long)n);
+        if (c < C)
 #pragma unroll 8
-        for (int i = mine * share + r; i < end; i += 8) {
-            sg += channel[(long long)i * 2 * C + c];
-            sx += channel[(long long)i * 2 * C + C + c];
+            for (int i = mine * share + r; i < end; i += 8) {
+                sg += channel[(long long)i * 2 * C + c];
+                sx += channel[(long long)i * 2 * C + C + c];
+            }
+        red[0][r][lane] = sg, red[1][r][lane] = sx;
+        __syncthreads();
+        if (threadIdx.x < 64 && c < C) {
+            const int which = threadIdx.x >> 5;
+            float t = 0.0f;
+            for (int i = 0; i < 8; ++i) t += red[which][i][lane];
+            if (part) part[((long long)mine * 2 + which) * C + c] = t;
+            else gn_param_store(which ? ggamma : gbeta, ptype, c, t);
         }
-    red[0][r][threadIdx.x & 31] = sg, red[1][r][threadIdx.x & 31] = sx;
-    __syncthreads();
-    if (threadIdx.x >= 64 || c >= C) return;
-    const int which = threadIdx.x >> 5;
-    float t = 0.0f;
-    for (int i = 0; i < 8; ++i) t += red[which][i][threadIdx.x & 31];
-    if (part) part[((long long)mine * 2 + which) * C + c] = t;
-    else gn_param_store(which ? ggamma : gbeta, ptype, c, t);
+        if (items - item <= gridDim.x) return;
+        __syncthreads();
+    }
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -717,6 +724,7 @@ static int gn_rows_per_step(const GnShape &s, int E, int threads) {
 #define GN_ONE_FORWARD(E) ((E) == 8 ? 10 : 12)
 #define GN_ONE_BACKWARD(E) ((E) == 8 ? 4 : 6)
 #define GN_SHARES 64  // of many samples, in the sums of the parameters' gradients
+#define GN_PARAM_BLOCKS (1 << 20)  // of their launch
 
 static GnShape gn_pieces_shape(int B, long long P, int C, int G, int E) {
     GnShape s = gn_tiles(B, P, C, G, E, GN_THREADS);
@@ -920,13 +928,16 @@ extern "C" int dl_group_norm_bwd(const void *x, const void *gy, const void *gamm
     if ((ggamma || gbeta) && !(threads && plan.rows == 1)) {
         int n = plan.rows;
         const float *rows = threads || s.pieces > 1 ? channel : part;
-        const int columns = dl_ceil_div(C, 32);
+        const auto blocks = [&](int shares) {  // of all channels, each of every shares' rows; the blocks go on where there are more than a launch takes
+            const long long all = (long long)dl_ceil_div(C, 32) * shares;
+            return (int)(all < GN_PARAM_BLOCKS ? all : GN_PARAM_BLOCKS);
+        };
         if (plan.shares) {
             float *sums = (float *)((char *)ws + plan.share_sums);
-            DL_TIMED("gn_param_grads", st, (gn_param_grads<<<columns * plan.shares, 256, 0, st>>>(rows, sums, nullptr, nullptr, ptype, n, C, plan.share)));
+            DL_TIMED("gn_param_grads", st, (gn_param_grads<<<blocks(plan.shares), 256, 0, st>>>(rows, sums, nullptr, nullptr, ptype, n, C, plan.share, plan.shares)));
             n = plan.shares, rows = sums;
         }
-        DL_TIMED("gn_param_grads", st, (gn_param_grads<<<columns, 256, 0, st>>>(rows, nullptr, ggamma, gbeta, ptype, n, C, n)));
+        DL_TIMED("gn_param_grads", st, (gn_param_grads<<<blocks(1), 256, 0, st>>>(rows, nullptr, ggamma, gbeta, ptype, n, C, n, 1)));
     }
     return dl_launch_status();
 }

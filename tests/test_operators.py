@@ -372,6 +372,26 @@ def test_group_norm_stays_within_its_workspaces(type, B, P, C, G):
         assert bool((space[n:] == 90).all())
 
 
+@pytest.mark.gpu
+def test_group_norm_gradients_of_more_channels_than_a_launch_takes():
+    """2^29 channels and more: 32 to a block of 256 threads would be 2^32 work items.  x of 1 and -1 in turn under statistics of 0 and 1:
+    the gradients are gy and gy x as they are (one sample, one position: nothing is added)."""
+    from difflut_amd import _native as nat
+
+    G, C = 64, 2 ** 29 + 64 * 6
+    x, ones = torch.ones(C, dtype=torch.bfloat16, device="cuda"), torch.ones(C, dtype=torch.bfloat16, device="cuda")
+    x[1::2] = -1
+    gy = (torch.arange(C, dtype=torch.int32, device="cuda") % 257 - 128).to(torch.bfloat16)  # (whole numbers that bf16 holds)
+    stats = torch.tensor([0.0, 1.0], device="cuda").repeat(G)
+    gw, gb = (torch.full((C,), 500.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    need = nat.lib().dl_group_norm_bwd_workspace_bytes(1, 1, 1, C, G)
+    space = torch.empty(need, dtype=torch.uint8, device="cuda")
+    at = lambda t: t.data_ptr()  # noqa: E731
+    assert nat.lib().dl_group_norm_bwd(at(x), at(gy), at(ones), None, at(stats), None, at(gw), at(gb), 1, 1, 1, 1, C, G, 0, at(space), need,
+                                       torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(gb, gy) and torch.equal(gw, gy * x)
+
+
 # ----------------------------------------------------------------------------- dropout
 def philox(seed, offset, numel, start=0):
     """By numpy's 64-bit products, from the generator's definition; words start .. (a multiple of 4)."""
