@@ -111,17 +111,21 @@ class Dropout(nn.Module):
     """Dropout, or (mode "flip") bit flips in front of a layer, whose mask is drawn from (seed, number of the call) and never
     stored.  The pair is the int64 buffer `state`: it travels with the state dict, so a resumed run goes on with the same masks, and
     it is read and moved on by the device, so that every replay of a captured step draws a new mask.  In evaluation the
-    input is returned as it is.  Modules with the same seed draw the same masks; a module is used on one stream at a time.
+    input is returned as it is.  Without a `seed` one is drawn from torch's default generator, so that modules have noise of their own,
+    and the same again after torch.manual_seed; where the state is the same (a seed given twice, a copied module, buffers broadcast from one
+    data-parallel rank) the masks are.  A module is used on one stream at a time.
     Each forward moves the state on, also one that activation checkpointing runs again: `ops.dropout` with a pair of one's own
     is the call for that."""
 
-    def __init__(self, p=0.5, mode="zero", seed=0):
+    def __init__(self, p=0.5, mode="zero", seed=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must be in [0, 1], got {p}")
         if mode not in ops.DROP_MODES:
             raise ValueError(f"mode must be one of {list(ops.DROP_MODES)}, got {mode!r}")
         self.p, self.mode = p, mode
+        if seed is None:
+            seed = int(torch.randint(-(1 << 63), (1 << 63) - 1, (), dtype=torch.int64, device="cpu"))
         self.register_buffer("state", torch.tensor([ops._signed64(seed), 0], dtype=torch.int64))
 
     def forward(self, x):

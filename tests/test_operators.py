@@ -475,6 +475,26 @@ def test_dropout_module(device):
     assert drop.eval()(x) is x
 
 
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("mode", ["zero", "flip"])
+def test_dropout_modules_have_noise_of_their_own(device, mode):
+    """Modules built without a seed draw different masks, and the same ones again after torch.manual_seed; a seed given is kept."""
+    from difflut_amd.utils import Dropout
+
+    def build():
+        torch.manual_seed(5)
+        return [Dropout(0.5, mode).to(device) for _ in range(3)]
+
+    x = torch.full((64, 64), 0.25, device=device)
+    hits = [drop(x) != x * (1 if mode == "flip" else 2) for drop in build()]
+    for i in range(3):
+        for j in range(i):  # of 4096 independent pairs half are equal, within 6 standard deviations of 32
+            assert abs(int((hits[i] == hits[j]).sum()) - 2048) <= 192
+    assert all(torch.equal(drop(x) != x * (1 if mode == "flip" else 2), hit) for drop, hit in zip(build(), hits))
+    assert torch.equal(Dropout(0.5, mode, seed=0).to(device)(x), ops.dropout(x, 0.5, (0, 0), mode))
+    assert Dropout(0.5, seed=7).state.tolist() == [7, 0]
+
+
 @pytest.mark.gpu
 def test_more_than_two_to_the_31_elements():
     """Offsets past 32 bits: the last entries of a dropout, a lookup and a gradient."""
