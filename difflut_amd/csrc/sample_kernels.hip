@@ -1255,7 +1255,6 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
     if (B == 0) return DL_OK;
     if (!logits || !uniform || !out) return DL_ERR_NULL;
     if (V > (1 << 30)) return DL_ERR_UNSUPPORTED;
-    if (!top_k && top_k_all < 0) top_k_all = 0;
     if (B > SMP_MOST_ROWS) {  // halves: each still has a block or a wavefront per row, and no workspace
         const int m = B / 2;
         const int rc = dl_sample(logits, ldl, type, uniform, temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all, out,
@@ -1265,7 +1264,7 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
                                             min_p ? min_p + m : nullptr, temperature_all, top_k_all, top_p_all, min_p_all, out + m, ws, ws_bytes,
                                             B - m, V, stream);
     }
-    const int k_rule = top_k ? -1 : top_k_all;
+    const int k_rule = top_k ? -1 : top_k_all;  // (as the size function was asked: by the number itself)
     const float p_rule = top_p ? -1.0f : top_p_all;
     const size_t need = dl_sample_workspace_bytes(B, V, k_rule, p_rule);
     if (need && !ws) return DL_ERR_NULL;
@@ -1273,7 +1272,7 @@ extern "C" int dl_sample(const void *logits, long long ldl, int type, const floa
     hipStream_t s = (hipStream_t)stream;
     SampleArgs a = {};
     a.logits = logits, a.ldl = ldl, a.uniform = uniform, a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
-    a.T = temperature_all, a.k = top_k_all, a.p = top_p_all, a.m = min_p_all, a.out = out, a.B = B, a.V = V;
+    a.T = temperature_all, a.k = top_k_all > 0 ? top_k_all : 0, a.p = top_p_all, a.m = min_p_all, a.out = out, a.B = B, a.V = V;
     int bits = 0;
     while ((1LL << bits) < V) ++bits;
     a.shift = 62 - bits < 51 ? 62 - bits : 51;

@@ -537,7 +537,7 @@ int dl_dropout(const void *x, void *y, int type, long long numel, double p, int 
  * first of the order; -1 where no logit is above -infinity (NaN counts as that).
  * Settings: device arrays [B] where given, else the numbers behind them for every row.
  * Workspace: dl_sample_workspace_bytes(B, V, top_k_all or -1 with an array, top_p_all or -1 with an array), 0 for all but few
- * long rows. */
+ * long rows.  V <= 2^30 (DL_ERR_UNSUPPORTED beyond). */
 size_t dl_sample_workspace_bytes(int B, int V, int top_k_all, float top_p_all);
 int dl_sample(const void *logits, long long ldl, int type, const float *uniform, const float *temperature, const int *top_k,
               const float *top_p, const float *min_p, float temperature_all, int top_k_all, float top_p_all, float min_p_all,

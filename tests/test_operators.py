@@ -695,6 +695,23 @@ def test_sample_weights_of_nothing(device, V):
         assert ops.sample(logits.to(device), torch.zeros(2, device=device), **settings).tolist() == [V - 1, 1 if settings.get("top_p", 1) == 1 else V - 1]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,V,top_p", [(1, 50000, 1.0), (3, 40000, 1.0), (20, 40000, 1.0), (1, 300000, 1.0), (1, 70000, 0.5), (2, 900, 0.5)])
+def test_sample_negative_top_k_keeps_all(B, V, top_p):
+    """The C entry point's top_k_all <= 0 keeps all, with the workspace that is asked for with the same number."""
+    from difflut_amd import _native as nat
+
+    lib, g = nat.lib(), gen(V)
+    logits, uniform = torch.randn(B, V, generator=g).cuda(), torch.rand(B, generator=g).cuda()
+    want = ops.sample(logits, uniform, top_p=top_p)
+    for k in (-5, -1, 0, -2 ** 31):
+        need = lib.dl_sample_workspace_bytes(B, V, k, top_p)
+        space, out = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda"), torch.full((B,), -7, device="cuda")
+        assert lib.dl_sample(logits.data_ptr(), V, 0, uniform.data_ptr(), None, None, None, None, 1.0, k, top_p, 0.0, out.data_ptr(),
+                             space.data_ptr() if need else None, need, B, V, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, want), k
+
+
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 def test_sample_strides_and_empty(device):
     g = gen(6)
