@@ -9,10 +9,12 @@
 //
 // Neighbouring running sums lie close together, so weights are 64-bit integers, round(2^shift w) with shift = min(51, 62 - ceil(log2 V)),
 // from exponentials in double: sums fit, are exact in any order - blocks and atomics can split them as they like, every run gives the
-// same index - and a weight is off by 2^-(shift + 1), 2^-46 at V = 131072.
+// same index - and a weight is off by 2^-(shift + 1), 2^-46 at V = 131072.  Only top-p's limit, and the weight before the classes that its
+// cut can be in, come from other sums in rows of more than SMP_WAVE columns: of classes (smp_class_term), whole numbers as well, off from the
+// weights' by as much as a weight and a few roundings of a double.
 //
 // Up to 64 columns: a few lanes per row compare every pair.  Up to SMP_WAVE: a wavefront per row, in its registers.  More: a block per row
-// (sample_row), which reads it once into its registers where it fits; or, for few long rows, four launches over pieces of rows
+// (sample_row), which reads it anew for every pass, mostly from the L2; or, for few long rows, four launches over pieces of rows
 // (sample_max, sample_hist, sample_collect, sample_draw).  Both go the same way:
 //   - the largest logit;
 //   - number or weight of the logits in SMP_BINS classes of (max - l) / T, a monotone function of l: they say which classes the cuts
@@ -498,11 +500,14 @@ __device__ __forceinline__ int smp_bin(uint32_t key, uint32_t top, const SampleR
     return smp_bin(key, top, r, rest);
 }
 // A class's weight is e^(-class / 32) times the sum of e^(-rest / 32) over its logits; that sum, whose terms lie within 1.6 % of 1, is kept
-// as 2^(62 - ceil(log2 V)) of it: a polynomial of degree 4 (off by 6 2^-44) and no power of two per logit.
+// as 2^(62 - ceil(log2 V)) of it: a polynomial of degree 5 and no power of two per logit.  The polynomial is Taylor's with d^6 / 720 taken
+// into the even terms (least largest error on |d| <= 1/64 with 1 kept at 0): off by 2^-50.1; of degree 4, Taylor's is off by 2^-36.9, which
+// moves a nucleus' end by a logit where its limit comes that near to one.
 __device__ __forceinline__ u64 smp_class_term(double rest, double unit) {
     const double d = rest * (-1.0 / SMP_BINS_PER_Z);
-    double e = fma(d, 1.0 / 24.0, 1.0 / 6.0);
-    e = fma(e, d, 0.5);
+    double e = fma(d, 1.0 / 120.0, 0.04166713877524326);
+    e = fma(e, d, 1.0 / 6.0);
+    e = fma(e, d, 0.49999999996433814);
     e = fma(e, d, 1.0);
     e = fma(e, d, 1.0);
     return (u64)__double_as_longlong(fma(e, unit, 4503599627370496.0)) & ((1ull << 52) - 1);

@@ -584,7 +584,9 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     weight is at least min_p; the first always stays.  The answer is the first kept index whose running sum, in index order, exceeds
     uniform times the kept sum.  temperature 0 takes the first of the order.  NaN counts as -infinity; a row with nothing above
     that gives -1.  Weights are summed in 64 bits, as multiples of 2^-51 (2^-(62 - ceil(log2 V)) where V
-    is more than 2048), so the answer does not depend on how the work is split; one of less than half of that is never drawn.
+    is more than 2048), so the answer does not depend on how the work is split; one of less than half of that is never drawn.  (top_p's
+    limit on rows of more than 1024 is off by about as much as a weight: which one is the last kept can differ where the limit lies
+    within that of a weight's border.)
 
     Each setting is a number or a tensor [B] with every row's own (whose values are not looked at on the host: temperature <= 0,
     top_p <= 0 and min_p > 1 leave the first index alone)."""

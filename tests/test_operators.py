@@ -6,6 +6,7 @@ half a step of it, eps(t) / 2 times its size.  A float32 sum of terms a_i in whi
 off by d u sum |a_i|; the bounds below are taken element by element from the exact values.
 """
 import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -693,6 +694,31 @@ def test_sample_weights_of_nothing(device, V):
     logits[1, 1] = 35.0
     for settings in (dict(), dict(top_p=1 - 2.0 ** -24), dict(top_k=V)):
         assert ops.sample(logits.to(device), torch.zeros(2, device=device), **settings).tolist() == [V - 1, 1 if settings.get("top_p", 1) == 1 else V - 1]
+
+
+# columns, their distance from the largest logit, top-p: what is kept ends 2 to 5 parts in 10^12 from a logit's border.  Rows with a list of what
+# is open, rows that are searched, rows over blocks.
+BORDERS = [(4001, 1 / 64, "0x1.5d5a720000000p-1"), (4006, 1 / 64, "0x1.8f47920000000p-3"), (4013, 3 / 64, "0x1.feda0c0000000p-1"),
+           (4021, 3 / 64, "0x1.d30f020000000p-2"), (1831, 1 / 64, "0x1.7f17a20000000p-1"), (1830, 3 / 64, "0x1.0629680000000p-1"),
+           (5005, 1 / 64, "0x1.365f9c0000000p-2"), (5006, 3 / 64, "0x1.3341f20000000p-3")]
+
+
+@pytest.mark.parametrize("device,V,distance,p", [pytest.param(d, *case, marks=[pytest.mark.gpu] * (d == "cuda")) for d in ("cpu", "cuda") for case in BORDERS] + [
+    pytest.param("cuda", *case, marks=pytest.mark.gpu) for case in ((70001, 1 / 64, "0x1.621fb00000000p-3"), (70002, 3 / 64, "0x1.de66740000000p-3"))])
+def test_sample_nucleus_ends_where_the_weights_say(device, V, distance, p):
+    """The largest logit first, the others equal.  Weights are whole numbers, so what top-p keeps is known exactly; the last of it is drawn.
+    The limit's roundings: a weight's, at most 2^-46 of it at these sizes, a few of a double's, the 64-bit oracle's V 2^-53 on the CPU - in
+    all less than 10^-12 of it, and the border is more than 2 10^-12 away."""
+    shift = min(51, 62 - (V - 1).bit_length())
+    first, each = 1 << shift, round(math.exp(-distance) * 2 ** shift)
+    limit = Fraction(float.fromhex(p)) * (first + (V - 1) * each)
+    kept = 1 + max(0, math.ceil((limit - first) / each))
+    borders = [abs(1 - (first + n * each) / limit) for n in (kept - 2, kept - 1)]
+    assert 2e-12 < min(borders) < 5e-12 and kept < V
+    logits = torch.full((1, V), -distance)
+    logits[0, 0] = 0.0
+    uniform = torch.tensor([1 - 2.0 ** -24])  # (short of the whole by 2^-24 of it, less than the last weight)
+    assert ops.sample(logits.to(device), uniform.to(device), top_p=float.fromhex(p)).item() == kept - 1
 
 
 @pytest.mark.gpu
