@@ -416,6 +416,32 @@ def test_philox_known_answers():
         assert philox_words(ops._signed64(seed), ops._signed64(offset), 1001).tolist() == philox(seed, offset, 1001).tolist()
 
 
+def philox_4x32(counter, key):
+    """Ten rounds on four words under two, in Python's whole numbers."""
+    (c0, c1, c2, c3), (k0, k1) = counter, key
+    for _ in range(10):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57
+        c0, c1, c2, c3 = (b >> 32) ^ c1 ^ k0, b % 2 ** 32, (a >> 32) ^ c3 ^ k1, a % 2 ** 32
+        k0, k1 = (k0 + 0x9E3779B9) % 2 ** 32, (k1 + 0xBB67AE85) % 2 ** 32
+    return [c0, c1, c2, c3]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_philox_words_where_they_belong(device):
+    """The three answers that are published with the generator (zeros, ones, digits of pi), then the order of the words: seed and offset have
+    four different ones, and each decides the mask."""
+    ones = 0xFFFFFFFF
+    for counter, key, answer in (((0,) * 4, (0, 0), "6627e8d5 e169c58d bc57ac4c 9b00dbd8"), ((ones,) * 4, (ones, ones), "408f276d 41c83b0e a20bc7c6 6d5451fd"),
+                                 ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0), "d16cfe09 94fdcceb 5001e420 24126ea1")):
+        assert " ".join(f"{w:08x}" for w in philox_4x32(counter, key)) == answer
+    low, high, k0, k1 = 0x13198A2E, 0x03707344, 0xA4093822, 0x299F31D0
+    words = [w for i in range(250) for w in philox_4x32((i, 0, low, high), (k0, k1))]
+    for p in (0.5, 0.1, 0.9):
+        hit = torch.tensor([w < math.floor(p * 2.0 ** 32 + 0.5) for w in words])
+        y = ops.dropout(torch.full((1000,), 0.25, device=device), p, (k1 << 32 | k0, high << 32 | low), mode="flip")
+        assert torch.equal(y.cpu() == 0.75, hit)
+
+
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 @pytest.mark.parametrize("shape", [(1,), (3, 5), (64, 100), (7, 1025), (0, 4)])
 @pytest.mark.parametrize("dtype", TYPES)
