@@ -4,7 +4,8 @@
 //
 // A token outside [0, V) gives a row of zeros and adds nothing to the gradient; one that equals `padding` adds nothing either.
 //
-// The gradient of many tokens takes three launches and no atomics on floats, so its bits do not depend on the schedule:
+// The gradient of many tokens takes three launches (six where a long list is parted first) and no atomics on floats, so its bits do not
+// depend on the schedule:
 //   embed_sort   positions sorted by token, ascending within one.  Block b owns the tokens v with v mod blocks = b and reads
 //                the whole token list (it stays in the L2): how many tokens belong to lower blocks is where its own begin.  Owning
 //                every blocks-th token spreads the frequent ones, which lie together at the low ids of a vocabulary.
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(EMB_SORT_THREADS) void embed_sort_part(const int *_
 struct EmbArgs {
     const int *order, *token_of, *begin_of, *count, *total;
     float *part;  // [pieces][2][D]: of the token that began in an earlier piece, of the one that goes on into the next
-    long long V, ldg;
+    long long V;
     int D, lane_bits, pieces, piece;  // sorted positions are walked in `pieces` pieces of `piece`
     unsigned sum_blocks;
     float scale;
@@ -573,11 +574,15 @@ extern "C" int dl_embedding_fwd(const void *tokens, int token_bits, const void *
 }
 
 // Sorted positions per piece: a piece ends inside a token's run twice, for two partials to write and to read again, so longer ones move
-// less; but there have to be enough teams.  (65521 x 1024 bf16: 32; 12544 x 784 fp32: 16, 17 us for 24.)
+// less; but there have to be enough teams.  The gradient in us with 16 / 32 positions, by tokens x features in millions: 4.2 (16384 x 256)
+// 24.4 / 29.0, 8.4 (65521 x 128) 47.7 / 53.6, 9.8 (12544 x 784) 32.0 / 37.1, 16.8 (32768 x 512) 42.7 / 45.8, 19.3 (24576 x 784) 49.0 / 48.7,
+// 25.2 (65521 x 384) 63.9 / 63.0, 25.7 (32768 x 784) 57.8 / 56.6, 33.6 (131072 x 256) 77.3 / 74.5, 67 (65521 x 1024 bf16) 109.0 / 105.6.
 static int emb_piece(long long n, int D) { return n * D >= (1LL << 24) + (1LL << 23) ? 32 : 16; }
 static long long emb_pieces(long long n, int D) { return (n + emb_piece(n, D) - 1) / emb_piece(n, D); }
 
-// Parting a long list: chunks of whole groups of 64 tokens, and the owners that their counts' LDS has room for
+// Parting a long list: chunks of whole groups of 64 tokens, and the owners that their counts' LDS has room for: up to 1024 of 512 rows.  A
+// larger vocabulary's blocks all read the whole list, so time goes by tokens times rows (rows of 16 floats, us, 524288 rows / 524289 /
+// 4194304: 131072 tokens 66 / 154 / 552, 1048576 tokens 226 / 1132 / 3837).
 static int emb_chunk(long long n) {
     const long long chunk = (n + EMB_CHUNKS - 1) / EMB_CHUNKS;
     return (int)((chunk > 4096 ? chunk + 63 : 4096) / 64 * 64);

@@ -528,7 +528,8 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
 
 def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
     """Group norm of x [B, ..., C] (channels last) over the positions and the C / groups channels of each group, then weight [C]
-    and bias [C] (of one type; either may be missing), then `activation`: "none", "relu", "silu" or "sigmoid"."""
+    and bias [C] (of one type; either may be missing), then `activation`: "none", "relu", "silu" or "sigmoid".  On the device a batch
+    whose launches would have 2^32 threads or more raises (2^22 samples and more, by their size)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     if x.dim() < 2 or x.numel() == 0:

@@ -507,7 +507,9 @@ int dl_embedding_bwd(const void *tokens, int token_bits, const void *gy, void *g
 
 /* Group norm over channels-last activations x [B, P, C] (P positions, G groups of C / G neighbouring channels), with an
  * activation: y = act((x - mean) * rstd * gamma + beta), rstd = 1 / sqrt(var + eps); gamma / beta [C] may be null (1 / 0).
- * stats [B, G, 2] receives mean and rstd for the backward, which writes gx, ggamma, gbeta (each may be null). */
+ * stats [B, G, 2] receives mean and rstd for the backward, which writes gx, ggamma, gbeta (each may be null).
+ * A block of 256 or 1024 threads takes a sample's tile of up to 2048 channels (small samples share one, large ones are split); a batch
+ * whose launch would have 2^32 threads or more, or B * G >= 2^24 where samples are split, is refused (DL_ERR_UNSUPPORTED). */
 #define DL_ACT_NONE 0
 #define DL_ACT_RELU 1
 #define DL_ACT_SILU 2
