@@ -24,10 +24,10 @@
 //   - the list, sorted, gives the cut; then the piece that the target falls into, then the index.  A list that is too long
 //     (many equal logits) is searched over the whole row instead.
 //
-// What bounds it: short rows, the chain of barriers and wavefront sums; long ones, instructions per logit - 25 for its class's sum, an
-// exponential's 30 for the few that are kept.  us: 256 rows of 131072 fp32, top-p of 0.9: 99 (largest 20, classes 24, pieces and list
+// What bounds it: short rows, the chain of barriers and wavefront sums; long ones, instructions per logit - 26 for its class's sum, an
+// exponential's 30 for the few that are kept.  us: 256 rows of 131072 fp32, top-p of 0.9: 100 (largest 20, classes 25, pieces and list
 // 26, the rest 22; 260 in four launches with library exponentials); one row of 49999 bf16, all filters: 15; 64 rows of 32768
-// fp16, top-k up to 80: 17, 32 with a row that has no top-k; 8192 x 1000 fp32, top-k and top-p: 48 (178 sorted in LDS); 8192 x 10: 5.
+// fp16, top-k up to 80: 17, 32 with a row that has no top-k; 8192 x 1000 fp32, top-k and top-p: 45 (178 sorted in LDS); 8192 x 10: 5.
 #include "dl_types.h"
 
 #define SMP_WAVE 1024
