@@ -116,6 +116,17 @@ SIGNATURES = {
     "dl_dropout": (_I, [_P, _P, _I, _L, ctypes.c_double, _I, ctypes.c_ulonglong, ctypes.c_ulonglong, _P, _P, _P]),
     "dl_sample_workspace_bytes": (_Z, [_I, _I, _I, _F]),
     "dl_sample": (_I, [_P, _L, _I, _P, _P, _P, _P, _P, _F, _I, _F, _F, _P, _P, _Z, _I, _I, _P]),
+    "dl_rms_norm_fwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _L, _I, _F, _P]),
+    "dl_quantize_rows": (_I, [_P, _L, _P, _P, _I, _L, _I, _P]),
+    "dl_rms_norm_bwd_workspace_bytes": (_Z, [_L, _I]),
+    "dl_rms_norm_bwd": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _P, _Z, _P]),
+    "dl_linear_fwd_workspace_bytes": (_Z, [_P, _L, _P, _L, _I, _L, _L, _L, _I]),
+    "dl_linear_fwd": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _L, _P, _P, _I, _I, _L, _L, _L, _I, _I, _P, _Z, _P]),
+    "dl_linear_bwd_workspace_bytes": (_Z, [_P, _L, _P, _L, _P, _P, _I, _I, _L, _L, _L]),
+    "dl_linear_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _I, _P, _Z, _P]),
+    "dl_beam_step_workspace_bytes": (_Z, [_I] * 4),
+    "dl_beam_step": (_I, [_P, _L, _I, _P, _P, _L, _P, _P, _P, _P, _Z, _I, _I, _I, _I, _P]),
+    "dl_beam_reorder": (_I, [_P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "dl_profile_enable": (_I, [_I]),
     "dl_profile_read": (_I, [ctypes.c_char_p, _Z, ctypes.POINTER(_F), _I]),
 }

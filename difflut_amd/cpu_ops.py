@@ -383,3 +383,121 @@ def sample(logits, uniform, temperature, top_k, top_p, min_p):
     last = torch.where(kept > 0, rank, -1).amax(1)
     token = torch.minimum((running <= u * running[:, -1:]).sum(1), last)
     return torch.where(top.view(B) > -math.inf, token, -1)
+
+
+# ----------------------------------------------------------------------------- dense blocks between the layers, search over answers
+CODE_MAX = 448.0  # the largest float8_e4m3fn
+
+
+def _stream(x, residual):
+    if residual is not None and residual.dtype is not x.dtype:
+        raise TypeError(f"x and residual must be of one type, got {x.dtype} and {residual.dtype}")
+    if residual is None:
+        return _wide(x)
+    wide = _wide(x) + _wide(residual)
+    return _PassGradient.apply(wide, wide.detach().to(x.dtype).to(wide.dtype))  # rounded; its gradients are summed in 32 bits, as on the device
+
+
+def _normed(wide, weight, eps):
+    y = wide / torch.sqrt(wide.square().mean(-1, keepdim=True) + eps)
+    return y if weight is None else y * _wide(weight)
+
+
+def rms_norm(x, weight, eps, residual):
+    h = _stream(x, residual)
+    y = _normed(h, weight, eps).to(x.dtype).contiguous()
+    return y if residual is None else (y, h.to(x.dtype).contiguous())
+
+
+def _codes(y):
+    if y.shape[:-1].numel() == 0:
+        return y.to(torch.float8_e4m3fn), torch.zeros(y.shape[:-1], device=y.device)
+    scale = (y.abs().amax(-1) / CODE_MAX).float()
+    factor = torch.where(scale == 0, 0.0, 1.0 / scale)
+    return (y.float() * factor.unsqueeze(-1)).clamp(-CODE_MAX, CODE_MAX).to(torch.float8_e4m3fn), scale
+
+
+@torch.no_grad()
+def rms_norm_codes(x, weight, eps, residual):
+    h = _stream(x, residual)
+    codes, scale = _codes(_normed(h, weight, eps))
+    return (codes, scale) if residual is None else (codes, scale, h.to(x.dtype).contiguous())
+
+
+@torch.no_grad()
+def quantize_rows(x):
+    return _codes(_wide(x))
+
+
+def _activated(z, activation):
+    if activation == "sigmoid":
+        return torch.sigmoid(z)
+    if activation == "silu":
+        return z * torch.sigmoid(z)
+    return torch.relu(z) if activation == "relu" else z
+
+
+def _followed(z, bias, activation, residual, gated):
+    if bias is not None:
+        z = z + _wide(bias)
+    if gated:
+        gate, up = z.chunk(2, dim=-1)
+        y = _activated(gate, activation) * up
+    else:
+        y = _activated(z, activation)
+    return y if residual is None else y + _wide(residual)
+
+
+def linear(x, weight, bias, activation, residual, gated):
+    for t in (weight, bias, residual):
+        if t is not None and t.dtype is not x.dtype:
+            raise TypeError(f"x, weight, bias and residual must be of one type, got {x.dtype} and {t.dtype}")
+    return _followed(torch.matmul(_wide(x), _wide(weight).t()), bias, activation, residual, gated).to(x.dtype)
+
+
+@torch.no_grad()
+def linear_codes(x, x_scale, weight, weight_scale, bias, activation, residual, gated, dtype):
+    for t in (bias, residual):
+        if t is not None and t.dtype is not dtype:
+            raise TypeError(f"bias and residual must be of the result's type, got {t.dtype}, expected {dtype}")
+    z = torch.matmul(x.float(), weight.float().t()) * x_scale.unsqueeze(-1) * weight_scale
+    return _followed(z, bias, activation, residual, gated).to(dtype)
+
+
+@torch.no_grad()
+def beam_step(logits, scores, beams, finished, end):
+    x = logits.double()
+    x = torch.where(x.isnan(), -math.inf, x).clamp(max=torch.finfo(torch.float32).max)
+    B, K, V = x.shape
+    top = x.amax(2, keepdim=True)
+    known = top > -math.inf
+    x = torch.where(known, x, 0.0)
+    norm = torch.where(known, top, 0.0)
+    norm = norm + torch.exp(x - norm).sum(2, keepdim=True).log()
+    total = torch.where(known, scores.double().unsqueeze(2) + (x - norm), -math.inf)
+    if finished is not None:
+        alone = torch.full_like(total, -math.inf)
+        alone[:, :, 0] = scores.double()
+        total = torch.where(finished.unsqueeze(2), alone, total)
+    total = torch.where(total.isnan(), -math.inf, total).view(B, K * V)
+    best, at = torch.sort(total, dim=1, descending=True, stable=True)
+    best, at = best[:, :beams], at[:, :beams]
+    short = beams - best.shape[1]
+    if short > 0:
+        best, at = torch.nn.functional.pad(best, (0, short), value=-math.inf), torch.nn.functional.pad(at, (0, short))
+    parents, tokens = at // V, at % V
+    if finished is not None:
+        tokens = torch.where(finished.gather(1, parents), end, tokens)
+    none = best == -math.inf
+    return best.float(), torch.where(none, 0, parents), torch.where(none, -1, tokens)
+
+
+@torch.no_grad()
+def beam_reorder(states, parents):
+    rows = torch.arange(parents.shape[0]).unsqueeze(1)
+    results = []
+    for s in states:
+        known = ((parents >= 0) & (parents < s.shape[1])).view(*parents.shape, *([1] * (s.dim() - 2)))
+        moved = s[rows, parents.clamp(0, s.shape[1] - 1)]
+        results.append(torch.where(known, moved, torch.zeros_like(moved)))
+    return results

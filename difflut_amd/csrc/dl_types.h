@@ -7,7 +7,7 @@ typedef __bf16 dl_bf16;
 typedef _Float16 dl_f16;
 
 template <typename T, int N>
-struct alignas(sizeof(T) * N) DlVec {
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) DlVec {
     T v[N];
 };
 template <typename T, int N>

@@ -39,7 +39,10 @@ namespace {
     X(dl_dwn_layer_bwd_chain_first) X(dl_cross_entropy_workspace_bytes) X(dl_cross_entropy) X(dl_adam_step) \
     X(dl_embedding_fwd) X(dl_embedding_bwd_workspace_bytes) X(dl_embedding_bwd) X(dl_group_norm_fwd_workspace_bytes)     \
     X(dl_group_norm_fwd) X(dl_group_norm_bwd_workspace_bytes) X(dl_group_norm_bwd) X(dl_dropout)                         \
-    X(dl_sample_workspace_bytes) X(dl_sample)
+    X(dl_sample_workspace_bytes) X(dl_sample)                                                                             \
+    X(dl_rms_norm_fwd) X(dl_quantize_rows) X(dl_rms_norm_bwd_workspace_bytes) X(dl_rms_norm_bwd)                         \
+    X(dl_linear_fwd_workspace_bytes) X(dl_linear_fwd) X(dl_linear_bwd_workspace_bytes) X(dl_linear_bwd)                  \
+    X(dl_beam_step_workspace_bytes) X(dl_beam_step) X(dl_beam_reorder)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     DL_FUNCTIONS(X)
@@ -936,6 +939,238 @@ Tensor sample(const Tensor &logits_, const Tensor &uniform_, const Maybe &temper
     return tokens;
 }
 
+// ------------------------------------------------------------------ dense blocks between the layers, and the search over answers
+// x as rows [n, size of the last dimension] that may lie apart, else a contiguous copy
+Tensor rows_of(const Tensor &x) {
+    const int64_t D = x.size(-1);
+    if (x.dim() == 2 && x.stride(1) == 1 && (x.stride(0) >= D || x.size(0) <= 1)) return x;
+    return x.contiguous().view({-1, D});
+}
+int64_t ld_of(const Tensor &rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+Tensor like_rows(const Tensor &x, int64_t D, at::ScalarType dtype) {
+    auto sizes = x.sizes().vec();
+    sizes.back() = D;
+    return at::empty(sizes, x.options().dtype(dtype).requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+}
+
+// -> (y, h): h is x itself where there is no residual (and not handed on)
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x_, const Maybe &weight_, const Maybe &residual_, double eps, bool keep) {
+        const c10::DeviceGuard guard(x_.device());
+        const Tensor x = rows_of(x_), weight = weight_ ? weight_->contiguous() : Tensor(), residual = residual_ ? rows_of(*residual_) : Tensor();
+        const int64_t rows = x.size(0), D = size_int(x.size(1), "a row");
+        const Tensor y = like_rows(x_, D, x.scalar_type()), h = residual.defined() ? like_rows(x_, D, x.scalar_type()) : Tensor(),
+                     rstd = keep ? floats({rows}, x) : Tensor();
+        const int type = type_of(x, "x"), ptype = weight.defined() ? type_of(weight, "weight") : type;
+        check(L.dl_rms_norm_fwd(raw_in(x), ld_of(x), raw_in(residual), residual.defined() ? ld_of(residual) : 0, raw_in(weight), raw(h), raw(y), out(rstd),
+                                nullptr, type, ptype, rows, D, (float)eps, stream()));
+        ctx->set_materialize_grads(false);
+        if (!keep) return residual.defined() ? variable_list{y, h} : variable_list{y};
+        ctx->save_for_backward({residual.defined() ? h : x_, weight, rstd});
+        ctx->saved_data["residual"] = residual.defined();
+        return residual.defined() ? variable_list{y, h} : variable_list{y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        once("rms_norm");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &h_ = saved[0], &weight = saved[1], &rstd = saved[2];
+        const bool residual = ctx->saved_data["residual"].toBool();
+        const c10::DeviceGuard guard(h_.device());
+        const Tensor h = rows_of(h_), gy = grads[0].defined() ? grads[0].contiguous() : Tensor(),
+                     gh = residual && grads[1].defined() ? grads[1].contiguous() : Tensor();
+        // (inputs are counted without those that are missing)
+        const bool want_x = ctx->needs_input_grad(0), want_w = weight.defined() && ctx->needs_input_grad(1),
+                   want_r = residual && ctx->needs_input_grad(weight.defined() ? 2 : 1);
+        Tensor gx, gw;
+        if (gy.defined() || gh.defined()) {
+            const int64_t rows = h.size(0), D = h.size(1);
+            const int type = type_of(h, "x"), ptype = weight.defined() ? type_of(weight, "weight") : type;
+            if (want_x || want_r) gx = like_rows(h_, D, h.scalar_type());
+            if (want_w) gw = at::empty_like(weight);
+            const size_t need = want_w ? L.dl_rms_norm_bwd_workspace_bytes(rows, D) : 0;
+            const Tensor ws = need ? bytes(need, h) : Tensor();
+            check(L.dl_rms_norm_bwd(raw_in(h), ld_of(h), raw_in(weight), in(rstd), raw_in(gy), raw_in(gh), raw(gx), raw(gw), type, ptype, rows, D, raw(ws),
+                                    need, stream()));
+        }
+        return {want_x ? gx : Tensor(), gw, want_r ? gx : Tensor(), Tensor(), Tensor()};
+    }
+};
+void check_norm(const Tensor &x, const Tensor &weight, const Tensor &residual) {
+    require_device(x);
+    same_device(x, weight, "weight");
+    same_device(x, residual, "residual");
+    type_of(x, "x");
+    if (weight.defined()) type_of(weight, "weight");
+    TORCH_CHECK_TYPE(!residual.defined() || residual.scalar_type() == x.scalar_type(), "x and residual must be of one type, got ", x.scalar_type(), " and ",
+                     residual.defined() ? residual.scalar_type() : x.scalar_type());
+}
+bool differentiates(std::initializer_list<Tensor> inputs) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor &t : inputs)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+variable_list rms_norm(const Tensor &x, const Maybe &weight, const Maybe &residual, double eps) {
+    check_norm(x, tensor_of(weight), tensor_of(residual));
+    return RmsNorm::apply(x, weight, residual, eps, differentiates({x, tensor_of(weight), tensor_of(residual)}));
+}
+
+// -> (codes, scale) or (codes, scale, h)
+std::vector<Tensor> rms_norm_codes(const Tensor &x_, const Maybe &weight_, const Maybe &residual_, double eps) {
+    at::NoGradGuard no_grad;
+    check_norm(x_, tensor_of(weight_), tensor_of(residual_));
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = rows_of(x_), weight = weight_ ? weight_->contiguous() : Tensor(), residual = residual_ ? rows_of(*residual_) : Tensor();
+    const int64_t rows = x.size(0), D = size_int(x.size(1), "a row");
+    const Tensor codes = like_rows(x_, D, at::kFloat8_e4m3fn), h = residual.defined() ? like_rows(x_, D, x.scalar_type()) : Tensor(),
+                 scale = floats(x_.sizes().slice(0, x_.dim() - 1), x);
+    const int type = type_of(x, "x"), ptype = weight.defined() ? type_of(weight, "weight") : type;
+    check(L.dl_rms_norm_fwd(raw_in(x), ld_of(x), raw_in(residual), residual.defined() ? ld_of(residual) : 0, raw_in(weight), raw(h), raw(codes), nullptr,
+                            out(scale), type, ptype, rows, D, (float)eps, stream()));
+    return residual.defined() ? std::vector<Tensor>{codes, scale, h} : std::vector<Tensor>{codes, scale};
+}
+std::vector<Tensor> quantize_rows(const Tensor &x_) {
+    at::NoGradGuard no_grad;
+    require_device(x_);
+    const c10::DeviceGuard guard(x_.device());
+    const int type = type_of(x_, "x");
+    const Tensor x = rows_of(x_), codes = like_rows(x_, x.size(1), at::kFloat8_e4m3fn), scale = floats(x_.sizes().slice(0, x_.dim() - 1), x);
+    check(L.dl_quantize_rows(raw_in(x), ld_of(x), raw(codes), out(scale), type, x.size(0), size_int(x.size(1), "a row"), stream()));
+    return {codes, scale};
+}
+
+// y = act(x w^T + bias) + residual; gated: the activated first half of the columns times the second
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &weight_, const Maybe &bias_, const Maybe &residual_, int64_t act, bool gated, bool keep) {
+        const c10::DeviceGuard guard(x_.device());
+        const Tensor x = rows_of(x_), weight = rows_of(weight_), bias = bias_ ? bias_->contiguous() : Tensor(), residual = residual_ ? rows_of(*residual_) : Tensor();
+        const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
+        const int type = type_of(x, "x");
+        const Tensor y = like_rows(x_, gated ? N / 2 : N, x.scalar_type());
+        const Tensor z = keep && (gated || act != DL_ACT_NONE) ? at::empty({M, N}, y.options()) : Tensor();
+        const size_t need = L.dl_linear_fwd_workspace_bytes(raw_in(x), ld_of(x), raw_in(weight), ld_of(weight), type, M, N, K, gated);
+        const Tensor ws = need ? bytes(need, x) : Tensor();
+        check(L.dl_linear_fwd(raw_in(x), ld_of(x), nullptr, raw_in(weight), ld_of(weight), nullptr, raw_in(bias), raw_in(residual),
+                              residual.defined() ? ld_of(residual) : 0, raw(y), raw(z), type, type, M, N, K, (int)act, gated, raw(ws), need, stream()));
+        if (keep) {
+            ctx->save_for_backward({x_, weight_, z});
+            ctx->saved_data["act"] = act;
+            ctx->saved_data["gated"] = gated;
+            ctx->saved_data["bias"] = bias.defined();
+            ctx->saved_data["residual"] = residual.defined();
+        }
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        once("linear");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x_ = saved[0], &weight_ = saved[1], &z = saved[2];
+        const bool gated = ctx->saved_data["gated"].toBool(), bias = ctx->saved_data["bias"].toBool(), residual = ctx->saved_data["residual"].toBool();
+        const c10::DeviceGuard guard(x_.device());
+        const Tensor x = rows_of(x_), weight = rows_of(weight_), gy = grads[0].contiguous();
+        const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
+        const int type = type_of(x, "x");
+        const Tensor gx = ctx->needs_input_grad(0) ? like_rows(x_, K, x.scalar_type()) : Tensor(),
+                     gw = ctx->needs_input_grad(1) ? at::empty({N, K}, gy.options()) : Tensor(),
+                     gb = bias && ctx->needs_input_grad(2) ? at::empty({N}, gy.options()) : Tensor();
+        const int wants = (gx.defined() ? 1 : 0) | (gw.defined() ? 2 : 0) | (gb.defined() ? 4 : 0);
+        if (wants) {
+            const size_t need = L.dl_linear_bwd_workspace_bytes(raw_in(x), ld_of(x), raw_in(weight), ld_of(weight), raw_in(z), raw_in(gy), wants, type, M, N, K);
+            const Tensor ws = need ? bytes(need, x) : Tensor();
+            check(L.dl_linear_bwd(raw_in(x), ld_of(x), raw_in(weight), ld_of(weight), raw_in(z), raw_in(gy), raw(gx), raw(gw), raw(gb), type, M, N, K,
+                                  (int)ctx->saved_data["act"].toInt(), gated, raw(ws), need, stream()));
+        }
+        const bool want_r = residual && ctx->needs_input_grad(bias ? 3 : 2);
+        return {gx, gw, gb, want_r ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+Tensor linear(const Tensor &x, const Tensor &weight, const Maybe &bias_, const Maybe &residual_, int64_t act, bool gated) {
+    const Tensor bias = tensor_of(bias_), residual = tensor_of(residual_);
+    require_device(x);
+    same_device(x, weight, "weight");
+    same_device(x, bias, "bias");
+    same_device(x, residual, "residual");
+    type_of(x, "x");
+    for (const Tensor &t : {weight, bias, residual})
+        TORCH_CHECK_TYPE(!t.defined() || t.scalar_type() == x.scalar_type(), "x, weight, bias and residual must be of one type, got ", x.scalar_type(), " and ",
+                         t.defined() ? t.scalar_type() : x.scalar_type());
+    return Linear::apply(x, weight, bias_, residual_, act, gated, differentiates({x, weight, bias, residual}));
+}
+Tensor linear_codes(const Tensor &x_, const Tensor &x_scale_, const Tensor &weight_, const Tensor &weight_scale_, const Maybe &bias_, const Maybe &residual_,
+                    int64_t act, bool gated, at::ScalarType dtype) {
+    at::NoGradGuard no_grad;
+    require_device(x_);
+    same_device(x_, x_scale_, "x_scale");
+    same_device(x_, weight_, "weight");
+    same_device(x_, weight_scale_, "weight_scale");
+    same_device(x_, tensor_of(bias_), "bias");
+    same_device(x_, tensor_of(residual_), "residual");
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = rows_of(x_), weight = rows_of(weight_), bias = bias_ ? bias_->contiguous() : Tensor(), residual = residual_ ? rows_of(*residual_) : Tensor();
+    const Tensor x_scale = x_scale_.contiguous(), weight_scale = weight_scale_.contiguous();
+    const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
+    const Tensor y = like_rows(x_, gated ? N / 2 : N, dtype);
+    const int type = type_of(y, "the result");
+    for (const Tensor &t : {bias, residual})
+        TORCH_CHECK_TYPE(!t.defined() || t.scalar_type() == dtype, "bias and residual must be of the result's type, got ",
+                         t.defined() ? t.scalar_type() : dtype, ", expected ", dtype);
+    const size_t need = L.dl_linear_fwd_workspace_bytes(raw_in(x), ld_of(x), raw_in(weight), ld_of(weight), DL_E4M3, M, N, K, gated);
+    const Tensor ws = need ? bytes(need, x) : Tensor();
+    check(L.dl_linear_fwd(raw_in(x), ld_of(x), in(x_scale), raw_in(weight), ld_of(weight), in(weight_scale), raw_in(bias), raw_in(residual),
+                          residual.defined() ? ld_of(residual) : 0, raw(y), nullptr, DL_E4M3, type, M, N, K, (int)act, gated, raw(ws), need, stream()));
+    return y;
+}
+
+// -> (scores, parents, tokens)
+std::vector<Tensor> beam_step(const Tensor &logits_, const Tensor &scores_, int64_t count, const Maybe &ended_, int64_t end) {
+    at::NoGradGuard no_grad;
+    require_device(logits_);
+    same_device(logits_, scores_, "scores");
+    same_device(logits_, tensor_of(ended_), "finished");
+    const c10::DeviceGuard guard(logits_.device());
+    const int64_t B = size_int(logits_.size(0), "a batch"), K = size_int(logits_.size(1), "a number of beams"), V = size_int(logits_.size(2), "a vocabulary");
+    const int type = type_of(logits_, "logits");
+    // rows may lie apart where they do so evenly
+    const bool even = logits_.stride(2) == 1 && logits_.stride(1) >= V && (B <= 1 || logits_.stride(0) == K * logits_.stride(1));
+    const Tensor logits = even ? logits_ : logits_.contiguous(), scores = scores_.contiguous(), ended = ended_ ? ended_->contiguous() : Tensor();
+    const auto longs = logits.options().dtype(at::kLong).requires_grad(false);
+    const Tensor best = floats({B, count}, logits), parents = at::empty({B, count}, longs), tokens = at::empty({B, count}, longs);
+    if (B == 0) return {best, parents, tokens};
+    const Tensor ws = bytes(L.dl_beam_step_workspace_bytes((int)B, (int)K, (int)V, (int)count), logits);
+    check(L.dl_beam_step(raw_in(logits), logits.stride(1) >= V ? logits.stride(1) : V, type, in(scores),
+                         ended.defined() ? (const uint8_t *)ended.const_data_ptr() : nullptr, end, out(best), (long long *)raw(parents), (long long *)raw(tokens),
+                         raw(ws), ws.numel(), (int)B, (int)K, (int)V, (int)count, stream()));
+    return {best, parents, tokens};
+}
+std::vector<Tensor> beam_reorder(const std::vector<Tensor> &states, const Tensor &parents_) {
+    at::NoGradGuard no_grad;
+    require_device(parents_);
+    const c10::DeviceGuard guard(parents_.device());
+    const Tensor parents = parents_.contiguous();
+    const int64_t B = parents.size(0), count = parents.size(1), K = states.empty() ? 0 : size_int(states[0].size(1), "a number of beams");
+    std::vector<Tensor> results, kept;
+    std::vector<const void *> src;
+    std::vector<void *> dst;
+    std::vector<long long> row;
+    const auto flush = [&] {
+        if (!src.empty()) check(L.dl_beam_reorder(src.data(), dst.data(), row.data(), (int)src.size(), (const long long *)raw_in(parents), size_int(B, "a batch"), (int)K, (int)count, stream()));
+        src.clear(), dst.clear(), row.clear();
+    };
+    for (const Tensor &s_ : states) {
+        same_device(parents_, s_, "a state");
+        const Tensor s = s_.contiguous();
+        auto sizes = s.sizes().vec();
+        sizes[1] = count;
+        const Tensor d = at::empty(sizes, s.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+        results.push_back(d), kept.push_back(s);
+        if (d.numel() == 0) continue;
+        src.push_back(raw_in(s)), dst.push_back(raw(d)), row.push_back((long long)(s.numel() / (B * K) * s.element_size()));
+        if (src.size() == DL_BEAM_STATES) flush();
+    }
+    flush();
+    return results;
+}
+
 // Whether rows 0, n - 1 and `count` rows from `start` on (around the end) of a bank's nodes still hold the views the bank handed out:
 // nodes[keys[row]]._buffers[name] is views[row].  In Python, 18 rows took 3.5 us a bank, two banks a call of a layer.
 bool views_hold(const py::dict &nodes, const py::tuple &keys, const py::str &name, const py::list &views, Py_ssize_t start, Py_ssize_t count) {
@@ -983,5 +1218,12 @@ PYBIND11_MODULE(difflut_host, m) {
     m.def("group_norm", &group_norm, free_gil);
     m.def("dropout", &dropout, free_gil);
     m.def("sample", &sample, free_gil);
+    m.def("rms_norm", &rms_norm, free_gil);
+    m.def("rms_norm_codes", &rms_norm_codes, free_gil);
+    m.def("quantize_rows", &quantize_rows, free_gil);
+    m.def("linear", &linear, free_gil);
+    m.def("linear_codes", &linear_codes, free_gil);
+    m.def("beam_step", &beam_step, free_gil);
+    m.def("beam_reorder", &beam_reorder, free_gil);
     m.def("cross_entropy", [](const Tensor &logits, const Tensor &labels) { return CrossEntropy::apply(logits, labels); }, free_gil);
 }

@@ -612,3 +612,144 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     tensors = [v if torch.is_tensor(v) else None for v in settings.values()]
     numbers = [0 if torch.is_tensor(v) else v for v in settings.values()]
     return nat.host().sample(logits, uniform, *tensors, float(numbers[0]), int(numbers[1]), float(numbers[2]), float(numbers[3]))
+
+
+# ----------------------------------------------------------------------------- dense blocks between the layers, search over answers
+# As above: float32, bfloat16 and float16 as they are (on the CPU float64 as well), sums in 32 bits or more, on the tensors' own device.
+CODES = torch.float8_e4m3fn  # rows in 8 bits: code * scale[row], the largest of a row at the type's largest value, 448
+BEAM_MOST = 64
+
+
+def _check_norm(name, x, weight, eps, residual):
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{name} expects (..., features), got shape {tuple(x.shape)}")
+    if weight is not None and tuple(weight.shape) != (x.shape[-1],):
+        raise ValueError(f"{name} weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"{name} residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None):
+    """x / sqrt(mean(x^2) + eps) over the last dimension, times weight [features] (of any float type; it may be missing).
+
+    With a `residual` of x's shape and type: h = x + residual, rounded to that type, takes x's place, and (norm, h) are returned: h is the
+    stream that the next block adds to. Gradients are those of both results. Rows of x may lie apart (a slice of a wider matrix)."""
+    _check_norm("rms_norm", x, weight, eps, residual)
+    if not x.is_cuda or x.numel() == 0:
+        return cpu_ops.rms_norm(x, weight, float(eps), residual)
+    out = nat.host().rms_norm(x, weight, residual, float(eps))
+    return tuple(out) if residual is not None else out[0]
+
+
+def rms_norm_codes(x, weight=None, eps=1e-6, residual=None):
+    """rms_norm whose result is left in 8 bits for linear_codes: (codes, scale), or (codes, scale, h) with a residual. codes are
+    float8_e4m3fn of x's shape, scale float32 has one value per row: code * scale is the norm, rounded to three bits behind the leading
+    one; scale = max |norm| / 448, in a row of zeros 0. No gradient."""
+    _check_norm("rms_norm_codes", x, weight, eps, residual)
+    if not x.is_cuda or x.numel() == 0:
+        return cpu_ops.rms_norm_codes(x, weight, float(eps), residual)
+    return tuple(nat.host().rms_norm_codes(x, weight, residual, float(eps)))
+
+
+def quantize_rows(x):
+    """x (..., features) in 8 bits with a scale per row: (codes, scale) as rms_norm_codes leaves them. No gradient."""
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"quantize_rows expects (..., features), got shape {tuple(x.shape)}")
+    if not x.is_cuda or x.numel() == 0:
+        return cpu_ops.quantize_rows(x)
+    return tuple(nat.host().quantize_rows(x))
+
+
+def _check_linear(name, x, weight, bias, activation, residual, gated):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"{name} weight must be a non-empty matrix (out features, in features), got {tuple(weight.shape)}")
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{name} expects (..., {weight.shape[1]}), got shape {tuple(x.shape)}")
+    out = weight.shape[0]
+    if gated and out % 2 != 0:
+        raise ValueError(f"{name} weight must have an even number of rows, the gate's first, got {out}")
+    if bias is not None and tuple(bias.shape) != (out,):
+        raise ValueError(f"{name} bias must be [{out}], got {tuple(bias.shape)}")
+    shape = (*x.shape[:-1], out // 2 if gated else out)
+    if residual is not None and tuple(residual.shape) != shape:
+        raise ValueError(f"{name} residual must be {list(shape)}, got {tuple(residual.shape)}")
+
+
+def linear(x, weight, bias=None, activation="none", residual=None):
+    """activation(x weight^T + bias) + residual: x (..., in features), weight [out, in], bias [out], residual (..., out), all of one
+    type; activation "none", "relu", "silu" or "sigmoid".  A product and what follows it are one launch; for the backward the values in
+    front of an activation are kept in x's type, and the gradient behind it is rounded to that type before the backward's products.
+    float32 is multiplied to within its own rounding; there, products with infinities are NaN."""
+    _check_linear("linear", x, weight, bias, activation, residual, False)
+    if not x.is_cuda or x.numel() == 0:
+        return cpu_ops.linear(x, weight, bias, activation, residual, False)
+    return nat.host().linear(x, weight, bias, residual, ACTIVATIONS[activation], False)
+
+
+def gated_linear(x, weight, bias=None, activation="silu", residual=None):
+    """activation(gate) * up + residual, where gate and up are the two halves of x weight^T + bias: weight [2 out, in] holds the gate's
+    rows, then the others', bias [2 out] likewise, residual is (..., out).  Both projections are one product; types and roundings are
+    those of `linear`."""
+    _check_linear("gated_linear", x, weight, bias, activation, residual, True)
+    if not x.is_cuda or x.numel() == 0:
+        return cpu_ops.linear(x, weight, bias, activation, residual, True)
+    return nat.host().linear(x, weight, bias, residual, ACTIVATIONS[activation], True)
+
+
+def linear_codes(x, x_scale, weight, weight_scale, bias=None, activation="none", residual=None, gated=False, dtype=torch.bfloat16):
+    """`linear` (or with gated=True `gated_linear`) on rows in 8 bits: x (..., in) with x_scale (...), weight [out, in] with
+    weight_scale [out], as rms_norm_codes and quantize_rows leave them; bias, residual and the result are of `dtype`. Sums are
+    float32; of the products that the 8-bit matrix cores add at once (up to 64) they leave out what lies below 2^-13 of the largest. No gradient."""
+    _check_linear("linear_codes", x, weight, bias, activation, residual, gated)
+    for name, t in (("x", x), ("weight", weight)):
+        if t.dtype is not CODES:
+            raise TypeError(f"linear_codes {name} must be {CODES}, got {t.dtype}")
+    for name, t, shape in (("x_scale", x_scale, x.shape[:-1]), ("weight_scale", weight_scale, weight.shape[:1])):
+        if t.shape != shape or t.dtype is not torch.float32:
+            raise ValueError(f"linear_codes {name} must be float32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+    if not x.is_cuda or x.numel() == 0:
+        return cpu_ops.linear_codes(x, x_scale, weight, weight_scale, bias, activation, residual, gated, dtype)
+    return nat.host().linear_codes(x, x_scale, weight, weight_scale, bias, residual, ACTIVATIONS[activation], bool(gated), dtype)
+
+
+def beam_step(logits, scores, beams=None, finished=None, end=0):
+    """One step of beam search: of every sequence's beams the best continuations -> (scores, parents, tokens), each [batch, beams].
+
+    logits [batch, beams in, vocabulary], scores float32 [batch, beams in]; a continuation's score is its beam's plus the token's
+    log-softmax, the `beams` (as many as came in unless given) largest are returned, largest first, equal ones by beam, then token.
+    A beam that is `finished` (bool [batch, beams in]) goes on by one continuation alone, the token `end` at its own score; its logits are not
+    looked at.  NaN logits are no continuations, infinite ones count as the largest number; where there are fewer continuations above
+    -infinity than asked for, the rest have score -infinity, parent 0 and token -1.  Beams start as [0, -infinity, ...].
+    Scores are compared as doubles.  Up to 64 beams.  No gradient."""
+    if logits.dim() != 3 or logits.shape[1] == 0 or logits.shape[2] == 0:
+        raise ValueError(f"beam_step expects logits (batch, beams, vocabulary), got shape {tuple(logits.shape)}")
+    shape = tuple(logits.shape[:2])
+    if tuple(scores.shape) != shape or scores.dtype is not torch.float32:
+        raise ValueError(f"scores must be float32 {list(shape)}, got {scores.dtype} {tuple(scores.shape)}")
+    if finished is not None and (tuple(finished.shape) != shape or finished.dtype is not torch.bool):
+        raise ValueError(f"finished must be bool {list(shape)}, got {finished.dtype} {tuple(finished.shape)}")
+    beams = shape[1] if beams is None else beams
+    if not isinstance(beams, int) or not 0 < beams <= BEAM_MOST or shape[1] > BEAM_MOST:
+        raise ValueError(f"beams must be in [1, {BEAM_MOST}], got {shape[1]} and {beams}")
+    if not logits.is_cuda:
+        return cpu_ops.beam_step(logits, scores, beams, finished, int(end))
+    return tuple(nat.host().beam_step(logits, scores, beams, finished, int(end)))
+
+
+def beam_reorder(states, parents):
+    """The beams' states in the order of beam_step's answer: for each tensor [batch, beams, ...] of the list `states`, of any type, a
+    new one whose entry [b, j] is its entry [b, parents[b, j]], all in one launch.  A parent outside the beams gives zeros.  No gradient."""
+    if parents.dim() != 2 or parents.dtype is not torch.int64:
+        raise ValueError(f"parents must be int64 [batch, beams], got {parents.dtype} {tuple(parents.shape)}")
+    for s in states:
+        if s.dim() < 2 or s.shape[0] != parents.shape[0] or s.shape[1] == 0 or s.shape[1] != states[0].shape[1]:
+            raise ValueError(f"states must be [{parents.shape[0]}, beams, ...] with the same beams, got {[tuple(t.shape) for t in states]}")
+    if not parents.is_cuda:
+        return cpu_ops.beam_reorder(states, parents)
+    return nat.host().beam_reorder(states, parents)

@@ -1,6 +1,7 @@
 """GroupSum head (difflut/utils/modules.py:20-163): split the features into k contiguous groups
 (zero-padded to a multiple of k), sum each group, divide by tau; its loss; and what stands around LUT layers in models over tokens and
-in deep stacks (no counterpart in the reference): token embedding, group norm, counter-based dropout, sampling."""
+in deep stacks (no counterpart in the reference): token embedding, group norm, counter-based dropout, sampling, RMS norm,
+projections, beam search."""
 import math
 import warnings
 
@@ -144,3 +145,83 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One class per row of logits [batch, classes] (e.g. what GroupSum returns), drawn with the random numbers `uniform` [batch]:
     see `ops.sample`."""
     return ops.sample(logits, uniform, temperature, top_k, top_p, min_p)
+
+
+class RMSNorm(nn.Module):
+    """Root-mean-square norm over the last dimension of (..., features).  Called with a residual it adds that first and returns
+    (norm, sum): see `ops.rms_norm`.  `codes=True` leaves the norm in 8 bits with a scale per row, for Linear8: (codes, scale), or (codes,
+    scale, sum); no gradient goes through these."""
+
+    def __init__(self, features, eps=1e-6, affine=True, codes=False):
+        super().__init__()
+        if not isinstance(features, int) or features <= 0:
+            raise ValueError(f"features must be a positive integer, got {features}")
+        self.features, self.eps, self.codes = features, eps, codes
+        self.weight = nn.Parameter(torch.ones(features)) if affine else None
+
+    def forward(self, x, residual=None):
+        if x.dim() < 1 or x.shape[-1] != self.features:
+            raise ValueError(f"RMSNorm expects (..., {self.features}), got {tuple(x.shape)}")
+        return (ops.rms_norm_codes if self.codes else ops.rms_norm)(x, self.weight, self.eps, residual)
+
+    def extra_repr(self):
+        return f"{self.features}, eps={self.eps}, affine={self.weight is not None}, codes={self.codes}"
+
+
+class Linear(nn.Module):
+    """activation(x weight^T + bias) + residual for x (..., in_features): a projection with what follows it in one launch; with `gated`
+    activation(gate) * up of two projections, the gate's rows first in `weight`.  "sigmoid" brings features to (0, 1) around the 1/2 that LUT nodes
+    threshold at.  The weight begins uniformly within 1 / sqrt(in_features), the bias likewise.  `to_codes()` gives the same projection on 8-bit
+    rows, for inference."""
+
+    def __init__(self, in_features, out_features, bias=True, activation="none", gated=False):
+        super().__init__()
+        if not isinstance(in_features, int) or in_features <= 0 or not isinstance(out_features, int) or out_features <= 0:
+            raise ValueError(f"in_features and out_features must be positive integers, got {in_features} and {out_features}")
+        if activation not in ops.ACTIVATIONS:
+            raise ValueError(f"activation must be one of {list(ops.ACTIVATIONS)}, got {activation!r}")
+        self.in_features, self.out_features, self.activation, self.gated = in_features, out_features, activation, bool(gated)
+        rows, limit = out_features * (2 if gated else 1), 1.0 / math.sqrt(in_features)
+        self.weight = nn.Parameter(torch.empty(rows, in_features).uniform_(-limit, limit))
+        self.bias = nn.Parameter(torch.empty(rows).uniform_(-limit, limit)) if bias else None
+
+    def forward(self, x, residual=None):
+        return (ops.gated_linear if self.gated else ops.linear)(x, self.weight, self.bias, self.activation, residual)
+
+    def to_codes(self):
+        return Linear8(self)
+
+    def extra_repr(self):
+        return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, activation={self.activation!r}, gated={self.gated}"
+
+
+class Linear8(nn.Module):
+    """A trained Linear on 8-bit rows: the weight is kept as codes with a scale per row (buffers), the bias in `linear`'s type, which is the
+    result's.  Takes (codes, scale) as RMSNorm(codes=True) leaves them, or rows of a float type, which it quantizes."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.activation, self.gated, self.dtype = linear.activation, linear.gated, linear.weight.dtype
+        codes, scale = ops.quantize_rows(linear.weight.detach())
+        self.register_buffer("weight", codes)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+
+    def forward(self, x, scale=None, residual=None):
+        if scale is None:
+            x, scale = ops.quantize_rows(x)
+        return ops.linear_codes(x, scale, self.weight, self.weight_scale, self.bias, self.activation, residual, self.gated, self.dtype)
+
+    def extra_repr(self):
+        return f"{self.weight.shape[1]}, {self.weight.shape[0] // (2 if self.gated else 1)}, activation={self.activation!r}, gated={self.gated}"
+
+
+def beam_step(logits, scores, beams=None, finished=None, end=0):
+    """The best continuations of every sequence's beams, from logits [batch, beams, classes] (e.g. what GroupSum returns, reshaped) and
+    scores [batch, beams]: see `ops.beam_step`.  `beam_reorder` brings the beams' states into their order."""
+    return ops.beam_step(logits, scores, beams, finished, end)
+
+
+def beam_reorder(states, parents):
+    """The beams' states [batch, beams, ...] in the order of beam_step's answer: see `ops.beam_reorder`."""
+    return ops.beam_reorder(states, parents)

@@ -546,6 +546,57 @@ int dl_sample(const void *logits, long long ldl, int type, const float *uniform,
               long long *out, void *ws, size_t ws_bytes, int B, int V, void *stream);
 
 /* ------------------------------------------------------------------------
+ * The dense blocks between the layers in models over tokens, and the search over their answers.  No counterpart in the reference.
+ * Types as above; sums and statistics in float or more.  Rows and columns are below 2^31 - 65536 (DL_ERR_SHAPE).
+ * ------------------------------------------------------------------------ */
+#define DL_E4M3 3 /* 8 bits with a scale per row: the value is code * scale[row] */
+
+/* Root-mean-square norm: h = x + residual (rounded to `type`; without a residual h = x and is not written), rstd = 1 / sqrt(mean(h^2) + eps),
+ * y = h rstd gamma; x and residual with ldx and ldr elements between rows, h and y [rows, D]; gamma [D] may be null (1).
+ * rstd [rows] (nullable) is kept for the backward.  With `scale` [rows], y is e4m3 codes of D bytes a row, scale = max |y| / 448 (a row of
+ * zeros: 0).  dl_quantize_rows: the same codes of x itself.
+ * Backward: gx = rstd (g - hat mean(g hat)) + gh with g = gy gamma, hat = h rstd; gh (nullable) is the gradient that reaches h itself, gy
+ * may be null where nothing reaches y; ggamma [D] = sum over rows of gy hat.  gx is the gradient of x and of the residual.
+ * Workspace only where ggamma is asked for. */
+int dl_rms_norm_fwd(const void *x, long long ldx, const void *residual, long long ldr, const void *gamma, void *h, void *y, float *rstd, float *scale,
+                    int type, int ptype, long long rows, int D, float eps, void *stream);
+int dl_quantize_rows(const void *x, long long ldx, void *codes, float *scale, int type, long long rows, int D, void *stream);
+size_t dl_rms_norm_bwd_workspace_bytes(long long rows, int D);
+int dl_rms_norm_bwd(const void *h, long long ldh, const void *gamma, const float *rstd, const void *gy, const void *gh, void *gx, void *ggamma, int type,
+                    int ptype, long long rows, int D, void *ws, size_t ws_bytes, void *stream);
+
+/* Matrix product with what follows it: s = x w^T + bias over x [M, K], w [N, K] (ldx, ldw elements between rows), y = act(s) + residual [M, N];
+ * gated: N is even, the first N / 2 rows of w are the gate's, y = act(s[:, :N/2]) * s[:, N/2:] + residual [M, N / 2].  z [M, N] (nullable)
+ * receives s in y's type, for the backward.  bias, residual (ldr) and z may be null.  All of type `type` = out_type, or x and w of DL_E4M3 with
+ * their rows' scales and the rest of out_type (inference; no z needed).  y and z are contiguous.
+ * Backward: from gy (contiguous, y's shape) the gradients gx [M, K], gw [N, K], gb [N], each nullable; z as the forward left it (null where act
+ * is DL_ACT_NONE and not gated); the residual's gradient is gy.  `wants` of the size query: 1 gx, 2 gw, 4 gb.
+ * The size queries look at pointers for their alignment alone.  Rows of operands up to 2^23 bytes, in the backward also M and N up to 2^22
+ * (DL_ERR_UNSUPPORTED beyond). */
+size_t dl_linear_fwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, int type, long long M, long long N, long long K, int gated);
+int dl_linear_fwd(const void *x, long long ldx, const float *x_scale, const void *w, long long ldw, const float *w_scale, const void *bias,
+                  const void *residual, long long ldr, void *y, void *z, int type, int out_type, long long M, long long N, long long K, int act, int gated,
+                  void *ws, size_t ws_bytes, void *stream);
+size_t dl_linear_bwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, int wants, int type,
+                                     long long M, long long N, long long K);
+int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, void *gx, void *gw, void *gb, int type,
+                  long long M, long long N, long long K, int act, int gated, void *ws, size_t ws_bytes, void *stream);
+
+/* A step of beam search: of every sequence's K beams over V tokens the `count` continuations with the largest
+ * scores[b, k] + log_softmax(logits[b, k, :])[v], largest first, equal ones by beam, then token.  logits [B * K, V] (ldl between rows), scores
+ * [B, K]; ended (nullable) [B, K]: a beam with a non-zero byte goes on by (its score, token `end`) alone, its logits are not read.
+ * NaN logits are no candidates, infinite ones count as the largest number.  Where there are fewer candidates above -infinity: score
+ * -infinity, parent 0, token -1.  K and count up to 64, V up to 2^30 (DL_ERR_UNSUPPORTED).
+ * dl_beam_reorder: dst[t][b, j] = src[t][b, parents[b, j]] for n tensors of row_bytes[t] bytes per beam (src, dst, row_bytes: HOST arrays);
+ * a parent outside [0, K) gives zeros.  dst does not overlap src. */
+#define DL_BEAM_STATES 8
+size_t dl_beam_step_workspace_bytes(int B, int K, int V, int count);
+int dl_beam_step(const void *logits, long long ldl, int type, const float *scores, const uint8_t *ended, long long end, float *out_scores,
+                 long long *parents, long long *tokens, void *ws, size_t ws_bytes, int B, int K, int V, int count, void *stream);
+int dl_beam_reorder(const void *const *src, void *const *dst, const long long *row_bytes, int n, const long long *parents, int B, int K, int count,
+                    void *stream);
+
+/* ------------------------------------------------------------------------
  * Per-kernel timing.  No counterpart in the reference (it has no tracing at all).
  * After dl_profile_enable(1) every kernel launched by the entry points above is
  * bracketed by HIP events on its stream (at most 64 kernels between two reads).
