@@ -1,0 +1,8 @@
+// The product kernel on 8-bit operands.
+#include "linear.h"
+
+int lin_launch_e4m3(LinArgs &g, const LinPlan &p, int out_type, bool gated, hipStream_t s) {
+    int code = DL_ERR_UNSUPPORTED;
+    DL_BY_TYPE(out_type, Out, (code = lin_launch<LinE4m3, Out, false, false>(g, p, gated, s)));
+    return code;
+}
