@@ -27,6 +27,7 @@ typedef int intx8 __attribute__((ext_vector_type(8)));
 #define LIN_STAGE_BYTES 128  // of a row in a stage: 32 float32, 64 16-bit or 128 8-bit values
 #define LIN_PLANES 3
 #define LIN_CUS 256
+enum { LIN_SUMS, LIN_PLAIN, LIN_ENDS, LIN_ODD };
 
 struct LinF32 { static constexpr int SIZE = 4; };
 struct LinBf16 { static constexpr int SIZE = 2; };
@@ -92,14 +93,15 @@ __device__ __forceinline__ DlVec<Out, 8> lin_residual(const LinEnd &g, int width
     return f;
 }
 // Eight columns from c on of row r, from their sums v (gated: the gate's, u the other half's), the row's scale and the residual
-template <typename Out, bool GATED>
+template <typename Out, bool GATED, bool SCALED>
 __device__ __forceinline__ void lin_finish(const LinEnd &g, const LinColumns<Out, GATED> &k, int r, int c, float (&v)[8], float (&u)[8], float row_scale, const DlVec<Out, 8> &res) {
     const int width = GATED ? g.F : g.C;
     if (r >= g.R || c >= width) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        v[i] = fmaf(v[i], row_scale * k.scale[0][i], k.bias[0][i]);
-        if (GATED) u[i] = fmaf(u[i], row_scale * k.scale[LinColumns<Out, GATED>::H - 1][i], k.bias[LinColumns<Out, GATED>::H - 1][i]);
+        constexpr int H = GATED ? 1 : 0;
+        v[i] = SCALED ? fmaf(v[i], row_scale * k.scale[0][i], k.bias[0][i]) : v[i] + k.bias[0][i];
+        if (GATED) u[i] = SCALED ? fmaf(u[i], row_scale * k.scale[H][i], k.bias[H][i]) : u[i] + k.bias[H][i];
     }
     if (g.z) {
         Out *z = (Out *)g.z + (long long)r * g.C + c;
@@ -143,15 +145,25 @@ struct LinArgs {
     long long lda, ldb;          // bytes
     long long K;                 // of the reduction, values
     int stages, chunk;           // of the reduction; of a block (all of them without PARTIAL)
-    int row_tiles, col_tiles;
+    int row_tiles, col_tiles, splits;
     float *part;                 // PARTIAL: sums [splits][R][C]
     LinEnd end;
 };
 __device__ const uint4 lin_zeros = {0, 0, 0, 0};  // what lies behind a reduction's end
 
 // Loads that bypass the registers: lane l's 16 bytes land at LDS address lds + 16 l.  The compiler does not count them: a stage waits.
-__device__ __forceinline__ void lin_to_lds(unsigned lds, const char *base, unsigned voff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(voff), "s"(base) : "memory", "m0");
+// A buffer of no bytes is not read.
+__device__ __forceinline__ void lin_to_lds(unsigned lds, intx4 buffer, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(buffer) : "memory", "m0");
+}
+__device__ __forceinline__ intx4 lin_buffer(uint64_t at, int size) {  // size: -1, or 0 for none
+    return intx4{(int)(uint32_t)at, (int)(uint32_t)(at >> 32), size, DL_BUFFER_WORD3};
+}
+// what is the same in every lane, in scalar registers also where the compiler works it out in the lanes' (loads above take nothing else)
+__device__ __forceinline__ uint64_t lin_scalar(uint64_t v) {
+    int low = (int)(uint32_t)v, high = (int)(uint32_t)(v >> 32);
+    asm("" : "+v"(low), "+v"(high));
+    return (uint64_t)(uint32_t)dl_uniform(high) << 32 | (uint32_t)dl_uniform(low);
 }
 __device__ __forceinline__ void lin_to_lds_far(unsigned lds, const char *at) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory", "m0");
@@ -201,7 +213,8 @@ __device__ __forceinline__ floatx16 lin_mfma(const LinFragment<In> &a, const Lin
 
 // An operand's tile in the LDS: T rows (or columns) of C by a stage of the reduction, loaded by 1 KB per wavefront and load.
 // Reduction along the memory's rows: T rows of 128 bytes, whose eight units of 16 bytes are kept in turned order (unit u in slot
-//   u ^ (row & 7)), so that the eight lanes of an LDS read that take one unit of eight rows find them on different banks.
+//   u ^ (row / 2 & 7)), so that the sixteen lanes that an LDS read serves at once, one unit of eight even and eight odd rows, find them on
+//   different banks.
 // Reduction across them (TURNED): LIN_STAGE_BYTES / SIZE rows of T values.  16-bit values are turned by ds_read_b64_tr_b16, sixteen lanes
 //   of which read four rows of 16 values: units of row k are kept in slots u ^ 4 (k & 3).  float32 values are read one by one, lanes along
 //   the row, half the wavefront eight rows further on: slots u ^ 8 (k / 8 & 1).
@@ -214,7 +227,7 @@ struct LinTile {
     static __device__ __forceinline__ int row_of(int load, int lane) { return load * PER + lane / UNITS; }
     static __device__ __forceinline__ int unit_of(int row, int lane) {
         const int slot = lane % UNITS;
-        return !TURNED ? slot ^ (row & 7) : SIZE == 2 ? slot ^ (4 * (row & 3)) : slot ^ (8 * (row >> 3 & 1));
+        return !TURNED ? slot ^ (row >> 1 & 7) : SIZE == 2 ? slot ^ (4 * (row & 3)) : slot ^ (8 * (row >> 3 & 1));
     }
 };
 
@@ -229,7 +242,7 @@ struct LinReader {
     unsigned turn;  // the lane's unit of the first step
     __device__ __forceinline__ LinReader(int first, int lane) {
         const int kh = lane >> 5, l32 = lane & 31;
-        turn = (unsigned)(((Tile::SIZE == 4 ? 2 * kh : kh) ^ (lane & 7)) * 16);
+        turn = (unsigned)(((Tile::SIZE == 4 ? 2 * kh : kh) ^ (lane >> 1 & 7)) * 16);
 #pragma unroll
         for (int i = 0; i < F; ++i) {
             if (!TURNED) at[i] = (first + i * 32 + l32) * Tile::ROW;
@@ -276,102 +289,220 @@ __device__ __forceinline__ void lin_each(F f) {
     if constexpr (TO > FROM) lin_each_of<FROM>(std::make_integer_sequence<int, TO - FROM>(), f);
 }
 
-// A block of four wavefronts makes a tile of TR x TC, a wavefront a quarter of it, in stages of 128 bytes along the reduction: three of A and two of
+__device__ __forceinline__ void lin_lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <bool FIRST, typename A, typename B>
+struct LinChoose { typedef A type; };
+template <typename A, typename B>
+struct LinChoose<false, A, B> { typedef B type; };
+
+// A wavefront's place in the LDS for 32 rows of WIDTH values on their way to or from memory: units of 16 bytes of a row in turned order, so that
+// sixteen rows' units of one column, and sixteen units of one row, lie on different banks.
+template <typename T, int WIDTH>
+struct LinPlace {
+    static constexpr int E = 16 / sizeof(T), UNITS = WIDTH / E, TURNS = 32 * UNITS / 64, BYTES = 32 * WIDTH * (int)sizeof(T), SHARED = UNITS >= 16 ? 0 : UNITS == 8 ? 1 : 2;
+    static_assert(UNITS >= 4 && 64 % UNITS == 0, "a lane has the same unit in every turn");
+    static __device__ __forceinline__ int spot(int row, int unit) { return (row * UNITS + (unit ^ ((row >> SHARED) & (UNITS >= 16 ? 15 : UNITS - 1)))) * 16; }
+    static __device__ __forceinline__ int four(int row, int column) { return spot(row, column / E) + column % E * (int)sizeof(T); }
+    // four values from a column that is a multiple of four
+    static __device__ __forceinline__ void put(char *place, int row, int column, const float (&f)[4]) { dl_store<T, 4>((T *)(place + four(row, column)), f); }
+    static __device__ __forceinline__ void get(const char *place, int row, int column, float (&f)[4]) { dl_load<T, 4>((const T *)(place + four(row, column)), f); }
+    // to memory: `to` is the place's first value's, `rows` and `columns` are there.  HALVES: the second half of a row goes `apart` further on.
+    template <bool HALVES = false>
+    static __device__ __forceinline__ void send(const char *place, int lane, T *to, long long ld, int rows, int columns, bool vec, int apart = 0) {
+        constexpr int PART = HALVES ? WIDTH / 2 : WIDTH;
+        if (vec) {
+            const int unit = lane % UNITS, column = unit * E % PART;
+            T *const p = to + column + (HALVES && unit * E >= PART ? apart : 0);
+            dl_words v[TURNS];
+#pragma unroll
+            for (int t = 0; t < TURNS; ++t) v[t] = *reinterpret_cast<const dl_words *>(place + spot(t * (64 / UNITS) + lane / UNITS, unit));
+            lin_lds_done();  // (all of them are read before the first is written)
+            T *at = p + lane / UNITS * ld;
+            if (rows >= 32 && columns >= PART) {
+#pragma unroll
+                for (int t = 0; t < TURNS; ++t, at += 64 / UNITS * ld) *reinterpret_cast<dl_words *>(at) = v[t];
+            } else if (column < columns) {
+#pragma unroll
+                for (int t = 0; t < TURNS; ++t, at += 64 / UNITS * ld)
+                    if (t * (64 / UNITS) + lane / UNITS < rows) *reinterpret_cast<dl_words *>(at) = v[t];
+            }
+            return;
+        }
+#pragma unroll 1
+        for (int e = lane; e < 32 * WIDTH; e += 64) {
+            const int row = e / WIDTH, at = e % WIDTH, column = at % PART;
+            if (row < rows && column < columns) to[row * ld + column + (HALVES && at >= PART ? apart : 0)] = *reinterpret_cast<const T *>(place + spot(row, at / E) + at % E * (int)sizeof(T));
+        }
+    }
+    // from memory: vectors by way of registers, asked for early; the rest value by value
+    static __device__ __forceinline__ void fetch(dl_words (&v)[TURNS], int lane, const T *from, long long ld, int rows, int columns) {
+        const int column = lane % UNITS * E;
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) {
+            const int row = t * (64 / UNITS) + lane / UNITS;
+            v[t] = dl_words{0, 0, 0, 0};
+            if (row < rows && column < columns) v[t] = *reinterpret_cast<const dl_words *>(from + row * ld + column);
+        }
+    }
+    static __device__ __forceinline__ void keep(char *place, int lane, const dl_words (&v)[TURNS]) {
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) *reinterpret_cast<dl_words *>(place + spot(t * (64 / UNITS) + lane / UNITS, lane % UNITS)) = v[t];
+    }
+    static __device__ __forceinline__ void bring(char *place, int lane, const T *from, long long ld, int rows, int columns) {
+#pragma unroll 1
+        for (int e = lane; e < 32 * WIDTH; e += 64) {
+            const int row = e / WIDTH, column = e % WIDTH;
+            *reinterpret_cast<T *>(place + spot(row, column / E) + column % E * (int)sizeof(T)) = row < rows && column < columns ? from[row * ld + column] : (T)0.0f;
+        }
+    }
+};
+// Four values that belong to columns, bias or scales, as they lie
+template <typename T>
+struct LinFour {
+    uint32_t w[sizeof(T)];
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (__is_same(T, dl_bf16)) return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        else return (float)__builtin_bit_cast(dl_f16, (uint16_t)(w[i / 2] >> (i % 2 * 16)));
+    }
+    __device__ __forceinline__ void again() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i) asm volatile("" : "+v"(w[i]));
+    }
+    // columns from `column` on of the `width` that begin at p + from (p null: `otherwise`); ones that are not there are as the last
+    __device__ __forceinline__ void load(const T *p, long long from, int column, int width, bool vec, T otherwise) {
+        DlVec<T, 4> v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v.v[i] = otherwise;
+        if (p) {
+            if (vec) v = *reinterpret_cast<const DlVec<T, 4> *>(p + from + min(column, width - 4));
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v.v[i] = p[from + min(column + i, width - 1)];
+        }
+        __builtin_memcpy(w, &v, sizeof(w));
+    }
+};
+
+// What follows from it is worked out where it is needed, not held through a loop around
+__device__ __forceinline__ int lin_anew(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// A block of four wavefronts makes tiles of TR x TC, a wavefront a quarter of one, in stages of 128 bytes along the reduction: three of A and two of
 // B are in the LDS.  A stage has 2 or 4 steps of the matrix cores; a step's fragments are read while the one before is worked on, across
 // stages too: by the last step of a stage all of it has been read and the next one has landed.  B's stage after the next is sent for
 // then, into the same place, A's one step later, so that loads are spread over the matrix instructions and have a stage's time to land.  One wavefront
 // a SIMD issues everything, so reads, loads and (of float32) cuts stand between the matrix instructions in the order written here; left
 // to itself the compiler puts the reads in front of their use.  Where the reduction ends inside a stage, that stage comes first.
+// WHAT becomes of the sums: LIN_SUMS partial sums, LIN_PLAIN nothing but the result, LIN_ENDS what follows in whole vectors, LIN_ODD the same value by value.
+// There are as many blocks as the chip holds; one sends for its next tile's first stages before it writes a tile out.
 // Gated, a wavefront's columns are those of the gate, then the ones that belong to them.
-template <typename In, typename Out, int TR, int TC, bool TURN_A, bool TURN_B, bool GATED, bool PARTIAL>
+template <typename In, typename Out, int TR, int TC, bool TURN_A, bool TURN_B, bool GATED, int WHAT>
 __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(LinArgs g) {
     extern __shared__ __align__(16) char lds[];
     typedef LinTile<In, TR, TURN_A> TileA;
     typedef LinTile<In, TC, TURN_B> TileB;
-    constexpr int WAVES = 4, FA = TR / 64, FB = TC / 64, B_PLACE = 3 * TileA::BYTES, KS = TileA::KS;
+    constexpr int WAVES = 4, FA = TR / 64, FB = TC / 64, KS = TileA::KS;
+    constexpr int A0 = 0, A1 = TileA::BYTES, B0 = 2 * TileA::BYTES, B1 = B0 + TileB::BYTES, A2 = B1 + TileB::BYTES;  // places; tiles are written out through the last two
     constexpr int NA = TileA::LOADS / WAVES, NB = TileB::LOADS / WAVES, STEPS = In::SIZE == 2 ? 4 : 2, HALF = FB * 16;
     static_assert(STEPS % 2 == 0, "a stage begins in the first of two sets of fragments");
     typedef __attribute__((address_space(3))) char lds_char;
     const unsigned lds_base = (unsigned)(uintptr_t)(lds_char *)lds;
     const int lane = threadIdx.x & 63, wave = dl_uniform(threadIdx.x >> 6);
 
-    // tiles: every XCD takes a run of them, eight rows of tiles at a time, so that its L2 holds what neighbours share
-    const int tiles = g.row_tiles * g.col_tiles, per = (tiles + DL_XCDS - 1) / DL_XCDS;
-    const int split = blockIdx.x / (per * DL_XCDS), id = blockIdx.x % (per * DL_XCDS);
-    const int tile = (id % DL_XCDS) * per + id / DL_XCDS;
-    if (tile >= tiles) return;
-    const int band = tile / (8 * g.col_tiles), in_band = tile % (8 * g.col_tiles), band_rows = min(8, g.row_tiles - band * 8);
-    const int r0 = (band * 8 + in_band % band_rows) * TR, c0 = in_band / band_rows * (GATED ? TC / 2 : TC);
-    const int first = split * g.chunk, count = min(g.stages - first, g.chunk);
-
-    // ---- what this lane fetches: offsets from the tile's first row and the stage's first value
-    unsigned a_off[NA], b_off[NB];
-    const char *a_base = TURN_A ? g.A : g.A + (long long)r0 * g.lda;
-    const char *b_base = TURN_B ? g.B : g.B + (long long)c0 * g.ldb, *b_other = GATED ? b_base + g.end.F * g.ldb : b_base;
-#pragma unroll
-    for (int j = 0; j < NA; ++j) {
-        const int row = TileA::row_of(wave + j * WAVES, lane), unit = TileA::unit_of(row, lane);
-        a_off[j] = TURN_A ? (unsigned)row * (unsigned)g.lda + (unsigned)min(r0 * In::SIZE + unit * 16, (g.end.R * In::SIZE + 15) / 16 * 16 - 16)
-                          : (unsigned)(min(r0 + row, g.end.R - 1) - r0) * (unsigned)g.lda + unit * 16;
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        const int row = TileB::row_of(wave + j * WAVES, lane), unit = TileB::unit_of(row, lane);
-        // (gated: rows of the tile are HALF of the gate, HALF of the other, and so on)
-        const int f = GATED ? row / (2 * HALF) * HALF + row % HALF : row, most = GATED ? g.end.F : g.end.C;
-        b_off[j] = TURN_B ? (unsigned)row * (unsigned)g.ldb + (unsigned)min(c0 * In::SIZE + unit * 16, (g.end.C * In::SIZE + 15) / 16 * 16 - 16)
-                          : (unsigned)(min(c0 + f, most - 1) - c0) * (unsigned)g.ldb + unit * 16;
-    }
-    static_assert(!GATED || (WAVES * TileB::PER <= HALF && HALF % (WAVES * TileB::PER) == 0), "the four wavefronts' loads are of one half");
-    constexpr auto other = [](int j) { return GATED && j * WAVES * TileB::PER % (2 * HALF) >= HALF; };
-    // where the reduction ends inside a stage: that stage is the block's first
-    const int whole = (int)(g.K / KS), left = (int)(g.K - (long long)whole * KS), tail = first + count - min(first + count, whole);
-    const auto stage_of = [&](int s) { return s == 0 ? first + (count - 1) * tail : first + s - tail; };
-    const auto begin_a = [&](int s) { return a_base + (long long)stage_of(s) * KS * (TURN_A ? g.lda : In::SIZE); };
-    const auto begin_b = [&](int s, const char *base) { return base + (long long)stage_of(s) * KS * (TURN_B ? g.ldb : In::SIZE); };
-    const auto load_a = [&](const char *from, unsigned to, int j) __attribute__((always_inline)) { lin_to_lds(to + (wave + j * WAVES) * 1024, from, a_off[j]); };
-    const auto load_b = [&](const char *from, const char *from_other, unsigned to, int j) __attribute__((always_inline)) {
-        lin_to_lds(to + (wave + j * WAVES) * 1024, other(j) ? from_other : from, b_off[j]);
+    // tiles: every XCD takes a run of them, eight rows of tiles at a time, so that its L2 holds what neighbours share; its blocks take turns
+    const int tiles = g.row_tiles * g.col_tiles, per = (tiles + DL_XCDS - 1) / DL_XCDS, xcd = blockIdx.x % DL_XCDS, items = per * g.splits;
+    int item = blockIdx.x / DL_XCDS;
+    const auto settle = [&]() __attribute__((always_inline)) {
+        while (item < items && xcd * per + item % per >= tiles) item += gridDim.x / DL_XCDS;
+        return item < items;
     };
+    if (!settle()) return;
 
-    floatx16 acc[FA][FB];
-#pragma unroll
-    for (int i = 0; i < FA; ++i)
-#pragma unroll
-        for (int j = 0; j < FB; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
-
-    const int kh = lane >> 5, l32 = lane & 31, wr = wave / 2 * (TR / 2), wc = wave % 2 * (TC / 2);
-    const LinReader<In, TR, TURN_A, FA> read_a(wr, lane);
-    const LinReader<In, TC, TURN_B, FB> read_b(wc, lane);
-    LinFragment<In> a[2][FA], b[2][FB];
-
-    // the first two stages
-    if (tail) {
+    // ---- what this lane fetches of a tile: offsets from its first row and the stage's first value
+    int r0, c0, split, first, count, tail;
+    unsigned a_off[NA], b_off[NB];
+    uint64_t a_first, a_second, b_first, b_second;  // where its first two stages begin; the others follow
+    const int whole = (int)(g.K / KS), left = (int)(g.K - (long long)whole * KS);
+    const uint64_t a_step = TURN_A ? g.lda * KS : LIN_STAGE_BYTES, b_step = TURN_B ? g.ldb * KS : LIN_STAGE_BYTES, b_half = GATED ? lin_scalar(g.end.F * g.ldb) : 0;
+    const unsigned band_tiles = 8 * g.col_tiles, band_reciprocal = dl_uniform(0xFFFFFFFFu / band_tiles);  // (its product is short by one at most)
+    bool inside = false;  // the offsets are those of a tile that ends at no edge
+    const auto place = [&]() __attribute__((always_inline)) {
+        const int of_split = g.splits == 1 ? item : item % per;
+        const unsigned tile = xcd * per + of_split;
+        unsigned band = __umulhi(tile, band_reciprocal), in_band = tile - band * band_tiles;
+        if (in_band >= band_tiles) ++band, in_band -= band_tiles;
+        const unsigned band_rows = min(8, g.row_tiles - (int)band * 8), column = band_rows == 8 ? in_band / 8 : in_band / band_rows;
+        r0 = (int)(band * 8 + in_band - column * band_rows) * TR, c0 = (int)column * (GATED ? TC / 2 : TC);
+        split = g.splits == 1 ? 0 : item / per, first = split * g.chunk, count = min(g.stages - first, g.chunk);
+        tail = first + count - min(first + count, whole);  // 1: the reduction ends inside the last stage, which comes first
+        const char *const a = g.A + (long long)r0 * (TURN_A ? In::SIZE : g.lda), *const b = g.B + (long long)c0 * (TURN_B ? In::SIZE : g.ldb);
+        const uint64_t first_stage = first + (count - 1) * tail, second_stage = first + 1 - tail;
+        a_first = lin_scalar((uint64_t)a + first_stage * a_step), a_second = lin_scalar((uint64_t)a + second_stage * a_step);
+        b_first = lin_scalar((uint64_t)b + first_stage * b_step), b_second = lin_scalar((uint64_t)b + second_stage * b_step);
+        const int most = GATED ? g.end.F : g.end.C;
+        const bool ends = r0 + TR > g.end.R || c0 + (GATED ? TC / 2 : TC) > most;
+        if (inside && !ends) return;
+        inside = !ends;
+        const int lane = lin_anew(threadIdx.x & 63);
 #pragma unroll
         for (int j = 0; j < NA; ++j) {
-            const int row = TileA::row_of(wave + j * WAVES, lane), value = TURN_A ? row : TileA::unit_of(row, lane) * (16 / In::SIZE);
-            lin_to_lds_far(lds_base + (wave + j * WAVES) * 1024, value < left ? begin_a(0) + a_off[j] : (const char *)&lin_zeros);
+            const int row = TileA::row_of(wave + j * WAVES, lane), unit = TileA::unit_of(row, lane);
+            a_off[j] = TURN_A ? (unsigned)row * (unsigned)g.lda + (unsigned)min(unit * 16, (g.end.R * In::SIZE + 15) / 16 * 16 - 16 - r0 * In::SIZE)
+                              : (unsigned)min(row, g.end.R - 1 - r0) * (unsigned)g.lda + unit * 16;
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const int row = TileB::row_of(wave + j * WAVES, lane), value = TURN_B ? row : TileB::unit_of(row, lane) * (16 / In::SIZE);
-            lin_to_lds_far(lds_base + B_PLACE + (wave + j * WAVES) * 1024, value < left ? begin_b(0, other(j) ? b_other : b_base) + b_off[j] : (const char *)&lin_zeros);
+            const int row = TileB::row_of(wave + j * WAVES, lane), unit = TileB::unit_of(row, lane);
+            // (gated: rows of the tile are HALF of the gate, HALF of the other, and so on)
+            const int f = GATED ? row / (2 * HALF) * HALF + row % HALF : row;
+            b_off[j] = TURN_B ? (unsigned)row * (unsigned)g.ldb + (unsigned)min(unit * 16, (g.end.C * In::SIZE + 15) / 16 * 16 - 16 - c0 * In::SIZE)
+                              : (unsigned)min(f, most - 1 - c0) * (unsigned)g.ldb + unit * 16;
         }
-    } else {
+    };
+    static_assert(!GATED || (WAVES * TileB::PER <= HALF && HALF % (WAVES * TileB::PER) == 0), "the four wavefronts' loads are of one half");
+    constexpr auto other = [](int j) { return GATED && j * WAVES * TileB::PER % (2 * HALF) >= HALF; };
+    const auto load_a = [&](intx4 from, unsigned to, int j) __attribute__((always_inline)) { lin_to_lds(to + (wave + j * WAVES) * 1024, from, a_off[j]); };
+    const auto load_b = [&](intx4 from, intx4 from_other, unsigned to, int j) __attribute__((always_inline)) {
+        lin_to_lds(to + (wave + j * WAVES) * 1024, other(j) ? from_other : from, b_off[j]);
+    };
+
+    const auto there = [&](int s) {
+        int behind = s - count;
+        asm("" : "+s"(behind));  // (as a comparison it would be taken through the lanes' registers)
+        return behind >> 31;
+    };
+    // a tile's first stages: the first of both, the second of A
+    const auto begin = [&]() __attribute__((always_inline)) {
+        if (tail) {
+            const int lane = lin_anew(threadIdx.x & 63);
 #pragma unroll
-        for (int j = 0; j < NA; ++j) load_a(begin_a(0), lds_base, j);
+            for (int j = 0; j < NA; ++j) {
+                const int row = TileA::row_of(wave + j * WAVES, lane), value = TURN_A ? row : TileA::unit_of(row, lane) * (16 / In::SIZE);
+                lin_to_lds_far(lds_base + A0 + (wave + j * WAVES) * 1024, value < left ? (const char *)a_first + a_off[j] : (const char *)&lin_zeros);
+            }
 #pragma unroll
-        for (int j = 0; j < NB; ++j) load_b(begin_b(0, b_base), begin_b(0, b_other), lds_base + B_PLACE, j);
-    }
-    if (count > 1) {
+            for (int j = 0; j < NB; ++j) {
+                const int row = TileB::row_of(wave + j * WAVES, lane), value = TURN_B ? row : TileB::unit_of(row, lane) * (16 / In::SIZE);
+                lin_to_lds_far(lds_base + B0 + (wave + j * WAVES) * 1024, value < left ? (const char *)b_first + (other(j) ? b_half : 0) + b_off[j] : (const char *)&lin_zeros);
+            }
+        } else {
 #pragma unroll
-        for (int j = 0; j < NA; ++j) load_a(begin_a(1), lds_base + TileA::BYTES, j);
+            for (int j = 0; j < NA; ++j) load_a(lin_buffer(a_first, -1), lds_base + A0, j);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) load_b(begin_b(1, b_base), begin_b(1, b_other), lds_base + B_PLACE + TileB::BYTES, j);
-        lin_stage_barrier<NA + NB>();
-    } else lin_stage_barrier<0>();
+            for (int j = 0; j < NB; ++j) load_b(lin_buffer(b_first, -1), lin_buffer(b_first + b_half, -1), lds_base + B0, j);
+        }
+#pragma unroll
+        for (int j = 0; j < NA; ++j) load_a(lin_buffer(a_second, there(1)), lds_base + A1, j);
+    };
+
+    const int wr = wave / 2 * (TR / 2), wc = wave % 2 * (TC / 2);
+    const LinReader<In, TR, TURN_A, FA> read_a(wr, lane);
+    const LinReader<In, TC, TURN_B, FB> read_b(wc, lane);
+    floatx16 acc[FA][FB];
+    LinFragment<In> a[2][FA], b[2][FB];
 
     // Side work of a step, one piece after the other: fragments in the order in which the next step takes them (A's first, all of B, the rest of A)
     constexpr bool CUT = __is_same(In, LinF32);
@@ -385,125 +516,215 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
             constexpr int f = o / 5, r = o % 5, q = f - 1;
             if constexpr (r == 0 && f < FRAGMENTS) {
                 if constexpr (f == 0 || f > FB) read_a.read_raw(lds + from_a, step, f == 0 ? 0 : f - FB, raw[f & 1]);
-                else read_b.read_raw(lds + B_PLACE + from_b, step, f - 1, raw[f & 1]);
+                else read_b.read_raw(lds + from_b, step, f - 1, raw[f & 1]);
             }
             if constexpr (r > 0 && f > 0) {
                 if constexpr (q == 0 || q > FB) lin_cut(raw[q & 1], r - 1, a[set][q == 0 ? 0 : q - FB]);
                 else lin_cut(raw[q & 1], r - 1, b[set][q - 1]);
             }
         } else if constexpr (o < PA) read_a.read(lds + from_a, step, 0, o, a[set][0]);
-        else if constexpr (o < PA + FB * PB) read_b.read(lds + B_PLACE + from_b, step, (o - PA) / PB, (o - PA) % PB, b[set][(o - PA) / PB]);
+        else if constexpr (o < PA + FB * PB) read_b.read(lds + from_b, step, (o - PA) / PB, (o - PA) % PB, b[set][(o - PA) / PB]);
         else read_a.read(lds + from_a, step, (o - FB * PB) / PA, (o - FB * PB) % PA, a[set][(o - FB * PB) / PA]);
     };
-    lin_each<0, PIECES>([&](auto o) __attribute__((always_inline)) { piece(o, 0, 0, 0, 0); });
 
-    unsigned a_now = 0, a_next = TileA::BYTES, a_free = 2 * TileA::BYTES, b_now = 0;
-    const char *from_a = begin_a(2);  // (not followed where there are no three stages)
-    const char *from_b = begin_b(2, b_base), *from_other = begin_b(2, b_other);
-    // MORE: stages behind this one, 2 standing for two or more
-    const auto stage = [&](auto more) __attribute__((always_inline)) {
-        constexpr int MORE = decltype(more)::value;
+    unsigned a_now, a_next, a_free, b_now;
+    intx4 from_a, from_b, from_other;
+    // A stage, FIRST of a tile or another.  What it sends for and reads behind the last one is not there, and not used.
+    const auto stage = [&](auto is_first) __attribute__((always_inline)) {
+        constexpr bool FIRST = decltype(is_first)::value;
         lin_each<0, STEPS>([&](auto step) __attribute__((always_inline)) {
             constexpr int st = decltype(step)::value;
             constexpr bool last = st + 1 == STEPS;
-            if constexpr (last && MORE > 0) lin_stage_barrier<MORE == 2 ? NA : 0>();  // the next stage is there, and nobody reads this one any more
+            if constexpr (last) lin_stage_barrier<NA>();  // the next stage is there, and nobody reads this one any more
             __builtin_amdgcn_sched_barrier(0);
             lin_each<0, SLOTS>([&](auto slot) __attribute__((always_inline)) {
                 constexpr int m = decltype(slot)::value, o0 = m * PIECES / READ_SLOTS, o1 = (m + 1) * PIECES / READ_SLOTS;
-                if constexpr (!last || MORE > 0)
-                    lin_each<(o0 < PIECES ? o0 : PIECES), (o1 < PIECES ? o1 : PIECES)>([&](auto o) __attribute__((always_inline)) {
-                        piece(o, last ? a_next : a_now, last ? TileB::BYTES - b_now : b_now, last ? 0 : st + 1, (st + 1) & 1);
-                    });
-                if constexpr (MORE == 2 && last)
-                    lin_each<m * NB / SLOTS, (m + 1) * NB / SLOTS>([&](auto j) __attribute__((always_inline)) { load_b(from_b, from_other, lds_base + B_PLACE + b_now, decltype(j)::value); });
-                if constexpr (MORE == 2 && st == 0)
+                lin_each<(o0 < PIECES ? o0 : PIECES), (o1 < PIECES ? o1 : PIECES)>([&](auto o) __attribute__((always_inline)) {
+                    piece(o, last ? a_next : a_now, last ? B0 + B1 - b_now : b_now, last ? 0 : st + 1, (st + 1) & 1);
+                });
+                if constexpr (last)
+                    lin_each<m * NB / SLOTS, (m + 1) * NB / SLOTS>([&](auto j) __attribute__((always_inline)) { load_b(from_b, from_other, lds_base + b_now, decltype(j)::value); });
+                if constexpr (st == 0)
                     lin_each<m * NA / SLOTS, (m + 1) * NA / SLOTS>([&](auto j) __attribute__((always_inline)) { load_a(from_a, lds_base + a_free, decltype(j)::value); });
                 constexpr int i = m / (FB * PRODUCTS), t = m / FB % PRODUCTS, j = m % FB;
-                acc[i][j] = lin_mfma<In>(a[st & 1][i], b[st & 1][j], acc[i][j], t);
+                if constexpr (FIRST && st == 0 && t == 0) {
+                    floatx16 none;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) none[v] = 0.0f;
+                    acc[i][j] = lin_mfma<In>(b[0][j], a[0][i], none, 0);
+                } else acc[i][j] = lin_mfma<In>(b[st & 1][j], a[st & 1][i], acc[i][j], t);
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
         const unsigned was = a_now;
         a_now = a_next, a_next = a_free, a_free = was;
-        b_now = TileB::BYTES - b_now;
-        from_a += KS * (TURN_A ? g.lda : In::SIZE), from_b += KS * (TURN_B ? g.ldb : In::SIZE), from_other += KS * (TURN_B ? g.ldb : In::SIZE);
+        b_now = B0 + B1 - b_now;
     };
-    for (int s = 0; s + 2 < count; ++s) stage(LinIs<2>());
-    if (count > 1) stage(LinIs<1>());
-    stage(LinIs<0>());
 
-    // C: row (v % 4) + 8 (v / 4) + 4 (lane / 32) of a tile of 32 x 32, column lane % 32
-    if (PARTIAL) {
-        float *part = g.part + (long long)split * g.end.R * g.end.C;
+    // C: a lane has row lane % 32 of a tile of 32 x 32, and columns (v % 4) + 8 (v / 4) + 4 (lane / 32) of it
+    constexpr int W = FB * 32, H = GATED ? FB / 2 : FB;
+    constexpr bool PARTIAL = WHAT == LIN_SUMS;
+    typedef typename LinChoose<PARTIAL, float, Out>::type Stored;
+    typedef LinPlace<Stored, W> Products;               // z, or partial sums
+    typedef LinPlace<Stored, GATED ? HALF : W> Results;
+    static_assert(WAVES * Products::BYTES <= TileA::BYTES + TileB::BYTES, "fits the last two places");
+    constexpr bool SCALED = In::SIZE == 1, VEC = WHAT != LIN_ODD;
+    static_assert(WHAT != LIN_PLAIN || (!SCALED && !GATED), "something follows");
+    const auto write_plain = [&](int row0, int column0, int plane) __attribute__((always_inline)) {
+        const int lane = lin_anew(threadIdx.x & 63), c = column0 + wc;
+        Stored *const out = PARTIAL ? (Stored *)(void *)g.part + (long long)plane * g.end.R * g.end.C : (Stored *)g.end.y;
+        const bool vec = PARTIAL ? g.end.C % 4 == 0 : g.end.vec;
+        char *mine = lds + B1 + wave * Products::BYTES;
+        lin_each<0, FA>([&](auto phase) __attribute__((always_inline)) {
+            constexpr int i = decltype(phase)::value;
+            const int r = row0 + wr + i * 32;
+            if constexpr (TR * TC > 128 * 128) {
 #pragma unroll
-        for (int i = 0; i < FA; ++i)
+                for (int j = 0; j < FB; ++j) asm volatile("" : "+a"(acc[i][j]));  // (no earlier than here out of the accumulators' registers)
+            }
+#pragma unroll
+            for (int j = 0; j < FB; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float f[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    Products::put(mine, lane & 31, j * 32 + 8 * q + 4 * (lane >> 5), f);
+                }
+            lin_lds_done();
+            Products::send(mine, lane, out + (long long)r * g.end.C + c, g.end.C, g.end.R - r, g.end.C - c, vec);
+            lin_lds_done();
+        });
+    };
+    const auto write = [&](int row0, int column0) __attribute__((always_inline)) {
+        const int lane = lin_anew(threadIdx.x & 63), kh = lane >> 5, l32 = lane & 31;
+        const LinEnd &e = g.end;
+        char *mine = lds + B1 + wave * Products::BYTES;
+        const int width = GATED ? e.F : e.C, c = column0 + (GATED ? wc / 2 : wc), columns = width - c;
+        LinFour<Stored> bias[FB][4];
+        LinFour<float> scale[SCALED ? FB : 1][4];
+        const auto of_columns = [&]() __attribute__((always_inline)) {
+            const int first = lin_anew(c + 4 * kh);
+#pragma unroll
+            for (int j = 0; j < FB; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const long long from = (j / H) * (long long)e.F;  // (gated: of the gate's or the other's columns)
+                    const int column = first + j % H * 32 + 8 * q;
+                    bias[j][q].load((const Stored *)e.bias, from, column, width, VEC, (Stored)0.0f);
+                    if (SCALED) scale[SCALED ? j : 0][q].load(e.col_scale, from, column, width, VEC, 1.0f);
+                }
+        };
+        constexpr bool HELD = sizeof(Stored) == 2;  // through the tile; more would not fit the registers
+        if (HELD) of_columns();
+        lin_each<0, FA>([&](auto phase) __attribute__((always_inline)) {
+            constexpr int i = decltype(phase)::value;
+            const int r = row0 + wr + i * 32, rows = e.R - r;
+            if constexpr (TR * TC > 128 * 128) {
+#pragma unroll
+                for (int j = 0; j < FB; ++j) asm volatile("" : "+a"(acc[i][j]));  // (no earlier than here out of the accumulators' registers)
+            }
+            const Stored *const res = (const Stored *)e.res + r * e.ldr + c;
+            dl_words residual[Results::TURNS];
+            if (e.res && VEC && !SCALED) Results::fetch(residual, lane, res, e.ldr, rows, columns);  // (scales take the registers that it would wait in)
+            const float row_scale = SCALED ? e.row_scale[min(r + l32, e.R - 1)] : 1.0f;
+            if (!HELD) of_columns();
+            else {
+#pragma unroll
+                for (int j = 0; j < FB; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        bias[j][q].again();  // (held as words, not as what they become)
+                        if (SCALED) scale[SCALED ? j : 0][q].again();
+                    }
+            }
+            float f[FB][16];
 #pragma unroll
             for (int j = 0; j < FB; ++j)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const int r = r0 + wr + i * 32 + (v & 3) + 8 * (v >> 2) + 4 * kh, c = c0 + wc + j * 32 + l32;
-                    if (r < g.end.R && c < g.end.C) part[(long long)r * g.end.C + c] = acc[i][j][v];
+                    const float b = bias[j][v / 4].value(v % 4);
+                    f[j][v] = SCALED ? fmaf(acc[i][j][v], row_scale * scale[SCALED ? j : 0][v / 4].value(v % 4), b) : acc[i][j][v] + b;
                 }
-        return;
-    }
-    // through the LDS, 64 rows at a time, every wavefront in a place of its own: a lane then has eight columns of a row
-    constexpr int W = FB * 32, LD = W + 4, COLUMNS = GATED ? HALF : W, LANES = COLUMNS / 8, ROWS = 64 / LANES, TURNS = 4;  // lanes of a row, rows at a time
-    static_assert(FA % 2 == 0 && 64 % (ROWS * TURNS) == 0 && WAVES * 64 * LD * 4 <= 3 * TileA::BYTES + 2 * TileB::BYTES, "fits the stages");
-    lin_stage_barrier<0>();
-    float *mine = reinterpret_cast<float *>(lds) + wave * 64 * LD;
-    const int width = GATED ? g.end.F : g.end.C, begin = c0 + (GATED ? wc / 2 : wc), col = lane % LANES * 8, c = begin + col;
-    const LinColumns<Out, GATED> columns(g.end, g.end.vec ? c : width);
-    lin_each<0, FA / 2>([&](auto phase) __attribute__((always_inline)) {
-        constexpr int i0 = 2 * decltype(phase)::value;
-        const int first_row = r0 + wr + i0 * 32;
-        DlVec<Out, 8> next[TURNS];  // residuals, asked for a round ahead
-        float next_scale[TURNS];
-        const auto ask = [&](int row) __attribute__((always_inline)) {
+            if (e.z) {
 #pragma unroll
-            for (int t = 0; t < TURNS; ++t) {
-                const int r = first_row + row + t * ROWS;
-                next[t] = lin_residual<Out>(g.end, row < 64 ? width : 0, r, c);
-                next_scale[t] = g.end.row_scale && r < g.end.R ? g.end.row_scale[r] : 1.0f;
+                for (int j = 0; j < FB; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) Products::put(mine, l32, j * 32 + 8 * q + 4 * kh, {f[j][4 * q], f[j][4 * q + 1], f[j][4 * q + 2], f[j][4 * q + 3]});
+                lin_lds_done();
+                Products::template send<GATED>(mine, lane, (Stored *)e.z + (long long)r * e.C + c, e.C, rows, columns, VEC, e.F);
+                lin_lds_done();
             }
-        };
-        if (g.end.vec) ask(lane / LANES);
+            if (e.res) {
+                if (VEC && SCALED) Results::fetch(residual, lane, res, e.ldr, rows, columns);
+                if (VEC) Results::keep(mine, lane, residual);
+                else Results::bring(mine, lane, res, e.ldr, rows, columns);
+                lin_lds_done();
+            }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < H; ++j) {
+                if (e.act == DL_ACT_RELU) {
 #pragma unroll
-            for (int j = 0; j < FB; ++j)
+                    for (int v = 0; v < 16; ++v) f[j][v] = lin_act(f[j][v], DL_ACT_RELU);
+                } else if (e.act != DL_ACT_NONE) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) mine[(i * 32 + (v & 3) + 8 * (v >> 2) + 4 * kh) * LD + j * 32 + l32] = acc[i0 + i][j][v];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (g.end.vec) {
-#pragma unroll 1
-            for (int row = lane / LANES; row < 64; row += ROWS * TURNS) {
-                DlVec<Out, 8> res[TURNS];
-                float scale[TURNS];
-#pragma unroll
-                for (int t = 0; t < TURNS; ++t) res[t] = next[t], scale[t] = next_scale[t];
-                ask(row + ROWS * TURNS);
-#pragma unroll
-                for (int t = 0; t < TURNS; ++t) {
-                    const float *at = mine + (row + t * ROWS) * LD + col;
-                    float v[8], u[8];
-                    *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(at);
-                    *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(at + 4);
-                    if (GATED) {
-                        *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(at + HALF);
-                        *reinterpret_cast<float4 *>(u + 4) = *reinterpret_cast<const float4 *>(at + HALF + 4);
+                    for (int v = 0; v < 16; ++v) {
+                        const float s = lin_sigmoid(f[j][v]);
+                        f[j][v] = e.act == DL_ACT_SILU ? f[j][v] * s : s;
                     }
-                    lin_finish<Out, GATED>(g.end, columns, first_row + row + t * ROWS, c, v, u, scale[t], res[t]);
                 }
+                if (GATED) {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) f[j][v] *= f[j + FB - H][v];
+                }
+                if (e.res) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float r4[4];
+                        Results::get(mine, l32, j * 32 + 8 * q + 4 * kh, r4);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) f[j][4 * q + v] += r4[v];
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) Results::put(mine, l32, j * 32 + 8 * q + 4 * kh, {f[j][4 * q], f[j][4 * q + 1], f[j][4 * q + 2], f[j][4 * q + 3]});
             }
-        } else {
-#pragma unroll 1
-            for (int e = lane; e < 64 * COLUMNS; e += 64) {
-                const float *at = mine + e / COLUMNS * LD + e % COLUMNS;
-                lin_finish_one<Out, GATED>(g.end, first_row + e / COLUMNS, begin + e % COLUMNS, at[0], GATED ? at[HALF] : 0.0f);
-            }
+            lin_lds_done();
+            Results::send(mine, lane, (Stored *)e.y + (long long)r * width + c, width, rows, columns, VEC);
+            lin_lds_done();
+        });
+    };
+
+    place();
+    begin();
+    for (;;) {
+        lin_stage_barrier<0>();  // the first stages are there, and the tile before is written out of the LDS
+#pragma unroll
+        for (int j = 0; j < NB; ++j) load_b(lin_buffer(b_second, there(1)), lin_buffer(b_second + b_half, there(1)), lds_base + B1, j);
+        a_now = A0, a_next = A1, a_free = A2, b_now = B0;
+        uint64_t at_a = a_second, at_b = b_second;
+        const auto send_for = [&](int s) __attribute__((always_inline)) {
+            at_a += a_step, at_b += b_step;
+            from_a = lin_buffer(at_a, there(s)), from_b = lin_buffer(at_b, there(s)), from_other = lin_buffer(at_b + b_half, there(s));
+        };
+        lin_each<0, PIECES>([&](auto o) __attribute__((always_inline)) { piece(o, A0, B0, 0, 0); });
+        send_for(2);
+        stage(LinIs<1>());
+        for (int s = 1; s < count; ++s) {
+            send_for(s + 2);
+            stage(LinIs<0>());
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    });
+
+        const int row = r0, column = c0, plane = split;
+        item += gridDim.x / DL_XCDS;
+        const bool more = settle();
+        lin_stage_barrier<0>();  // everybody has read the last stage
+        if (more) {
+            place();
+            begin();
+        }
+        if constexpr (WHAT == LIN_SUMS || WHAT == LIN_PLAIN) write_plain(row, column, plane);
+        else write(row, column);
+        if (!more) return;
+    }
 }
 
 // The sums of a reduction that was split, in order, and what follows
@@ -539,40 +760,46 @@ __global__ __launch_bounds__(256) void lin_join(LinArgs g, int splits) {
                 if (GATED) u[i] += q[i];
             }
         }
-        lin_finish<Out, GATED>(g.end, LinColumns<Out, GATED>(g.end, c), r, c, v, u, g.end.row_scale ? g.end.row_scale[r] : 1.0f, res);
+        lin_finish<Out, GATED, true>(g.end, LinColumns<Out, GATED>(g.end, c), r, c, v, u, g.end.row_scale ? g.end.row_scale[r] : 1.0f, res);
     }
 }
 
 // ------------------------------------------------------------------ launches
 struct LinPlan {
-    int tile_rows, tile_cols;
+    int tile;
     int splits, chunk;  // parts of the reduction, and their stages
     size_t a_bytes, b_bytes, part_bytes;
     size_t bytes() const { return a_bytes + b_bytes + part_bytes; }
 };
-template <typename In, typename Out, int TR, int TC, bool TURN_A, bool TURN_B, bool GATED, bool PARTIAL>
-static int lin_go(const LinArgs &g, int splits, hipStream_t s) {
-    constexpr int BYTES = (3 * TR + 2 * TC) * LIN_STAGE_BYTES;
-    const long long blocks = (long long)splits * DL_XCDS * dl_ceil_div((long long)g.row_tiles * g.col_tiles, DL_XCDS);
-    if (!dl_grid_ok(blocks, 256)) return DL_ERR_UNSUPPORTED;
-    const auto kernel = lin_product<In, Out, TR, TC, TURN_A, TURN_B, GATED, PARTIAL>;
-    if (BYTES > 65536) {
-        const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
-        if (room != hipSuccess) return (int)room;
-    }
-    DL_TIMED("lin_product", s, hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), BYTES, s, g));
+template <typename In, typename Out, int T, bool TURN_A, bool TURN_B, bool GATED, int WHAT>
+static int lin_go(const LinArgs &g, hipStream_t s) {
+    constexpr int BYTES = 5 * T * LIN_STAGE_BYTES;
+    const long long items = (long long)g.splits * DL_XCDS * (((long long)g.row_tiles * g.col_tiles + DL_XCDS - 1) / DL_XCDS), most = LIN_CUS * (T > 128 ? 1 : 2);
+    if (items >= 1LL << 30) return DL_ERR_UNSUPPORTED;
+    const auto kernel = lin_product<In, Out, T, T, TURN_A, TURN_B, GATED, WHAT>;
+    const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    if (room != hipSuccess) return (int)room;
+    DL_TIMED("lin_product", s, hipLaunchKernelGGL(kernel, dim3((unsigned)(items < most ? items : most)), dim3(256), BYTES, s, g));
     return DL_OK;
 }
+// (the backward's products: nothing follows)
 template <typename In, typename Out, int T, bool TURN_A, bool TURN_B>
-static int lin_launch_tile(const LinArgs &g, int splits, bool gated, hipStream_t s) {
-    if (splits > 1) return lin_go<In, Out, T, T, TURN_A, TURN_B, false, true>(g, splits, s);
-    if constexpr (!TURN_A && !TURN_B)
-        if (gated) return lin_go<In, Out, T, T, false, false, true, false>(g, splits, s);
-    return lin_go<In, Out, T, T, TURN_A, TURN_B, false, false>(g, splits, s);
+static int lin_launch_tile(const LinArgs &g, bool gated, hipStream_t s) {
+    const LinEnd &e = g.end;
+    if (g.splits > 1) return lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_SUMS>(g, s);
+    if constexpr (TURN_B) return lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_PLAIN>(g, s);
+    else {
+        constexpr bool SCALED = In::SIZE == 1;
+        if constexpr (!SCALED)
+            if (!gated && !e.bias && !e.res && !e.z && e.act == DL_ACT_NONE) return lin_go<In, Out, T, false, false, false, LIN_PLAIN>(g, s);
+        if (e.vec) return gated ? lin_go<In, Out, T, false, false, true, LIN_ENDS>(g, s) : lin_go<In, Out, T, false, false, false, LIN_ENDS>(g, s);
+        if constexpr (T <= 128) return gated ? lin_go<In, Out, T, false, false, true, LIN_ODD>(g, s) : lin_go<In, Out, T, false, false, false, LIN_ODD>(g, s);
+    }
+    return DL_ERR_UNSUPPORTED;  // (the plan gives small tiles to what is not in whole vectors)
 }
 template <typename In, typename Out, bool TURN_A, bool TURN_B>
 static int lin_launch(LinArgs &g, const LinPlan &p, bool gated, hipStream_t s) {
-    const int code = p.tile_rows == 256 ? lin_launch_tile<In, Out, 256, TURN_A, TURN_B>(g, p.splits, gated, s) : lin_launch_tile<In, Out, 128, TURN_A, TURN_B>(g, p.splits, gated, s);
+    const int code = p.tile == 256 ? lin_launch_tile<In, Out, 256, TURN_A, TURN_B>(g, gated, s) : lin_launch_tile<In, Out, 128, TURN_A, TURN_B>(g, gated, s);
     if (code != DL_OK || p.splits == 1) return code;
     const long long blocks = ((long long)g.end.R * ((gated ? g.end.F : g.end.C) / (g.end.vec ? 8 : 1)) + 255) / 256;
     const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));

@@ -1,5 +1,7 @@
 // Entry points of the matrix products, their plans, and the gradient in front of the backward's products (linear.h has the mathematics and
 // the product kernel).
+#include <math.h>
+
 #include "linear.h"
 
 // ------------------------------------------------------------------ operands whose rows are not whole units
@@ -110,19 +112,25 @@ static long long lin_padded(const LinOperand &o, int type) { const int unit = 16
 static size_t lin_operand_bytes(const LinOperand &o, int type) {
     return lin_direct(o, type) ? 0 : dl_align256((size_t)o.rows * (size_t)lin_padded(o, type) * lin_size(type));
 }
-// Tile and split.
+// Tile and split: the least of an estimate over both tiles and the splits that leave a part four stages.  A stage takes a block of 256 x 256
+// 1.55 us, the two blocks of 128 x 128 that share a CU 0.95, one that has it alone 0.6 (float32: three times that); a tile's beginning and end
+// take 5 and 3 us; sums are written and read at 4 bytes/ps, with 4 us for the launch that joins them.  (bf16, 8192^3: 256 787 us, 128 970; 1024 x 4096 over
+// 12544, us with the join: 256 in 4 parts 98, 128 in 2 parts 104, 256 whole 360.)
 static LinPlan lin_plan(const LinOperand &a, const LinOperand &b, int type, long long K) {
     LinPlan p;
-    const long long R = a.count(), C = b.count();
+    const long long R = a.count(), C = b.count(), stages = (K * lin_size(type) + LIN_STAGE_BYTES - 1) / LIN_STAGE_BYTES;
     p.a_bytes = lin_operand_bytes(a, type), p.b_bytes = lin_operand_bytes(b, type);
-    const auto tiles = [&](int tr, int tc) { return (double)((R + tr - 1) / tr) * (double)((C + tc - 1) / tc); };
-    p.tile_rows = p.tile_cols = tiles(256, 256) >= 0.7 * LIN_CUS ? 256 : 128;
-    const long long stages = (K * lin_size(type) + LIN_STAGE_BYTES - 1) / LIN_STAGE_BYTES;
-    p.splits = 1;
-    if (p.tile_rows == 128)
-        while (p.splits < 64 && tiles(128, 128) * p.splits * 2 <= 2 * LIN_CUS && stages / (p.splits * 2) >= 4) p.splits *= 2;
-    p.chunk = (int)((stages + p.splits - 1) / p.splits);
-    p.splits = (int)((stages + p.chunk - 1) / p.chunk);  // (none without a stage)
+    double best = 1e30;
+    for (int tile = 128; tile <= 256; tile += 128) {
+        const double tiles = (double)((R + tile - 1) / tile) * (double)((C + tile - 1) / tile), slots = tile == 256 ? LIN_CUS : 2 * LIN_CUS;
+        for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits / 2) {
+            if (splits > 1 && (stages / splits < 4 || tiles * (splits - 1) >= slots)) break;
+            const long long chunk = (stages + splits - 1) / splits;
+            const double stage = (type == DL_F32 ? 3.0 : 1.0) * (tile == 256 ? 1.55 : tiles * splits <= LIN_CUS ? 0.6 : 0.95), rounds = ceil(tiles * splits / slots);
+            const double us = rounds * ((double)chunk * stage + (tile == 256 ? 5.0 : 3.0)) + (splits > 1 ? 4.0 + 8.0 * splits * (double)R * (double)C / 4e6 : 0.0);
+            if (us < best) best = us, p.tile = tile, p.splits = (int)((stages + chunk - 1) / chunk), p.chunk = (int)chunk;  // (no part is without a stage)
+        }
+    }
     p.part_bytes = p.splits > 1 ? dl_align256((size_t)p.splits * (size_t)R * (size_t)C * 4) : 0;
     return p;
 }
@@ -148,18 +156,18 @@ static const char *lin_lay_out(const LinOperand &o, int type, void *room, long l
 
 // One product: operands laid out, tiles, what follows
 static int lin_run(const LinOperand &a, const LinOperand &b, int type, int out_type, long long K, bool gated, LinEnd end, char *ws, hipStream_t s) {
-    const LinPlan p = lin_plan(a, b, type, K);
+    LinPlan p = lin_plan(a, b, type, K);
     LinArgs g{};
     g.A = lin_lay_out(a, type, ws, g.lda, s);
     g.B = lin_lay_out(b, type, ws + p.a_bytes, g.ldb, s);
     if (g.lda > LIN_MOST_ROW || g.ldb > LIN_MOST_ROW) return DL_ERR_UNSUPPORTED;
     g.part = (float *)(ws + p.a_bytes + p.b_bytes);
-    g.K = K, g.stages = dl_ceil_div(K * lin_size(type), LIN_STAGE_BYTES), g.chunk = p.chunk;
     end.R = (int)a.count(), end.C = (int)b.count(), end.F = end.C / 2;
-    const bool halves = gated && p.splits == 1;
-    g.row_tiles = dl_ceil_div(end.R, p.tile_rows), g.col_tiles = halves ? dl_ceil_div(end.F, p.tile_cols / 2) : dl_ceil_div(end.C, p.tile_cols);
     const int width = gated ? end.F : end.C, size = dl_type_bytes(out_type);
     end.vec = width % 8 == 0 && dl_aligned16(end.y) && dl_aligned16(end.z) && dl_aligned16(end.bias) && dl_aligned16(end.res) && dl_aligned16(end.col_scale) && end.ldr * size % 16 == 0;
+    if (p.splits == 1 && !end.vec && !b.turned) p.tile = 128;  // (value by value: the smaller tile alone)
+    g.K = K, g.stages = dl_ceil_div(K * lin_size(type), LIN_STAGE_BYTES), g.chunk = p.chunk, g.splits = p.splits;
+    g.row_tiles = dl_ceil_div(end.R, p.tile), g.col_tiles = gated && p.splits == 1 ? dl_ceil_div(end.F, p.tile / 2) : dl_ceil_div(end.C, p.tile);
     g.end = end;
     int code = DL_ERR_UNSUPPORTED;
     if (type == DL_E4M3) code = lin_launch_e4m3(g, p, out_type, gated, s);
