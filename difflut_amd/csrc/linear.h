@@ -180,21 +180,27 @@ struct LinFragment {
     static constexpr int WORDS = __is_same(In, LinE4m3) ? 8 : 4, PLANES = __is_same(In, LinF32) ? LIN_PLANES : 1;
     int w[PLANES][WORDS];
 };
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ unsigned lin_pk_bf16(float a, float b) {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     typedef float floatx2 __attribute__((ext_vector_type(2)));
     const floatx2 v = {a, b};
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
 }
-// values 2 i and 2 i + 1
-__device__ __forceinline__ void lin_cut(const float (&f)[8], int i, LinFragment<LinF32> &out) {
-    float a = f[2 * i], b = f[2 * i + 1];
+// Eight values into planes in five parts: the first plane, what it leaves, the second, what it leaves, the third.  What is left of a value is
+// its product with -1 of the plane's pair, and 0 of its neighbour, added to it: exact, and at once from the packed pair.  (Cycles of one wavefront: rounding
+// a pair 8.6, such a product 6.4, to unpack or subtract 5.6 each, so a pair takes 51 instead of 71.  The parts keep results away from their use, which
+// would cost waits.)
+__device__ __forceinline__ void lin_cut(float (&f)[8], int part, LinFragment<LinF32> &out) {
+    unsigned low = 0x0000BF80u, high = 0xBF800000u;  // (-1, 0) and (0, -1)
+    asm("" : "+s"(low), "+s"(high));  // in registers: as the instruction's own constant -1 the first would stand in the other half
 #pragma unroll
-    for (int p = 0; p < LIN_PLANES; ++p) {
-        const unsigned w = lin_pk_bf16(a, b);
-        out.w[p][i] = (int)w;
-        a -= __uint_as_float(w << 16);
-        b -= __uint_as_float(w & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) {
+        int &w = out.w[part / 2][i];
+        if (part % 2 == 0) w = (int)lin_pk_bf16(f[2 * i], f[2 * i + 1]);
+        else {
+            f[2 * i] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, low), f[2 * i], false);
+            f[2 * i + 1] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, high), f[2 * i + 1], false);
+        }
     }
 }
 template <typename In>
@@ -232,8 +238,8 @@ struct LinTile {
 };
 
 // The F fragments of 32 rows each, from row `first` of the tile on.  Lane l has row l % 32 of a fragment, and of a step's values along the
-// reduction the eight (of 8 bits 2 x 16) at l / 32.  A fragment comes in PER reads; float32 fragments come raw, and are cut a pair of
-// values at a time.
+// reduction the eight (of 8 bits 2 x 16) at l / 32.  A fragment comes in PER reads; float32 fragments come raw, and are cut a part
+// at a time.
 template <typename In, int T, bool TURNED, int F>
 struct LinReader {
     typedef LinTile<In, T, TURNED> Tile;
@@ -413,36 +419,37 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
     const int lane = threadIdx.x & 63, wave = dl_uniform(threadIdx.x >> 6);
 
     // tiles: every XCD takes a run of them, eight rows of tiles at a time, so that its L2 holds what neighbours share; its blocks take turns
-    const int tiles = g.row_tiles * g.col_tiles, per = (tiles + DL_XCDS - 1) / DL_XCDS, xcd = blockIdx.x % DL_XCDS, items = per * g.splits;
-    int item = blockIdx.x / DL_XCDS;
+    const int tiles = g.row_tiles * g.col_tiles, per = (tiles + DL_XCDS - 1) / DL_XCDS, xcd = blockIdx.x % DL_XCDS, items = per * g.splits, most = GATED ? g.end.F : g.end.C;
+    const unsigned band_tiles = 8 * g.col_tiles, band_reciprocal = dl_uniform(0xFFFFFFFFu / band_tiles);  // (its product is short by one at most)
+    int item = blockIdx.x / DL_XCDS, r0, c0;
     const auto settle = [&]() __attribute__((always_inline)) {
-        while (item < items && xcd * per + item % per >= tiles) item += gridDim.x / DL_XCDS;
-        return item < items;
+        for (; item < items; item += gridDim.x / DL_XCDS) {
+            const unsigned tile = xcd * per + (g.splits == 1 ? item : item % per);
+            if (tile >= (unsigned)tiles) continue;
+            unsigned band = __umulhi(tile, band_reciprocal), in_band = tile - band * band_tiles;
+            if (in_band >= band_tiles) ++band, in_band -= band_tiles;
+            const unsigned band_rows = min(8, g.row_tiles - (int)band * 8), column = band_rows == 8 ? in_band / 8 : in_band / band_rows;
+            r0 = (int)(band * 8 + in_band - column * band_rows) * TR, c0 = (int)column * (GATED ? TC / 2 : TC);
+            return true;
+        }
+        return false;
     };
     if (!settle()) return;
 
     // ---- what this lane fetches of a tile: offsets from its first row and the stage's first value
-    int r0, c0, split, first, count, tail;
+    int split, first, count, tail;
     unsigned a_off[NA], b_off[NB];
     uint64_t a_first, a_second, b_first, b_second;  // where its first two stages begin; the others follow
     const int whole = (int)(g.K / KS), left = (int)(g.K - (long long)whole * KS);
     const uint64_t a_step = TURN_A ? g.lda * KS : LIN_STAGE_BYTES, b_step = TURN_B ? g.ldb * KS : LIN_STAGE_BYTES, b_half = GATED ? lin_scalar(g.end.F * g.ldb) : 0;
-    const unsigned band_tiles = 8 * g.col_tiles, band_reciprocal = dl_uniform(0xFFFFFFFFu / band_tiles);  // (its product is short by one at most)
     bool inside = false;  // the offsets are those of a tile that ends at no edge
     const auto place = [&]() __attribute__((always_inline)) {
-        const int of_split = g.splits == 1 ? item : item % per;
-        const unsigned tile = xcd * per + of_split;
-        unsigned band = __umulhi(tile, band_reciprocal), in_band = tile - band * band_tiles;
-        if (in_band >= band_tiles) ++band, in_band -= band_tiles;
-        const unsigned band_rows = min(8, g.row_tiles - (int)band * 8), column = band_rows == 8 ? in_band / 8 : in_band / band_rows;
-        r0 = (int)(band * 8 + in_band - column * band_rows) * TR, c0 = (int)column * (GATED ? TC / 2 : TC);
         split = g.splits == 1 ? 0 : item / per, first = split * g.chunk, count = min(g.stages - first, g.chunk);
         tail = first + count - min(first + count, whole);  // 1: the reduction ends inside the last stage, which comes first
         const char *const a = g.A + (long long)r0 * (TURN_A ? In::SIZE : g.lda), *const b = g.B + (long long)c0 * (TURN_B ? In::SIZE : g.ldb);
         const uint64_t first_stage = first + (count - 1) * tail, second_stage = first + 1 - tail;
         a_first = lin_scalar((uint64_t)a + first_stage * a_step), a_second = lin_scalar((uint64_t)a + second_stage * a_step);
         b_first = lin_scalar((uint64_t)b + first_stage * b_step), b_second = lin_scalar((uint64_t)b + second_stage * b_step);
-        const int most = GATED ? g.end.F : g.end.C;
         const bool ends = r0 + TR > g.end.R || c0 + (GATED ? TC / 2 : TC) > most;
         if (inside && !ends) return;
         inside = !ends;
@@ -507,13 +514,13 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
     // Side work of a step, one piece after the other: fragments in the order in which the next step takes them (A's first, all of B, the rest of A)
     constexpr bool CUT = __is_same(In, LinF32);
     constexpr int FRAGMENTS = FA + FB, PA = LinReader<In, TR, TURN_A, FA>::PER, PB = LinReader<In, TC, TURN_B, FB>::PER;
-    constexpr int PIECES = CUT ? 5 * (FRAGMENTS + 1) : FA * PA + FB * PB, PRODUCTS = CUT ? 6 : 1, SLOTS = FA * FB * PRODUCTS;
+    constexpr int PIECES = CUT ? 6 * (FRAGMENTS + 1) : FA * PA + FB * PB, PRODUCTS = CUT ? 6 : 1, SLOTS = FA * FB * PRODUCTS;
     constexpr int READ_SLOTS = CUT ? SLOTS : SLOTS * 3 / 4;  // (the last reads are answered by the next step)
     float raw[2][8];
     const auto piece = [&](auto number, unsigned from_a, unsigned from_b, int step, int set) __attribute__((always_inline)) {
         constexpr int o = decltype(number)::value;
         if constexpr (CUT) {  // read a fragment, then cut the one before
-            constexpr int f = o / 5, r = o % 5, q = f - 1;
+            constexpr int f = o / 6, r = o % 6, q = f - 1;
             if constexpr (r == 0 && f < FRAGMENTS) {
                 if constexpr (f == 0 || f > FB) read_a.read_raw(lds + from_a, step, f == 0 ? 0 : f - FB, raw[f & 1]);
                 else read_b.read_raw(lds + from_b, step, f - 1, raw[f & 1]);
@@ -764,8 +771,176 @@ __global__ __launch_bounds__(256) void lin_join(LinArgs g, int splits) {
     }
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 64 rows of x, a token or some: what counts is that w is read once, at the memory's rate, by as many wavefronts as there are.  A wavefront takes
+// 16 rows of w (G times, gated: 16 of the gate and theirs of the other), straight into the registers as the matrix cores take them (four lanes read 64
+// bytes of a row); x comes out of the caches.  Of a block's eight wavefronts SHARING have the same rows, every one a step of 64 or 128 bytes in turn; their
+// sums are added in order in the LDS, and what follows is done there: one launch, no workspace, rows of any alignment.
+// Which of those: up to 16 always; up to 32 float32, but for few long rows of w, and of the others what w has up to 2^23 values of; up to 64 that and gated (x
+// serves gate and other), not float32.  (us, so and by tiles: bf16 8 x 1024 over 8192 6.8, 11.2, over 131072 52, 51; 32 x 1024 over 8192 8.1, 12.0,
+// over 32768 22, 18; gated 64 x 1024 over 2 x 4096 8.9, 11.7, not gated 14, 11; float32 32 x 1024 over 32768 37, 54, 32 x 4096 over 1024 24, 18.)
+static inline bool lin_few_rows(long long M, long long N, long long K, int size, bool gated) {
+    const bool small = N * K <= 1LL << 23 && K <= 2048;
+    return M <= 16 || (M <= 32 && (size == 4 ? K <= 2048 || N >= 4096 : small)) || (M <= 64 && gated && size < 4 && small);
+}
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+template <typename In>
+__device__ __forceinline__ floatx4 lin_mfma16(const LinFragment<In> &a, const LinFragment<In> &b, floatx4 c) {
+    if constexpr (__is_same(In, LinE4m3)) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(intx8, a), __builtin_bit_cast(intx8, b), c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+    } else if constexpr (__is_same(In, LinBf16)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else if constexpr (__is_same(In, LinF16)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+    } else {
+        constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 6; ++t)
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.w[PA[t]]), __builtin_bit_cast(bf16x8, b.w[PB[t]]), c, 0, 0, 0);
+        return c;
+    }
+}
+template <typename In, typename Out, int MT, int G, bool GATED, int SHARING>
+__global__ __launch_bounds__(512) void lin_few(LinArgs g) {
+    constexpr int WAVES = 8, Q = In::SIZE == 2 ? 1 : 2, STEP = 64 * Q, ROOM = (MT == 1 ? 12 : 8) / (Q * (G + MT)), U = ROOM > 4 ? 4 : ROOM > 1 ? ROOM : 1;  // steps asked for at once: two such sets fit the registers
+    __shared__ float sums[WAVES][G][MT][256];
+    struct Raw { uint32_t w[4 * Q]; };
+    const int lane = threadIdx.x & 63, wave = dl_uniform(threadIdx.x >> 6), row = lane & 15, unit = (lane >> 4) * 16;
+    constexpr int H = GATED ? 1 : G;
+    constexpr int GROUPS = WAVES / SHARING;
+    const int part = wave % SHARING, group = wave / SHARING, width = GATED ? g.end.F : g.end.C;
+    const long long n_first = (long long)blockIdx.x * GROUPS * 16 * H;
+    const int n0 = (int)(n_first + group * 16 * H < width ? n_first + group * 16 * H : width - 1);  // (wavefronts without rows go along: there is a barrier)
+    const char *w[G], *x[MT];
+#pragma unroll
+    for (int i = 0; i < G; ++i) w[i] = g.B + (long long)(GATED ? i * g.end.F + min(n0 + row, width - 1) : min(n0 + 16 * i + row, width - 1)) * g.ldb;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) x[t] = g.A + (long long)min(16 * t + row, g.end.R - 1) * g.lda;
+    const long long bytes = g.K * In::SIZE;
+    const int whole = (int)(bytes / STEP);
+    const auto fetch = [&](const char *from, int step, Raw &to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) __builtin_memcpy(to.w + 4 * q, from + (long long)step * STEP + q * 64 + unit, 16);  // (of any alignment)
+    };
+    const auto fragment = [&](const Raw &from) __attribute__((always_inline)) {
+        LinFragment<In> f;
+        if constexpr (__is_same(In, LinF32)) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(from.w[i]);
+#pragma unroll
+            for (int part = 0; part < 5; ++part) lin_cut(v, part, f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4 * Q; ++i) f.w[0][i] = (int)from.w[i];
+        }
+        return f;
+    };
+    floatx4 acc[G][MT];
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[i][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto multiply = [&](const Raw (&rw)[G], const Raw (&rx)[MT]) __attribute__((always_inline)) {
+        LinFragment<In> fw[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) fw[i] = fragment(rw[i]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const LinFragment<In> fx = fragment(rx[t]);
+#pragma unroll
+            for (int i = 0; i < G; ++i) acc[i][t] = lin_mfma16<In>(fw[i], fx, acc[i][t]);
+        }
+    };
+    Raw rw[2][U][G], rx[2][U][MT];
+    const auto batch = [&](int step, int set) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = step + u * SHARING;
+            if (at < whole) {
+#pragma unroll
+                for (int i = 0; i < G; ++i) fetch(w[i], at, rw[set][u][i]);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) fetch(x[t], at, rx[set][u][t]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < G; ++i) rw[set][u][i] = Raw{};
+#pragma unroll
+                for (int t = 0; t < MT; ++t) rx[set][u][t] = Raw{};
+            }
+        }
+    };
+    batch(part, 0);
+    for (int step = part; step < whole; step += 2 * U * SHARING) {
+        batch(step + U * SHARING, 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(rw[0][u], rx[0][u]);
+        batch(step + 2 * U * SHARING, 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(rw[1][u], rx[1][u]);
+    }
+    if (whole * (long long)STEP < bytes && whole % SHARING == part) {  // the reduction ends inside a step: value by value
+        Raw tw[G], tx[MT];
+        const auto some = [&](const char *from, Raw &to) __attribute__((always_inline)) {
+            to = Raw{};
+#pragma unroll
+            for (int e = 0; e < 16 * Q / In::SIZE; ++e) {
+                const long long at = (long long)whole * STEP + e * In::SIZE / 16 * 64 + unit + e * In::SIZE % 16;
+                if (at >= bytes) continue;
+                uint32_t v = 0;
+                __builtin_memcpy(&v, from + at, In::SIZE);
+                to.w[e * In::SIZE / 4] |= v << (e * In::SIZE % 4 * 8);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < G; ++i) some(w[i], tw[i]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) some(x[t], tx[t]);
+        multiply(tw, tx);
+    }
+    // a lane has x's row lane % 16, and of w's four from 4 (lane / 16) on
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) *reinterpret_cast<floatx4 *>(&sums[wave][i][t][lane * 4]) = acc[i][t];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 256 * MT * H * GROUPS; e += 512) {
+        const int n = e % (16 * H * GROUPS), m = e / (16 * H * GROUPS), i = n / 16 % H, from = n / (16 * H) * SHARING, at = (n % 16 / 4 * 16 + m % 16) * 4 + n % 4;
+        float v = 0.0f, u = 0.0f;
+        for (int q = 0; q < SHARING; ++q) {
+            v += sums[from + q][i][m / 16][at];
+            if (GATED) u += sums[from + q][G - 1][m / 16][at];
+        }
+        if (n_first + n < width) lin_finish_one<Out, GATED>(g.end, m, (int)n_first + n, v, u);
+    }
+}
+template <typename In, typename Out>
+static int lin_launch_few(LinArgs &g, bool gated, hipStream_t s) {
+    const int width = gated ? g.end.F : g.end.C, rows = g.end.R;
+    // 32 rows of w a wavefront where x has more than 16 (its loads serve both) or 1024 have some; two to share them instead of eight where eight would
+    // have less than four steps each and 512 blocks are left
+    const bool pairs = !gated && (rows > 16 || width >= 1024 * 32);
+    const int rows_each = pairs ? 32 : 16;
+    const bool two = g.K * In::SIZE < 32 * (In::SIZE == 2 ? 64 : 128) && width >= 512 * 4 * rows_each;
+    const long long blocks = dl_ceil_div(width, rows_each * (two ? 4 : 1));
+    if (!dl_grid_ok(blocks, 512)) return DL_ERR_UNSUPPORTED;
+#define LIN_FEW_GO(MT, G, GATED, SHARING) hipLaunchKernelGGL((lin_few<In, Out, MT, G, GATED, SHARING>), dim3((unsigned)blocks), dim3(512), 0, s, g)
+#define LIN_FEW_ROWS(SHARING) \
+    do { \
+        if (gated) { if (rows <= 16) LIN_FEW_GO(1, 2, true, SHARING); else if (rows <= 32) LIN_FEW_GO(2, 2, true, SHARING); else if constexpr (In::SIZE < 4) LIN_FEW_GO(4, 2, true, SHARING); } \
+        else if (rows > 16) LIN_FEW_GO(2, 2, false, SHARING); \
+        else if (pairs) LIN_FEW_GO(1, 2, false, SHARING); \
+        else LIN_FEW_GO(1, 1, false, SHARING); \
+    } while (0)
+    DL_TIMED("lin_few", s, if (two) LIN_FEW_ROWS(2); else LIN_FEW_ROWS(8));
+#undef LIN_FEW_ROWS
+#undef LIN_FEW_GO
+    return DL_OK;
+}
+
 // ------------------------------------------------------------------ launches
 struct LinPlan {
+    bool few;    // by lin_few
     int tile;
     int splits, chunk;  // parts of the reduction, and their stages
     size_t a_bytes, b_bytes, part_bytes;
@@ -810,6 +985,7 @@ static int lin_launch(LinArgs &g, const LinPlan &p, bool gated, hipStream_t s) {
 // (forward: neither is turned; gx: the second; gw: both)
 template <typename In, typename Out>
 static int lin_launch_turned(LinArgs &g, const LinPlan &p, bool turn_a, bool turn_b, bool gated, hipStream_t s) {
+    if (p.few) return lin_launch_few<In, Out>(g, gated, s);
     if (turn_a) return lin_launch<In, Out, true, true>(g, p, gated, s);
     return turn_b ? lin_launch<In, Out, false, true>(g, p, gated, s) : lin_launch<In, Out, false, false>(g, p, gated, s);
 }

@@ -3,6 +3,6 @@
 
 int lin_launch_e4m3(LinArgs &g, const LinPlan &p, int out_type, bool gated, hipStream_t s) {
     int code = DL_ERR_UNSUPPORTED;
-    DL_BY_TYPE(out_type, Out, (code = lin_launch<LinE4m3, Out, false, false>(g, p, gated, s)));
+    DL_BY_TYPE(out_type, Out, (code = p.few ? lin_launch_few<LinE4m3, Out>(g, gated, s) : lin_launch<LinE4m3, Out, false, false>(g, p, gated, s)));
     return code;
 }

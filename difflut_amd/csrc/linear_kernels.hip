@@ -116,10 +116,15 @@ static size_t lin_operand_bytes(const LinOperand &o, int type) {
 // 1.55 us, the two blocks of 128 x 128 that share a CU 0.95, one that has it alone 0.6 (float32: three times that); a tile's beginning and end
 // take 5 and 3 us; sums are written and read at 4 bytes/ps, with 4 us for the launch that joins them.  (bf16, 8192^3: 256 787 us, 128 970; 1024 x 4096 over
 // 12544, us with the join: 256 in 4 parts 98, 128 in 2 parts 104, 256 whole 360.)
-static LinPlan lin_plan(const LinOperand &a, const LinOperand &b, int type, long long K) {
+static LinPlan lin_plan(const LinOperand &a, const LinOperand &b, int type, long long K, bool gated) {
     LinPlan p;
     const long long R = a.count(), C = b.count(), stages = (K * lin_size(type) + LIN_STAGE_BYTES - 1) / LIN_STAGE_BYTES;
-    p.a_bytes = lin_operand_bytes(a, type), p.b_bytes = lin_operand_bytes(b, type);
+    p.a_bytes = lin_operand_bytes(a, type), p.b_bytes = lin_operand_bytes(b, type), p.part_bytes = 0;
+    p.few = !a.turned && !b.turned && lin_few_rows(R, C, K, lin_size(type), gated);
+    if (p.few) {
+        p.a_bytes = p.b_bytes = 0, p.tile = 0, p.splits = p.chunk = 1;
+        return p;
+    }
     double best = 1e30;
     for (int tile = 128; tile <= 256; tile += 128) {
         const double tiles = (double)((R + tile - 1) / tile) * (double)((C + tile - 1) / tile), slots = tile == 256 ? LIN_CUS : 2 * LIN_CUS;
@@ -156,18 +161,18 @@ static const char *lin_lay_out(const LinOperand &o, int type, void *room, long l
 
 // One product: operands laid out, tiles, what follows
 static int lin_run(const LinOperand &a, const LinOperand &b, int type, int out_type, long long K, bool gated, LinEnd end, char *ws, hipStream_t s) {
-    LinPlan p = lin_plan(a, b, type, K);
+    LinPlan p = lin_plan(a, b, type, K, gated);
     LinArgs g{};
-    g.A = lin_lay_out(a, type, ws, g.lda, s);
-    g.B = lin_lay_out(b, type, ws + p.a_bytes, g.ldb, s);
-    if (g.lda > LIN_MOST_ROW || g.ldb > LIN_MOST_ROW) return DL_ERR_UNSUPPORTED;
+    if (p.few) g.A = (const char *)a.p, g.lda = a.ld * lin_size(type), g.B = (const char *)b.p, g.ldb = b.ld * lin_size(type);
+    else g.A = lin_lay_out(a, type, ws, g.lda, s), g.B = lin_lay_out(b, type, ws + p.a_bytes, g.ldb, s);
+    if (!p.few && (g.lda > LIN_MOST_ROW || g.ldb > LIN_MOST_ROW)) return DL_ERR_UNSUPPORTED;
     g.part = (float *)(ws + p.a_bytes + p.b_bytes);
     end.R = (int)a.count(), end.C = (int)b.count(), end.F = end.C / 2;
     const int width = gated ? end.F : end.C, size = dl_type_bytes(out_type);
     end.vec = width % 8 == 0 && dl_aligned16(end.y) && dl_aligned16(end.z) && dl_aligned16(end.bias) && dl_aligned16(end.res) && dl_aligned16(end.col_scale) && end.ldr * size % 16 == 0;
     if (p.splits == 1 && !end.vec && !b.turned) p.tile = 128;  // (value by value: the smaller tile alone)
     g.K = K, g.stages = dl_ceil_div(K * lin_size(type), LIN_STAGE_BYTES), g.chunk = p.chunk, g.splits = p.splits;
-    g.row_tiles = dl_ceil_div(end.R, p.tile), g.col_tiles = gated && p.splits == 1 ? dl_ceil_div(end.F, p.tile / 2) : dl_ceil_div(end.C, p.tile);
+    if (!p.few) g.row_tiles = dl_ceil_div(end.R, p.tile), g.col_tiles = gated && p.splits == 1 ? dl_ceil_div(end.F, p.tile / 2) : dl_ceil_div(end.C, p.tile);
     g.end = end;
     int code = DL_ERR_UNSUPPORTED;
     if (type == DL_E4M3) code = lin_launch_e4m3(g, p, out_type, gated, s);
@@ -189,7 +194,7 @@ static int lin_check(int type, int out_type, long long M, long long N, long long
 extern "C" size_t dl_linear_fwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, int type, long long M, long long N, long long K,
                                                 int gated) {
     if (lin_check(type, type == DL_E4M3 ? DL_F32 : type, M, N, K, 0, gated) != DL_OK) return 0;
-    return lin_plan({x, ldx, M, K, false}, {w, ldw, N, K, false}, type, K).bytes();
+    return lin_plan({x, ldx, M, K, false}, {w, ldw, N, K, false}, type, K, gated != 0).bytes();
 }
 
 extern "C" int dl_linear_fwd(const void *x, long long ldx, const float *x_scale, const void *w, long long ldw, const float *w_scale, const void *bias,
@@ -217,14 +222,16 @@ static LinBack lin_back(const LinOperand &gz, const LinOperand &x, const LinOper
     LinBack b{};
     const long long M = gz.rows;
     b.gz = kept ? dl_align256((size_t)M * (size_t)N * lin_size(type)) : 0;
-    b.rows = LIN_SLOPE_ROWS;
-    while ((M + b.rows - 1) / b.rows > 1024) b.rows *= 2;
+    // rows of a block: from one a team up, as few as leave 1024 blocks or fewer over the columns (vectors of 16 bytes)
+    const long long across = (N + 64 * (16 / lin_size(type)) - 1) / (64 * (16 / lin_size(type)));
+    b.rows = 4;
+    while ((M + b.rows - 1) / b.rows * across > 1024 && (b.rows < LIN_SLOPE_ROWS || (M + b.rows - 1) / b.rows > 1024)) b.rows *= 2;
     b.pieces = dl_ceil_div(M, b.rows);
     b.shares = wants & 4 ? dl_align256((size_t)b.pieces * (size_t)N * 4) : 0;
     const LinOperand gt = {gz.p, gz.ld, M, N, true}, wt = {w.p, w.ld, N, K, true}, xt = {x.p, x.ld, M, K, true};
-    if (wants & 1) b.products = lin_plan(gz, wt, type, N).bytes();
+    if (wants & 1) b.products = lin_plan(gz, wt, type, N, false).bytes();
     if (wants & 2) {
-        const size_t n = lin_plan(gt, xt, type, M).bytes();
+        const size_t n = lin_plan(gt, xt, type, M, false).bytes();
         if (n > b.products) b.products = n;
     }
     return b;

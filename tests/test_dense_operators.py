@@ -647,10 +647,10 @@ def test_c_entry_points_refuse():
 
     def linear(x=p, ldx=64, sx=0, w=p, ldw=64, sw=0, r=0, ldr=0, y=p, t=1, ot=1, M=4, N=8, K=64, act=0, gated=0, ws=p, size=1 << 30):
         return lib.dl_linear_fwd(x, ldx, sx, w, ldw, sw, None, r, ldr, y, None, t, ot, M, N, K, act, gated, ws, size, None)
-    assert [linear(x=0), linear(w=0), linear(y=0), linear(sx=p), linear(t=3), linear(t=3, sx=p), linear(ldx=72, x=p + 2, ws=0)] == [NULL] * 7
+    assert [linear(x=0), linear(w=0), linear(y=0), linear(sx=p), linear(t=3), linear(t=3, sx=p), linear(ldx=72, x=p + 2, ws=0, M=100)] == [NULL] * 7
     assert [linear(M=0), linear(N=0), linear(K=0), linear(ldx=63), linear(ldw=63), linear(gated=1, N=7), linear(r=p, ldr=7), linear(M=2 ** 31)] == [SHAPE] * 8
     assert [linear(t=5), linear(ot=0), linear(t=3, sx=p, sw=p, ot=3), linear(act=4), linear(K=2 ** 22 + 8, ldx=2 ** 23, ldw=2 ** 23)] == [UNSUPPORTED] * 5
-    assert linear(x=p + 2, size=16) == WORKSPACE and linear(x=p + 2, ws=p + 4) == WORKSPACE
+    assert linear(x=p + 2, size=16, M=100) == WORKSPACE and linear(x=p + 2, ws=p + 4, M=100) == WORKSPACE
 
     def linear_back(x=p, ldx=64, w=p, ldw=64, z=p, gy=p, gx=p, gw=p, gb=p, t=1, M=4, N=8, K=64, act=2, gated=0, ws=p, size=1 << 30):
         return lib.dl_linear_bwd(x, ldx, w, ldw, z, gy, gx, gw, gb, t, M, N, K, act, gated, ws, size, None)
