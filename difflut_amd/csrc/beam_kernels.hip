@@ -3,22 +3,25 @@
 //   candidate (k, v) of a sequence:  c = scores[k] + logits[k, v] - log sum_u exp(logits[k, u]);  a beam that has ended: (k, end) alone, c = scores[k]
 //   the `count` largest, equal ones by k, then v
 //
-// The best of all are among the best `count` logits of each beam.  One pass over the logits: a block takes a row or a piece of one in
-// rounds of BEAM_ROUND, keeps the running maximum and sum of the softmax (float within a round, double over rounds) and a list of what
-// may be among the best in the LDS.  The first round bounds them from below - of the threads' largest logits the count-th is passed by
-// `count` values at least - later ones append what passes the bound, a few values a round; a list that grows is cut to the best
-// and the bound raised to the last of these.  A second launch joins the pieces and picks among the rows' lists.
+// The best of all are among the best `count` logits of each beam.  One pass over the logits: a block takes a row or a piece of one, each of its
+// wavefronts in rounds of BEAM_ROUND / 4 values, without waiting for the others.  A thread keeps the sum of the softmax (float within a round,
+// double over rounds) on a maximum that it changes only where a logit lies far above; a wavefront keeps a list of what may be among
+// the best in the LDS.  The first round bounds them from below - the count-th of the lanes' largest logits is passed by `count` values at
+// least - later ones append what passes the bound, a few values a round; a list that grows is cut and the bound raised.  The thresholds are
+// searched bit by bit, with a ballot for a count.  A second launch joins the pieces and picks among the rows' lists.
 // Values are compared as doubles, c from double logarithms, so that neighbours of different beams stand in the right order.
 #include "dl_types.h"
 
 #define BEAM_THREADS 256
+#define BEAM_WAVES 4
 #define BEAM_PER_THREAD 16
 #define BEAM_ROUND (BEAM_THREADS * BEAM_PER_THREAD)
-#define BEAM_CUT 512       // list length from which it is cut
-#define BEAM_RANK 1024     // list length up to which ranks are counted
+#define BEAM_CUT 128       // length from which a wavefront's list is cut, at most
+#define BEAM_LIST (BEAM_CUT + 64 * 8)  // and what eight values a lane may append
 #define BEAM_MOST 64       // beams, and answers
 #define BEAM_PICKS 4096    // candidates that the second launch takes
 #define BEAM_LOG2E 1.44269504f
+#define BEAM_LOWEST 0x00800000u  // the order of the lowest number; below it is -infinity's
 
 typedef unsigned long long beam_key;  // the logit's order above, the index's order (lowest first) below; 0: none
 
@@ -52,23 +55,61 @@ struct BeamArgs {
     int B, K, V, count, pieces, piece;
 };
 
-// The best `count` of the list's n keys, in order, to out (LDS or device memory; past n: 0).  Every thread of the block; the list is left as it was.
-__device__ void beam_select(const beam_key *list, int n, int count, beam_key *out, beam_key *best) {
-    const int tid = threadIdx.x;
-    if (n <= BEAM_RANK) {  // every key counts the better ones
-        for (int e = tid; e < n; e += BEAM_THREADS) {
-            const beam_key mine = list[e];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > mine ? 1 : 0;
-            if (rank < count) out[rank] = mine;
-        }
-        for (int e = n + tid; e < count; e += BEAM_THREADS) out[e] = 0;
-        return;
+__device__ __forceinline__ uint32_t beam_order(beam_key k) { return (uint32_t)(k >> 32); }
+// the largest T of which BITS from the top may be set with `count` lanes or more whose values (V a lane) reach it; 0 where there are fewer
+template <int BITS, int V>
+__device__ __forceinline__ uint32_t beam_threshold(const uint32_t (&order)[V], int count) {
+    uint32_t t = 0;
+#pragma unroll 4
+    for (int bit = 31; bit > 31 - BITS; --bit) {
+        const uint32_t higher = t | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) n += __popcll(__ballot(order[i] >= higher));
+        if (n >= count) t = higher;
     }
-    beam_key below = ~0ull;  // the largest below the last one found, `count` times
+    return t;
+}
+// a wavefront's own LDS reads and writes, in the order written
+__device__ __forceinline__ void beam_in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// A wavefront's list of n keys, cut: to those that reach the count-th value, or where these are too many (equal ones, a long list) to exactly
+// `count`.  Returns how many; `past`: keys up to it are out.
+__device__ int beam_shorten(beam_key *list, int n, int count, int most, beam_key &past) {
+    const int lane = threadIdx.x & 63;
+    if (n <= 256) {
+        beam_key mine[4];
+        uint32_t order[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = i * 64 + lane;
+            mine[i] = e < n ? list[e] : 0;
+            order[i] = beam_order(mine[i]);
+        }
+        const uint32_t t = beam_threshold<32>(order, count);
+        int kept = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kept += __popcll(__ballot(mine[i] != 0 && order[i] >= t));
+        if (kept <= most) {
+            beam_in_order();
+            int at = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool keep = mine[i] != 0 && order[i] >= t;
+                const unsigned long long those = __ballot(keep);
+                if (keep) list[at + __popcll(those & ((1ull << lane) - 1))] = mine[i];
+                at += __popcll(those);
+            }
+            beam_in_order();
+            if (((beam_key)t << 32) > past + 1) past = ((beam_key)t << 32) - 1;  // (lower values are out)
+            return kept;
+        }
+    }
+    // the largest below the last one found, `count` times; they take the places that it has passed
+    beam_key below = ~0ull, first = 0;
     for (int k = 0; k < count; ++k) {
         beam_key mine = 0;
-        for (int e = tid; e < n; e += BEAM_THREADS) {
+        for (int e = lane; e < n; e += 64) {
             const beam_key v = list[e];
             if (v < below && v > mine) mine = v;
         }
@@ -77,30 +118,32 @@ __device__ void beam_select(const beam_key *list, int n, int count, beam_key *ou
             const beam_key v = __shfl_xor(mine, o);
             mine = v > mine ? v : mine;
         }
-        if ((tid & 63) == 0) best[tid >> 6] = mine;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < BEAM_THREADS / 64; ++w) mine = best[w] > mine ? best[w] : mine;
-        __syncthreads();
-        if (tid == 0) out[k] = mine;
         below = mine;
+        if (lane == k) first = mine;  // (count is 64 at most)
     }
+    beam_in_order();
+    if (lane < count) list[lane] = first;
+    beam_in_order();
+    past = below;
+    return count;
 }
 
 template <typename T, int E>
 __global__ __launch_bounds__(BEAM_THREADS) void beam_rows(BeamArgs g) {
     constexpr int Q = BEAM_PER_THREAD / E;
-    __shared__ beam_key list[BEAM_CUT + BEAM_ROUND], chosen[BEAM_MOST], best[BEAM_THREADS / 64];
-    __shared__ float tops[BEAM_THREADS], bound_of;
-    __shared__ double sums[BEAM_THREADS / 64];
-    __shared__ int length;
-    const int tid = threadIdx.x;
+    __shared__ beam_key lists[BEAM_WAVES][BEAM_LIST];
+    __shared__ __align__(16) beam_key merged[BEAM_WAVES * BEAM_CUT];
+    __shared__ float tops[BEAM_WAVES];
+    __shared__ double sums[BEAM_WAVES];
+    __shared__ int lengths[BEAM_WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = dl_uniform(tid >> 6);
     const long long row = blockIdx.x / g.pieces;
     const int piece = blockIdx.x % g.pieces;
     if (g.ended && g.ended[row]) return;
     const T *logits = (const T *)g.logits + row * g.ldl;
-    const int v0 = piece * g.piece, v1 = min(v0 + g.piece, g.V);
+    const int v0 = piece * g.piece, v1 = min(v0 + g.piece, g.V), most = g.count <= 32 ? 64 : BEAM_CUT;
     const float inf = __builtin_inff();
+    beam_key *list = lists[wave];
 
     float next[Q][E];
     auto fetch = [&](int at) __attribute__((always_inline)) {
@@ -113,10 +156,10 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows(BeamArgs g) {
                 for (int i = 0; i < E; ++i) next[q][i] = -inf;
         }
     };
-    if (tid == 0) length = 0;
-    float largest = -inf, bound = -inf;
-    beam_key past = 0;  // keys up to it are out
+    float ref = -inf, bound = -inf;  // of the thread's sum; of the wavefront's list
+    beam_key past = 0;
     double sum = 0.0;
+    int length = 0;
     fetch(v0);
     for (int at = v0; at < v1; at += BEAM_ROUND) {
         float v[Q][E], top = -inf;
@@ -124,152 +167,204 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows(BeamArgs g) {
         for (int q = 0; q < Q; ++q)
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float x = next[q][i];
-                v[q][i] = x != x ? -inf : fminf(x, 3.4028234663852886e38f);  // NaN: no candidate; infinity: the largest number
+                v[q][i] = fminf(fmaxf(next[q][i], -inf), 3.4028234663852886e38f);  // NaN: no candidate; infinity: the largest number
                 top = fmaxf(top, v[q][i]);
             }
         if (at + BEAM_ROUND < v1) fetch(at + BEAM_ROUND);
-        if (top > largest) {
-            sum *= (double)__builtin_amdgcn_exp2f((largest - top) * BEAM_LOG2E);
-            largest = top;
+        if (top > ref + 8.0f || (ref == -inf && top > -inf)) {  // (no higher, as the exponent's rounding grows with it)
+            sum *= ref == -inf ? 0.0 : exp((double)ref - (double)top);
+            ref = top;
         }
-        if (largest > -inf) {
+        if (ref > -inf) {
             float part = 0.0f;
 #pragma unroll
             for (int q = 0; q < Q; ++q)
 #pragma unroll
-                for (int i = 0; i < E; ++i) part += __builtin_amdgcn_exp2f((v[q][i] - largest) * BEAM_LOG2E);
+                for (int i = 0; i < E; ++i) part += __builtin_amdgcn_exp2f((v[q][i] - ref) * BEAM_LOG2E);
             sum += (double)part;
         }
         if (at == v0) {
-            tops[tid] = top;
-            if (tid == 0) bound_of = -inf;
-            __syncthreads();
-            int rank = 0;
-            for (int j = 0; j < BEAM_THREADS; ++j) rank += tops[j] > top || (tops[j] == top && j < tid) ? 1 : 0;
-            if (rank == g.count - 1) bound_of = top;
-            __syncthreads();
-            bound = bound_of;
+            const uint32_t order[1] = {beam_order(beam_make(top, 0))}, t = beam_threshold<20>(order, g.count);
+            if (t >= BEAM_LOWEST) bound = beam_value((beam_key)t << 32);
         }
-        if (top >= bound && top > -inf) {
+        if (!__ballot(top >= bound && top > -inf)) continue;
 #pragma unroll
-            for (int q = 0; q < Q; ++q)
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    if (!(v[q][i] >= bound && v[q][i] > -inf)) continue;
-                    const beam_key key = beam_make(v[q][i], (uint32_t)(at + (q * BEAM_THREADS + tid) * E + i));
-                    if (key > past) list[atomicAdd(&length, 1)] = key;
-                }
-        }
-        __syncthreads();
-        const int n = length;
-        __syncthreads();
-        if (n > BEAM_CUT) {  // (then there are more than `count`)
-            beam_select(list, n, g.count, chosen, best);
-            __syncthreads();
-            if (tid < g.count) list[tid] = chosen[tid];
-            past = chosen[g.count - 1], bound = beam_value(past);
-            if (tid == 0) length = g.count;
-            __syncthreads();
+        for (int e = 0; e < BEAM_PER_THREAD; ++e) {
+            const int q = e / E, i = e % E;
+            if (__ballot(v[q][i] >= bound)) {
+                const beam_key key = beam_make(v[q][i], (uint32_t)(at + (q * BEAM_THREADS + tid) * E + i));
+                const bool in = v[q][i] >= bound && v[q][i] > -inf && key > past;
+                const unsigned long long those = __ballot(in);
+                if (in) list[length + __popcll(those & ((1ull << lane) - 1))] = key;
+                length += __popcll(those);
+            }
+            if (e % 8 == 7 && length > most) {  // (then there are more than `count`)
+                beam_in_order();
+                length = beam_shorten(list, length, g.count, most, past);
+                const float last = beam_value(past + 1);
+                bound = last > bound ? last : bound;
+            }
         }
     }
-    const int n = length;
-    beam_select(list, n, g.count, g.keys + (row * g.pieces + piece) * g.count, best);
+
+    // the wavefronts' lists are one; every key counts the better ones
+    if (lane == 0) lengths[wave] = length;
+    __syncthreads();
+    int before = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < BEAM_WAVES; ++w) {
+        before += w < wave ? lengths[w] : 0;
+        n += lengths[w];
+    }
+    for (int e = lane; e < length; e += 64) merged[before + e] = list[e];
+    if (tid == 0 && (n & 1)) merged[n] = 0;  // (n is odd: below the end)
+    __syncthreads();
+    beam_key *out = g.keys + (row * g.pieces + piece) * g.count;
+    for (int e = tid; e < n; e += BEAM_THREADS) {
+        const beam_key mine = merged[e];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(merged + j);
+            rank += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+        }
+        if (rank < g.count) out[rank] = mine;
+    }
+    for (int e = n + tid; e < g.count; e += BEAM_THREADS) out[e] = 0;
 
     // the threads' sums, on one maximum, in a fixed order
-    float most = largest;
+    float largest = ref;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-    __syncthreads();
-    if ((tid & 63) == 0) tops[tid >> 6] = most;
+    for (int o = 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor(largest, o));
+    if (lane == 0) tops[wave] = largest;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < BEAM_THREADS / 64; ++w) most = fmaxf(most, tops[w]);
-    sum = largest > -inf ? sum * exp((double)largest - (double)most) : 0.0;
+    for (int w = 0; w < BEAM_WAVES; ++w) largest = fmaxf(largest, tops[w]);
+    sum = ref > -inf ? sum * exp((double)ref - (double)largest) : 0.0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if ((tid & 63) == 0) sums[tid >> 6] = sum;
+    if (lane == 0) sums[wave] = sum;
     __syncthreads();
     if (tid == 0) {
         sum = 0.0;
-        for (int w = 0; w < BEAM_THREADS / 64; ++w) sum += sums[w];
-        g.parts[row * g.pieces + piece] = {sum, most, 0};
+        for (int w = 0; w < BEAM_WAVES; ++w) sum += sums[w];
+        g.parts[row * g.pieces + piece] = {sum, largest, 0};
     }
 }
 
-// A block of THREADS takes a sequence's K * pieces * count candidates.
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void beam_pick(BeamArgs g) {
-    __shared__ double value[BEAM_PICKS], norm[BEAM_MOST], wave_value[THREADS / 64];
-    __shared__ int wave_at[THREADS / 64];
-    const int tid = threadIdx.x, b = blockIdx.x, per = g.pieces * g.count, n = g.K * per;
+// A block takes a sequence's K * pieces lists of `count` candidates, best first.  The count-th of the lists' best bounds them from below, where
+// there are as many lists; every candidate that passes it counts the better ones.
+#define BEAM_RANKS 1024  // candidates that are ranked; from more the best is taken `count` times
+__device__ __forceinline__ bool beam_before(double a, int at, double b, int bt) { return a > b || (a == b && at < bt); }
+__global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
+    __shared__ double value[BEAM_PICKS], norm[BEAM_MOST], base[BEAM_MOST], wave_value[BEAM_WAVES], bound;
+    __shared__ double kept_value[BEAM_RANKS];
+    __shared__ int kept_at[BEAM_RANKS], wave_at[BEAM_WAVES], kept, ended[BEAM_MOST];
+    const int tid = threadIdx.x, b = blockIdx.x, per = g.pieces * g.count, n = g.K * per, lists = g.K * g.pieces;
     const double inf = __builtin_inf();
+    const beam_key *keys = g.keys + (long long)b * n;
+
+    // the rows' logarithms: every list's share of its row's sum (in `value`), then a thread a row
+    const BeamPart *parts = g.parts + (long long)b * lists;
     if (tid < g.K) {
         const long long row = (long long)b * g.K + tid;
-        double result = inf;  // nothing to go on with
-        if (!(g.ended && g.ended[row])) {
-            const BeamPart *p = g.parts + row * g.pieces;
-            float most = -__builtin_inff();
-            for (int i = 0; i < g.pieces; ++i) most = fmaxf(most, p[i].largest);
-            if (most > -__builtin_inff()) {
-                double sum = 0.0;
-                for (int i = 0; i < g.pieces; ++i)
-                    if (p[i].sum > 0.0) sum += p[i].sum * exp((double)p[i].largest - (double)most);
-                result = (double)most + log(sum);
-            }
-        }
-        norm[tid] = result;
+        ended[tid] = g.ended && g.ended[row] ? 1 : 0;
+        base[tid] = (double)g.scores[row];
+    }
+    if (tid == 0) kept = 0, bound = -inf;
+    __syncthreads();
+    for (int e = tid; e < lists; e += BEAM_THREADS) {
+        const int k = e / g.pieces;
+        if (ended[k]) continue;
+        float most = -__builtin_inff();
+        for (int i = 0; i < g.pieces; ++i) most = fmaxf(most, parts[k * g.pieces + i].largest);
+        const BeamPart p = parts[e];
+        value[e] = p.sum > 0.0 ? p.sum * exp((double)p.largest - (double)most) : 0.0;
+        if (e % g.pieces == 0) norm[k] = (double)most;
     }
     __syncthreads();
-    const beam_key *keys = g.keys + (long long)b * n;
-    double mine = -inf;
-    int mine_at = n;
-    for (int e = tid; e < n; e += THREADS) {
+    if (tid < g.K && !ended[tid]) {
+        double sum = 0.0;
+        for (int i = 0; i < g.pieces; ++i) sum += value[tid * g.pieces + i];
+        norm[tid] = norm[tid] > -inf ? norm[tid] + log(sum) : inf;  // (infinity: nothing to go on with)
+    }
+    __syncthreads();
+    for (int e = tid; e < n; e += BEAM_THREADS) {
         const int k = e / per;
-        const long long row = (long long)b * g.K + k;
         double c = -inf;
-        if (g.ended && g.ended[row]) {
-            if (e == k * per) c = (double)g.scores[row];
+        if (ended[k]) {
+            if (e == k * per) c = base[k];
         } else {
             const beam_key key = keys[e];
-            if (key) c = (double)g.scores[row] + ((double)beam_value(key) - norm[k]);
+            if (key) c = base[k] + ((double)beam_value(key) - norm[k]);
         }
-        if (c != c) c = -inf;
-        value[e] = c;
-        if (c > mine) mine = c, mine_at = e;
+        value[e] = c == c ? c : -inf;
     }
-    for (int j = 0; j < g.count; ++j) {
-        // the largest, the first of equal ones
+    __syncthreads();
+    if (lists >= g.count && lists <= 2 * BEAM_THREADS)
+        for (int e = tid; e < lists; e += BEAM_THREADS) {
+            const double mine = value[e * g.count];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < lists; ++j) rank += beam_before(value[j * g.count], j, mine, e) ? 1 : 0;
+            if (rank == g.count - 1) bound = mine;
+        }
+    __syncthreads();
+    const double least = bound;
+    for (int e = tid; e < n; e += BEAM_THREADS) {
+        const double c = value[e];
+        if (!(c >= least && c > -inf)) continue;
+        const int at = atomicAdd(&kept, 1);  // (their order plays no part)
+        if (at < BEAM_RANKS) kept_value[at] = c, kept_at[at] = e;
+    }
+    __syncthreads();
+    const auto answer = [&](int j, double c, int at) __attribute__((always_inline)) {
+        const long long out = (long long)b * g.count + j;
+        const int k = at < 0 ? 0 : at / per;
+        g.out_scores[out] = (float)c;
+        g.parents[out] = k;
+        g.tokens[out] = at < 0 ? -1 : ended[k] ? g.end : (long long)beam_index(keys[at]);
+    };
+    const int m = kept;
+    for (int j = m + tid; j < g.count; j += BEAM_THREADS) answer(j, -inf, -1);
+    if (m <= BEAM_RANKS) {
+        for (int e = tid; e < m; e += BEAM_THREADS) {
+            const double mine = kept_value[e];
+            const int at = kept_at[e];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < m; ++j) rank += beam_before(kept_value[j], kept_at[j], mine, at) ? 1 : 0;
+            if (rank < g.count) answer(rank, mine, at);
+        }
+        return;
+    }
+    double mine = -inf;
+    int mine_at = n;
+    const auto own_best = [&]() __attribute__((always_inline)) {
+        mine = -inf, mine_at = n;
+        for (int e = tid; e < n; e += BEAM_THREADS)
+            if (value[e] > mine) mine = value[e], mine_at = e;
+    };
+    own_best();
+    for (int j = 0; j < g.count; ++j) {  // (there are more than `count` above -infinity)
         double best = mine;
         int at = mine_at;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             const double v = __shfl_xor(best, o);
             const int w = __shfl_xor(at, o);
-            if (v > best || (v == best && w < at)) best = v, at = w;
+            if (beam_before(v, w, best, at)) best = v, at = w;
         }
-        if (THREADS > 64) {
-            if ((tid & 63) == 0) wave_value[tid >> 6] = best, wave_at[tid >> 6] = at;
-            __syncthreads();
+        if ((tid & 63) == 0) wave_value[tid >> 6] = best, wave_at[tid >> 6] = at;
+        __syncthreads();
 #pragma unroll
-            for (int w = 0; w < THREADS / 64; ++w)
-                if (wave_value[w] > best || (wave_value[w] == best && wave_at[w] < at)) best = wave_value[w], at = wave_at[w];
-            __syncthreads();
-        }
-        const bool none = at >= n || best == -inf;
-        if (tid == 0) {
-            const long long out = (long long)b * g.count + j;
-            const int k = none ? 0 : at / per;
-            const long long row = (long long)b * g.K + k;
-            g.out_scores[out] = (float)best;
-            g.parents[out] = k;
-            g.tokens[out] = none ? -1 : g.ended && g.ended[row] ? g.end : (long long)beam_index(keys[at]);
-        }
-        if (!none && at % THREADS == tid) {  // its next one
+        for (int w = 0; w < BEAM_WAVES; ++w)
+            if (beam_before(wave_value[w], wave_at[w], best, at)) best = wave_value[w], at = wave_at[w];
+        __syncthreads();
+        if (tid == 0) answer(j, best, at);
+        if (at % BEAM_THREADS == tid) {  // its next one
             value[at] = -inf;
-            mine = -inf, mine_at = n;
-            for (int e = tid; e < n; e += THREADS)
-                if (value[e] > mine) mine = value[e], mine_at = e;
+            own_best();
         }
     }
 }
@@ -355,8 +450,7 @@ extern "C" int dl_beam_step(const void *logits, long long ldl, int type, const f
         else
             DL_TIMED("beam_rows", s, hipLaunchKernelGGL((beam_rows<T, 1>), dim3((unsigned)blocks), dim3(BEAM_THREADS), 0, s, g));
     });
-    if (K * g.pieces * count <= 1024) DL_TIMED("beam_pick", s, hipLaunchKernelGGL((beam_pick<64>), dim3(B), dim3(64), 0, s, g));
-    else DL_TIMED("beam_pick", s, hipLaunchKernelGGL((beam_pick<256>), dim3(B), dim3(256), 0, s, g));
+    DL_TIMED("beam_pick", s, hipLaunchKernelGGL(beam_pick, dim3(B), dim3(BEAM_THREADS), 0, s, g));
     return dl_launch_status();
 }
 
