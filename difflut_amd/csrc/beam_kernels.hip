@@ -259,28 +259,37 @@ __device__ __forceinline__ bool beam_before(double a, int at, double b, int bt) 
 __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
     __shared__ double value[BEAM_PICKS], norm[BEAM_MOST], base[BEAM_MOST], wave_value[BEAM_WAVES], bound;
     __shared__ double kept_value[BEAM_RANKS];
+    __shared__ float largest[BEAM_PICKS];
     __shared__ int kept_at[BEAM_RANKS], wave_at[BEAM_WAVES], kept, ended[BEAM_MOST];
     const int tid = threadIdx.x, b = blockIdx.x, per = g.pieces * g.count, n = g.K * per, lists = g.K * g.pieces;
     const double inf = __builtin_inf();
     const beam_key *keys = g.keys + (long long)b * n;
 
-    // the rows' logarithms: every list's share of its row's sum (in `value`), then a thread a row
+    // everything that is read, asked for at once
     const BeamPart *parts = g.parts + (long long)b * lists;
+    constexpr int EARLY = 4;
+    beam_key early[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) early[i] = i * BEAM_THREADS + tid < n ? keys[i * BEAM_THREADS + tid] : 0;
     if (tid < g.K) {
         const long long row = (long long)b * g.K + tid;
         ended[tid] = g.ended && g.ended[row] ? 1 : 0;
         base[tid] = (double)g.scores[row];
     }
+    for (int e = tid; e < lists; e += BEAM_THREADS) {
+        const BeamPart p = parts[e];
+        value[e] = p.sum, largest[e] = p.largest;
+    }
     if (tid == 0) kept = 0, bound = -inf;
     __syncthreads();
+    // the rows' logarithms: every list's share of its row's sum, then a thread a row  (what was never written of rows that have ended is not used)
     for (int e = tid; e < lists; e += BEAM_THREADS) {
-        const int k = e / g.pieces;
-        if (ended[k]) continue;
+        const int first = e / g.pieces * g.pieces;
+        if (ended[e / g.pieces]) continue;
         float most = -__builtin_inff();
-        for (int i = 0; i < g.pieces; ++i) most = fmaxf(most, parts[k * g.pieces + i].largest);
-        const BeamPart p = parts[e];
-        value[e] = p.sum > 0.0 ? p.sum * exp((double)p.largest - (double)most) : 0.0;
-        if (e % g.pieces == 0) norm[k] = (double)most;
+        for (int i = 0; i < g.pieces; ++i) most = fmaxf(most, largest[first + i]);
+        value[e] = value[e] > 0.0 ? value[e] * exp((double)largest[e] - (double)most) : 0.0;
+        if (e == first) norm[e / g.pieces] = (double)most;
     }
     __syncthreads();
     if (tid < g.K && !ended[tid]) {
@@ -289,17 +298,18 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
         norm[tid] = norm[tid] > -inf ? norm[tid] + log(sum) : inf;  // (infinity: nothing to go on with)
     }
     __syncthreads();
-    for (int e = tid; e < n; e += BEAM_THREADS) {
+    const auto candidate = [&](int e, beam_key key) __attribute__((always_inline)) {
         const int k = e / per;
         double c = -inf;
         if (ended[k]) {
             if (e == k * per) c = base[k];
-        } else {
-            const beam_key key = keys[e];
-            if (key) c = base[k] + ((double)beam_value(key) - norm[k]);
-        }
+        } else if (key) c = base[k] + ((double)beam_value(key) - norm[k]);
         value[e] = c == c ? c : -inf;
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i)
+        if (i * BEAM_THREADS + tid < n) candidate(i * BEAM_THREADS + tid, early[i]);
+    for (int e = EARLY * BEAM_THREADS + tid; e < n; e += BEAM_THREADS) candidate(e, keys[e]);
     __syncthreads();
     if (lists >= g.count && lists <= 2 * BEAM_THREADS)
         for (int e = tid; e < lists; e += BEAM_THREADS) {
