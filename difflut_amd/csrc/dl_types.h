@@ -59,6 +59,33 @@ __device__ __forceinline__ void dl_store_past(T *p, const float (&f)[N]) {
     }
 }
 
+// The same of any alignment (global memory takes it), and of the first `n` of E values only: the rest are 0, or not written
+template <typename T, int E>
+__device__ __forceinline__ void dl_load_some(const T *p, int n, float (&f)[E]) {
+    if (n >= E) {
+        DlVec<T, E> v;
+        __builtin_memcpy(&v, p, sizeof(v));
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = (float)v.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void dl_store_some(T *p, int n, const float (&f)[E]) {
+    if (n >= E) {
+        DlVec<T, E> v;
+#pragma unroll
+        for (int i = 0; i < E; ++i) v.v[i] = (T)f[i];
+        __builtin_memcpy(p, &v, sizeof(v));
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (i < n) p[i] = (T)f[i];
+    }
+}
+
 static inline bool dl_type_known(int type) { return type == DL_F32 || type == DL_BF16 || type == DL_F16; }
 static inline int dl_type_bytes(int type) { return type == DL_F32 ? 4 : 2; }
 static inline bool dl_grid_ok(long long blocks, int threads) { return blocks * threads < (1LL << 32); }  // work items of a launch

@@ -27,7 +27,7 @@ typedef int intx8 __attribute__((ext_vector_type(8)));
 #define LIN_STAGE_BYTES 128  // of a row in a stage: 32 float32, 64 16-bit or 128 8-bit values
 #define LIN_PLANES 3
 #define LIN_CUS 256
-enum { LIN_SUMS, LIN_PLAIN, LIN_ENDS, LIN_ODD };
+enum { LIN_SUMS, LIN_PLAIN, LIN_PLAIN_ODD, LIN_ENDS, LIN_ENDS_ODD };
 
 struct LinF32 { static constexpr int SIZE = 4; };
 struct LinBf16 { static constexpr int SIZE = 2; };
@@ -64,7 +64,7 @@ struct LinEnd {
     const float *row_scale, *col_scale;  // of 8-bit operands
     long long ldr;
     int R, C, F, act;           // C: rows of w; F: columns of y where gated
-    bool vec;                   // whole vectors of eight everywhere
+    bool vec;                   // whole vectors of eight of everything, aligned
 };
 
 // What belongs to eight columns from c on, whatever the row; gated: of the gate and of the other half.  Past the last column: nothing.
@@ -312,53 +312,53 @@ struct LinPlace {
     // four values from a column that is a multiple of four
     static __device__ __forceinline__ void put(char *place, int row, int column, const float (&f)[4]) { dl_store<T, 4>((T *)(place + four(row, column)), f); }
     static __device__ __forceinline__ void get(const char *place, int row, int column, float (&f)[4]) { dl_load<T, 4>((const T *)(place + four(row, column)), f); }
-    // to memory: `to` is the place's first value's, `rows` and `columns` are there.  HALVES: the second half of a row goes `apart` further on.
-    template <bool HALVES = false>
-    static __device__ __forceinline__ void send(const char *place, int lane, T *to, long long ld, int rows, int columns, bool vec, int apart = 0) {
+    // to memory of any alignment: `to` is the place's first value's, `rows` and `columns` are there.  HALVES: the second half of a row goes `apart`
+    // further on.  ODD: a row may end inside a unit, which goes value by value, all lanes taking some.
+    template <bool ODD, bool HALVES = false>
+    static __device__ __forceinline__ void send(const char *place, int lane, T *to, long long ld, int rows, int columns, int apart = 0) {
         constexpr int PART = HALVES ? WIDTH / 2 : WIDTH;
-        if (vec) {
-            const int unit = lane % UNITS, column = unit * E % PART;
-            T *const p = to + column + (HALVES && unit * E >= PART ? apart : 0);
-            dl_words v[TURNS];
+        const int unit = lane % UNITS, column = unit * E % PART, ends = ODD && columns > 0 && columns < PART ? columns % E : 0;
+        T *at = to + column + (HALVES && unit * E >= PART ? apart : 0) + lane / UNITS * ld;
+        dl_words v[TURNS];
 #pragma unroll
-            for (int t = 0; t < TURNS; ++t) v[t] = *reinterpret_cast<const dl_words *>(place + spot(t * (64 / UNITS) + lane / UNITS, unit));
-            lin_lds_done();  // (all of them are read before the first is written)
-            T *at = p + lane / UNITS * ld;
-            if (rows >= 32 && columns >= PART) {
+        for (int t = 0; t < TURNS; ++t) v[t] = *reinterpret_cast<const dl_words *>(place + spot(t * (64 / UNITS) + lane / UNITS, unit));
+        lin_lds_done();  // (all of them are read before the first is written)
+        if (rows >= 32 && columns >= PART) {
 #pragma unroll
-                for (int t = 0; t < TURNS; ++t, at += 64 / UNITS * ld) *reinterpret_cast<dl_words *>(at) = v[t];
-            } else if (column < columns) {
+            for (int t = 0; t < TURNS; ++t, at += 64 / UNITS * ld) __builtin_memcpy(at, &v[t], 16);
+        } else if (column + E <= columns) {
 #pragma unroll
-                for (int t = 0; t < TURNS; ++t, at += 64 / UNITS * ld)
-                    if (t * (64 / UNITS) + lane / UNITS < rows) *reinterpret_cast<dl_words *>(at) = v[t];
-            }
-            return;
+            for (int t = 0; t < TURNS; ++t, at += 64 / UNITS * ld)
+                if (t * (64 / UNITS) + lane / UNITS < rows) __builtin_memcpy(at, &v[t], 16);
         }
+        if (ends == 0) return;
 #pragma unroll 1
-        for (int e = lane; e < 32 * WIDTH; e += 64) {
-            const int row = e / WIDTH, at = e % WIDTH, column = at % PART;
-            if (row < rows && column < columns) to[row * ld + column + (HALVES && at >= PART ? apart : 0)] = *reinterpret_cast<const T *>(place + spot(row, at / E) + at % E * (int)sizeof(T));
+        for (int e = lane; e < 32 * ends * (HALVES ? 2 : 1); e += 64) {
+            const int half = e / (32 * ends), row = e / ends % 32, i = e % ends, c = columns - ends + i;
+            if (row < rows) to[row * ld + half * apart + c] = *reinterpret_cast<const T *>(place + spot(row, (half * PART + c) / E) + c % E * (int)sizeof(T));
         }
     }
-    // from memory: vectors by way of registers, asked for early; the rest value by value
+    template <bool ODD>
+    static __device__ __forceinline__ void keep(char *place, int lane, const dl_words (&v)[TURNS], const T *from, long long ld, int rows, int columns) {
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) *reinterpret_cast<dl_words *>(place + spot(t * (64 / UNITS) + lane / UNITS, lane % UNITS)) = v[t];
+        const int ends = ODD && columns > 0 && columns < WIDTH ? columns % E : 0;
+        if (ends == 0) return;
+        lin_lds_done();
+#pragma unroll 1
+        for (int e = lane; e < 32 * ends; e += 64) {
+            const int row = e / ends, c = columns - ends + e % ends;
+            if (row < rows) *reinterpret_cast<T *>(place + spot(row, c / E) + c % E * (int)sizeof(T)) = from[row * ld + c];
+        }
+    }
+    // from memory of any alignment: whole units by way of registers, asked for early; then these and the unit that a row ends in into the place
     static __device__ __forceinline__ void fetch(dl_words (&v)[TURNS], int lane, const T *from, long long ld, int rows, int columns) {
         const int column = lane % UNITS * E;
 #pragma unroll
         for (int t = 0; t < TURNS; ++t) {
             const int row = t * (64 / UNITS) + lane / UNITS;
             v[t] = dl_words{0, 0, 0, 0};
-            if (row < rows && column < columns) v[t] = *reinterpret_cast<const dl_words *>(from + row * ld + column);
-        }
-    }
-    static __device__ __forceinline__ void keep(char *place, int lane, const dl_words (&v)[TURNS]) {
-#pragma unroll
-        for (int t = 0; t < TURNS; ++t) *reinterpret_cast<dl_words *>(place + spot(t * (64 / UNITS) + lane / UNITS, lane % UNITS)) = v[t];
-    }
-    static __device__ __forceinline__ void bring(char *place, int lane, const T *from, long long ld, int rows, int columns) {
-#pragma unroll 1
-        for (int e = lane; e < 32 * WIDTH; e += 64) {
-            const int row = e / WIDTH, column = e % WIDTH;
-            *reinterpret_cast<T *>(place + spot(row, column / E) + column % E * (int)sizeof(T)) = row < rows && column < columns ? from[row * ld + column] : (T)0.0f;
+            if (row < rows && column + E <= columns) __builtin_memcpy(&v[t], from + row * ld + column, 16);
         }
     }
 };
@@ -402,7 +402,8 @@ __device__ __forceinline__ int lin_anew(int v) {
 // then, into the same place, A's one step later, so that loads are spread over the matrix instructions and have a stage's time to land.  One wavefront
 // a SIMD issues everything, so reads, loads and (of float32) cuts stand between the matrix instructions in the order written here; left
 // to itself the compiler puts the reads in front of their use.  Where the reduction ends inside a stage, that stage comes first.
-// WHAT becomes of the sums: LIN_SUMS partial sums, LIN_PLAIN nothing but the result, LIN_ENDS what follows in whole vectors, LIN_ODD the same value by value.
+// WHAT becomes of the sums: LIN_SUMS partial sums, LIN_PLAIN nothing but the result, LIN_ENDS what follows; ODD: not all is in aligned
+// whole vectors.
 // There are as many blocks as the chip holds; one sends for its next tile's first stages before it writes a tile out.
 // Gated, a wavefront's columns are those of the gate, then the ones that belong to them.
 template <typename In, typename Out, int TR, int TC, bool TURN_A, bool TURN_B, bool GATED, int WHAT>
@@ -570,17 +571,16 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
 
     // C: a lane has row lane % 32 of a tile of 32 x 32, and columns (v % 4) + 8 (v / 4) + 4 (lane / 32) of it
     constexpr int W = FB * 32, H = GATED ? FB / 2 : FB;
-    constexpr bool PARTIAL = WHAT == LIN_SUMS;
+    constexpr bool PARTIAL = WHAT == LIN_SUMS, PLAIN = WHAT == LIN_PLAIN || WHAT == LIN_PLAIN_ODD, ODD = WHAT != LIN_PLAIN && WHAT != LIN_ENDS;
     typedef typename LinChoose<PARTIAL, float, Out>::type Stored;
     typedef LinPlace<Stored, W> Products;               // z, or partial sums
     typedef LinPlace<Stored, GATED ? HALF : W> Results;
     static_assert(WAVES * Products::BYTES <= TileA::BYTES + TileB::BYTES, "fits the last two places");
-    constexpr bool SCALED = In::SIZE == 1, VEC = WHAT != LIN_ODD;
-    static_assert(WHAT != LIN_PLAIN || (!SCALED && !GATED), "something follows");
+    constexpr bool SCALED = In::SIZE == 1;
+    static_assert(!PLAIN || (!SCALED && !GATED), "something follows");
     const auto write_plain = [&](int row0, int column0, int plane) __attribute__((always_inline)) {
         const int lane = lin_anew(threadIdx.x & 63), c = column0 + wc;
         Stored *const out = PARTIAL ? (Stored *)(void *)g.part + (long long)plane * g.end.R * g.end.C : (Stored *)g.end.y;
-        const bool vec = PARTIAL ? g.end.C % 4 == 0 : g.end.vec;
         char *mine = lds + B1 + wave * Products::BYTES;
         lin_each<0, FA>([&](auto phase) __attribute__((always_inline)) {
             constexpr int i = decltype(phase)::value;
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
                     Products::put(mine, lane & 31, j * 32 + 8 * q + 4 * (lane >> 5), f);
                 }
             lin_lds_done();
-            Products::send(mine, lane, out + (long long)r * g.end.C + c, g.end.C, g.end.R - r, g.end.C - c, vec);
+            Products::template send<ODD>(mine, lane, out + (long long)r * g.end.C + c, g.end.C, g.end.R - r, g.end.C - c);
             lin_lds_done();
         });
     };
@@ -616,8 +616,8 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
                 for (int q = 0; q < 4; ++q) {
                     const long long from = (j / H) * (long long)e.F;  // (gated: of the gate's or the other's columns)
                     const int column = first + j % H * 32 + 8 * q;
-                    bias[j][q].load((const Stored *)e.bias, from, column, width, VEC, (Stored)0.0f);
-                    if (SCALED) scale[SCALED ? j : 0][q].load(e.col_scale, from, column, width, VEC, 1.0f);
+                    bias[j][q].load((const Stored *)e.bias, from, column, width, !ODD, (Stored)0.0f);
+                    if (SCALED) scale[SCALED ? j : 0][q].load(e.col_scale, from, column, width, !ODD, 1.0f);
                 }
         };
         constexpr bool HELD = sizeof(Stored) == 2;  // through the tile; more would not fit the registers
@@ -631,7 +631,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
             }
             const Stored *const res = (const Stored *)e.res + r * e.ldr + c;
             dl_words residual[Results::TURNS];
-            if (e.res && VEC && !SCALED) Results::fetch(residual, lane, res, e.ldr, rows, columns);  // (scales take the registers that it would wait in)
+            if (e.res && !SCALED) Results::fetch(residual, lane, res, e.ldr, rows, columns);  // (scales take the registers that it would wait in)
             const float row_scale = SCALED ? e.row_scale[min(r + l32, e.R - 1)] : 1.0f;
             if (!HELD) of_columns();
             else {
@@ -657,13 +657,12 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
 #pragma unroll
                     for (int q = 0; q < 4; ++q) Products::put(mine, l32, j * 32 + 8 * q + 4 * kh, {f[j][4 * q], f[j][4 * q + 1], f[j][4 * q + 2], f[j][4 * q + 3]});
                 lin_lds_done();
-                Products::template send<GATED>(mine, lane, (Stored *)e.z + (long long)r * e.C + c, e.C, rows, columns, VEC, e.F);
+                Products::template send<ODD, GATED>(mine, lane, (Stored *)e.z + (long long)r * e.C + c, e.C, rows, columns, e.F);
                 lin_lds_done();
             }
             if (e.res) {
-                if (VEC && SCALED) Results::fetch(residual, lane, res, e.ldr, rows, columns);
-                if (VEC) Results::keep(mine, lane, residual);
-                else Results::bring(mine, lane, res, e.ldr, rows, columns);
+                if (SCALED) Results::fetch(residual, lane, res, e.ldr, rows, columns);
+                Results::template keep<ODD>(mine, lane, residual, res, e.ldr, rows, columns);
                 lin_lds_done();
             }
 #pragma unroll
@@ -695,7 +694,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
                 for (int q = 0; q < 4; ++q) Results::put(mine, l32, j * 32 + 8 * q + 4 * kh, {f[j][4 * q], f[j][4 * q + 1], f[j][4 * q + 2], f[j][4 * q + 3]});
             }
             lin_lds_done();
-            Results::send(mine, lane, (Stored *)e.y + (long long)r * width + c, width, rows, columns, VEC);
+            Results::template send<ODD>(mine, lane, (Stored *)e.y + (long long)r * width + c, width, rows, columns);
             lin_lds_done();
         });
     };
@@ -728,7 +727,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
             place();
             begin();
         }
-        if constexpr (WHAT == LIN_SUMS || WHAT == LIN_PLAIN) write_plain(row, column, plane);
+        if constexpr (PARTIAL || PLAIN) write_plain(row, column, plane);
         else write(row, column);
         if (!more) return;
     }
@@ -962,15 +961,14 @@ template <typename In, typename Out, int T, bool TURN_A, bool TURN_B>
 static int lin_launch_tile(const LinArgs &g, bool gated, hipStream_t s) {
     const LinEnd &e = g.end;
     if (g.splits > 1) return lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_SUMS>(g, s);
-    if constexpr (TURN_B) return lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_PLAIN>(g, s);
-    else {
-        constexpr bool SCALED = In::SIZE == 1;
-        if constexpr (!SCALED)
-            if (!gated && !e.bias && !e.res && !e.z && e.act == DL_ACT_NONE) return lin_go<In, Out, T, false, false, false, LIN_PLAIN>(g, s);
-        if (e.vec) return gated ? lin_go<In, Out, T, false, false, true, LIN_ENDS>(g, s) : lin_go<In, Out, T, false, false, false, LIN_ENDS>(g, s);
-        if constexpr (T <= 128) return gated ? lin_go<In, Out, T, false, false, true, LIN_ODD>(g, s) : lin_go<In, Out, T, false, false, false, LIN_ODD>(g, s);
+    const bool plain = TURN_B || (!gated && !e.row_scale && !e.bias && !e.res && !e.z && e.act == DL_ACT_NONE);
+    if constexpr (In::SIZE > 1)
+        if (plain) return e.vec ? lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_PLAIN>(g, s) : lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_PLAIN_ODD>(g, s);
+    if constexpr (!TURN_B) {
+        if (gated) return e.vec ? lin_go<In, Out, T, false, false, true, LIN_ENDS>(g, s) : lin_go<In, Out, T, false, false, true, LIN_ENDS_ODD>(g, s);
+        return e.vec ? lin_go<In, Out, T, false, false, false, LIN_ENDS>(g, s) : lin_go<In, Out, T, false, false, false, LIN_ENDS_ODD>(g, s);
     }
-    return DL_ERR_UNSUPPORTED;  // (the plan gives small tiles to what is not in whole vectors)
+    return DL_ERR_UNSUPPORTED;
 }
 template <typename In, typename Out, bool TURN_A, bool TURN_B>
 static int lin_launch(LinArgs &g, const LinPlan &p, bool gated, hipStream_t s) {

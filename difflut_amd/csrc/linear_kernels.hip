@@ -21,30 +21,36 @@ __global__ __launch_bounds__(256) void lin_pad(const T *__restrict__ src, long l
 }
 
 // ------------------------------------------------------------------ the gradient in front of the products, and its column sums
-// gz [M, N] (null: not written) from gy and z (null: no activation, gz is gy), and a share of sum_m gz per block of rows (null: not asked for).
-// A thread takes E columns of every fourth row of its block's; gated: of the gate and of the other half.
+// gz [M, ldg] (null: not written) from gy and z (null: no activation, gz is gy), and a share of sum_m gz per block of rows (null: not asked for).
+// A thread takes E columns of every fourth row of its block's; gated: of the gate and of the other half.  Rows of gz are whole units of 16 bytes,
+// zeros behind the N-th column, as the products read them; those of gy and z
+// may begin anywhere and end inside a unit (ODD).
 #define LIN_SLOPE_ROWS 64
-template <typename T, int E, bool GATED>
+template <typename T, bool GATED, bool ODD>
 __global__ __launch_bounds__(256) void lin_gradient(const T *__restrict__ gy, const T *__restrict__ z, T *__restrict__ gz, float *__restrict__ shares,
-                                                    long long M, int N, int act, int col_tiles, int rows) {
-    constexpr int H = GATED ? 2 : 1;
+                                                    long long M, int N, long long ldg, int act, int col_tiles, int rows) {
+    constexpr int H = GATED ? 2 : 1, E = 16 / sizeof(T);
     __shared__ float part[H * 4][64 * E];
     const int lane = threadIdx.x & 63, team = threadIdx.x >> 6, width = GATED ? N / 2 : N;
-    const int c = ((int)(blockIdx.x % col_tiles) * 64 + lane) * E;
+    const int c = ((int)(blockIdx.x % col_tiles) * 64 + lane) * E, n = width - c;
     const long long piece = blockIdx.x / col_tiles, m0 = piece * rows, m1 = m0 + rows < M ? m0 + rows : M;
     float sum[H][E];
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int i = 0; i < E; ++i) sum[h][i] = 0.0f;
-    if (c < width)
+    if (n > 0)
         for (long long m = m0 + team; m < m1; m += 4) {
+            const auto load = [&](const T *p, float (&f)[E]) __attribute__((always_inline)) {
+                if (ODD) dl_load_some<T, E>(p, n, f);
+                else dl_load<T, E>(p, f);
+            };
             float g[H][E];
-            dl_load<T, E>(gy + m * width + c, g[0]);
+            load(gy + m * width + c, g[0]);
             if (z) {
                 float a[H][E];
-                dl_load<T, E>(z + m * N + c, a[0]);
-                if (GATED) dl_load<T, E>(z + m * N + width + c, a[H - 1]);
+                load(z + m * N + c, a[0]);
+                if (GATED) load(z + m * N + width + c, a[H - 1]);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     float value;
@@ -55,10 +61,13 @@ __global__ __launch_bounds__(256) void lin_gradient(const T *__restrict__ gy, co
             }
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                if (gz) dl_store<T, E>(gz + m * N + h * width + c, g[h]);
+                if (gz && ODD) dl_store_some<T, E>(gz + m * ldg + h * width + c, n, g[h]);
+                if (gz && !ODD) dl_store<T, E>(gz + m * ldg + h * width + c, g[h]);
 #pragma unroll
                 for (int i = 0; i < E; ++i) sum[h][i] += g[h][i];
             }
+            if (ODD && gz && c == 0)
+                for (int i = N; i < ldg; ++i) gz[m * ldg + i] = (T)0.0f;
         }
     if (!shares) return;
 #pragma unroll
@@ -66,11 +75,12 @@ __global__ __launch_bounds__(256) void lin_gradient(const T *__restrict__ gy, co
 #pragma unroll
         for (int i = 0; i < E; ++i) part[h * 4 + team][i * 64 + lane] = sum[h][i];
     __syncthreads();
-    if (team != 0 || c >= width) return;
+    if (team != 0) return;
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int i = 0; i < E; ++i) {
+            if (i >= n) continue;
             float t = 0.0f;
             for (int q = 0; q < 4; ++q) t += part[h * 4 + q][i * 64 + lane];
             shares[piece * N + h * width + c + i] = t;
@@ -102,11 +112,12 @@ struct LinOperand {
     const void *p;
     long long ld, rows, length;
     bool turned;
+    bool padded = false;  // rows go on to a whole unit, with zeros
     long long count() const { return turned ? length : rows; }
 };
 static bool lin_direct(const LinOperand &o, int type) {
     const int size = lin_size(type);
-    return dl_aligned16(o.p) && o.ld * size % 16 == 0 && o.length * size % 16 == 0;
+    return dl_aligned16(o.p) && o.ld * size % 16 == 0 && (o.padded || o.length * size % 16 == 0);
 }
 static long long lin_padded(const LinOperand &o, int type) { const int unit = 16 / lin_size(type); return (o.length + unit - 1) / unit * unit; }
 static size_t lin_operand_bytes(const LinOperand &o, int type) {
@@ -170,7 +181,6 @@ static int lin_run(const LinOperand &a, const LinOperand &b, int type, int out_t
     end.R = (int)a.count(), end.C = (int)b.count(), end.F = end.C / 2;
     const int width = gated ? end.F : end.C, size = dl_type_bytes(out_type);
     end.vec = width % 8 == 0 && dl_aligned16(end.y) && dl_aligned16(end.z) && dl_aligned16(end.bias) && dl_aligned16(end.res) && dl_aligned16(end.col_scale) && end.ldr * size % 16 == 0;
-    if (p.splits == 1 && !end.vec && !b.turned) p.tile = 128;  // (value by value: the smaller tile alone)
     g.K = K, g.stages = dl_ceil_div(K * lin_size(type), LIN_STAGE_BYTES), g.chunk = p.chunk, g.splits = p.splits;
     if (!p.few) g.row_tiles = dl_ceil_div(end.R, p.tile), g.col_tiles = gated && p.splits == 1 ? dl_ceil_div(end.F, p.tile / 2) : dl_ceil_div(end.C, p.tile);
     g.end = end;
@@ -221,14 +231,14 @@ struct LinBack {
 static LinBack lin_back(const LinOperand &gz, const LinOperand &x, const LinOperand &w, int type, bool kept, int wants, long long N, long long K) {
     LinBack b{};
     const long long M = gz.rows;
-    b.gz = kept ? dl_align256((size_t)M * (size_t)N * lin_size(type)) : 0;
+    b.gz = kept ? dl_align256((size_t)M * (size_t)gz.ld * lin_size(type)) : 0;
     // rows of a block: from one a team up, as few as leave 1024 blocks or fewer over the columns (vectors of 16 bytes)
     const long long across = (N + 64 * (16 / lin_size(type)) - 1) / (64 * (16 / lin_size(type)));
     b.rows = 4;
     while ((M + b.rows - 1) / b.rows * across > 1024 && (b.rows < LIN_SLOPE_ROWS || (M + b.rows - 1) / b.rows > 1024)) b.rows *= 2;
     b.pieces = dl_ceil_div(M, b.rows);
     b.shares = wants & 4 ? dl_align256((size_t)b.pieces * (size_t)N * 4) : 0;
-    const LinOperand gt = {gz.p, gz.ld, M, N, true}, wt = {w.p, w.ld, N, K, true}, xt = {x.p, x.ld, M, K, true};
+    const LinOperand gt = {gz.p, gz.ld, M, N, true, gz.padded}, wt = {w.p, w.ld, N, K, true}, xt = {x.p, x.ld, M, K, true};
     if (wants & 1) b.products = lin_plan(gz, wt, type, N, false).bytes();
     if (wants & 2) {
         const size_t n = lin_plan(gt, xt, type, M, false).bytes();
@@ -236,13 +246,17 @@ static LinBack lin_back(const LinOperand &gz, const LinOperand &x, const LinOper
     }
     return b;
 }
-// (the workspace begins on 16 bytes, as gz in it does, so a pointer of that alignment stands for it)
-static const void *lin_gz_place(const void *ws, const void *gy, bool kept) { return kept ? (ws ? ws : (const void *)256) : gy; }
+// gz: gy itself, or in the workspace's beginning (on 16 bytes: any pointer of that alignment stands for it) in rows of whole units
+static LinOperand lin_gz(const void *ws, const void *gy, bool kept, int type, long long M, long long N) {
+    if (!kept) return {gy, N, M, N, false};
+    const long long unit = 16 / lin_size(type);
+    return {ws ? ws : (const void *)256, (N + unit - 1) / unit * unit, M, N, false, true};
+}
 
 extern "C" size_t dl_linear_bwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, int wants, int type,
                                                 long long M, long long N, long long K) {
     if (lin_check(type, type, M, N, K, 0, 0) != DL_OK) return 0;
-    return lin_back({lin_gz_place(nullptr, gy, z != nullptr), N, M, N, false}, {x, ldx, M, K, false}, {w, ldw, N, K, false}, type, z != nullptr, wants, N, K).bytes();
+    return lin_back(lin_gz(nullptr, gy, z != nullptr, type, M, N), {x, ldx, M, K, false}, {w, ldw, N, K, false}, type, z != nullptr, wants, N, K).bytes();
 }
 
 extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, void *gx, void *gw, void *gb, int type,
@@ -255,7 +269,7 @@ extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long l
     const int wants = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
     if (!wants) return DL_OK;
     const bool kept = z != nullptr;
-    const LinOperand gz = {lin_gz_place(ws, gy, kept), N, M, N, false}, xo = {x, ldx, M, K, false}, wo = {w, ldw, N, K, false};
+    const LinOperand gz = lin_gz(ws, gy, kept, type, M, N), xo = {x, ldx, M, K, false}, wo = {w, ldw, N, K, false};
     const LinBack p = lin_back(gz, xo, wo, type, kept, wants, N, K);
     if (p.bytes() && !ws) return DL_ERR_NULL;
     if (ws_bytes < p.bytes() || !dl_aligned16(ws)) return DL_ERR_WORKSPACE;
@@ -263,16 +277,15 @@ extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long l
     float *shares = gb ? (float *)((char *)ws + p.gz) : nullptr;
     if (kept || gb) {
         void *out = kept ? ws : nullptr;
-#define LIN_GRADIENT(E, GATED) hipLaunchKernelGGL((lin_gradient<T, E, GATED>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)gy, (const T *)z, (T *)out, shares, M, (int)N, act, col_tiles, p.rows)
         const int width = (int)(gated ? N / 2 : N);
+#define LIN_GRADIENT(GATED, ODD) hipLaunchKernelGGL((lin_gradient<T, GATED, ODD>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)gy, (const T *)z, (T *)out, shares, M, (int)N, gz.ld, act, col_tiles, p.rows)
         DL_BY_TYPE(type, T, {
-            constexpr int E = 16 / sizeof(T);
-            const bool vec = width % E == 0 && dl_aligned16(gy) && dl_aligned16(z);
-            const int col_tiles = dl_ceil_div(width, 64 * (vec ? E : 1));
+            const int col_tiles = dl_ceil_div(width, 64 * (16 / (int)sizeof(T)));
             const long long blocks = (long long)col_tiles * p.pieces;
             if (!dl_grid_ok(blocks, 256)) return DL_ERR_UNSUPPORTED;
-            DL_TIMED("lin_gradient", s, if (gated) { if (vec) LIN_GRADIENT(E, true); else LIN_GRADIENT(1, true); }
-                     else if (vec) LIN_GRADIENT(E, false); else LIN_GRADIENT(1, false));
+            const bool odd = width % (16 / (int)sizeof(T)) != 0 || !dl_aligned16(gy) || !dl_aligned16(z);
+            DL_TIMED("lin_gradient", s, if (gated) { if (odd) LIN_GRADIENT(true, true); else LIN_GRADIENT(true, false); }
+                     else if (odd) LIN_GRADIENT(false, true); else LIN_GRADIENT(false, false));
             if (gb) DL_TIMED("lin_columns", s, hipLaunchKernelGGL((lin_columns<T>), dim3(dl_ceil_div(N, 16)), dim3(256), 0, s, shares, (T *)gb, p.pieces, (int)N));
         });
 #undef LIN_GRADIENT
@@ -286,7 +299,7 @@ extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long l
     }
     if (gw) {
         end.y = gw;
-        const int code = lin_run({gz.p, N, M, N, true}, {x, ldx, M, K, true}, type, type, M, false, end, room, s);
+        const int code = lin_run({gz.p, gz.ld, M, N, true, gz.padded}, {x, ldx, M, K, true}, type, type, M, false, end, room, s);
         if (code != DL_OK) return code;
     }
     return dl_launch_status();
