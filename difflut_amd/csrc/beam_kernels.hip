@@ -128,9 +128,10 @@ __device__ int beam_shorten(beam_key *list, int n, int count, int most, beam_key
     return count;
 }
 
-template <typename T, int E>
+// ODD: rows begin anywhere, and may end inside a vector of 16 bytes.
+template <typename T, bool ODD>
 __global__ __launch_bounds__(BEAM_THREADS) void beam_rows(BeamArgs g) {
-    constexpr int Q = BEAM_PER_THREAD / E;
+    constexpr int E = 16 / sizeof(T), Q = BEAM_PER_THREAD / E;
     __shared__ beam_key lists[BEAM_WAVES][BEAM_LIST];
     __shared__ __align__(16) beam_key merged[BEAM_WAVES * BEAM_CUT];
     __shared__ float tops[BEAM_WAVES];
@@ -150,7 +151,11 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows(BeamArgs g) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
             const int c = at + (q * BEAM_THREADS + tid) * E;
-            if (c < v1) dl_load<T, E>(logits + c, next[q]);
+            if (!ODD && c < v1) dl_load<T, E>(logits + c, next[q]);
+            else if (ODD && c + E <= v1) dl_load_some<T, E>(logits + c, E, next[q]);
+            else if (ODD && c < v1)
+#pragma unroll
+                for (int i = 0; i < E; ++i) next[q][i] = c + i < v1 ? (float)logits[c + i] : -inf;
             else
 #pragma unroll
                 for (int i = 0; i < E; ++i) next[q][i] = -inf;
@@ -456,9 +461,9 @@ extern "C" int dl_beam_step(const void *logits, long long ldl, int type, const f
     DL_BY_TYPE(type, T, {
         constexpr int E = 16 / sizeof(T);
         if (V % E == 0 && ldl % E == 0 && dl_aligned16(logits))
-            DL_TIMED("beam_rows", s, hipLaunchKernelGGL((beam_rows<T, E>), dim3((unsigned)blocks), dim3(BEAM_THREADS), 0, s, g));
+            DL_TIMED("beam_rows", s, hipLaunchKernelGGL((beam_rows<T, false>), dim3((unsigned)blocks), dim3(BEAM_THREADS), 0, s, g));
         else
-            DL_TIMED("beam_rows", s, hipLaunchKernelGGL((beam_rows<T, 1>), dim3((unsigned)blocks), dim3(BEAM_THREADS), 0, s, g));
+            DL_TIMED("beam_rows", s, hipLaunchKernelGGL((beam_rows<T, true>), dim3((unsigned)blocks), dim3(BEAM_THREADS), 0, s, g));
     });
     DL_TIMED("beam_pick", s, hipLaunchKernelGGL(beam_pick, dim3(B), dim3(BEAM_THREADS), 0, s, g));
     return dl_launch_status();

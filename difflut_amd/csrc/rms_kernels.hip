@@ -5,7 +5,7 @@
 //   backward, g = gy gamma, hat = h rstd:   gh = rstd (g - hat mean(g hat)) + (gradient that reached h itself),   ggamma_c = sum gy hat
 //
 // A team of 8 to 1024 threads takes a row and holds it in registers, V vectors of 16 bytes a thread, so that every tensor is read once
-// and written once; rows of more than RMS_WIDEST values are read again instead (they are in the L2 by then).  The backward's teams go
+// and written once; rows that 1024 threads cannot hold so (16384 values of float32, 32768 of 16 bits) are read again instead, from the L2.  The backward's teams go
 // through rows in steps and keep their columns' sums of ggamma in registers: a share per block, added up in order by one more launch.
 // Sums are floats in a fixed order: the same bits from run to run.
 #include "dl_types.h"
@@ -45,33 +45,40 @@ __device__ __forceinline__ float rms_reduce(float v, float *part) {
     return v;
 }
 
-__device__ __forceinline__ float rms_gamma(const void *p, int type, long long c) {
-    if (!p) return 1.0f;
-    if (type == DL_F32) return ((const float *)p)[c];
-    return type == DL_BF16 ? (float)((const dl_bf16 *)p)[c] : (float)((const dl_f16 *)p)[c];
+// E values of a row, `left` of them there and at any alignment (ODD), or all and aligned
+template <bool ODD, typename T, int E>
+__device__ __forceinline__ void rms_load(const T *p, int left, float (&f)[E]) {
+    if constexpr (ODD) dl_load_some<T, E>(p, left, f);
+    else dl_load<T, E>(p, f);
 }
-template <int E>
-__device__ __forceinline__ void rms_gammas(const void *p, int type, int c, float (&f)[E]) {
+template <bool ODD, typename T, int E>
+__device__ __forceinline__ void rms_store(T *p, int left, const float (&f)[E]) {
+    if constexpr (ODD) dl_store_some<T, E>(p, left, f);
+    else dl_store<T, E>(p, f);
+}
+template <bool ODD, int E>
+__device__ __forceinline__ void rms_gammas(const void *p, int type, int c, int left, float (&f)[E]) {
 #pragma unroll
     for (int i = 0; i < E; ++i) f[i] = 1.0f;
     if (!p) return;
-    DL_BY_TYPE(type, T, dl_load<T, E>((const T *)p + c, f));
+    DL_BY_TYPE(type, T, (rms_load<ODD, T, E>((const T *)p + c, left, f)));
 }
 
-// eight (or fewer) values as e4m3, rounded to nearest even
-template <int E>
-__device__ __forceinline__ void rms_store_codes(rms_code *p, const float (&f)[E]) {
-    if constexpr (E == 1) {
-        *p = (rms_code)__builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[0], 0, false);
-    } else {
-        DlVec<uint32_t, E / 4> w;
+// values as e4m3, rounded to nearest even
+template <bool ODD, int E>
+__device__ __forceinline__ void rms_store_codes(rms_code *p, int left, const float (&f)[E]) {
+    DlVec<uint32_t, E / 4> w;
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i) {
-            int t = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
-            w.v[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], t, true);
-        }
-        *reinterpret_cast<DlVec<uint32_t, E / 4> *>(p) = w;
+    for (int i = 0; i < E / 4; ++i) {
+        const int t = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+        w.v[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], t, true);
     }
+    if (!ODD) *reinterpret_cast<DlVec<uint32_t, E / 4> *>(p) = w;
+    else if (left >= E) __builtin_memcpy(p, &w, E);
+    else
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (i < left) p[i] = (rms_code)(w.v[i / 4] >> (i % 4 * 8));
 }
 __device__ __forceinline__ float rms_clamped(float v) { return v > RMS_CODE_MAX ? RMS_CODE_MAX : v < -RMS_CODE_MAX ? -RMS_CODE_MAX : v; }
 
@@ -84,8 +91,9 @@ struct RmsArgs {
     float eps;
 };
 
-// CODES: y is bytes, and the rows' scales are written.  HELD: the row stays in registers (V vectors of E a thread).
-template <typename T, int E, int V, int TEAM, bool CODES, bool HELD>
+// CODES: y is bytes, and the rows' scales are written.  HELD: the row stays in registers (V vectors of E a thread).  ODD: rows begin anywhere and may
+// end inside a vector.
+template <typename T, int E, int V, int TEAM, bool CODES, bool HELD, bool ODD>
 __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
     constexpr int TEAMS = RmsTeam<TEAM>::TEAMS, THREADS = RmsTeam<TEAM>::THREADS, UNROLL = HELD ? V : 1;
     __shared__ float part[2][THREADS / 64];
@@ -103,10 +111,10 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
 #pragma unroll
         for (int i = 0; i < E; ++i) f[i] = 0.0f;
         if (c >= g.D) return;
-        dl_load<T, E>(x + c, f);
+        rms_load<ODD, T, E>(x + c, g.D - c, f);
         if (res) {
             float r[E];
-            dl_load<T, E>(res + c, r);
+            rms_load<ODD, T, E>(res + c, g.D - c, r);
 #pragma unroll
             for (int i = 0; i < E; ++i) f[i] = (float)(T)(f[i] + r[i]);
         }
@@ -116,7 +124,7 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
         float(&f)[E] = v[HELD ? j : 0];
         fetch(j, f);
         const int c = (j * TEAM + lane) * E;
-        if (h && real && c < g.D) dl_store<T, E>(h + c, f);
+        if (h && real && c < g.D) rms_store<ODD, T, E>(h + c, g.D - c, f);
 #pragma unroll
         for (int i = 0; i < E; ++i) sum = fmaf(f[i], f[i], sum);
     }
@@ -134,14 +142,14 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
         if (!HELD) fetch(j, f);
         if (c >= g.D) continue;
         float w[E];
-        rms_gammas<E>(g.gamma, g.ptype, c, w);
+        rms_gammas<ODD, E>(g.gamma, g.ptype, c, g.D - c, w);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             f[i] = f[i] * rstd * w[i];
             const float a = fabsf(f[i]);
             if (CODES) big = a > big || a != a ? a : big;
         }
-        if (!CODES && real) dl_store<T, E>((T *)g.y + row * g.D + c, f);
+        if (!CODES && real) rms_store<ODD, T, E>((T *)g.y + row * g.D + c, g.D - c, f);
     }
     if (!CODES) return;
     big = rms_reduce<TEAM, true>(big, part[1]);
@@ -157,18 +165,18 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
         if (!HELD) {
             float w[E];
             fetch(j, f);
-            rms_gammas<E>(g.gamma, g.ptype, c, w);
+            rms_gammas<ODD, E>(g.gamma, g.ptype, c, g.D - c, w);
 #pragma unroll
             for (int i = 0; i < E; ++i) f[i] = f[i] * rstd * w[i];
         }
 #pragma unroll
         for (int i = 0; i < E; ++i) f[i] = rms_clamped(f[i] * factor);
-        rms_store_codes<E>((rms_code *)g.y + row * g.D + c, f);
+        rms_store_codes<ODD, E>((rms_code *)g.y + row * g.D + c, g.D - c, f);
     }
 }
 
 // shares [gridDim.x][D] of ggamma (null: not asked for), in the order of rows, then teams
-template <typename T, int E, int V, int TEAM, bool HELD>
+template <typename T, int E, int V, int TEAM, bool HELD, bool ODD>
 __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_bwd(RmsArgs g) {
     constexpr int TEAMS = RmsTeam<TEAM>::TEAMS, THREADS = RmsTeam<TEAM>::THREADS, UNROLL = HELD ? V : 1;
     __shared__ float part[2][THREADS / 64];
@@ -199,15 +207,15 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_bwd(RmsArgs g) {
             for (int i = 0; i < E; ++i) hat[i] = gw[i] = 0.0f;
             if (c >= g.D) return;
             float w[E];
-            dl_load<T, E>(h + c, hat);
-            if (gy) dl_load<T, E>(gy + c, gw);
-            rms_gammas<E>(g.gamma, g.ptype, c, w);
+            rms_load<ODD, T, E>(h + c, g.D - c, hat);
+            if (gy) rms_load<ODD, T, E>(gy + c, g.D - c, gw);
+            rms_gammas<ODD, E>(g.gamma, g.ptype, c, g.D - c, w);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 hat[i] *= rstd;
                 if (sum && real) {
                     if (HELD) gg[HELD ? j : 0][i] = fmaf(gw[i], hat[i], gg[HELD ? j : 0][i]);
-                    else if (share) share[c + i] = fmaf(gw[i], hat[i], share[c + i]);
+                    else if (share && c + i < g.D) share[c + i] = fmaf(gw[i], hat[i], share[c + i]);
                 }
                 gw[i] *= w[i];
                 if (sum) dot = fmaf(gw[i], hat[i], dot);
@@ -226,10 +234,10 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_bwd(RmsArgs g) {
             float r[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) r[i] = 0.0f;
-            if (g.gh) dl_load<T, E>((const T *)g.gh + row * g.D + c, r);
+            if (g.gh) rms_load<ODD, T, E>((const T *)g.gh + row * g.D + c, g.D - c, r);
 #pragma unroll
             for (int i = 0; i < E; ++i) r[i] = fmaf(rstd, gw[i] - hat[i] * mean, r[i]);
-            dl_store<T, E>((T *)g.gx + row * g.D + c, r);
+            rms_store<ODD, T, E>((T *)g.gx + row * g.D + c, g.D - c, r);
         }
     }
     if (!HELD || !share) return;
@@ -237,7 +245,7 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_bwd(RmsArgs g) {
     for (int j = 0; j < V; ++j) {
         const int c = (j * TEAM + lane) * E;
         if (TEAMS == 1) {
-            if (c < g.D) dl_store<float, E>(share + c, gg[HELD ? j : 0]);
+            if (c < g.D) rms_store<ODD, float, E>(share + c, g.D - c, gg[HELD ? j : 0]);
             continue;
         }
         __syncthreads();
@@ -274,23 +282,24 @@ __global__ __launch_bounds__(256) void rms_join(const float *__restrict__ shares
 static int rms_team(int D, int e) { return D <= 8 * 4 * e ? 8 : D <= 64 * 4 * e ? 64 : D <= 256 * 4 * e ? 256 : D <= 1024 * 4 * e ? 1024 : -1; }
 static int rms_team_rows(int team) { return team < 0 || team > RMS_THREADS ? 1 : RMS_THREADS / team; }
 
-// vectors of 16 bytes where every row of every tensor starts on one, single values otherwise
-static int rms_vector(const RmsArgs &g, int type, int out_bytes) {
+// whether rows begin off a vector of 16 bytes, or end inside one
+static bool rms_odd(const RmsArgs &g, int type, int out_bytes) {
     const int size = dl_type_bytes(type), e = 16 / size;
     const int psize = g.gamma ? dl_type_bytes(g.ptype) : 2;
     const auto fits = [&](const void *p, int width) { return ((uintptr_t)p & (uintptr_t)(width * e < 16 ? width * e - 1 : 15)) == 0; };
     const bool fine = g.D % e == 0 && g.ldx % e == 0 && g.ldr % e == 0 && fits(g.x, size) && fits(g.res, size) && fits(g.h, size) &&
                       fits(g.gy, size) && fits(g.gh, size) && fits(g.gx, size) && fits(g.y, out_bytes) && fits(g.gamma, psize);
     // (gamma of float next to 16-bit rows: two loads of 16 bytes)
-    return fine ? e : 1;
+    return !fine;
 }
 
-template <typename T, int E, bool CODES>
+template <typename T, bool CODES, bool ODD>
 static void rms_launch_fwd(const RmsArgs &g, hipStream_t s) {
+    constexpr int E = 16 / sizeof(T);
     const int team = rms_team(g.D, E);
     const long long blocks = (g.rows + rms_team_rows(team) - 1) / rms_team_rows(team);
     const int vectors = team > 0 ? (g.D + team * E - 1) / (team * E) : 0;
-#define RMS_FWD(TEAM, V, HELD) hipLaunchKernelGGL((rms_fwd<T, E, V, TEAM, CODES, HELD>), dim3((unsigned)blocks), dim3(RmsTeam<TEAM>::THREADS), 0, s, g)
+#define RMS_FWD(TEAM, V, HELD) hipLaunchKernelGGL((rms_fwd<T, E, V, TEAM, CODES, HELD, ODD>), dim3((unsigned)blocks), dim3(RmsTeam<TEAM>::THREADS), 0, s, g)
 #define RMS_FWD_V(TEAM) \
     do { if (vectors <= 1) RMS_FWD(TEAM, 1, true); else if (vectors <= 2) RMS_FWD(TEAM, 2, true); else RMS_FWD(TEAM, 4, true); } while (0)
     DL_TIMED("rms_fwd", s, if (team == 8) RMS_FWD_V(8); else if (team == 64) RMS_FWD_V(64); else if (team == 256) RMS_FWD_V(256);
@@ -298,10 +307,11 @@ static void rms_launch_fwd(const RmsArgs &g, hipStream_t s) {
 #undef RMS_FWD_V
 #undef RMS_FWD
 }
-template <typename T, int E>
+template <typename T, bool ODD>
 static void rms_launch_bwd(const RmsArgs &g, int blocks, hipStream_t s) {
+    constexpr int E = 16 / sizeof(T);
     const int team = rms_team(g.D, E), vectors = team > 0 ? (g.D + team * E - 1) / (team * E) : 0;
-#define RMS_BWD(TEAM, V, HELD) hipLaunchKernelGGL((rms_bwd<T, E, V, TEAM, HELD>), dim3((unsigned)blocks), dim3(RmsTeam<TEAM>::THREADS), 0, s, g)
+#define RMS_BWD(TEAM, V, HELD) hipLaunchKernelGGL((rms_bwd<T, E, V, TEAM, HELD, ODD>), dim3((unsigned)blocks), dim3(RmsTeam<TEAM>::THREADS), 0, s, g)
 #define RMS_BWD_V(TEAM) \
     do { if (vectors <= 1) RMS_BWD(TEAM, 1, true); else if (vectors <= 2) RMS_BWD(TEAM, 2, true); else RMS_BWD(TEAM, 4, true); } while (0)
     DL_TIMED("rms_bwd", s, if (team == 8) RMS_BWD_V(8); else if (team == 64) RMS_BWD_V(64); else if (team == 256) RMS_BWD_V(256);
@@ -310,7 +320,7 @@ static void rms_launch_bwd(const RmsArgs &g, int blocks, hipStream_t s) {
 #undef RMS_BWD
 }
 
-// blocks of the backward: as many as have rows, up to RMS_SHARES (a team is smallest, and a block's rows most, without vectors)
+// blocks of the backward: as many as have rows, up to RMS_SHARES 
 static long long rms_bwd_blocks(long long rows, int team) {
     const long long need = (rows + rms_team_rows(team) - 1) / rms_team_rows(team);
     return need < RMS_SHARES ? need : RMS_SHARES;
@@ -337,14 +347,13 @@ extern "C" int dl_rms_norm_fwd(const void *x, long long ldx, const void *residua
     RmsArgs g{};
     g.x = x, g.ldx = ldx, g.res = residual, g.ldr = residual ? ldr : 0, g.gamma = gamma, g.h = residual ? h : nullptr, g.y = y, g.rstd = rstd, g.scale = scale;
     g.rows = rows, g.D = D, g.ptype = ptype, g.eps = eps;
-    const int e = rms_vector(g, type, scale ? 1 : dl_type_bytes(type));
-    if (!rms_grid_fits(rows, D, e)) return DL_ERR_UNSUPPORTED;
+    const bool odd = rms_odd(g, type, scale ? 1 : dl_type_bytes(type));
+    if (!rms_grid_fits(rows, D, 16 / dl_type_bytes(type))) return DL_ERR_UNSUPPORTED;
     const hipStream_t s = (hipStream_t)stream;
     DL_BY_TYPE(type, T, {
-        constexpr int E = 16 / sizeof(T);
-        if (scale) { if (e > 1) rms_launch_fwd<T, E, true>(g, s); else rms_launch_fwd<T, 1, true>(g, s); }
-        else if (e > 1) rms_launch_fwd<T, E, false>(g, s);
-        else rms_launch_fwd<T, 1, false>(g, s);
+        if (scale) { if (odd) rms_launch_fwd<T, true, true>(g, s); else rms_launch_fwd<T, true, false>(g, s); }
+        else if (odd) rms_launch_fwd<T, false, true>(g, s);
+        else rms_launch_fwd<T, false, false>(g, s);
     });
     return dl_launch_status();
 }
@@ -356,12 +365,11 @@ extern "C" int dl_quantize_rows(const void *x, long long ldx, void *codes, float
     if (ldx < D) return DL_ERR_SHAPE;
     RmsArgs g{};
     g.x = x, g.ldx = ldx, g.y = codes, g.scale = scale, g.rows = rows, g.D = D, g.plain = 1;
-    const int e = rms_vector(g, type, 1);
-    if (!rms_grid_fits(rows, D, e)) return DL_ERR_UNSUPPORTED;
+    const bool odd = rms_odd(g, type, 1);
+    if (!rms_grid_fits(rows, D, 16 / dl_type_bytes(type))) return DL_ERR_UNSUPPORTED;
     const hipStream_t s = (hipStream_t)stream;
     DL_BY_TYPE(type, T, {
-        constexpr int E = 16 / sizeof(T);
-        if (e > 1) rms_launch_fwd<T, E, true>(g, s); else rms_launch_fwd<T, 1, true>(g, s);
+        if (odd) rms_launch_fwd<T, true, true>(g, s); else rms_launch_fwd<T, true, false>(g, s);
     });
     return dl_launch_status();
 }
@@ -383,12 +391,11 @@ extern "C" int dl_rms_norm_bwd(const void *h, long long ldh, const void *gamma, 
     RmsArgs g{};
     g.x = h, g.ldx = ldh, g.gamma = gamma, g.rstd = const_cast<float *>(rstd), g.gy = gy, g.gh = gh, g.gx = gx, g.shares = ggamma ? (float *)ws : nullptr;
     g.rows = rows, g.D = D, g.ptype = ptype;
-    const int e = rms_vector(g, type, dl_type_bytes(type));
-    const int blocks = (int)rms_bwd_blocks(rows, rms_team(D, e));
+    const bool odd = rms_odd(g, type, dl_type_bytes(type));
+    const int blocks = (int)rms_bwd_blocks(rows, rms_team(D, 16 / dl_type_bytes(type)));
     const hipStream_t s = (hipStream_t)stream;
     DL_BY_TYPE(type, T, {
-        constexpr int E = 16 / sizeof(T);
-        if (e > 1) rms_launch_bwd<T, E>(g, blocks, s); else rms_launch_bwd<T, 1>(g, blocks, s);
+        if (odd) rms_launch_bwd<T, true>(g, blocks, s); else rms_launch_bwd<T, false>(g, blocks, s);
     });
     if (ggamma) DL_TIMED("rms_join", s, hipLaunchKernelGGL(rms_join, dim3(dl_ceil_div(D, 16)), dim3(256), 0, s, (const float *)ws, ggamma, ptype, blocks, D));
     return dl_launch_status();
