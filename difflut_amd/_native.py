@@ -121,6 +121,7 @@ SIGNATURES = {
     "dl_rms_norm_bwd_workspace_bytes": (_Z, [_L, _I]),
     "dl_rms_norm_bwd": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _P, _Z, _P]),
     "dl_linear_fwd_workspace_bytes": (_Z, [_P, _L, _P, _L, _I, _L, _L, _L, _I]),
+    "dl_linear_kept_bytes": (_Z, [_I, _L, _L, _I]),
     "dl_linear_fwd": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _L, _P, _P, _I, _I, _L, _L, _L, _I, _I, _P, _Z, _P]),
     "dl_linear_bwd_workspace_bytes": (_Z, [_P, _L, _P, _L, _P, _P, _I, _I, _L, _L, _L]),
     "dl_linear_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _L, _L, _L, _I, _I, _P, _Z, _P]),

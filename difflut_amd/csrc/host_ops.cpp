@@ -41,7 +41,7 @@ namespace {
     X(dl_group_norm_fwd) X(dl_group_norm_bwd_workspace_bytes) X(dl_group_norm_bwd) X(dl_dropout)                         \
     X(dl_sample_workspace_bytes) X(dl_sample)                                                                             \
     X(dl_rms_norm_fwd) X(dl_quantize_rows) X(dl_rms_norm_bwd_workspace_bytes) X(dl_rms_norm_bwd)                         \
-    X(dl_linear_fwd_workspace_bytes) X(dl_linear_fwd) X(dl_linear_bwd_workspace_bytes) X(dl_linear_bwd)                  \
+    X(dl_linear_fwd_workspace_bytes) X(dl_linear_kept_bytes) X(dl_linear_fwd) X(dl_linear_bwd_workspace_bytes) X(dl_linear_bwd)                  \
     X(dl_beam_step_workspace_bytes) X(dl_beam_step) X(dl_beam_reorder)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -1047,7 +1047,7 @@ struct Linear : torch::autograd::Function<Linear> {
         const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
         const int type = type_of(x, "x");
         const Tensor y = like_rows(x_, gated ? N / 2 : N, x.scalar_type());
-        const Tensor z = keep && (gated || act != DL_ACT_NONE) ? at::empty({M, N}, y.options()) : Tensor();
+        const Tensor z = keep && (gated || act != DL_ACT_NONE) ? bytes(L.dl_linear_kept_bytes(type, M, N, gated), x) : Tensor();
         const size_t need = L.dl_linear_fwd_workspace_bytes(raw_in(x), ld_of(x), raw_in(weight), ld_of(weight), type, M, N, K, gated);
         const Tensor ws = need ? bytes(need, x) : Tensor();
         check(L.dl_linear_fwd(raw_in(x), ld_of(x), nullptr, raw_in(weight), ld_of(weight), nullptr, raw_in(bias), raw_in(residual),

@@ -4,6 +4,8 @@
 //   linear    z[m,n] = sum_k x[m,k] w[n,k] + b[n],   y = act(z) + residual
 //   gated     z over 2 F rows of w, gate first:      y[m,f] = act(z[m,f]) z[m,F+f]
 //   backward  gz = gy act'(z)   (gated: gz[f] = gy z[F+f] act'(z[f]),  gz[F+f] = gy act(z[f])),  gb = sum_m gz,  gx = gz w,  gw = gz^T x
+//   kept for the backward: z.  In 16 bits that and gz would be two roundings, together with the gradient's own three of one size; so of 16-bit types
+//   24 bits of a float are kept, as a plane of 16 and one of 8.
 //
 // One product kernel serves all of them: C[r,c] = sum_k A(r,k) B(c,k).  An operand lies with the reduction along its rows of memory, or
 // (w for gx, gz and x for gw) with the reduction across them, and is turned on the way out of the LDS.  Operands whose rows do not
@@ -27,7 +29,7 @@ typedef int intx8 __attribute__((ext_vector_type(8)));
 #define LIN_STAGE_BYTES 128  // of a row in a stage: 32 float32, 64 16-bit or 128 8-bit values
 #define LIN_PLANES 3
 #define LIN_CUS 256
-enum { LIN_SUMS, LIN_PLAIN, LIN_PLAIN_ODD, LIN_ENDS, LIN_ENDS_ODD };
+enum { LIN_SUMS, LIN_PLAIN, LIN_PLAIN_ODD, LIN_ENDS, LIN_ENDS_ODD, LIN_KEEPS, LIN_KEEPS_ODD };
 
 struct LinF32 { static constexpr int SIZE = 4; };
 struct LinBf16 { static constexpr int SIZE = 2; };
@@ -36,16 +38,17 @@ struct LinE4m3 { static constexpr int SIZE = 1; };
 
 // (exponential and reciprocal as the hardware has them: an ulp each, and |z| u from the product with log2 e)
 __device__ __forceinline__ float lin_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+__device__ __forceinline__ float lin_relu(float z) { return z > 0.0f || z != z ? z : 0.0f; }
 __device__ __forceinline__ float lin_act(float z, int act) {
-    if (act == DL_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;
-    if (act == DL_ACT_SILU) return z * lin_sigmoid(z);
-    if (act == DL_ACT_SIGMOID) return lin_sigmoid(z);
-    return z;
+    if (act == DL_ACT_RELU) return lin_relu(z);
+    if (act == DL_ACT_NONE) return z;
+    const float s = lin_sigmoid(z);
+    return act == DL_ACT_SILU ? z * s : s;
 }
 // the activation's value and slope
 __device__ __forceinline__ float lin_slope(float z, int act, float &value) {
     if (act == DL_ACT_RELU) {
-        value = z > 0.0f || z != z ? z : 0.0f;
+        value = lin_relu(z);
         return z > 0.0f ? 1.0f : 0.0f;
     }
     if (act == DL_ACT_NONE) {
@@ -59,13 +62,32 @@ __device__ __forceinline__ float lin_slope(float z, int act, float &value) {
 
 // ------------------------------------------------------------------ what follows a product
 struct LinEnd {
-    void *y, *z;                // z (null: not kept): what the activation is applied to, in y's type
+    void *y, *kept;             // kept (null: not) for the backward: ldk values a row, gated the other half from `half` on; of 16-bit types their upper halves,
+    uint8_t *kept_low;          // and the eight bits below them
+    long long ldk;
+    int half;
     const void *bias, *res;
     const float *row_scale, *col_scale;  // of 8-bit operands
     long long ldr;
     int R, C, F, act;           // C: rows of w; F: columns of y where gated
     bool vec;                   // whole vectors of eight of everything, aligned
 };
+
+// rounded to 24 bits (what comes of 16-bit values carries no NaN that this would turn over)
+__device__ __forceinline__ uint32_t lin_kept_bits(float f) { return __float_as_uint(f) + 0x80u; }
+template <typename Out, int E>
+__device__ __forceinline__ void lin_keep(const LinEnd &g, int r, int c, const float (&f)[E]) {
+    const long long at = r * g.ldk + c;
+    if constexpr (sizeof(Out) == 4) dl_store<float, E>((float *)g.kept + at, f);
+    else {
+        DlVec<uint16_t, E> high;
+        DlVec<uint8_t, E> low;
+#pragma unroll
+        for (int i = 0; i < E; ++i) high.v[i] = (uint16_t)(lin_kept_bits(f[i]) >> 16), low.v[i] = (uint8_t)(lin_kept_bits(f[i]) >> 8);
+        *reinterpret_cast<DlVec<uint16_t, E> *>((uint16_t *)g.kept + at) = high;
+        *reinterpret_cast<DlVec<uint8_t, E> *>(g.kept_low + at) = low;
+    }
+}
 
 // What belongs to eight columns from c on, whatever the row; gated: of the gate and of the other half.  Past the last column: nothing.
 template <typename Out, bool GATED>
@@ -103,21 +125,12 @@ __device__ __forceinline__ void lin_finish(const LinEnd &g, const LinColumns<Out
         v[i] = SCALED ? fmaf(v[i], row_scale * k.scale[0][i], k.bias[0][i]) : v[i] + k.bias[0][i];
         if (GATED) u[i] = SCALED ? fmaf(u[i], row_scale * k.scale[H][i], k.bias[H][i]) : u[i] + k.bias[H][i];
     }
-    if (g.z) {
-        Out *z = (Out *)g.z + (long long)r * g.C + c;
-        dl_store<Out, 8>(z, v);
-        if (GATED) dl_store<Out, 8>(z + g.F, u);
+    if (g.kept) {
+        lin_keep<Out, 8>(g, r, c, v);
+        if (GATED) lin_keep<Out, 8>(g, r, g.half + c, u);
     }
-    if (g.act == DL_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = lin_act(v[i], DL_ACT_RELU);
-    } else if (g.act != DL_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float s = lin_sigmoid(v[i]);
-            v[i] = g.act == DL_ACT_SILU ? v[i] * s : s;
-        }
-    }
+    for (int i = 0; i < 8; ++i) v[i] = lin_act(v[i], g.act);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (GATED ? v[i] * u[i] : v[i]) + (float)res.v[i];
     dl_store<Out, 8>((Out *)g.y + (long long)r * width + c, v);
@@ -130,10 +143,10 @@ __device__ __forceinline__ void lin_finish_one(const LinEnd &g, int r, int c, fl
     const float row_scale = g.row_scale ? g.row_scale[r] : 1.0f;
     v = fmaf(v, row_scale * (g.col_scale ? g.col_scale[c] : 1.0f), g.bias ? (float)((const Out *)g.bias)[c] : 0.0f);
     if (GATED) u = fmaf(u, row_scale * (g.col_scale ? g.col_scale[g.F + c] : 1.0f), g.bias ? (float)((const Out *)g.bias)[g.F + c] : 0.0f);
-    if (g.z) {
-        Out *z = (Out *)g.z + (long long)r * g.C + c;
-        z[0] = (Out)v;
-        if (GATED) z[g.F] = (Out)u;
+    if (g.kept) {
+        const float first[1] = {v}, second[1] = {u};
+        lin_keep<Out, 1>(g, r, c, first);
+        if (GATED) lin_keep<Out, 1>(g, r, g.half + c, second);
     }
     const float y = lin_act(v, g.act);
     ((Out *)g.y)[(long long)r * width + c] = (Out)((GATED ? y * u : y) + (g.res ? (float)((const Out *)g.res)[r * g.ldr + c] : 0.0f));
@@ -402,8 +415,8 @@ __device__ __forceinline__ int lin_anew(int v) {
 // then, into the same place, A's one step later, so that loads are spread over the matrix instructions and have a stage's time to land.  One wavefront
 // a SIMD issues everything, so reads, loads and (of float32) cuts stand between the matrix instructions in the order written here; left
 // to itself the compiler puts the reads in front of their use.  Where the reduction ends inside a stage, that stage comes first.
-// WHAT becomes of the sums: LIN_SUMS partial sums, LIN_PLAIN nothing but the result, LIN_ENDS what follows; ODD: not all is in aligned
-// whole vectors.
+// WHAT becomes of the sums: LIN_SUMS partial sums, LIN_PLAIN nothing but the result, LIN_ENDS what follows, LIN_KEEPS that and
+// what is kept for the backward; ODD: not all is in aligned whole vectors.
 // There are as many blocks as the chip holds; one sends for its next tile's first stages before it writes a tile out.
 // Gated, a wavefront's columns are those of the gate, then the ones that belong to them.
 template <typename In, typename Out, int TR, int TC, bool TURN_A, bool TURN_B, bool GATED, int WHAT>
@@ -571,17 +584,20 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
 
     // C: a lane has row lane % 32 of a tile of 32 x 32, and columns (v % 4) + 8 (v / 4) + 4 (lane / 32) of it
     constexpr int W = FB * 32, H = GATED ? FB / 2 : FB;
-    constexpr bool PARTIAL = WHAT == LIN_SUMS, PLAIN = WHAT == LIN_PLAIN || WHAT == LIN_PLAIN_ODD, ODD = WHAT != LIN_PLAIN && WHAT != LIN_ENDS;
+    constexpr bool PARTIAL = WHAT == LIN_SUMS, PLAIN = WHAT == LIN_PLAIN || WHAT == LIN_PLAIN_ODD, ODD = WHAT != LIN_PLAIN && WHAT != LIN_ENDS && WHAT != LIN_KEEPS, KEEPS = WHAT == LIN_KEEPS || WHAT == LIN_KEEPS_ODD;
     typedef typename LinChoose<PARTIAL, float, Out>::type Stored;
-    typedef LinPlace<Stored, W> Products;               // z, or partial sums
+    typedef LinPlace<Stored, W> Products;               // partial sums, results of the backward
+    typedef LinPlace<uint16_t, W> KeptHigh;
+    typedef LinPlace<uint8_t, W> KeptLow;
     typedef LinPlace<Stored, GATED ? HALF : W> Results;
-    static_assert(WAVES * Products::BYTES <= TileA::BYTES + TileB::BYTES, "fits the last two places");
+    constexpr int PLACE = (TileA::BYTES + TileB::BYTES) / WAVES;  // of a wavefront, in the last two places
+    static_assert(Products::BYTES <= PLACE && KeptHigh::BYTES + KeptLow::BYTES <= PLACE, "fits the last two places");
     constexpr bool SCALED = In::SIZE == 1;
     static_assert(!PLAIN || (!SCALED && !GATED), "something follows");
     const auto write_plain = [&](int row0, int column0, int plane) __attribute__((always_inline)) {
         const int lane = lin_anew(threadIdx.x & 63), c = column0 + wc;
         Stored *const out = PARTIAL ? (Stored *)(void *)g.part + (long long)plane * g.end.R * g.end.C : (Stored *)g.end.y;
-        char *mine = lds + B1 + wave * Products::BYTES;
+        char *mine = lds + B1 + wave * PLACE;
         lin_each<0, FA>([&](auto phase) __attribute__((always_inline)) {
             constexpr int i = decltype(phase)::value;
             const int r = row0 + wr + i * 32;
@@ -602,14 +618,14 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
         });
     };
     const auto write = [&](int row0, int column0) __attribute__((always_inline)) {
-        const int lane = lin_anew(threadIdx.x & 63), kh = lane >> 5, l32 = lane & 31;
+        const int lane0 = threadIdx.x & 63;
         const LinEnd &e = g.end;
-        char *mine = lds + B1 + wave * Products::BYTES;
+        char *mine = lds + B1 + wave * PLACE;
         const int width = GATED ? e.F : e.C, c = column0 + (GATED ? wc / 2 : wc), columns = width - c;
         LinFour<Stored> bias[FB][4];
         LinFour<float> scale[SCALED ? FB : 1][4];
         const auto of_columns = [&]() __attribute__((always_inline)) {
-            const int first = lin_anew(c + 4 * kh);
+            const int first = lin_anew(c + 4 * (lane0 >> 5));
 #pragma unroll
             for (int j = 0; j < FB; ++j)
 #pragma unroll
@@ -624,6 +640,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
         if (HELD) of_columns();
         lin_each<0, FA>([&](auto phase) __attribute__((always_inline)) {
             constexpr int i = decltype(phase)::value;
+            const int lane = lin_anew(lane0), kh = lane >> 5, l32 = lane & 31;
             const int r = row0 + wr + i * 32, rows = e.R - r;
             if constexpr (TR * TC > 128 * 128) {
 #pragma unroll
@@ -651,13 +668,33 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
                     const float b = bias[j][v / 4].value(v % 4);
                     f[j][v] = SCALED ? fmaf(acc[i][j][v], row_scale * scale[SCALED ? j : 0][v / 4].value(v % 4), b) : acc[i][j][v] + b;
                 }
-            if (e.z) {
+            const auto keep = [&](int column, const float (&v)[16]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int j = 0; j < FB; ++j)
+                for (int q = 0; q < 4; ++q) {
+                    const int at = column + 8 * q + 4 * kh;
+                    if constexpr (sizeof(Stored) == 4) Products::put(mine, l32, at, {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
+                    else {
+                        uint32_t w[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) Products::put(mine, l32, j * 32 + 8 * q + 4 * kh, {f[j][4 * q], f[j][4 * q + 1], f[j][4 * q + 2], f[j][4 * q + 3]});
+                        for (int i = 0; i < 4; ++i) w[i] = lin_kept_bits(v[4 * q + i]);
+                        // (selectors: bytes 3 and 2 of both; byte 1 of both)
+                        *reinterpret_cast<uint2 *>(mine + KeptHigh::four(l32, at)) = uint2{__builtin_amdgcn_perm(w[1], w[0], 0x07060302), __builtin_amdgcn_perm(w[3], w[2], 0x07060302)};
+                        *reinterpret_cast<uint32_t *>(mine + KeptHigh::BYTES + KeptLow::four(l32, at)) =
+                            __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0501), __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0501), 0x05040100);
+                    }
+                }
+            };
+            if constexpr (KEEPS) {
+#pragma unroll
+                for (int j = 0; j < FB; ++j) keep(j * 32, f[j]);
+                const long long at = r * e.ldk + c;
+                const int padded = (columns + 15) / 16 * 16;  // (its rows are)
                 lin_lds_done();
-                Products::template send<ODD, GATED>(mine, lane, (Stored *)e.z + (long long)r * e.C + c, e.C, rows, columns, e.F);
+                if constexpr (sizeof(Stored) == 4) Products::template send<false, GATED>(mine, lane, (Stored *)e.kept + at, e.ldk, rows, padded, e.half);
+                else {
+                    KeptHigh::template send<false, GATED>(mine, lane, (uint16_t *)e.kept + at, e.ldk, rows, padded, e.half);
+                    KeptLow::template send<false, GATED>(mine + KeptHigh::BYTES, lane, e.kept_low + at, e.ldk, rows, padded, e.half);
+                }
                 lin_lds_done();
             }
             if (e.res) {
@@ -667,20 +704,17 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
             }
 #pragma unroll
             for (int j = 0; j < H; ++j) {
-                if (e.act == DL_ACT_RELU) {
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) f[j][v] = lin_act(f[j][v], DL_ACT_RELU);
-                } else if (e.act != DL_ACT_NONE) {
+                const auto follow = [&](int act) __attribute__((always_inline)) {
 #pragma unroll
                     for (int v = 0; v < 16; ++v) {
-                        const float s = lin_sigmoid(f[j][v]);
-                        f[j][v] = e.act == DL_ACT_SILU ? f[j][v] * s : s;
+                        f[j][v] = lin_act(f[j][v], act);
+                        if (GATED) f[j][v] *= f[j + FB - H][v];
                     }
-                }
-                if (GATED) {
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) f[j][v] *= f[j + FB - H][v];
-                }
+                };
+                if (e.act == DL_ACT_NONE) follow(DL_ACT_NONE);
+                else if (e.act == DL_ACT_RELU) follow(DL_ACT_RELU);
+                else if (e.act == DL_ACT_SILU) follow(DL_ACT_SILU);
+                else follow(DL_ACT_SIGMOID);
                 if (e.res) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -961,10 +995,15 @@ template <typename In, typename Out, int T, bool TURN_A, bool TURN_B>
 static int lin_launch_tile(const LinArgs &g, bool gated, hipStream_t s) {
     const LinEnd &e = g.end;
     if (g.splits > 1) return lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_SUMS>(g, s);
-    const bool plain = TURN_B || (!gated && !e.row_scale && !e.bias && !e.res && !e.z && e.act == DL_ACT_NONE);
+    const bool plain = TURN_B || (!gated && !e.row_scale && !e.bias && !e.res && !e.kept && e.act == DL_ACT_NONE);
     if constexpr (In::SIZE > 1)
         if (plain) return e.vec ? lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_PLAIN>(g, s) : lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_PLAIN_ODD>(g, s);
     if constexpr (!TURN_B) {
+        if constexpr (In::SIZE > 1)
+            if (e.kept) {
+                if (gated) return e.vec ? lin_go<In, Out, T, false, false, true, LIN_KEEPS>(g, s) : lin_go<In, Out, T, false, false, true, LIN_KEEPS_ODD>(g, s);
+                return e.vec ? lin_go<In, Out, T, false, false, false, LIN_KEEPS>(g, s) : lin_go<In, Out, T, false, false, false, LIN_KEEPS_ODD>(g, s);
+            }
         if (gated) return e.vec ? lin_go<In, Out, T, false, false, true, LIN_ENDS>(g, s) : lin_go<In, Out, T, false, false, true, LIN_ENDS_ODD>(g, s);
         return e.vec ? lin_go<In, Out, T, false, false, false, LIN_ENDS>(g, s) : lin_go<In, Out, T, false, false, false, LIN_ENDS_ODD>(g, s);
     }

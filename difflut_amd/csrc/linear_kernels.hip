@@ -21,14 +21,29 @@ __global__ __launch_bounds__(256) void lin_pad(const T *__restrict__ src, long l
 }
 
 // ------------------------------------------------------------------ the gradient in front of the products, and its column sums
-// gz [M, ldg] (null: not written) from gy and z (null: no activation, gz is gy), and a share of sum_m gz per block of rows (null: not asked for).
-// A thread takes E columns of every fourth row of its block's; gated: of the gate and of the other half.  Rows of gz are whole units of 16 bytes,
-// zeros behind the N-th column, as the products read them; those of gy and z
-// may begin anywhere and end inside a unit (ODD).
+// gz [M, ldg] (null: not written) from gy and z as it was kept (null: no activation, gz is gy), and a share of sum_m gz per block of rows (null: not
+// asked for).  A thread takes E columns of every fourth row of its block's; gated: of the gate and of the other half.  Rows of gz are whole units of
+// 16 bytes, zeros behind the N-th column, as the products read them; those of gy may begin anywhere and end inside a unit (ODD).
 #define LIN_SLOPE_ROWS 64
+struct LinKept {
+    const void *high;
+    const uint8_t *low;
+    long long ld;
+    int half;
+};
+template <typename T, int E>
+__device__ __forceinline__ void lin_kept(const LinKept &k, long long at, float (&f)[E]) {
+    if constexpr (sizeof(T) == 4) dl_load<float, E>((const float *)k.high + at, f);
+    else {
+        const DlVec<uint16_t, E> high = *reinterpret_cast<const DlVec<uint16_t, E> *>((const uint16_t *)k.high + at);
+        const DlVec<uint8_t, E> low = *reinterpret_cast<const DlVec<uint8_t, E> *>(k.low + at);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = __uint_as_float((uint32_t)high.v[i] << 16 | (uint32_t)low.v[i] << 8);
+    }
+}
 template <typename T, bool GATED, bool ODD>
-__global__ __launch_bounds__(256) void lin_gradient(const T *__restrict__ gy, const T *__restrict__ z, T *__restrict__ gz, float *__restrict__ shares,
-                                                    long long M, int N, long long ldg, int act, int col_tiles, int rows) {
+__global__ __launch_bounds__(256) void lin_gradient(const T *__restrict__ gy, LinKept kept, T *__restrict__ gz, float *__restrict__ shares, long long M, int N,
+                                                    long long ldg, int act, int col_tiles, int rows) {
     constexpr int H = GATED ? 2 : 1, E = 16 / sizeof(T);
     __shared__ float part[H * 4][64 * E];
     const int lane = threadIdx.x & 63, team = threadIdx.x >> 6, width = GATED ? N / 2 : N;
@@ -41,16 +56,13 @@ __global__ __launch_bounds__(256) void lin_gradient(const T *__restrict__ gy, co
         for (int i = 0; i < E; ++i) sum[h][i] = 0.0f;
     if (n > 0)
         for (long long m = m0 + team; m < m1; m += 4) {
-            const auto load = [&](const T *p, float (&f)[E]) __attribute__((always_inline)) {
-                if (ODD) dl_load_some<T, E>(p, n, f);
-                else dl_load<T, E>(p, f);
-            };
             float g[H][E];
-            load(gy + m * width + c, g[0]);
-            if (z) {
+            if (ODD) dl_load_some<T, E>(gy + m * width + c, n, g[0]);
+            else dl_load<T, E>(gy + m * width + c, g[0]);
+            if (kept.high) {
                 float a[H][E];
-                load(z + m * N + c, a[0]);
-                if (GATED) load(z + m * N + width + c, a[H - 1]);
+                lin_kept<T, E>(kept, m * kept.ld + c, a[0]);
+                if (GATED) lin_kept<T, E>(kept, m * kept.ld + kept.half + c, a[H - 1]);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     float value;
@@ -180,7 +192,7 @@ static int lin_run(const LinOperand &a, const LinOperand &b, int type, int out_t
     g.part = (float *)(ws + p.a_bytes + p.b_bytes);
     end.R = (int)a.count(), end.C = (int)b.count(), end.F = end.C / 2;
     const int width = gated ? end.F : end.C, size = dl_type_bytes(out_type);
-    end.vec = width % 8 == 0 && dl_aligned16(end.y) && dl_aligned16(end.z) && dl_aligned16(end.bias) && dl_aligned16(end.res) && dl_aligned16(end.col_scale) && end.ldr * size % 16 == 0;
+    end.vec = width % 8 == 0 && dl_aligned16(end.y) && dl_aligned16(end.bias) && dl_aligned16(end.res) && dl_aligned16(end.col_scale) && end.ldr * size % 16 == 0;
     g.K = K, g.stages = dl_ceil_div(K * lin_size(type), LIN_STAGE_BYTES), g.chunk = p.chunk, g.splits = p.splits;
     if (!p.few) g.row_tiles = dl_ceil_div(end.R, p.tile), g.col_tiles = gated && p.splits == 1 ? dl_ceil_div(end.F, p.tile / 2) : dl_ceil_div(end.C, p.tile);
     g.end = end;
@@ -207,18 +219,33 @@ extern "C" size_t dl_linear_fwd_workspace_bytes(const void *x, long long ldx, co
     return lin_plan({x, ldx, M, K, false}, {w, ldw, N, K, false}, type, K, gated != 0).bytes();
 }
 
+// what is kept for the backward: rows of whole sixteens (gated: of both halves), of 16-bit types in two planes
+static void lin_keep_in(LinEnd &end, void *kept, int type, long long M, long long N, bool gated) {
+    end.half = (int)((N / 2 + 15) / 16 * 16), end.ldk = gated ? 2LL * end.half : (N + 15) / 16 * 16, end.kept = kept;
+    end.kept_low = kept && type != DL_F32 ? (uint8_t *)kept + dl_align256((size_t)M * end.ldk * 2) : nullptr;
+}
+extern "C" size_t dl_linear_kept_bytes(int type, long long M, long long N, int gated) {
+    if (lin_check(type, type, M, N, 1, 0, gated) != DL_OK || !dl_type_known(type)) return 0;
+    LinEnd end{};
+    lin_keep_in(end, nullptr, type, M, N, gated != 0);
+    return type == DL_F32 ? (size_t)M * end.ldk * 4 : dl_align256((size_t)M * end.ldk * 2) + (size_t)M * end.ldk;
+}
+
 extern "C" int dl_linear_fwd(const void *x, long long ldx, const float *x_scale, const void *w, long long ldw, const float *w_scale, const void *bias,
-                             const void *residual, long long ldr, void *y, void *z, int type, int out_type, long long M, long long N, long long K, int act,
+                             const void *residual, long long ldr, void *y, void *kept, int type, int out_type, long long M, long long N, long long K, int act,
                              int gated, void *ws, size_t ws_bytes, void *stream) {
     if (!x || !w || !y || ((x_scale || w_scale) != (type == DL_E4M3)) || (type == DL_E4M3 && (!x_scale || !w_scale))) return DL_ERR_NULL;
     const int bad = lin_check(type, out_type, M, N, K, act, gated);
     if (bad) return bad;
     if (ldx < K || ldw < K || (residual && ldr < (gated ? N / 2 : N))) return DL_ERR_SHAPE;
+    if (kept && type == DL_E4M3) return DL_ERR_UNSUPPORTED;
+    if (!dl_aligned16(kept)) return DL_ERR_WORKSPACE;
     const size_t need = dl_linear_fwd_workspace_bytes(x, ldx, w, ldw, type, M, N, K, gated);
     if (need && !ws) return DL_ERR_NULL;
     if (ws_bytes < need || (need && !dl_aligned16(ws))) return DL_ERR_WORKSPACE;
     LinEnd end{};
-    end.y = y, end.z = z, end.bias = bias, end.res = residual, end.ldr = residual ? ldr : 0, end.row_scale = x_scale, end.col_scale = w_scale, end.act = act;
+    end.y = y, end.bias = bias, end.res = residual, end.ldr = residual ? ldr : 0, end.row_scale = x_scale, end.col_scale = w_scale, end.act = act;
+    if (kept) lin_keep_in(end, kept, type, M, N, gated != 0);
     return lin_run({x, ldx, M, K, false}, {w, ldw, N, K, false}, type, out_type, K, gated != 0, end, (char *)ws, (hipStream_t)stream);
 }
 
@@ -253,22 +280,23 @@ static LinOperand lin_gz(const void *ws, const void *gy, bool kept, int type, lo
     return {ws ? ws : (const void *)256, (N + unit - 1) / unit * unit, M, N, false, true};
 }
 
-extern "C" size_t dl_linear_bwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, int wants, int type,
+extern "C" size_t dl_linear_bwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, const void *kept, const void *gy, int wants, int type,
                                                 long long M, long long N, long long K) {
     if (lin_check(type, type, M, N, K, 0, 0) != DL_OK) return 0;
-    return lin_back(lin_gz(nullptr, gy, z != nullptr, type, M, N), {x, ldx, M, K, false}, {w, ldw, N, K, false}, type, z != nullptr, wants, N, K).bytes();
+    return lin_back(lin_gz(nullptr, gy, kept != nullptr, type, M, N), {x, ldx, M, K, false}, {w, ldw, N, K, false}, type, kept != nullptr, wants, N, K).bytes();
 }
 
-extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, void *gx, void *gw, void *gb, int type,
+extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, const void *keeping, const void *gy, void *gx, void *gw, void *gb, int type,
                              long long M, long long N, long long K, int act, int gated, void *ws, size_t ws_bytes, void *stream) {
-    if (!gy || (gx && !w) || (gw && !x) || ((gated || act != DL_ACT_NONE) && !z)) return DL_ERR_NULL;
+    if (!gy || (gx && !w) || (gw && !x) || ((gated || act != DL_ACT_NONE) && !keeping)) return DL_ERR_NULL;
     const int bad = lin_check(type, type, M, N, K, act, gated);
     if (bad) return bad;
     if (N * lin_size(type) > LIN_MOST_ROW) return DL_ERR_UNSUPPORTED;
     if ((gx && ldw < K) || (gw && ldx < K)) return DL_ERR_SHAPE;
     const int wants = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
     if (!wants) return DL_OK;
-    const bool kept = z != nullptr;
+    if (!dl_aligned16(keeping)) return DL_ERR_WORKSPACE;
+    const bool kept = keeping != nullptr;
     const LinOperand gz = lin_gz(ws, gy, kept, type, M, N), xo = {x, ldx, M, K, false}, wo = {w, ldw, N, K, false};
     const LinBack p = lin_back(gz, xo, wo, type, kept, wants, N, K);
     if (p.bytes() && !ws) return DL_ERR_NULL;
@@ -278,12 +306,18 @@ extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long l
     if (kept || gb) {
         void *out = kept ? ws : nullptr;
         const int width = (int)(gated ? N / 2 : N);
-#define LIN_GRADIENT(GATED, ODD) hipLaunchKernelGGL((lin_gradient<T, GATED, ODD>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)gy, (const T *)z, (T *)out, shares, M, (int)N, gz.ld, act, col_tiles, p.rows)
+        LinKept factors{};
+        if (kept) {
+            LinEnd layout{};
+            lin_keep_in(layout, const_cast<void *>(keeping), type, M, N, gated != 0);
+            factors = {keeping, layout.kept_low, layout.ldk, layout.half};
+        }
+#define LIN_GRADIENT(GATED, ODD) hipLaunchKernelGGL((lin_gradient<T, GATED, ODD>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)gy, factors, (T *)out, shares, M, (int)N, gz.ld, act, col_tiles, p.rows)
         DL_BY_TYPE(type, T, {
             const int col_tiles = dl_ceil_div(width, 64 * (16 / (int)sizeof(T)));
             const long long blocks = (long long)col_tiles * p.pieces;
             if (!dl_grid_ok(blocks, 256)) return DL_ERR_UNSUPPORTED;
-            const bool odd = width % (16 / (int)sizeof(T)) != 0 || !dl_aligned16(gy) || !dl_aligned16(z);
+            const bool odd = width % (16 / (int)sizeof(T)) != 0 || !dl_aligned16(gy);
             DL_TIMED("lin_gradient", s, if (gated) { if (odd) LIN_GRADIENT(true, true); else LIN_GRADIENT(true, false); }
                      else if (odd) LIN_GRADIENT(false, true); else LIN_GRADIENT(false, false));
             if (gb) DL_TIMED("lin_columns", s, hipLaunchKernelGGL((lin_columns<T>), dim3(dl_ceil_div(N, 16)), dim3(256), 0, s, shares, (T *)gb, p.pieces, (int)N));

@@ -566,20 +566,22 @@ int dl_rms_norm_bwd(const void *h, long long ldh, const void *gamma, const float
                     int ptype, long long rows, int D, void *ws, size_t ws_bytes, void *stream);
 
 /* Matrix product with what follows it: s = x w^T + bias over x [M, K], w [N, K] (ldx, ldw elements between rows), y = act(s) + residual [M, N];
- * gated: N is even, the first N / 2 rows of w are the gate's, y = act(s[:, :N/2]) * s[:, N/2:] + residual [M, N / 2].  z [M, N] (nullable)
- * receives s in y's type, for the backward.  bias, residual (ldr) and z may be null.  All of type `type` = out_type, or x and w of DL_E4M3 with
- * their rows' scales and the rest of out_type (inference; no z needed).  y and z are contiguous.
- * Backward: from gy (contiguous, y's shape) the gradients gx [M, K], gw [N, K], gb [N], each nullable; z as the forward left it (null where act
+ * gated: N is even, the first N / 2 rows of w are the gate's, y = act(s[:, :N/2]) * s[:, N/2:] + residual [M, N / 2].  bias, residual (ldr)
+ * and kept may be null.  All of type `type` = out_type, or x and w of DL_E4M3 with their rows' scales and the rest of out_type (inference: nothing kept).
+ * y is contiguous.  kept (dl_linear_kept_bytes, on 16 bytes) receives s for the backward, in 24 bits of a float or, of DL_F32, 32; its
+ * layout is the library's own.
+ * Backward: from gy (contiguous, y's shape) the gradients gx [M, K], gw [N, K], gb [N], each nullable; kept as the forward left it (null where act
  * is DL_ACT_NONE and not gated); the residual's gradient is gy.  `wants` of the size query: 1 gx, 2 gw, 4 gb.
  * The size queries look at pointers for their alignment alone.  Rows of operands up to 2^23 bytes, in the backward also M and N up to 2^22
  * (DL_ERR_UNSUPPORTED beyond). */
 size_t dl_linear_fwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, int type, long long M, long long N, long long K, int gated);
+size_t dl_linear_kept_bytes(int type, long long M, long long N, int gated);
 int dl_linear_fwd(const void *x, long long ldx, const float *x_scale, const void *w, long long ldw, const float *w_scale, const void *bias,
-                  const void *residual, long long ldr, void *y, void *z, int type, int out_type, long long M, long long N, long long K, int act, int gated,
+                  const void *residual, long long ldr, void *y, void *kept, int type, int out_type, long long M, long long N, long long K, int act, int gated,
                   void *ws, size_t ws_bytes, void *stream);
-size_t dl_linear_bwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, int wants, int type,
+size_t dl_linear_bwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, const void *kept, const void *gy, int wants, int type,
                                      long long M, long long N, long long K);
-int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, const void *z, const void *gy, void *gx, void *gw, void *gb, int type,
+int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, const void *kept, const void *gy, void *gx, void *gw, void *gb, int type,
                   long long M, long long N, long long K, int act, int gated, void *ws, size_t ws_bytes, void *stream);
 
 /* A step of beam search: of every sequence's K beams over V tokens the `count` continuations with the largest

@@ -208,7 +208,7 @@ def linear_64(x, w, b, r, act, gated, gy):
     if b is not None:
         z = z + b.double()
         z_off = z_off + z.abs() * U
-    zk_off = z_off + z.abs() * h  # as it is kept
+    zk_off = z_off + z.abs() * (0.0 if dtype is torch.float32 else 2.0 ** -16)  # as it is kept: 24 bits of a float, 16 of them the value's
 
     def followed(t, off):
         value, slope, curve = act_64(t, act)
