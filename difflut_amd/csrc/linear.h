@@ -992,7 +992,7 @@ static int lin_go(const LinArgs &g, hipStream_t s) {
 }
 // (the backward's products: nothing follows)
 template <typename In, typename Out, int T, bool TURN_A, bool TURN_B>
-static int lin_launch_tile(const LinArgs &g, bool gated, hipStream_t s) {
+int lin_launch_tile(const LinArgs &g, bool gated, hipStream_t s) {
     const LinEnd &e = g.end;
     if (g.splits > 1) return lin_go<In, Out, T, TURN_A, TURN_B, false, LIN_SUMS>(g, s);
     const bool plain = TURN_B || (!gated && !e.row_scale && !e.bias && !e.res && !e.kept && e.act == DL_ACT_NONE);
@@ -1027,7 +1027,8 @@ static int lin_launch_turned(LinArgs &g, const LinPlan &p, bool turn_a, bool tur
     return turn_b ? lin_launch<In, Out, false, true>(g, p, gated, s) : lin_launch<In, Out, false, false>(g, p, gated, s);
 }
 
-// One translation unit for every type of operands
+// Translation units: one for every type of operands, where its kernels are few; else these are instantiated in units of their own.
+#define LIN_TILE(In, Out, T, TURN_A, TURN_B) template int lin_launch_tile<In, Out, T, TURN_A, TURN_B>(const LinArgs &g, bool gated, hipStream_t s)
 int lin_launch_f32(LinArgs &g, const LinPlan &p, bool turn_a, bool turn_b, bool gated, hipStream_t s);
 int lin_launch_bf16(LinArgs &g, const LinPlan &p, bool turn_a, bool turn_b, bool gated, hipStream_t s);
 int lin_launch_f16(LinArgs &g, const LinPlan &p, bool turn_a, bool turn_b, bool gated, hipStream_t s);
