@@ -299,6 +299,63 @@ def test_linear_of_many_tiles(M, K, N, dtype, gated):
     check_linear("cuda", M, K, N, dtype, "silu", gated, True, True)
 
 
+# few rows: short and long reductions, rows of w shared by two wavefronts or eight, the last group inside a block, up to 16, 32 and 64 rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,dtype,gated", [
+    (1, 33, 70001, torch.bfloat16, False), (3, 100, 40000, torch.float16, False), (16, 96, 66000, torch.bfloat16, True), (5, 40, 33002, torch.float32, True),
+    (20, 64, 70010, torch.float16, False), (32, 1000, 4098, torch.float32, False), (31, 77, 66002, torch.float32, False), (48, 300, 2050, torch.bfloat16, True),
+    (64, 2047, 1030, torch.float16, True), (2, 4001, 17, torch.bfloat16, False), (16, 8200, 40, torch.float32, False), (1, 1, 50000, torch.float32, False)])
+def test_linear_of_few_rows(M, K, N, dtype, gated):
+    check_linear("cuda", M, K, N // 2 * 2 if gated else N, dtype, "sigmoid" if gated else "silu", gated, True, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(5, 64, 34), (40, 72, 514), (130, 257, 130), (300, 129, 2050), (4100, 200, 4104), (4101, 130, 4098), (9001, 64, 512)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "sigmoid"])
+def test_linear_of_inference_is_that_of_training(M, K, N, dtype, gated, act):
+    """Kernels that keep nothing for a backward give the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    x, w, b = (torch.randn(s, device="cuda", generator=g).to(dtype) for s in ((M, K), (N, K), (N,)))
+    r = torch.randn(M, N // 2 if gated else N, device="cuda", generator=g).to(dtype)
+    f = ops.gated_linear if gated else ops.linear
+    for bias, residual in ((b, r), (None, None)):
+        with torch.no_grad():
+            want = f(x, w, bias, activation=act, residual=residual)
+        assert torch.equal(f(x, w.detach().requires_grad_(), bias, activation=act, residual=residual), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_streams_at_once(dtype):
+    """The same operators on other data on two streams, turn by turn without waiting, are those of one after the other."""
+    p = block_parameters(dtype, "cuda")
+    data = []
+    for seed in (1, 2):
+        g = gen(seed)
+        data.append(([torch.randn(1500, 64, generator=g).to(dtype).cuda() for _ in range(3)], torch.randn(4, 6, 20001, generator=g).to(dtype).cuda()))
+
+    def everything(d):
+        (x, r, gy), logits = d
+        y = block_step(p, x, r)
+        grads = torch.autograd.grad(y, list(p.values()), gy)
+        step = ops.beam_step(logits, torch.zeros(4, 6, device="cuda"))
+        return [y, *grads, *step, *ops.beam_reorder([logits], step[1])]
+
+    want = [everything(d) for d in data]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in data], [[], []]
+    for _ in range(3):
+        for k, (s, d) in enumerate(zip(streams, data)):
+            with torch.cuda.stream(s):
+                got[k].append(everything(d))
+    torch.cuda.synchronize()
+    for a, runs in zip(want, got):
+        for b in runs:
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 @pytest.mark.parametrize("M,K,N", [(40, 100, 60), (300, 129, 257), (3, 640, 1000), (1, 24, 7)])
 @pytest.mark.parametrize("dtype", TYPES)
@@ -457,6 +514,25 @@ def test_linear_codes_of_strangers(device):
     y = ops.linear_codes(codes, scale, w, sw, dtype=torch.float32).cpu()
     assert not y[0].any() and y[1].isnan().all()
     close(y[2], torch.full((8,), 32.0), torch.full((8,), 32 * 40 * U), torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,dtype,gated", [(1, 5000, 40000, torch.bfloat16, False), (7, 100, 33000, torch.float32, True), (30, 260, 4100, torch.float16, False), (60, 512, 2052, torch.bfloat16, True),
+                                               (4200, 144, 4230, torch.bfloat16, True), (4200, 128, 4224, torch.float16, False)])
+def test_linear_codes_of_few_and_many_rows(M, K, N, dtype, gated):
+    g = gen(M + N)
+    (x, sx), (w, sw) = (tuple(t.cuda() for t in coded(s, g, d)) for s, d in (((M, K), 1.0), ((N, K), 1 / math.sqrt(K))))
+    out = N // 2 if gated else N
+    b, r = torch.randn(N, generator=g).to(dtype).cuda(), torch.randn(M, out, generator=g).to(dtype).cuda()
+    y = ops.linear_codes(x, sx, w, sw, b, "silu", r, gated, dtype)
+    wide, wide_w = x.double() * sx.double()[:, None], w.double() * sw.double()[:, None]
+    for rows in range(0, M, 600):  # (in pieces: what the sums leave out is a number for every product of a step)
+        part = slice(rows, min(M, rows + 600))
+        (want, off), *_ = linear_64(wide[part], wide_w, b, r[part], "silu", gated, torch.zeros(part.stop - part.start, out, device="cuda"))
+        size = wide[part].abs() @ wide_w.abs().t() * 4 * U + torch.cat([cut_64(q, wide_w) for q in wide[part].split(8)])
+        size = size[:, :out] + size[:, out:] if gated else size
+        other = 1.0 if not gated else 1 + (wide[part] @ wide_w.t() + b.double()).abs().amax()
+        close(y[part], want, off + size * other, dtype)
 
 
 # ----------------------------------------------------------------------------- beam search
