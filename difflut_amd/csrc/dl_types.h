@@ -86,6 +86,23 @@ __device__ __forceinline__ void dl_store_some(T *p, int n, const float (&f)[E]) 
     }
 }
 
+// Sum of a column of `count` rows of `width` floats, in a fixed order, by a block of 1024 that takes 16 columns: thread t rows t / 16, + 64, ...
+// The first 16 threads have it.
+__device__ __forceinline__ float dl_column_sum(const float *__restrict__ rows, int count, int width, int column) {
+    __shared__ float part[64][17];
+    const int k = threadIdx.x >> 4, c = threadIdx.x & 15;
+    float t = 0.0f;
+    if (column < width)
+#pragma unroll 8
+        for (int r = k; r < count; r += 64) t += rows[(long long)r * width + column];
+    part[k][c] = t;
+    __syncthreads();
+    if (k == 0)
+#pragma unroll 8
+        for (int i = 1; i < 64; ++i) t += part[i][c];
+    return t;
+}
+
 static inline bool dl_type_known(int type) { return type == DL_F32 || type == DL_BF16 || type == DL_F16; }
 static inline int dl_type_bytes(int type) { return type == DL_F32 ? 4 : 2; }
 static inline bool dl_grid_ok(long long blocks, int threads) { return blocks * threads < (1LL << 32); }  // work items of a launch

@@ -14,7 +14,9 @@
 // float32 values are cut into three bf16 planes on the way out of the LDS (8 + 8 + 8 significant bits, each the rounding of what the ones
 // above left); a product is the six plane products hi*lo, lo*hi, mid*mid, hi*mid, mid*hi, hi*hi, small ones first.  What is left out is
 // below 2^-26 of |a b|, less than the 2^-24 of one fp32 multiply-add.  Six bf16 products at 2.5 PFLOP/s are 417 TFLOP/s of fp32 work
-// against 157 on the fp32 matrix cores.  (Planes carry no infinities: such a product is NaN.)
+// against 157 on the fp32 matrix cores; 4096^3 takes 600 us (229 TFLOP/s), 2 M N K on the fp32 cores by the library 900.  What bounds it is the cuts'
+// instructions, which do not run beside a matrix instruction: 6144 cycles of these a stage of 256 x 256 and 3264 of those are the 4.7 us that one takes.
+// (Planes carry no infinities: such a product is NaN.)
 #pragma once
 #include <utility>
 
@@ -418,6 +420,9 @@ __device__ __forceinline__ int lin_anew(int v) {
 // WHAT becomes of the sums: LIN_SUMS partial sums, LIN_PLAIN nothing but the result, LIN_ENDS what follows, LIN_KEEPS that and
 // what is kept for the backward; ODD: not all is in aligned whole vectors.
 // There are as many blocks as the chip holds; one sends for its next tile's first stages before it writes a tile out.
+// bf16, 8192^3: 787 us, 1.40 PFLOP/s, a large library product's rate; what bounds it is power: the matrix cores are busy half of the time at 1.8 to 2.2 GHz
+// (2.4 without load), in every form tried.  8 bits, 8192 x 4096 x 16384 with silu: 480 us, 2.29 PFLOP/s.  A tile's end takes 5 us where nothing follows
+// the product (a stage takes 1.6), 9 with a gate and what is kept: 12544 x 1024 x 8192 gated and kept 267 us, the plain product 187.
 // Gated, a wavefront's columns are those of the gate, then the ones that belong to them.
 template <typename In, typename Out, int TR, int TC, bool TURN_A, bool TURN_B, bool GATED, int WHAT>
 __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(LinArgs g) {
@@ -808,7 +813,8 @@ __global__ __launch_bounds__(256) void lin_join(LinArgs g, int splits) {
 // Up to 64 rows of x, a token or some: what counts is that w is read once, at the memory's rate, by as many wavefronts as there are.  A wavefront takes
 // 16 rows of w (G times, gated: 16 of the gate and theirs of the other), straight into the registers as the matrix cores take them (four lanes read 64
 // bytes of a row); x comes out of the caches.  Of a block's eight wavefronts SHARING have the same rows, every one a step of 64 or 128 bytes in turn; their
-// sums are added in order in the LDS, and what follows is done there: one launch, no workspace, rows of any alignment.
+// sums are added in order in the LDS, and what follows is done there: one launch, no workspace, rows of any alignment.  A token of 1024 to 131072 in bf16,
+// 269 MB: 40 us, 6.7 TB/s (the memory and the last cache).
 // Which of those: up to 16 always; up to 32 float32, but for few long rows of w, and of the others what w has up to 2^23 values of; up to 64 that and gated (x
 // serves gate and other), not float32.  (us, so and by tiles: bf16 8 x 1024 over 8192 6.8, 11.2, over 131072 52, 51; 32 x 1024 over 8192 8.1, 12.0,
 // over 32768 22, 18; gated 64 x 1024 over 2 x 4096 8.9, 11.7, not gated 14, 11; float32 32 x 1024 over 32768 37, 54, 32 x 4096 over 1024 24, 18.)

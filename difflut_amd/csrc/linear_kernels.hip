@@ -23,7 +23,8 @@ __global__ __launch_bounds__(256) void lin_pad(const T *__restrict__ src, long l
 // ------------------------------------------------------------------ the gradient in front of the products, and its column sums
 // gz [M, ldg] (null: not written) from gy and z as it was kept (null: no activation, gz is gy), and a share of sum_m gz per block of rows (null: not
 // asked for).  A thread takes E columns of every fourth row of its block's; gated: of the gate and of the other half.  Rows of gz are whole units of
-// 16 bytes, zeros behind the N-th column, as the products read them; those of gy may begin anywhere and end inside a unit (ODD).
+// 16 bytes, zeros behind the N-th column, as the products read them; those of gy may begin anywhere and end inside a unit (ODD).  Memory bounds it:
+// 12544 x 8192 of a gate in bf16, 616 MB, 134 us, 4.6 TB/s.
 #define LIN_SLOPE_ROWS 64
 struct LinKept {
     const void *high;
@@ -98,19 +99,13 @@ __global__ __launch_bounds__(256) void lin_gradient(const T *__restrict__ gy, Li
             shares[piece * N + h * width + c + i] = t;
         }
 }
-// the shares of 16 columns per block, each column by 16 threads one after the other, then theirs
+// the shares of 16 columns per block, each column by 64 threads one after the other, then theirs  (784 shares of 1024 columns: 9.2 us by 16 threads, so
+// 4.9)
 template <typename T>
-__global__ __launch_bounds__(256) void lin_columns(const float *__restrict__ shares, T *__restrict__ out, int count, int N) {
-    __shared__ float part[16][17];
-    const int c = threadIdx.x & 15, k = threadIdx.x >> 4, column = (int)blockIdx.x * 16 + c;
-    float t = 0.0f;
-    if (column < N)
-        for (int s = k; s < count; s += 16) t += shares[(long long)s * N + column];
-    part[k][c] = t;
-    __syncthreads();
-    if (k != 0 || column >= N) return;
-    for (int i = 1; i < 16; ++i) t += part[i][c];
-    out[column] = (T)t;
+__global__ __launch_bounds__(1024) void lin_columns(const float *__restrict__ shares, T *__restrict__ out, int count, int N) {
+    const int column = (int)blockIdx.x * 16 + (threadIdx.x & 15);
+    const float t = dl_column_sum(shares, count, N, column);
+    if (threadIdx.x < 16 && column < N) out[column] = (T)t;
 }
 
 // ------------------------------------------------------------------ plans
@@ -320,7 +315,7 @@ extern "C" int dl_linear_bwd(const void *x, long long ldx, const void *w, long l
             const bool odd = width % (16 / (int)sizeof(T)) != 0 || !dl_aligned16(gy);
             DL_TIMED("lin_gradient", s, if (gated) { if (odd) LIN_GRADIENT(true, true); else LIN_GRADIENT(true, false); }
                      else if (odd) LIN_GRADIENT(false, true); else LIN_GRADIENT(false, false));
-            if (gb) DL_TIMED("lin_columns", s, hipLaunchKernelGGL((lin_columns<T>), dim3(dl_ceil_div(N, 16)), dim3(256), 0, s, shares, (T *)gb, p.pieces, (int)N));
+            if (gb) DL_TIMED("lin_columns", s, hipLaunchKernelGGL((lin_columns<T>), dim3(dl_ceil_div(N, 16)), dim3(1024), 0, s, shares, (T *)gb, p.pieces, (int)N));
         });
 #undef LIN_GRADIENT
     }
