@@ -1121,6 +1121,14 @@ Tensor linear_codes(const Tensor &x_, const Tensor &x_scale_, const Tensor &weig
     return y;
 }
 
+// x [B, K, V] as B K rows that lie evenly apart, and their distance: x itself, or a copy.  The stride of a dimension of one entry says nothing (and
+// x.contiguous() may be x with any such stride), so the distance is that of the dimension that has more.
+std::pair<Tensor, int64_t> even_rows(const Tensor &x) {
+    const int64_t B = x.size(0), K = x.size(1), V = x.size(2), ld = K > 1 ? x.stride(1) : B > 1 ? x.stride(0) : V;
+    if ((V == 1 || x.stride(2) == 1) && ld >= V && (B <= 1 || K == 1 || x.stride(0) == K * ld)) return {x, ld};
+    return {x.contiguous(), V};
+}
+
 // -> (scores, parents, tokens)
 std::vector<Tensor> beam_step(const Tensor &logits_, const Tensor &scores_, int64_t count, const Maybe &ended_, int64_t end) {
     at::NoGradGuard no_grad;
@@ -1130,14 +1138,13 @@ std::vector<Tensor> beam_step(const Tensor &logits_, const Tensor &scores_, int6
     const c10::DeviceGuard guard(logits_.device());
     const int64_t B = size_int(logits_.size(0), "a batch"), K = size_int(logits_.size(1), "a number of beams"), V = size_int(logits_.size(2), "a vocabulary");
     const int type = type_of(logits_, "logits");
-    // rows may lie apart where they do so evenly
-    const bool even = logits_.stride(2) == 1 && logits_.stride(1) >= V && (B <= 1 || logits_.stride(0) == K * logits_.stride(1));
-    const Tensor logits = even ? logits_ : logits_.contiguous(), scores = scores_.contiguous(), ended = ended_ ? ended_->contiguous() : Tensor();
+    const auto [logits, ldl] = even_rows(logits_);
+    const Tensor scores = scores_.contiguous(), ended = ended_ ? ended_->contiguous() : Tensor();
     const auto longs = logits.options().dtype(at::kLong).requires_grad(false);
     const Tensor best = floats({B, count}, logits), parents = at::empty({B, count}, longs), tokens = at::empty({B, count}, longs);
     if (B == 0) return {best, parents, tokens};
     const Tensor ws = bytes(L.dl_beam_step_workspace_bytes((int)B, (int)K, (int)V, (int)count), logits);
-    check(L.dl_beam_step(raw_in(logits), logits.stride(1) >= V ? logits.stride(1) : V, type, in(scores),
+    check(L.dl_beam_step(raw_in(logits), ldl, type, in(scores),
                          ended.defined() ? (const uint8_t *)ended.const_data_ptr() : nullptr, end, out(best), (long long *)raw(parents), (long long *)raw(tokens),
                          raw(ws), ws.numel(), (int)B, (int)K, (int)V, (int)count, stream()));
     return {best, parents, tokens};

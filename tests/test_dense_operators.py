@@ -657,6 +657,22 @@ def test_beam_step_strides_finished_and_empty(device):
 
 
 @pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_beam_step_strides_of_one_beam(device, dtype):
+    """One beam, one sequence, one class: the stride of a dimension of one entry says nothing about where rows lie."""
+    g = gen(16)
+    wide, line, scores = torch.randn(4, 6, 90, generator=g).to(dtype), torch.randn(1, 5, 70, generator=g).to(dtype), -torch.rand(5, 6, generator=g)
+    cuts = [lambda t: t[:, -1:], lambda t: t[:, -1:, 3:80], lambda t: t[::2, 1:2], lambda t: t[:1, 2:3], lambda t: t[:, 0][:, None], lambda t: t[:1, :, 5:69],
+            lambda t: t[:, :, :1], lambda t: t[:, 2:3, 4:5], lambda t: t[:1, 1:2].expand(3, 1, 90), lambda t: t[0].t()[:, None], lambda t: t[0].t()[:5, :, None], lambda t: t[:, ::3].transpose(0, 1)]
+    for source, cut in [(wide, c) for c in cuts] + [(line, lambda t: t.transpose(0, 1)), (line, lambda t: t.transpose(0, 1)[1:, :, 2:]), (line[:, :, :1].contiguous(), lambda t: t.transpose(0, 1))]:
+        x = cut(source)
+        s = scores.repeat(18, 1)[:x.shape[0], :x.shape[1]]
+        got = ops.beam_step(cut(source.to(device)), s.to(device), 4)
+        want = beam_64(x, s, 4, None, 0)
+        assert got[1].tolist() == [[f[1] for f in row] for row in want] and got[2].tolist() == [[int(f[2]) for f in row] for row in want]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
 def test_beam_reorder(device):
     g = gen(8)
     parents = torch.tensor([[2, 2, 0, 1], [0, 1, 2, 0], [-1, 3, 1, 2 ** 40]])
