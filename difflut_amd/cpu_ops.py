@@ -387,6 +387,7 @@ def sample(logits, uniform, temperature, top_k, top_p, min_p):
 
 # ----------------------------------------------------------------------------- dense blocks between the layers, search over answers
 CODE_MAX = 448.0  # the largest float8_e4m3fn
+CODE_SMALL = 2.0 ** -100  # scales below it are brought up before they are divided by
 
 
 def _stream(x, residual):
@@ -413,8 +414,9 @@ def _codes(y):
     if y.shape[:-1].numel() == 0:
         return y.to(torch.float8_e4m3fn), torch.zeros(y.shape[:-1], device=y.device)
     scale = (y.abs().amax(-1) / CODE_MAX).float()
-    factor = torch.where(scale == 0, 0.0, 1.0 / scale)
-    return (y.float() * factor.unsqueeze(-1)).clamp(-CODE_MAX, CODE_MAX).to(torch.float8_e4m3fn), scale
+    up = torch.where(scale < CODE_SMALL, 2.0 ** 64, 1.0)  # exact; without it the reciprocal of scales below 2^-128 is infinite
+    factor = torch.where(scale == 0, 0.0, 1.0 / (scale * up))
+    return (y.float() * up.unsqueeze(-1) * factor.unsqueeze(-1)).clamp(-CODE_MAX, CODE_MAX).to(torch.float8_e4m3fn), scale
 
 
 @torch.no_grad()

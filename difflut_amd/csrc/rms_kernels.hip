@@ -12,8 +12,9 @@
 #include "dl_types.h"
 
 #define RMS_THREADS 256
-#define RMS_SHARES 1024      // shares of ggamma at most
-#define RMS_CODE_MAX 448.0f  // largest e4m3 value
+#define RMS_SHARES 1024           // shares of ggamma at most
+#define RMS_CODE_MAX 448.0f       // largest e4m3 value
+#define RMS_CODE_SMALL 0x1p-100f  // scales below it are brought up before they are divided by
 
 typedef uint8_t rms_code;
 
@@ -135,7 +136,6 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
         rstd = 1.0f / sqrtf(sum / (float)g.D + g.eps);
         if (g.rstd && lane == 0 && real) g.rstd[row] = rstd;
     }
-    float factor = 1.0f, scale = 0.0f;
 #pragma unroll UNROLL
     for (int j = 0; j < turns; ++j) {
         const int c = (j * TEAM + lane) * E;
@@ -154,8 +154,8 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
     }
     if (!CODES) return;
     big = rms_reduce<TEAM, true>(big, part[1]);
-    scale = big / RMS_CODE_MAX;
-    factor = scale > 0.0f || scale != scale ? 1.0f / scale : 0.0f;  // a row of zeros: codes and scale 0
+    const float scale = big / RMS_CODE_MAX, up = scale < RMS_CODE_SMALL ? 0x1p64f : 1.0f;  // (exact; a scale below 2^-128 has no reciprocal)
+    const float factor = scale > 0.0f || scale != scale ? 1.0f / (scale * up) : 0.0f;      // a row of zeros: codes and scale 0
     if (!real) return;
     if (lane == 0) g.scale[row] = scale;
 #pragma unroll UNROLL
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(RmsTeam<TEAM>::THREADS) void rms_fwd(RmsArgs g) {
             for (int i = 0; i < E; ++i) f[i] = f[i] * rstd * w[i];
         }
 #pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = rms_clamped(f[i] * factor);
+        for (int i = 0; i < E; ++i) f[i] = rms_clamped(f[i] * up * factor);
         rms_store_codes<ODD, E>((rms_code *)g.y + row * g.D + c, g.D - c, f);
     }
 }

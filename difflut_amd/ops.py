@@ -646,7 +646,7 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None):
 def rms_norm_codes(x, weight=None, eps=1e-6, residual=None):
     """rms_norm whose result is left in 8 bits for linear_codes: (codes, scale), or (codes, scale, h) with a residual. codes are
     float8_e4m3fn of x's shape, scale float32 has one value per row: code * scale is the norm, rounded to three bits behind the leading
-    one; scale = max |norm| / 448, in a row of zeros 0. No gradient."""
+    one; scale = max |norm| / 448 as float32 has it, in a row of zeros, or of nothing above 448 * 2^-150, 0. No gradient."""
     _check_norm("rms_norm_codes", x, weight, eps, residual)
     if not x.is_cuda or x.numel() == 0:
         return cpu_ops.rms_norm_codes(x, weight, float(eps), residual)

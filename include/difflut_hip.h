@@ -553,8 +553,8 @@ int dl_sample(const void *logits, long long ldl, int type, const float *uniform,
 
 /* Root-mean-square norm: h = x + residual (rounded to `type`; without a residual h = x and is not written), rstd = 1 / sqrt(mean(h^2) + eps),
  * y = h rstd gamma; x and residual with ldx and ldr elements between rows, h and y [rows, D]; gamma [D] may be null (1).
- * rstd [rows] (nullable) is kept for the backward.  With `scale` [rows], y is e4m3 codes of D bytes a row, scale = max |y| / 448 (a row of
- * zeros: 0).  dl_quantize_rows: the same codes of x itself.
+ * rstd [rows] (nullable) is kept for the backward.  With `scale` [rows], y is e4m3 codes of D bytes a row, scale = max |y| / 448 (0, as are the codes, in a
+ * row of zeros or of nothing above 448 * 2^-150).  dl_quantize_rows: the same codes of x itself.
  * Backward: gx = rstd (g - hat mean(g hat)) + gh with g = gy gamma, hat = h rstd; gh (nullable) is the gradient that reaches h itself, gy
  * may be null where nothing reaches y; ggamma [D] = sum over rows of gy hat.  gx is the gradient of x and of the residual.
  * Workspace only where ggamma is asked for. */

@@ -185,6 +185,45 @@ def test_rows_in_8_bits_of_zeros_and_strangers(device):
     assert codes[3, 0] == 448 and not codes[3, 1:].any()
 
 
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [3, 32, 785, 33000])
+def test_rows_in_8_bits_of_very_small_values(device, dtype, D):
+    """From rows whose scale has no reciprocal in float32 down to its smallest subnormal; zeros among them stay zeros, other rows as they are."""
+    g = gen(D)
+    most = torch.tensor([1.0, 1e-28, 1e-30, 5e-34, 2e-36, 1.3e-36, 1e-36, 1e-37, 2.0 ** -126, 1e-39, 2.0 ** -133, 700 * 2.0 ** -149, 2.0 ** -140, 2.0 ** -149, 0.0])
+    shape = torch.rand(len(most), D, generator=g) * 2 - 1
+    shape[:, 0], shape[:, 1:2], shape[:, 2] = 1.0, 0.0, -0.5
+    x = (shape.double() * most[:, None].double()).to(dtype)
+    weight = torch.tensor([1.0, 0.5] * D)[:D]
+    w = (1e-37 * weight).to(dtype)  # the norm's: a weight that has decayed
+    y = x[:1].double() / torch.sqrt(x[:1].double().square().mean() + 1e-6) * w.double()
+    for got, want, rel in ((ops.quantize_rows(x.to(device)), x.double(), 0.0), (ops.rms_norm_codes(x[:1].to(device), w.to(device)), y, (54 + D / 1024) / 2 + 6)):
+        codes, scale = got[0].cpu().double(), got[1].cpu().double()
+        assert bool(codes.isfinite().all())
+        top = want.abs().amax(1)
+        # the scale is off by its rounding, of a subnormal 2^-150; (rel + 1) 2^-150: what came out as a subnormal itself
+        least = (1 + (rel > 0)) * 2.0 ** -150
+        assert bool(((scale - top / 448).abs() <= (rel + 1) * U * top / 448 + least).all())
+        s = scale[:, None]
+        # values beyond 448 of a scale that was rounded down are off by 448 times what that was
+        step = torch.maximum(want.abs() * E4M3_HALF, s * E4M3_LEAST)
+        limit = step * (1 + 8 * U) + want.abs() * (rel + 4) * U + (448 + 2) * least
+        assert bool(((codes * s - want).abs() <= limit).all())
+        assert not codes[want == 0].any()
+        if dtype is torch.float32 and rel == 0.0:
+            assert bool((codes.abs().amax(1) == 448)[top >= 1e-30].all())
+    # a row of a weight that has decayed: its column is next to nothing, the others are as they were
+    full = torch.randn(6, D, generator=g).to(dtype)
+    gone = full.clone()
+    gone[2] = x[7, :D]
+    rows = torch.randn(5, D, generator=g).to(dtype).to(device)
+    want, got = (ops.linear_codes(*ops.quantize_rows(rows), *ops.quantize_rows(t.to(device)), dtype=torch.float32) for t in (full, gone))
+    assert bool(got[:, 2].isfinite().all()) and float(got[:, 2].abs().max()) < 1e-30
+    keep = [0, 1, 3, 4, 5]
+    assert torch.equal(got[:, keep], want[:, keep])
+
+
 # ----------------------------------------------------------------------------- projections
 def act_64(z, act):
     """Value, slope, and a bound of the slope's slope"""
