@@ -471,7 +471,8 @@ def beam_step(logits, scores, beams, finished, end):
     x = logits.double()
     x = torch.where(x.isnan(), -math.inf, x).clamp(max=torch.finfo(torch.float32).max)
     B, K, V = x.shape
-    top = x.amax(2, keepdim=True)
+    x, order = torch.sort(x, dim=2, descending=True, stable=True)  # equal scores by beam, then logit, then token
+    top = x[:, :, :1]
     known = top > -math.inf
     x = torch.where(known, x, 0.0)
     norm = torch.where(known, top, 0.0)
@@ -481,13 +482,13 @@ def beam_step(logits, scores, beams, finished, end):
         alone = torch.full_like(total, -math.inf)
         alone[:, :, 0] = scores.double()
         total = torch.where(finished.unsqueeze(2), alone, total)
-    total = torch.where(total.isnan(), -math.inf, total).view(B, K * V)
+    total = torch.where(total.isnan(), -math.inf, total).reshape(B, K * V)
     best, at = torch.sort(total, dim=1, descending=True, stable=True)
     best, at = best[:, :beams], at[:, :beams]
     short = beams - best.shape[1]
     if short > 0:
         best, at = torch.nn.functional.pad(best, (0, short), value=-math.inf), torch.nn.functional.pad(at, (0, short))
-    parents, tokens = at // V, at % V
+    parents, tokens = at // V, order.reshape(B, K * V).gather(1, at)
     if finished is not None:
         tokens = torch.where(finished.gather(1, parents), end, tokens)
     none = best == -math.inf

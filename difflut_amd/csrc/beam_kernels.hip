@@ -1,7 +1,7 @@
 // A step of beam search: the best continuations of every sequence's beams over the vocabulary, and the beams' states in their order.
 //
 //   candidate (k, v) of a sequence:  c = scores[k] + logits[k, v] - log sum_u exp(logits[k, u]);  a beam that has ended: (k, end) alone, c = scores[k]
-//   the `count` largest, equal ones by k, then v
+//   the `count` largest, equal ones by k, then logit (they may differ where the scores are so far from zero that c does not), then v
 //
 // The best of all are among the best `count` logits of each beam.  One pass over the logits: a block takes a row or a piece of one, each of its
 // wavefronts in rounds of BEAM_ROUND / 4 values, without waiting for the others.  A thread keeps the sum of the softmax (float within a round,
@@ -262,7 +262,13 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows(BeamArgs g) {
 // A block takes a sequence's K * pieces lists of `count` candidates, best first.  The count-th of the lists' best bounds them from below, where
 // there are as many lists; every candidate that passes it counts the better ones.
 #define BEAM_RANKS 1024  // candidates that are ranked; from more the best is taken `count` times
-__device__ __forceinline__ bool beam_before(double a, int at, double b, int bt) { return a > b || (a == b && at < bt); }
+// Candidate a, at place `at` of the lists, before b: equal ones by beam, then key.  Places are in that order but for a beam of several lists (per: places of a
+// beam; 0: they are).
+__device__ __forceinline__ bool beam_before(double a, int at, double b, int bt, const beam_key *keys, int per) {
+    if (a != b || at == bt) return a > b;
+    if (per == 0 || at / per != bt / per) return at < bt;
+    return keys[at] > keys[bt];
+}
 __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
     __shared__ double value[BEAM_PICKS], norm[BEAM_MOST], base[BEAM_MOST], wave_value[BEAM_WAVES], bound;
     __shared__ double kept_value[BEAM_RANKS];
@@ -323,11 +329,12 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
             const double mine = value[e * g.count];
             int rank = 0;
 #pragma unroll 4
-            for (int j = 0; j < lists; ++j) rank += beam_before(value[j * g.count], j, mine, e) ? 1 : 0;
+            for (int j = 0; j < lists; ++j) rank += value[j * g.count] > mine || (value[j * g.count] == mine && j < e) ? 1 : 0;
             if (rank == g.count - 1) bound = mine;
         }
     __syncthreads();
     const double least = bound;
+    const int apart = g.pieces > 1 ? per : 0;
     for (int e = tid; e < n; e += BEAM_THREADS) {
         const double c = value[e];
         if (!(c >= least && c > -inf)) continue;
@@ -350,7 +357,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
             const int at = kept_at[e];
             int rank = 0;
 #pragma unroll 4
-            for (int j = 0; j < m; ++j) rank += beam_before(kept_value[j], kept_at[j], mine, at) ? 1 : 0;
+            for (int j = 0; j < m; ++j) rank += beam_before(kept_value[j], kept_at[j], mine, at, keys, apart) ? 1 : 0;
             if (rank < g.count) answer(rank, mine, at);
         }
         return;
@@ -360,7 +367,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
     const auto own_best = [&]() __attribute__((always_inline)) {
         mine = -inf, mine_at = n;
         for (int e = tid; e < n; e += BEAM_THREADS)
-            if (value[e] > mine) mine = value[e], mine_at = e;
+            if (value[e] > -inf && beam_before(value[e], e, mine, mine_at, keys, apart)) mine = value[e], mine_at = e;
     };
     own_best();
     for (int j = 0; j < g.count; ++j) {  // (there are more than `count` above -infinity)
@@ -370,13 +377,13 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
         for (int o = 32; o > 0; o >>= 1) {
             const double v = __shfl_xor(best, o);
             const int w = __shfl_xor(at, o);
-            if (beam_before(v, w, best, at)) best = v, at = w;
+            if (beam_before(v, w, best, at, keys, apart)) best = v, at = w;
         }
         if ((tid & 63) == 0) wave_value[tid >> 6] = best, wave_at[tid >> 6] = at;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < BEAM_WAVES; ++w)
-            if (beam_before(wave_value[w], wave_at[w], best, at)) best = wave_value[w], at = wave_at[w];
+            if (beam_before(wave_value[w], wave_at[w], best, at, keys, apart)) best = wave_value[w], at = wave_at[w];
         __syncthreads();
         if (tid == 0) answer(j, best, at);
         if (at % BEAM_THREADS == tid) {  // its next one

@@ -722,7 +722,8 @@ def beam_step(logits, scores, beams=None, finished=None, end=0):
     """One step of beam search: of every sequence's beams the best continuations -> (scores, parents, tokens), each [batch, beams].
 
     logits [batch, beams in, vocabulary], scores float32 [batch, beams in]; a continuation's score is its beam's plus the token's
-    log-softmax, the `beams` (as many as came in unless given) largest are returned, largest first, equal ones by beam, then token.
+    log-softmax, the `beams` (as many as came in unless given) largest are returned, largest first, equal ones by beam, then logit (a score of
+    -1e30 leaves no difference of a beam's logits in the sum), then token.
     A beam that is `finished` (bool [batch, beams in]) goes on by one continuation alone, the token `end` at its own score; its logits are not
     looked at.  NaN logits are no continuations, infinite ones count as the largest number; where there are fewer continuations above
     -infinity than asked for, the rest have score -infinity, parent 0 and token -1.  Beams start as [0, -infinity, ...].

@@ -585,8 +585,8 @@ int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, co
                   long long M, long long N, long long K, int act, int gated, void *ws, size_t ws_bytes, void *stream);
 
 /* A step of beam search: of every sequence's K beams over V tokens the `count` continuations with the largest
- * scores[b, k] + log_softmax(logits[b, k, :])[v], largest first, equal ones by beam, then token.  logits [B * K, V] (ldl between rows), scores
- * [B, K]; ended (nullable) [B, K]: a beam with a non-zero byte goes on by (its score, token `end`) alone, its logits are not read.
+ * scores[b, k] + log_softmax(logits[b, k, :])[v], largest first, equal ones by beam, then logit, then token.  logits [B * K, V] (ldl between rows),
+ * scores [B, K]; ended (nullable) [B, K]: a beam with a non-zero byte goes on by (its score, token `end`) alone, its logits are not read.
  * NaN logits are no candidates, infinite ones count as the largest number.  Where there are fewer candidates above -infinity: score
  * -infinity, parent 0, token -1.  K and count up to 64, V up to 2^30 (DL_ERR_UNSUPPORTED).
  * dl_beam_reorder: dst[t][b, j] = src[t][b, parents[b, j]] for n tensors of row_bytes[t] bytes per beam (src, dst, row_bytes: HOST arrays);

@@ -652,6 +652,38 @@ def test_beam_step_equal_logits(device, V):
     check_beam(device, torch.tensor([0.0, -0.0]).repeat(V)[:V].expand(1, 2, V).contiguous(), torch.zeros(1, 2), 4)
 
 
+# (beams in, vocabulary, answers): a piece of a row and several, few candidates and more than are ranked at once
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("K,V,beams", [(4, 5, 16), (3, 700, 8), (2, 20001, 16), (4, 40000, 64), (64, 300, 64), (20, 9000, 64)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_beam_step_scores_that_swallow_logits(device, K, V, beams, dtype):
+    """Different logits, the same score as a double: by beam, then logit, then token."""
+    g = gen(K + V)
+    x = (3 * torch.randn(2, K, V, generator=g)).to(dtype)
+    x[1, 0, V - 1] = x[1, 0].max()  # (twice: the lower token first)
+    tiny = (torch.randn(2, K, V, generator=g) * 1e-20).to(dtype)  # all of one probability as a double
+    mixed = torch.full((2, K), -1e30)
+    mixed[:, 0], mixed[0, K - 1] = 0.0, -1e9
+    ended = torch.zeros(2, K, dtype=torch.bool)
+    ended[:, 1] = True
+    for logits, scores, finished in [(x, torch.full((2, K), s), None) for s in (-1e30, -1e9, torch.finfo(torch.float32).min, math.inf)] + [
+            (x, mixed, None), (x, mixed, ended), (tiny, torch.zeros(2, K), None), (tiny, torch.full((2, K), -1e30), ended)]:
+        z, s = logits.double(), scores.double()
+        c = s[:, :, None] + torch.log_softmax(z, 2)
+        rank = torch.sort(z, dim=2, descending=True, stable=True).indices.argsort(2)  # of a beam's tokens
+        if finished is not None:
+            alone = torch.full_like(c, -math.inf)
+            alone[:, :, 3] = s
+            c = torch.where(finished[:, :, None], alone, c)
+        place = rank + V * torch.arange(K)[None, :, None]
+        got = ops.beam_step(logits.to(device), scores.to(device), beams, None if finished is None else finished.to(device), 3)
+        for b in range(2):
+            order = np.lexsort((place[b].flatten().numpy(), -c[b].flatten().numpy()))[:beams]
+            assert got[1][b].tolist() == (order // V).tolist() and got[2][b].tolist() == (order % V).tolist()
+            want = c[b].flatten()[order]
+            assert bool(((got[0][b].cpu().double() - want).abs() <= want.abs() * U + 40 * U).logical_or(want == math.inf).all()) and torch.equal(got[0][b].cpu() == math.inf, want == math.inf)
+
+
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 @pytest.mark.parametrize("V", [6, 700, 9001])
 def test_beam_step_masked_rows(device, V):
