@@ -197,15 +197,35 @@ class Linear(nn.Module):
 
 class Linear8(nn.Module):
     """A trained Linear on 8-bit rows: the weight is kept as codes with a scale per row (buffers), the bias in `linear`'s type, which is the
-    result's.  Takes (codes, scale) as RMSNorm(codes=True) leaves them, or rows of a float type, which it quantizes."""
+    result's.  Takes (codes, scale) as RMSNorm(codes=True) leaves them, or rows of a float type, which it quantizes.  `.to(dtype)` and its like
+    are of the bias and the result: codes and scales stay as they are."""
 
     def __init__(self, linear):
         super().__init__()
-        self.activation, self.gated, self.dtype = linear.activation, linear.gated, linear.weight.dtype
+        self.activation, self.gated = linear.activation, linear.gated
         codes, scale = ops.quantize_rows(linear.weight.detach())
         self.register_buffer("weight", codes)
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+        self.register_buffer("_result", linear.weight.new_empty(0), persistent=False)  # goes along with the module's type
+
+    @property
+    def dtype(self):
+        return self._result.dtype
+
+    def _apply(self, fn, recurse=True):
+        """Moves take codes and scales along as whole numbers, which no change of a float type converts."""
+        held = {name: self._buffers[name] for name in ("weight", "weight_scale")}
+        for name, t in held.items():
+            self._buffers[name] = t.view(torch.uint8 if name == "weight" else torch.int32)
+        try:
+            super()._apply(fn, recurse)
+        finally:
+            for name, t in held.items():
+                moved = self._buffers[name]
+                # (`.type(dtype)` converts those as well)
+                self._buffers[name] = moved.view(t.dtype) if not moved.is_floating_point() and moved.element_size() == t.element_size() else t.to(moved.device)
+        return self
 
     def forward(self, x, scale=None, residual=None):
         if scale is None:

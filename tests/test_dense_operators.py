@@ -761,6 +761,35 @@ def test_beam_reorder(device):
     assert ops.beam_reorder([], parents.to(device)) == []
 
 
+# ----------------------------------------------------------------------------- modules
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("bias", [False, True])
+def test_linear8_through_changes_of_type_and_device(device, bias):
+    """Codes and scales stay as they are; the bias and the result follow the module's type; a saved state is that of another module."""
+    from difflut_amd.utils import Linear8
+
+    torch.manual_seed(3)
+    linear = Linear(40, 24, bias=bias, activation="silu", gated=True).to(device)
+    x, r = torch.randn(5, 40, device=device), torch.randn(5, 24, device=device)
+    first = linear.to_codes()
+    want = first(x, residual=r)
+    codes, scale = first.weight.float().clone(), first.weight_scale.clone()
+    holds = lambda m: m.weight.dtype is torch.float8_e4m3fn and m.weight_scale.dtype is torch.float32 and torch.equal(m.weight.float(), codes) and torch.equal(m.weight_scale, scale)  # noqa: E731
+    for change, dtype in ((lambda m: m.to(torch.bfloat16), torch.bfloat16), (lambda m: m.half(), torch.float16), (lambda m: m.bfloat16(), torch.bfloat16), (lambda m: m.to(device, torch.float16), torch.float16),
+                          (lambda m: m.cpu().to(device), torch.float32), (lambda m: m.type(torch.float16), torch.float16), (lambda m: m.to(torch.float64).float(), torch.float32)):
+        m = change(torch.nn.Sequential(linear.to_codes()))[0]
+        assert m.dtype is dtype and (m.bias is None or m.bias.dtype is dtype) and holds(m)
+        assert sorted(m.state_dict()) == sorted(["weight", "weight_scale"] + ["bias"] * bias)
+        got = m(x, residual=r.to(dtype))
+        b = linear.bias.detach().to(dtype) if bias else None
+        assert got.dtype is dtype and torch.equal(got, ops.linear_codes(*ops.quantize_rows(x), first.weight, first.weight_scale, b, "silu", r.to(dtype), True, dtype))
+    empty = linear.to_codes().to("meta").to_empty(device=device)
+    empty.load_state_dict(first.state_dict())
+    assert holds(empty) and torch.equal(empty(x, residual=r), want)
+    import copy
+    assert torch.equal(copy.deepcopy(first)(x, residual=r), want)
+
+
 # ----------------------------------------------------------------------------- refusals
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 def test_refusals(device):
