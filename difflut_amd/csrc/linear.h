@@ -13,10 +13,10 @@
 //
 // float32 values are cut into three bf16 planes on the way out of the LDS (8 + 8 + 8 significant bits, each the rounding of what the ones
 // above left); a product is the six plane products hi*lo, lo*hi, mid*mid, hi*mid, mid*hi, hi*hi, small ones first.  What is left out is
-// below 2^-26 of |a b|, less than the 2^-24 of one fp32 multiply-add.  Six bf16 products at 2.5 PFLOP/s are 417 TFLOP/s of fp32 work
+// below 2^-24 of |a b|, what one fp32 multiply-add rounds off (root mean square: below 2^-27).  Six bf16 products at 2.5 PFLOP/s are 417 TFLOP/s of fp32 work
 // against 157 on the fp32 matrix cores; 4096^3 takes 600 us (229 TFLOP/s), 2 M N K on the fp32 cores by the library 900.  What bounds it is the cuts'
 // instructions, which do not run beside a matrix instruction: 6144 cycles of these a stage of 256 x 256 and 3264 of those are the 4.7 us that one takes.
-// (Planes carry no infinities: such a product is NaN.)
+// (Planes carry no infinities: such a product is NaN.  Nor anything below 2^-133: values under 2^-110 lose their last bits to that.)
 #pragma once
 #include <utility>
 
@@ -30,6 +30,7 @@ typedef int intx8 __attribute__((ext_vector_type(8)));
 
 #define LIN_STAGE_BYTES 128  // of a row in a stage: 32 float32, 64 16-bit or 128 8-bit values
 #define LIN_PLANES 3
+#define LIN_BF16_MAX 0x1.fep127f  // the largest
 #define LIN_CUS 256
 enum { LIN_SUMS, LIN_PLAIN, LIN_PLAIN_ODD, LIN_ENDS, LIN_ENDS_ODD, LIN_KEEPS, LIN_KEEPS_ODD };
 
@@ -204,14 +205,17 @@ __device__ __forceinline__ unsigned lin_pk_bf16(float a, float b) {
 // Eight values into planes in five parts: the first plane, what it leaves, the second, what it leaves, the third.  What is left of a value is
 // its product with -1 of the plane's pair, and 0 of its neighbour, added to it: exact, and at once from the packed pair.  (Cycles of one wavefront: rounding
 // a pair 8.6, such a product 6.4, to unpack or subtract 5.6 each, so a pair takes 51 instead of 71.  The parts keep results away from their use, which
-// would cost waits.)
+// would cost waits.)  From 2^128 - 2^119 on the first plane's rounding is infinite, and the value's products are NaN; WIDE: these too are cut, by the largest bf16,
+// for two instructions a pair more.
+template <bool WIDE>
 __device__ __forceinline__ void lin_cut(float (&f)[8], int part, LinFragment<LinF32> &out) {
     unsigned low = 0x0000BF80u, high = 0xBF800000u;  // (-1, 0) and (0, -1)
     asm("" : "+s"(low), "+s"(high));  // in registers: as the instruction's own constant -1 the first would stand in the other half
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         int &w = out.w[part / 2][i];
-        if (part % 2 == 0) w = (int)lin_pk_bf16(f[2 * i], f[2 * i + 1]);
+        if (WIDE && part == 0) w = (int)lin_pk_bf16(__builtin_amdgcn_fmed3f(f[2 * i], -LIN_BF16_MAX, LIN_BF16_MAX), __builtin_amdgcn_fmed3f(f[2 * i + 1], -LIN_BF16_MAX, LIN_BF16_MAX));
+        else if (part % 2 == 0) w = (int)lin_pk_bf16(f[2 * i], f[2 * i + 1]);
         else {
             f[2 * i] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, low), f[2 * i], false);
             f[2 * i + 1] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, high), f[2 * i + 1], false);
@@ -536,7 +540,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
     constexpr int PIECES = CUT ? 6 * (FRAGMENTS + 1) : FA * PA + FB * PB, PRODUCTS = CUT ? 6 : 1, SLOTS = FA * FB * PRODUCTS;
     constexpr int READ_SLOTS = CUT ? SLOTS : SLOTS * 3 / 4;  // (the last reads are answered by the next step)
     float raw[2][8];
-    const auto piece = [&](auto number, unsigned from_a, unsigned from_b, int step, int set) __attribute__((always_inline)) {
+    const auto piece = [&](auto number, auto wide, unsigned from_a, unsigned from_b, int step, int set) __attribute__((always_inline)) {
         constexpr int o = decltype(number)::value;
         if constexpr (CUT) {  // read a fragment, then cut the one before
             constexpr int f = o / 6, r = o % 6, q = f - 1;
@@ -545,8 +549,8 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
                 else read_b.read_raw(lds + from_b, step, f - 1, raw[f & 1]);
             }
             if constexpr (r > 0 && f > 0) {
-                if constexpr (q == 0 || q > FB) lin_cut(raw[q & 1], r - 1, a[set][q == 0 ? 0 : q - FB]);
-                else lin_cut(raw[q & 1], r - 1, b[set][q - 1]);
+                if constexpr (q == 0 || q > FB) lin_cut<decltype(wide)::value>(raw[q & 1], r - 1, a[set][q == 0 ? 0 : q - FB]);
+                else lin_cut<decltype(wide)::value>(raw[q & 1], r - 1, b[set][q - 1]);
             }
         } else if constexpr (o < PA) read_a.read(lds + from_a, step, 0, o, a[set][0]);
         else if constexpr (o < PA + FB * PB) read_b.read(lds + from_b, step, (o - PA) / PB, (o - PA) % PB, b[set][(o - PA) / PB]);
@@ -556,7 +560,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
     unsigned a_now, a_next, a_free, b_now;
     intx4 from_a, from_b, from_other;
     // A stage, FIRST of a tile or another.  What it sends for and reads behind the last one is not there, and not used.
-    const auto stage = [&](auto is_first) __attribute__((always_inline)) {
+    const auto stage = [&](auto is_first, auto wide) __attribute__((always_inline)) {
         constexpr bool FIRST = decltype(is_first)::value;
         lin_each<0, STEPS>([&](auto step) __attribute__((always_inline)) {
             constexpr int st = decltype(step)::value;
@@ -566,7 +570,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
             lin_each<0, SLOTS>([&](auto slot) __attribute__((always_inline)) {
                 constexpr int m = decltype(slot)::value, o0 = m * PIECES / READ_SLOTS, o1 = (m + 1) * PIECES / READ_SLOTS;
                 lin_each<(o0 < PIECES ? o0 : PIECES), (o1 < PIECES ? o1 : PIECES)>([&](auto o) __attribute__((always_inline)) {
-                    piece(o, last ? a_next : a_now, last ? B0 + B1 - b_now : b_now, last ? 0 : st + 1, (st + 1) & 1);
+                    piece(o, wide, last ? a_next : a_now, last ? B0 + B1 - b_now : b_now, last ? 0 : st + 1, (st + 1) & 1);
                 });
                 if constexpr (last)
                     lin_each<m * NB / SLOTS, (m + 1) * NB / SLOTS>([&](auto j) __attribute__((always_inline)) { load_b(from_b, from_other, lds_base + b_now, decltype(j)::value); });
@@ -741,21 +745,46 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
     place();
     begin();
     for (;;) {
-        lin_stage_barrier<0>();  // the first stages are there, and the tile before is written out of the LDS
-#pragma unroll
-        for (int j = 0; j < NB; ++j) load_b(lin_buffer(b_second, there(1)), lin_buffer(b_second + b_half, there(1)), lds_base + B1, j);
-        a_now = A0, a_next = A1, a_free = A2, b_now = B0;
-        uint64_t at_a = a_second, at_b = b_second;
-        const auto send_for = [&](int s) __attribute__((always_inline)) {
-            at_a += a_step, at_b += b_step;
-            from_a = lin_buffer(at_a, there(s)), from_b = lin_buffer(at_b, there(s)), from_other = lin_buffer(at_b + b_half, there(s));
+        const auto multiply = [&](auto wide) __attribute__((always_inline)) {
+            lin_stage_barrier<0>();  // the first stages are there, and the tile before is written out of the LDS
+    #pragma unroll
+            for (int j = 0; j < NB; ++j) load_b(lin_buffer(b_second, there(1)), lin_buffer(b_second + b_half, there(1)), lds_base + B1, j);
+            a_now = A0, a_next = A1, a_free = A2, b_now = B0;
+            uint64_t at_a = a_second, at_b = b_second;
+            const auto send_for = [&](int s) __attribute__((always_inline)) {
+                at_a += a_step, at_b += b_step;
+                from_a = lin_buffer(at_a, there(s)), from_b = lin_buffer(at_b, there(s)), from_other = lin_buffer(at_b + b_half, there(s));
+            };
+            lin_each<0, PIECES>([&](auto o) __attribute__((always_inline)) { piece(o, wide, A0, B0, 0, 0); });
+            send_for(2);
+            stage(LinIs<1>(), wide);
+            for (int s = 1; s < count; ++s) {
+                send_for(s + 2);
+                stage(LinIs<0>(), wide);
+            }
         };
-        lin_each<0, PIECES>([&](auto o) __attribute__((always_inline)) { piece(o, A0, B0, 0, 0); });
-        send_for(2);
-        stage(LinIs<1>());
-        for (int s = 1; s < count; ++s) {
-            send_for(s + 2);
-            stage(LinIs<0>());
+        multiply(LinIs<0>());
+        if constexpr (CUT) {
+            // A value that the planes do not hold makes every sum of its row or column NaN, so one column's and one row's sums show it; then the tile is
+            // multiplied again by cuts that hold it.  (In every cut these would take 3 to 7 % of a product's time.)
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < FA; ++i) sum += acc[i][0][0];
+#pragma unroll
+            for (int j = 0; j < FB; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) sum += acc[0][j][v];
+            lin_stage_barrier<0>();  // everybody has read the last stage
+            int *const marks = (int *)(lds + B1);
+            if (lane == 0) marks[wave] = 0;
+            if (sum != sum) marks[wave] = 1;
+            lin_stage_barrier<0>();
+            const int any = dl_uniform(marks[0] | marks[1] | marks[2] | marks[3]);
+            lin_stage_barrier<0>();
+            if (any) {
+                begin();
+                multiply(LinIs<1>());
+            }
         }
 
         const int row = r0, column = c0, plane = split;
@@ -868,7 +897,7 @@ __global__ __launch_bounds__(512) void lin_few(LinArgs g) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(from.w[i]);
 #pragma unroll
-            for (int part = 0; part < 5; ++part) lin_cut(v, part, f);
+            for (int part = 0; part < 5; ++part) lin_cut<true>(v, part, f);  // (it costs nothing here)
         } else {
 #pragma unroll
             for (int i = 0; i < 4 * Q; ++i) f.w[0][i] = (int)from.w[i];

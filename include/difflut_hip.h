@@ -568,6 +568,7 @@ int dl_rms_norm_bwd(const void *h, long long ldh, const void *gamma, const float
 /* Matrix product with what follows it: s = x w^T + bias over x [M, K], w [N, K] (ldx, ldw elements between rows), y = act(s) + residual [M, N];
  * gated: N is even, the first N / 2 rows of w are the gate's, y = act(s[:, :N/2]) * s[:, N/2:] + residual [M, N / 2].  bias, residual (ldr)
  * and kept may be null.  All of type `type` = out_type, or x and w of DL_E4M3 with their rows' scales and the rest of out_type (inference: nothing kept).
+ * DL_F32 is multiplied to within its own rounding, values below 2^-110 as multiples of 2^-133, infinities as NaN.
  * y is contiguous.  kept (dl_linear_kept_bytes, on 16 bytes) receives s for the backward, in 24 bits of a float or, of DL_F32, 32; its
  * layout is the library's own.
  * Backward: from gy (contiguous, y's shape) the gradients gx [M, K], gw [N, K], gb [N], each nullable; kept as the forward left it (null where act

@@ -338,6 +338,52 @@ def test_linear_of_many_tiles(M, K, N, dtype, gated):
     check_linear("cuda", M, K, N, dtype, "silu", gated, True, True)
 
 
+# few rows, small tiles, a split reduction, gated tiles, large tiles
+HUGE = [pytest.param("cpu", 3, 72, 40), pytest.param("cpu", 40, 72, 130)] + [
+    pytest.param("cuda", *s, marks=pytest.mark.gpu) for s in ((3, 72, 40), (32, 640, 514), (100, 72, 300), (300, 2080, 514), (1100, 96, 2050), (4100, 72, 4104))]
+
+
+@pytest.mark.parametrize("device,M,K,N", HUGE)
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_of_the_lowest_value_times_nothing(device, M, K, N, gated):
+    """A mask of the type's lowest (or largest) value in front of weights of zero adds nothing, whichever operand holds it."""
+    g = gen(M + N)
+    x, w = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g) / math.sqrt(K)
+    f = ops.gated_linear if gated else ops.linear
+    for value in (torch.finfo(torch.float32).min, torch.finfo(torch.float32).max):
+        for k in (0, 37, K - 1):
+            xs, ws = x.clone(), w.clone()
+            xs[:, k], ws[:, k] = 0.0, 0.0
+            want = f(xs.to(device), ws.to(device), activation="silu")
+            for masked, other in ((xs, ws), (ws, xs)):
+                a = masked.clone()
+                a[1::2, k] = value
+                assert torch.equal(f(*(t.to(device) for t in ((a, other) if masked is xs else (other, a))), activation="silu"), want)
+
+
+@pytest.mark.parametrize("device,M,K,N", HUGE)
+@pytest.mark.parametrize("where", ["x", "w", "gy"])
+def test_linear_of_values_up_to_the_largest(device, M, K, N, where):
+    """Float32 above the largest bfloat16 here and there, next to small ones: results and gradients within the bounds of any other value."""
+    g = gen(M * 3 + N)
+    most = torch.finfo(torch.float32).max
+    values = torch.tensor([most, -most, 2.0 ** 128 - 2.0 ** 119, -(2.0 ** 128 - 2.0 ** 119), 2.0 ** 128 - 2.0 ** 119 - 2.0 ** 104, 2.0 ** 128 - 2.0 ** 120, 3e38, 1e38])
+    t = {"x": torch.randn(M, K, generator=g), "w": torch.randn(N, K, generator=g), "gy": torch.randn(M, N, generator=g)}
+    for name in t:
+        t[name] *= 1e-4
+    some = torch.rand(t[where].shape, generator=g) < 0.02
+    some[1, 1] = True
+    t[where] = torch.where(some, values[torch.randint(0, len(values), t[where].shape, generator=g)], t[where])
+    x, w, gy = (v.to(device) for v in t.values())
+    (y, y_off), gx, gw, _ = linear_64(x, w, None, None, "none", False, gy)
+    x.requires_grad_(), w.requires_grad_()
+    got = ops.linear(x, w)
+    close(got, y, y_off, torch.float32)
+    for grad, (want, off) in zip(torch.autograd.grad(got, (x, w), gy), (gx, gw)):
+        assert float(want.abs().max()) < most
+        close(grad, want, off, torch.float32)
+
+
 # few rows: short and long reductions, rows of w shared by two wavefronts or eight, the last group inside a block, up to 16, 32 and 64 rows
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,K,N,dtype,gated", [
