@@ -71,7 +71,7 @@ def build(verbose=False, jobs=None):
         if verbose:
             print(" ".join(cmd))
 
-    srcs = sources()
+    srcs = sorted(sources(), key=lambda s: not os.path.basename(s).startswith("linear_"))  # the longest to compile begin
     with ThreadPoolExecutor(max_workers=jobs or min(8, len(srcs) + 1)) as pool:
         host = pool.submit(compile_host)
         objs = list(pool.map(compile_one, srcs))
