@@ -1039,20 +1039,21 @@ std::vector<Tensor> quantize_rows(const Tensor &x_) {
     return {codes, scale};
 }
 
-// y = act(x w^T + bias) + residual; gated: the activated first half of the columns times the second
+// y = act(x w^T + bias) + residual; gated: the activated first half of the columns times the second.  KEEP_RESIDUAL: only the residual's gradient is asked for.
 struct Linear : torch::autograd::Function<Linear> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &weight_, const Maybe &bias_, const Maybe &residual_, int64_t act, bool gated, bool keep) {
+    enum { KEEP_NOTHING, KEEP_RESIDUAL, KEEP_ALL };
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &weight_, const Maybe &bias_, const Maybe &residual_, int64_t act, bool gated, int64_t keep) {
         const c10::DeviceGuard guard(x_.device());
         const Tensor x = rows_of(x_), weight = rows_of(weight_), bias = bias_ ? bias_->contiguous() : Tensor(), residual = residual_ ? rows_of(*residual_) : Tensor();
         const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
         const int type = type_of(x, "x");
         const Tensor y = like_rows(x_, gated ? N / 2 : N, x.scalar_type());
-        const Tensor z = keep && (gated || act != DL_ACT_NONE) ? bytes(L.dl_linear_kept_bytes(type, M, N, gated), x) : Tensor();
+        const Tensor z = keep == KEEP_ALL && (gated || act != DL_ACT_NONE) ? bytes(L.dl_linear_kept_bytes(type, M, N, gated), x) : Tensor();
         const size_t need = L.dl_linear_fwd_workspace_bytes(raw_in(x), ld_of(x), raw_in(weight), ld_of(weight), type, M, N, K, gated);
         const Tensor ws = need ? bytes(need, x) : Tensor();
         check(L.dl_linear_fwd(raw_in(x), ld_of(x), nullptr, raw_in(weight), ld_of(weight), nullptr, raw_in(bias), raw_in(residual),
                               residual.defined() ? ld_of(residual) : 0, raw(y), raw(z), type, type, M, N, K, (int)act, gated, raw(ws), need, stream()));
-        if (keep) {
+        if (keep != KEEP_NOTHING) {
             ctx->save_for_backward({x_, weight_, z});
             ctx->saved_data["act"] = act;
             ctx->saved_data["gated"] = gated;
@@ -1094,7 +1095,11 @@ Tensor linear(const Tensor &x, const Tensor &weight, const Maybe &bias_, const M
     for (const Tensor &t : {weight, bias, residual})
         TORCH_CHECK_TYPE(!t.defined() || t.scalar_type() == x.scalar_type(), "x, weight, bias and residual must be of one type, got ", x.scalar_type(), " and ",
                          t.defined() ? t.scalar_type() : x.scalar_type());
-    return Linear::apply(x, weight, bias_, residual_, act, gated, differentiates({x, weight, bias, residual}));
+    const int64_t keep = differentiates({x, weight, bias}) ? Linear::KEEP_ALL : differentiates({residual}) ? Linear::KEEP_RESIDUAL : Linear::KEEP_NOTHING;
+    // (not first in the backward)
+    TORCH_CHECK(weight.size(0) * (int64_t)x.element_size() <= DL_LINEAR_ROW || keep != Linear::KEEP_ALL, "a weight of ", weight.size(0), " rows in ", x.scalar_type(),
+                " has no gradients: up to ", DL_LINEAR_ROW, " bytes of a result's row have");
+    return Linear::apply(x, weight, bias_, residual_, act, gated, keep);
 }
 Tensor linear_codes(const Tensor &x_, const Tensor &x_scale_, const Tensor &weight_, const Tensor &weight_scale_, const Maybe &bias_, const Maybe &residual_,
                     int64_t act, bool gated, at::ScalarType dtype) {

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(1024) void lin_columns(const float *__restrict__ sh
 
 // ------------------------------------------------------------------ plans
 #define LIN_MOST ((1LL << 31) - 65536)
-#define LIN_MOST_ROW (1LL << 23)  // bytes of an operand's row: what a tile and a stage read lies within 2^32 of its beginning
+#define LIN_MOST_ROW ((long long)DL_LINEAR_ROW)  // bytes of an operand's row: what a tile and a stage read lies within 2^32 of its beginning
 
 static int lin_size(int type) { return type == DL_E4M3 ? 1 : type == DL_F32 ? 4 : 2; }
 
@@ -233,7 +233,7 @@ extern "C" int dl_linear_fwd(const void *x, long long ldx, const float *x_scale,
     const int bad = lin_check(type, out_type, M, N, K, act, gated);
     if (bad) return bad;
     if (ldx < K || ldw < K || (residual && ldr < (gated ? N / 2 : N))) return DL_ERR_SHAPE;
-    if (kept && type == DL_E4M3) return DL_ERR_UNSUPPORTED;
+    if (kept && (type == DL_E4M3 || N * lin_size(type) > LIN_MOST_ROW)) return DL_ERR_UNSUPPORTED;  // (such rows have no backward)
     if (!dl_aligned16(kept)) return DL_ERR_WORKSPACE;
     const size_t need = dl_linear_fwd_workspace_bytes(x, ldx, w, ldw, type, M, N, K, gated);
     if (need && !ws) return DL_ERR_NULL;

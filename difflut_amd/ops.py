@@ -683,7 +683,8 @@ def linear(x, weight, bias=None, activation="none", residual=None):
     """activation(x weight^T + bias) + residual: x (..., in features), weight [out, in], bias [out], residual (..., out), all of one
     type; activation "none", "relu", "silu" or "sigmoid".  A product and what follows it are one launch; for the backward the values in
     front of an activation are kept in 24 bits (float32: 32), and the gradient behind it is rounded to x's type before the backward's products.
-    float32 is multiplied to within its own rounding, values below 2^-110 as multiples of 2^-133; there, products with infinities are NaN."""
+    float32 is multiplied to within its own rounding, values below 2^-110 as multiples of 2^-133; there, products with infinities are NaN.
+    Rows of x and weight have up to 2^23 bytes on the device, and with gradients the rows of x weight^T as well; beyond, the call raises."""
     _check_linear("linear", x, weight, bias, activation, residual, False)
     if not x.is_cuda or x.numel() == 0:
         return cpu_ops.linear(x, weight, bias, activation, residual, False)

@@ -573,8 +573,9 @@ int dl_rms_norm_bwd(const void *h, long long ldh, const void *gamma, const float
  * layout is the library's own.
  * Backward: from gy (contiguous, y's shape) the gradients gx [M, K], gw [N, K], gb [N], each nullable; kept as the forward left it (null where act
  * is DL_ACT_NONE and not gated); the residual's gradient is gy.  `wants` of the size query: 1 gx, 2 gw, 4 gb.
- * The size queries look at pointers for their alignment alone.  Rows of operands up to 2^23 bytes, in the backward also M and N up to 2^22
- * (DL_ERR_UNSUPPORTED beyond). */
+ * The size queries look at pointers for their alignment alone.  Rows of operands up to DL_LINEAR_ROW bytes, as are rows of N values where something is kept,
+ * and in the backward, which has them as an operand (DL_ERR_UNSUPPORTED beyond). */
+#define DL_LINEAR_ROW (1 << 23)
 size_t dl_linear_fwd_workspace_bytes(const void *x, long long ldx, const void *w, long long ldw, int type, long long M, long long N, long long K, int gated);
 size_t dl_linear_kept_bytes(int type, long long M, long long N, int gated);
 int dl_linear_fwd(const void *x, long long ldx, const float *x_scale, const void *w, long long ldw, const float *w_scale, const void *bias,

@@ -384,6 +384,35 @@ def test_linear_of_values_up_to_the_largest(device, M, K, N, where):
         close(grad, want, off, torch.float32)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,dtype,act", [(2, 1, 1 << 21, torch.float32, "none"), (3, 2, 1 << 22, torch.bfloat16, "silu"), ((1 << 22) + 5, 8, 8, torch.bfloat16, "silu"), ((1 << 22) + 5, 3, 2, torch.float32, "none")])
+def test_linear_up_to_its_limits(M, K, N, dtype, act):
+    """The longest rows that have a backward, and more rows than that."""
+    check_linear("cuda", M, K, N, dtype, act, False, True, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act,gated", [("none", False), ("silu", False), ("sigmoid", True)])
+def test_linear_of_rows_without_a_backward(dtype, act, gated):
+    """Refused by the call itself where gradients are asked for; without them, and of the residual's alone, it runs."""
+    N = (1 << 23) // dtype.itemsize + 2
+    g = gen(7)
+    x, w = torch.randn(2, 3, generator=g).to(dtype).cuda(), torch.randn(N, 3, generator=g).to(dtype).cuda()
+    f = ops.gated_linear if gated else ops.linear
+    (y, y_off), *_ = linear_64(x, w, None, None, act, gated, torch.zeros(2, N // 2 if gated else N, device="cuda"))
+    close(f(x, w, activation=act), y, y_off, dtype)
+    b = torch.zeros(N, dtype=dtype, device="cuda")
+    for leaves in ((x.clone().requires_grad_(), w, b), (x, w.clone().requires_grad_(), b), (x, w, b.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            f(*leaves, activation=act)
+        with torch.no_grad():
+            close(f(*leaves, activation=act), y, y_off, dtype)
+    r = torch.ones(2, N // 2 if gated else N, dtype=dtype, device="cuda").requires_grad_()
+    out = f(x, w, activation=act, residual=r)
+    assert torch.equal(torch.autograd.grad(out, r, torch.full_like(out, 2.0))[0], torch.full_like(out, 2.0))
+
+
 # few rows: short and long reductions, rows of w shared by two wavefronts or eight, the last group inside a block, up to 16, 32 and 64 rows
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,K,N,dtype,gated", [
@@ -907,6 +936,14 @@ def test_c_entry_points_refuse():
     order = lambda src=one, dst=one, n=1, parents=p, B=2: lib.dl_beam_reorder(src, dst, sizes, n, parents, B, 3, 3, None)  # noqa: E731
     assert [order(parents=0), order(src=zero), order(dst=zero)] == [NULL] * 3
     assert [order(n=0), order(B=0)] == [SHAPE] * 2 and order(n=9) == UNSUPPORTED
+
+
+def test_c_entry_point_refuses_to_keep_rows_without_a_backward():
+    from difflut_amd import _native as nat
+
+    p = 4096
+    call = lambda kept, N, t=1: nat.lib().dl_linear_fwd(p, 64, 0, p, 64, 0, None, 0, 0, p, kept, t, t, 4, N, 64, 2, 0, None, 0, None)  # noqa: E731
+    assert [call(p, 2 ** 22 + 1), call(p, 2 ** 21 + 1, 0), call(p, 2 ** 22 + 1, 2)] == [-3] * 3
 
 
 @pytest.mark.gpu
