@@ -9,7 +9,7 @@
 //
 // One product kernel serves all of them: C[r,c] = sum_k A(r,k) B(c,k).  An operand lies with the reduction along its rows of memory, or
 // (w for gx, gz and x for gw) with the reduction across them, and is turned on the way out of the LDS.  Operands whose rows do not
-// start on 16 bytes or end inside 16 are copied to rows that do, by a pass in front of it.
+// start on 16 bytes, end inside 16 or lie more than 2^23 bytes apart are copied to rows that do not, by a pass in front of it.
 //
 // float32 values are cut into three bf16 planes on the way out of the LDS (8 + 8 + 8 significant bits, each the rounding of what the ones
 // above left); a product is the six plane products hi*lo, lo*hi, mid*mid, hi*mid, mid*hi, hi*hi, small ones first.  What is left out is

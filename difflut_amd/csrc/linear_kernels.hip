@@ -4,7 +4,7 @@
 
 #include "linear.h"
 
-// ------------------------------------------------------------------ operands whose rows are not whole units
+// ------------------------------------------------------------------ operands whose rows are not whole units, or lie far apart
 // src [rows][n], ld apart -> dst [rows][padded], zeros from n on; padded is a multiple of 16 bytes
 template <typename T>
 __global__ __launch_bounds__(256) void lin_pad(const T *__restrict__ src, long long ld, T *__restrict__ dst, long long rows, long long n,
@@ -124,7 +124,7 @@ struct LinOperand {
 };
 static bool lin_direct(const LinOperand &o, int type) {
     const int size = lin_size(type);
-    return dl_aligned16(o.p) && o.ld * size % 16 == 0 && (o.padded || o.length * size % 16 == 0);
+    return dl_aligned16(o.p) && o.ld * size % 16 == 0 && o.ld * size <= LIN_MOST_ROW && (o.padded || o.length * size % 16 == 0);
 }
 static long long lin_padded(const LinOperand &o, int type) { const int unit = 16 / lin_size(type); return (o.length + unit - 1) / unit * unit; }
 static size_t lin_operand_bytes(const LinOperand &o, int type) {
@@ -183,7 +183,6 @@ static int lin_run(const LinOperand &a, const LinOperand &b, int type, int out_t
     LinArgs g{};
     if (p.few) g.A = (const char *)a.p, g.lda = a.ld * lin_size(type), g.B = (const char *)b.p, g.ldb = b.ld * lin_size(type);
     else g.A = lin_lay_out(a, type, ws, g.lda, s), g.B = lin_lay_out(b, type, ws + p.a_bytes, g.ldb, s);
-    if (!p.few && (g.lda > LIN_MOST_ROW || g.ldb > LIN_MOST_ROW)) return DL_ERR_UNSUPPORTED;
     g.part = (float *)(ws + p.a_bytes + p.b_bytes);
     end.R = (int)a.count(), end.C = (int)b.count(), end.F = end.C / 2;
     const int width = gated ? end.F : end.C, size = dl_type_bytes(out_type);

@@ -392,6 +392,26 @@ def test_linear_up_to_its_limits(M, K, N, dtype, act):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(5, 40), (5, 8), (70, 40)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("far", ["x", "w"])
+def test_linear_of_rows_far_apart(M, N, dtype, far):
+    """Some columns of a matrix with rows of more than 2^23 bytes: forward and backward, of few rows and by tiles."""
+    g = gen(M + N)
+    D, K = (1 << 23) // dtype.itemsize + 64, 64
+    x, w, gy = torch.randn(M, K, generator=g).to(dtype).cuda(), (torch.randn(N, K, generator=g) / 8).to(dtype).cuda(), torch.randn(M, N, generator=g).to(dtype).cuda()
+    wide = torch.empty(M if far == "x" else N, D, dtype=dtype, device="cuda")
+    cut = wide[:, 128:128 + K]
+    cut.copy_(x if far == "x" else w)
+    (y, y_off), gx, gw, _ = linear_64(x, w, None, None, "none", False, gy)
+    leaves = [t.requires_grad_() for t in ((cut.detach(), w) if far == "x" else (x, cut.detach()))]
+    got = ops.linear(*leaves)
+    close(got, y, y_off, dtype)
+    for grad, (want, off) in zip(torch.autograd.grad(got, leaves, gy), (gx, gw)):
+        close(grad, want, off, dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act,gated", [("none", False), ("silu", False), ("sigmoid", True)])
 def test_linear_of_rows_without_a_backward(dtype, act, gated):
