@@ -118,15 +118,15 @@ __device__ __forceinline__ DlVec<Out, 8> lin_residual(const LinEnd &g, int width
     return f;
 }
 // Eight columns from c on of row r, from their sums v (gated: the gate's, u the other half's), the row's scale and the residual
-template <typename Out, bool GATED, bool SCALED>
+template <typename Out, bool GATED>
 __device__ __forceinline__ void lin_finish(const LinEnd &g, const LinColumns<Out, GATED> &k, int r, int c, float (&v)[8], float (&u)[8], float row_scale, const DlVec<Out, 8> &res) {
     const int width = GATED ? g.F : g.C;
     if (r >= g.R || c >= width) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         constexpr int H = GATED ? 1 : 0;
-        v[i] = SCALED ? fmaf(v[i], row_scale * k.scale[0][i], k.bias[0][i]) : v[i] + k.bias[0][i];
-        if (GATED) u[i] = SCALED ? fmaf(u[i], row_scale * k.scale[H][i], k.bias[H][i]) : u[i] + k.bias[H][i];
+        v[i] = fmaf(v[i], row_scale * k.scale[0][i], k.bias[0][i]);
+        if (GATED) u[i] = fmaf(u[i], row_scale * k.scale[H][i], k.bias[H][i]);
     }
     if (g.kept) {
         lin_keep<Out, 8>(g, r, c, v);
@@ -834,7 +834,7 @@ __global__ __launch_bounds__(256) void lin_join(LinArgs g, int splits) {
                 if (GATED) u[i] += q[i];
             }
         }
-        lin_finish<Out, GATED, true>(g.end, LinColumns<Out, GATED>(g.end, c), r, c, v, u, g.end.row_scale ? g.end.row_scale[r] : 1.0f, res);
+        lin_finish<Out, GATED>(g.end, LinColumns<Out, GATED>(g.end, c), r, c, v, u, g.end.row_scale ? g.end.row_scale[r] : 1.0f, res);
     }
 }
 
