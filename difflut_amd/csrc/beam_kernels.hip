@@ -260,20 +260,18 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_rows(BeamArgs g) {
 }
 
 // A block takes a sequence's K * pieces lists of `count` candidates, best first.  The count-th of the lists' best bounds them from below, where
-// there are as many lists; every candidate that passes it counts the better ones.
-#define BEAM_RANKS 1024  // candidates that are ranked; from more the best is taken `count` times
-// Candidate a, at place `at` of the lists, before b: equal ones by beam, then key.  Places are in that order but for a beam of several lists (per: places of a
-// beam; 0: they are).
-__device__ __forceinline__ bool beam_before(double a, int at, double b, int bt, const beam_key *keys, int per) {
-    if (a != b || at == bt) return a > b;
-    if (per == 0 || at / per != bt / per) return at < bt;
-    return keys[at] > keys[bt];
-}
+// there are as many lists; every candidate that passes it counts the better ones, or where there are many the best of all is taken `count` times.
+// Ranking m takes about 0.3 ns m^2, taking the best count times 1.4 us each.
+#define BEAM_RANKS 512
+__device__ __forceinline__ bool beam_ranked(int m, int count) { return m <= BEAM_RANKS && m * m <= 4096 * count; }
+__device__ __forceinline__ bool beam_before(double a, beam_key ka, double b, beam_key kb) { return a > b || (a == b && ka > kb); }
 __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
     __shared__ double value[BEAM_PICKS], norm[BEAM_MOST], base[BEAM_MOST], wave_value[BEAM_WAVES], bound;
     __shared__ double kept_value[BEAM_RANKS];
-    __shared__ float largest[BEAM_PICKS];
-    __shared__ int kept_at[BEAM_RANKS], wave_at[BEAM_WAVES], kept, ended[BEAM_MOST];
+    // Of equal candidates the one with the larger key comes first: the earlier beam's, of one beam the larger logit's, then the one that lies first in
+    // the lists, at the place that the last bits say.  (Before that the lists' largest.)
+    __shared__ beam_key key[BEAM_PICKS], kept_key[BEAM_RANKS], wave_key[BEAM_WAVES];
+    __shared__ int kept, ended[BEAM_MOST];
     const int tid = threadIdx.x, b = blockIdx.x, per = g.pieces * g.count, n = g.K * per, lists = g.K * g.pieces;
     const double inf = __builtin_inf();
     const beam_key *keys = g.keys + (long long)b * n;
@@ -291,7 +289,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
     }
     for (int e = tid; e < lists; e += BEAM_THREADS) {
         const BeamPart p = parts[e];
-        value[e] = p.sum, largest[e] = p.largest;
+        value[e] = p.sum, key[e] = __float_as_uint(p.largest);
     }
     if (tid == 0) kept = 0, bound = -inf;
     __syncthreads();
@@ -300,8 +298,8 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
         const int first = e / g.pieces * g.pieces;
         if (ended[e / g.pieces]) continue;
         float most = -__builtin_inff();
-        for (int i = 0; i < g.pieces; ++i) most = fmaxf(most, largest[first + i]);
-        value[e] = value[e] > 0.0 ? value[e] * exp((double)largest[e] - (double)most) : 0.0;
+        for (int i = 0; i < g.pieces; ++i) most = fmaxf(most, __uint_as_float((uint32_t)key[first + i]));
+        value[e] = value[e] > 0.0 ? value[e] * exp((double)__uint_as_float((uint32_t)key[e]) - (double)most) : 0.0;
         if (e == first) norm[e / g.pieces] = (double)most;
     }
     __syncthreads();
@@ -311,13 +309,14 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
         norm[tid] = norm[tid] > -inf ? norm[tid] + log(sum) : inf;  // (infinity: nothing to go on with)
     }
     __syncthreads();
-    const auto candidate = [&](int e, beam_key key) __attribute__((always_inline)) {
+    const auto candidate = [&](int e, beam_key of_row) __attribute__((always_inline)) {
         const int k = e / per;
         double c = -inf;
         if (ended[k]) {
             if (e == k * per) c = base[k];
-        } else if (key) c = base[k] + ((double)beam_value(key) - norm[k]);
+        } else if (of_row) c = base[k] + ((double)beam_value(of_row) - norm[k]);
         value[e] = c == c ? c : -inf;
+        key[e] = (beam_key)(BEAM_MOST - k) << 44 | (beam_key)beam_order(of_row) << 12 | (beam_key)(BEAM_PICKS - 1 - e);
     };
 #pragma unroll
     for (int i = 0; i < EARLY; ++i)
@@ -334,12 +333,12 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
         }
     __syncthreads();
     const double least = bound;
-    const int apart = g.pieces > 1 ? per : 0;
+    const auto place = [](beam_key k) { return BEAM_PICKS - 1 - (int)(k & (BEAM_PICKS - 1)); };
     for (int e = tid; e < n; e += BEAM_THREADS) {
         const double c = value[e];
         if (!(c >= least && c > -inf)) continue;
         const int at = atomicAdd(&kept, 1);  // (their order plays no part)
-        if (at < BEAM_RANKS) kept_value[at] = c, kept_at[at] = e;
+        if (at < BEAM_RANKS) kept_value[at] = c, kept_key[at] = key[e];
     }
     __syncthreads();
     const auto answer = [&](int j, double c, int at) __attribute__((always_inline)) {
@@ -351,40 +350,48 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_pick(BeamArgs g) {
     };
     const int m = kept;
     for (int j = m + tid; j < g.count; j += BEAM_THREADS) answer(j, -inf, -1);
-    if (m <= BEAM_RANKS) {
+    if (beam_ranked(m, g.count)) {
         for (int e = tid; e < m; e += BEAM_THREADS) {
             const double mine = kept_value[e];
-            const int at = kept_at[e];
+            const beam_key mine_key = kept_key[e];
             int rank = 0;
 #pragma unroll 4
-            for (int j = 0; j < m; ++j) rank += beam_before(kept_value[j], kept_at[j], mine, at, keys, apart) ? 1 : 0;
-            if (rank < g.count) answer(rank, mine, at);
+            for (int j = 0; j < m; ++j) rank += beam_before(kept_value[j], kept_key[j], mine, mine_key) ? 1 : 0;
+            if (rank < g.count) answer(rank, mine, place(mine_key));
         }
         return;
     }
     double mine = -inf;
-    int mine_at = n;
+    beam_key mine_key = 0;
     const auto own_best = [&]() __attribute__((always_inline)) {
-        mine = -inf, mine_at = n;
+        mine = -inf, mine_key = 0;
+        if (g.pieces > 1) {
+            for (int e = tid; e < n; e += BEAM_THREADS)
+                if (beam_before(value[e], key[e], mine, mine_key)) mine = value[e], mine_key = key[e];
+            return;
+        }
+        int at = -1;  // of one list a beam the first of equal ones has the largest key  (1 x 64 x 50000: 227 us with the loop above, 200)
         for (int e = tid; e < n; e += BEAM_THREADS)
-            if (value[e] > -inf && beam_before(value[e], e, mine, mine_at, keys, apart)) mine = value[e], mine_at = e;
+            if (value[e] > mine) mine = value[e], at = e;
+        if (at >= 0) mine_key = key[at];
     };
     own_best();
     for (int j = 0; j < g.count; ++j) {  // (there are more than `count` above -infinity)
         double best = mine;
-        int at = mine_at;
+        beam_key best_key = mine_key;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             const double v = __shfl_xor(best, o);
-            const int w = __shfl_xor(at, o);
-            if (beam_before(v, w, best, at, keys, apart)) best = v, at = w;
+            const beam_key w = __shfl_xor(best_key, o);
+            if (beam_before(v, w, best, best_key)) best = v, best_key = w;
         }
-        if ((tid & 63) == 0) wave_value[tid >> 6] = best, wave_at[tid >> 6] = at;
+        if ((tid & 63) == 0) wave_value[tid >> 6] = best, wave_key[tid >> 6] = best_key;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < BEAM_WAVES; ++w)
-            if (beam_before(wave_value[w], wave_at[w], best, at, keys, apart)) best = wave_value[w], at = wave_at[w];
+            if (beam_before(wave_value[w], wave_key[w], best, best_key)) best = wave_value[w], best_key = wave_key[w];
         __syncthreads();
+        const int at = place(best_key);
         if (tid == 0) answer(j, best, at);
         if (at % BEAM_THREADS == tid) {  // its next one
             value[at] = -inf;
