@@ -846,7 +846,8 @@ __global__ __launch_bounds__(256) void lin_join(LinArgs g, int splits) {
 // 269 MB: 40 us, 6.7 TB/s (the memory and the last cache).
 // Which of those: up to 16 always; up to 32 float32, but for few long rows of w, and of the others what w has up to 2^23 values of; up to 64 that and gated (x
 // serves gate and other), not float32.  (us, so and by tiles: bf16 8 x 1024 over 8192 6.8, 11.2, over 131072 52, 51; 32 x 1024 over 8192 8.1, 12.0,
-// over 32768 22, 18; gated 64 x 1024 over 2 x 4096 8.9, 11.7, not gated 14, 11; float32 32 x 1024 over 32768 37, 54, 32 x 4096 over 1024 24, 18.)
+// over 10240 10.5, 10.8, over 12288 10.3, 8.2, over 32768 18, 13; gated 64 x 1024 over 2 x 4096 8.9, 11.7, over 2 x 5120 13.9, 9.8, over 2 x 16384
+// 25, 14, 48 x 1024 over 2 x 8192 12.7, 11.6; 64 x 1024 not gated 14, 11; float32 32 x 1024 over 32768 37, 54, 32 x 4096 over 1024 24, 18.)
 static inline bool lin_few_rows(long long M, long long N, long long K, int size, bool gated) {
     const bool small = N * K <= 1LL << 23 && K <= 2048;
     return M <= 16 || (M <= 32 && (size == 4 ? K <= 2048 || N >= 4096 : small)) || (M <= 64 && gated && size < 4 && small);

@@ -133,7 +133,8 @@ static size_t lin_operand_bytes(const LinOperand &o, int type) {
 // Tile and split: the least of an estimate over both tiles and the splits that leave a part four stages.  A stage takes a block of 256 x 256
 // 1.55 us, the two blocks of 128 x 128 that share a CU 0.95, one that has it alone 0.6 (float32: three times that); a tile's beginning and end
 // take 5 and 3 us; sums are written and read at 4 bytes/ps, with 4 us for the launch that joins them.  (bf16, 8192^3: 256 787 us, 128 970; 1024 x 4096 over
-// 12544, us with the join: 256 in 4 parts 98, 128 in 2 parts 104, 256 whole 360.)
+// 12544, us with the join: 256 in 4 parts 98, 128 in 2 parts 104, 256 whole 360.  The join's share is set too high: that of two parts is 9.7 us and
+// counted as 20.8, so that here the estimate, 118 and 117, takes the second.)
 static LinPlan lin_plan(const LinOperand &a, const LinOperand &b, int type, long long K, bool gated) {
     LinPlan p;
     const long long R = a.count(), C = b.count(), stages = (K * lin_size(type) + LIN_STAGE_BYTES - 1) / LIN_STAGE_BYTES;

@@ -11,7 +11,7 @@
 // every operand, times 2^24, is the EXACT sum of three bf16 planes (8 + 8 + 8 significant bits, each the rounding of what
 // the planes above left; the factor keeps the lowest plane of every fp32 value, denormal ones included, a normal number).
 // A product is the six plane products hi*hi, hi*mid, mid*hi, mid*mid, hi*lo, lo*hi.  The three products left out are
-// below 2^-26 of |a*b| (|mid| <= 2^-9 |a|, |lo| <= 2^-18 |a|), less than the 2^-24 by which one fp32 multiply-add rounds,
+// below 2^-24 of |a*b| (|mid| <= 2^-8 |a|, |lo| <= 2^-17 |a|; root mean square 2^-27), what one fp32 multiply-add rounds off,
 // and bf16 products are exact in fp32, so the result is an fp32 product sum, times 2^48.  Six bf16 products at
 // 2.5 PFLOP/s are 417 TFLOP/s of fp32 work against 157 on the fp32 matrix cores.
 // Where a sum of an operand's size could overflow with that factor, or as the sum before rs, while the result does not, and

@@ -728,7 +728,8 @@ def beam_step(logits, scores, beams=None, finished=None, end=0):
     A beam that is `finished` (bool [batch, beams in]) goes on by one continuation alone, the token `end` at its own score; its logits are not
     looked at.  NaN logits are no continuations, infinite ones count as the largest number; where there are fewer continuations above
     -infinity than asked for, the rest have score -infinity, parent 0 and token -1.  Beams start as [0, -infinity, ...].
-    Scores are compared as doubles.  Up to 64 beams.  No gradient."""
+    Scores are compared as doubles, which on the device hold a log-softmax that is right to about 2^-22: continuations of different beams that lie closer
+    may change places.  Up to 64 beams.  No gradient."""
     if logits.dim() != 3 or logits.shape[1] == 0 or logits.shape[2] == 0:
         raise ValueError(f"beam_step expects logits (batch, beams, vocabulary), got shape {tuple(logits.shape)}")
     shape = tuple(logits.shape[:2])

@@ -590,7 +590,7 @@ int dl_linear_bwd(const void *x, long long ldx, const void *w, long long ldw, co
  * scores[b, k] + log_softmax(logits[b, k, :])[v], largest first, equal ones by beam, then logit, then token.  logits [B * K, V] (ldl between rows),
  * scores [B, K]; ended (nullable) [B, K]: a beam with a non-zero byte goes on by (its score, token `end`) alone, its logits are not read.
  * NaN logits are no candidates, infinite ones count as the largest number.  Where there are fewer candidates above -infinity: score
- * -infinity, parent 0, token -1.  K and count up to 64, V up to 2^30 (DL_ERR_UNSUPPORTED).
+ * -infinity, parent 0, token -1.  Compared as doubles, of log_softmax values that are right to about 2^-22.  K and count up to 64, V up to 2^30 (DL_ERR_UNSUPPORTED).
  * dl_beam_reorder: dst[t][b, j] = src[t][b, parents[b, j]] for n tensors of row_bytes[t] bytes per beam (src, dst, row_bytes: HOST arrays);
  * a parent outside [0, K) gives zeros.  dst does not overlap src. */
 #define DL_BEAM_STATES 8
