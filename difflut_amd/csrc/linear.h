@@ -747,7 +747,7 @@ __global__ __launch_bounds__(256, TR * TC > 128 * 128 ? 1 : 2) void lin_product(
     for (;;) {
         const auto multiply = [&](auto wide) __attribute__((always_inline)) {
             lin_stage_barrier<0>();  // the first stages are there, and the tile before is written out of the LDS
-    #pragma unroll
+#pragma unroll
             for (int j = 0; j < NB; ++j) load_b(lin_buffer(b_second, there(1)), lin_buffer(b_second + b_half, there(1)), lds_base + B1, j);
             a_now = A0, a_next = A1, a_free = A2, b_now = B0;
             uint64_t at_a = a_second, at_b = b_second;

@@ -361,6 +361,26 @@ def test_linear_of_the_lowest_value_times_nothing(device, M, K, N, gated):
                 assert torch.equal(f(*(t.to(device) for t in ((a, other) if masked is xs else (other, a))), activation="silu"), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(32, 640, 514), (300, 72, 300), (300, 2080, 514), (4100, 72, 4104)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_of_one_largest_value_wherever_it_stands(M, K, N, gated):
+    """In any row of a tile of either operand: nothing but its product with zero comes of it."""
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    x, w = torch.randn(M, K, device="cuda", generator=g), torch.randn(N, K, device="cuda", generator=g) / math.sqrt(K)
+    f = ops.gated_linear if gated else ops.linear
+    k = 41
+    x[:, k], w[:, k] = 0.0, 0.0
+    want = f(x, w)
+    same = torch.ones((), dtype=torch.bool, device="cuda")
+    for t in (x, w):
+        for r in [*range(min(300, t.shape[0])), t.shape[0] - 1]:
+            t[r, k] = torch.finfo(torch.float32).max
+            same &= (f(x, w) == want).all()
+            t[r, k] = 0.0
+    assert bool(same)
+
+
 @pytest.mark.parametrize("device,M,K,N", HUGE)
 @pytest.mark.parametrize("where", ["x", "w", "gy"])
 def test_linear_of_values_up_to_the_largest(device, M, K, N, where):
